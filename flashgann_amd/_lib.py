@@ -21,11 +21,13 @@ FG_ENTRY_AUTO = 0xFFFFFFFF
 FG_COUNTERS_PER_QUERY = 6
 FG_PROFILE_SLOTS = 12
 FG_NOALLOC_STAGING_BYTES = 16 << 20
+FG_BF16 = 0
+FG_F16 = 1
 
 EXPORTED = (
     "fg_index_create", "fg_index_load", "fg_index_destroy", "fg_index_get_info", "fg_search", "fg_search_noalloc",
     "fg_search_device", "fg_search_stream", "fg_search_profile", "fg_lds_bytes", "fg_search_waves", "fg_search_launches", "fg_search_geometry", "fg_encode_rows", "fg_query_prepare", "fg_score_edges", "fg_last_error",
-    "fg_version",
+    "fg_version", "fg_cache_plan", "fg_cache_append", "fg_attend", "fg_attend_retrieved", "fg_attend_workspace_bytes",
 )
 
 
@@ -87,6 +89,15 @@ def lib():
         L.fg_query_prepare.argtypes = [vp, f32p, C.c_uint32, f32p, u8p, f32p, i32p]
         L.fg_score_edges.argtypes = [vp, f32p, C.c_uint32, u32p, u32p, u32p, C.c_uint32, f32p,
                                      f32p, f32p]
+        i64 = C.c_int64
+        L.fg_cache_plan.argtypes = [vp, vp, C.c_uint32, vp, i64, C.c_uint32, vp, C.c_uint32, C.c_uint32, C.c_uint32,
+                                    vp, vp, vp, vp, vp, vp]
+        # the structs arrive packed (flashgann_amd.attention)
+        L.fg_cache_append.argtypes = [C.c_char_p, vp, vp, i64, i64, i64, i64, vp, C.c_uint32, vp]
+        L.fg_attend.argtypes = [C.c_char_p, C.c_char_p, vp]
+        L.fg_attend_retrieved.argtypes = L.fg_attend.argtypes
+        L.fg_attend_workspace_bytes.argtypes = [C.c_uint32]
+        L.fg_attend_workspace_bytes.restype = C.c_uint64
         L.fg_last_error.restype = C.c_char_p
         L.fg_version.restype = C.c_char_p
         _lib = L

@@ -1,0 +1,522 @@
+// fg_attend.hip -- attention over a paged key/value cache.
+//
+// For a row with query q, scores s_j = scale2 * (q . k_j) of the visible tokens
+// (scale2 = scale * log2 e, so that weights are powers of two), maximum m:
+//   out = sum 2^(s_j - m) v_j / l,  l = sum 2^(s_j - m),  lse = ln 2 (m + log2 l)
+// in one pass over the tokens: a new maximum m' multiplies what is summed so far
+// by 2^(m - m').  Products run on the matrix unit, transposed: S' = K Q', then
+// O' = V' P', so that a query row is a lane's column in both.  Its weights leave
+// the first product in the lanes where the second wants them, once the second's
+// contraction takes the tokens in the order that the first leaves them, and V is
+// read from LDS in that order by the transposing read.
+#include "fg_attend.hpp"
+
+namespace fgk {
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+struct BF16 {
+    using vec = bf16x8;
+    static constexpr uint32_t kExponent = 0x7F80, kMantissa = 0x007F, kOne = 0x3F80;
+    static __device__ __forceinline__ f32x4 mfma16(vec a, vec b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+};
+struct F16 {
+    using vec = f16x8;
+    static constexpr uint32_t kExponent = 0x7C00, kMantissa = 0x03FF, kOne = 0x3C00;
+    static __device__ __forceinline__ f32x4 mfma16(vec a, vec b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+};
+
+// Four rows of one column each: lane i of 16 gets column i of the 4 x 16 block
+// whose row i / 4, columns 4 (i % 4) .. + 3 lie at lane i's address.
+__device__ __forceinline__ s16x4 read_transposed(const char *lds) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds));
+}
+
+template <class T>
+__device__ __forceinline__ bool any_special(uint4 w) {
+    bool s = false;
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        s |= (x[i] & T::kExponent) == T::kExponent || ((x[i] >> 16) & T::kExponent) == T::kExponent;
+    return s;
+}
+
+// a with its infinities and NaNs as zeros; ones in `pos` for +inf and NaN, in
+// `neg` for -inf and NaN.
+template <class T>
+__device__ __forceinline__ s16x8 split_special(s16x8 a, s16x8 *pos, s16x8 *neg) {
+    s16x8 fine;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t x = static_cast<uint16_t>(a[i]);
+        const bool special = (x & T::kExponent) == T::kExponent, nan = special && (x & T::kMantissa);
+        fine[i] = special ? 0 : a[i];
+        (*pos)[i] = nan || (special && !(x & 0x8000)) ? static_cast<short>(T::kOne) : 0;
+        (*neg)[i] = nan || (special && (x & 0x8000)) ? static_cast<short>(T::kOne) : 0;
+    }
+    return fine;
+}
+
+// ---------------------------------------------------------------- few rows
+//
+// Blocks of 16 query rows; each of the four waves takes every fourth tile of 32
+// tokens and keeps a softmax of its own, joined through LDS at the end.  Bound
+// by the cache's bytes: a tile is 32 x D keys and values against 16 rows.
+constexpr uint32_t kRows = 16;
+constexpr uint32_t kRowsUnit = 128;    // tokens a unit: one tile of each wave
+constexpr uint32_t kPlaces = 1024;     // token places resolved at a time
+constexpr uint32_t kWorkgroups = 512;  // at most: two a CU, two parts of the workspace each
+
+template <class T, int D, bool FOUND>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendParams P) {
+    using vec = typename T::vec;
+    constexpr int STEPS = D / 32, DB = D / 16;
+    constexpr uint32_t VROW = 2 * D + 32;  // bytes of a row of V in LDS: 16 rows' 32-byte pieces meet each bank twice
+    constexpr uint32_t OROW = D + 4;       // floats of a row of O in LDS
+    static_assert(kRows * OROW * 4 <= 32 * VROW);
+    __shared__ __attribute__((aligned(16))) char vbuf[4][32 * VROW];
+    __shared__ int2 place[kPlaces];
+    __shared__ float wave_m[4][kRows], wave_l[4][kRows];
+
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, col = lane % 16, quarter = lane / 16;
+    const uint32_t w = blockIdx.x, W = gridDim.x;
+    const Start start = find_start<FOUND, kRows, kRowsUnit>(P, w, W, 1);
+    if (P.join && tid == 0) P.joins[w].pieces = 0;
+    const uint64_t x1 = min((w + 1) * start.share, start.units);
+    uint64_t before = start.before;
+    uint32_t r = start.request;
+    char *const vmine = vbuf[wave];
+
+    for (uint64_t x = w * start.share; x < x1;) {
+        const Request rq = request_of<FOUND, kRows, kRowsUnit>(P, r);
+        const uint64_t all = static_cast<uint64_t>(rq.blocks) * rq.units * P.lists;
+        if (x >= before + all) {
+            before += all;
+            ++r;
+            continue;
+        }
+        const uint64_t item = (x - before) / rq.units;
+        const uint32_t u0 = static_cast<uint32_t>((x - before) - item * rq.units);
+        const uint32_t u1 = static_cast<uint32_t>(min(static_cast<uint64_t>(rq.units), u0 + (x1 - x)));
+        const uint32_t list = static_cast<uint32_t>(item / rq.blocks), block = static_cast<uint32_t>(item - static_cast<uint64_t>(list) * rq.blocks);
+        const Span sp = span_of<FOUND, kRows>(P, rq, block);
+        const int32_t t_lo = static_cast<int32_t>(min(static_cast<uint64_t>(u0) * kRowsUnit, static_cast<uint64_t>(sp.total)));
+        const int32_t t_hi = static_cast<int32_t>(min(static_cast<uint64_t>(u1) * kRowsUnit, static_cast<uint64_t>(sp.total)));
+        const int32_t row0 = static_cast<int32_t>(block * kRows);
+
+        // this lane's row: its query, and where its token stands
+        const int32_t row = row0 + static_cast<int32_t>(col);
+        const int32_t token = P.group.div(row);
+        const int32_t pos = sp.pos0 + token;
+        const bool ragged = !FOUND && P.group.div(row0) != P.group.div(min(row0 + static_cast<int32_t>(kRows), rq.rows) - 1);
+        vec qv[STEPS];
+        {
+            const int64_t head = static_cast<int64_t>(list) * P.group.d + (row - token * static_cast<int32_t>(P.group.d));
+            const char *src = P.q + (rq.q0 + static_cast<int64_t>(token)) * P.q_token + head * P.q_head + quarter * 16;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                uint4 v = {0, 0, 0, 0};
+                if (row < rq.rows) v = *reinterpret_cast<const uint4 *>(src + 64 * s);
+                qv[s] = __builtin_bit_cast(vec, v);
+            }
+        }
+        const uint32_t kv_head = list / P.list_heads;
+        const char *const kbase = P.cache.k + kv_head * P.cache.k_head + quarter * 16;
+        const char *const vbase = P.cache.v + kv_head * P.cache.v_head + quarter * 16;
+
+        float m = -INFINITY, l = 0.0f;
+        f32x4 o[DB];
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
+
+        for (int32_t c0 = t_lo; c0 < t_hi; c0 += kPlaces) {
+            const int32_t n = min(t_hi - c0, static_cast<int32_t>(kPlaces));
+            __syncthreads();
+            for (int32_t i = tid; i < ((n + 31) & ~31); i += 256) {
+                const int32_t t = c0 + i;
+                int2 at = {-1, 0};
+                if (t < min(t_hi, sp.dense)) {
+                    at = place_of(P, r, position_of(sp, t));
+                } else if (FOUND && t < t_hi) {
+                    const int32_t k = t - sp.dense;
+                    const uint32_t *ids = P.ids + (static_cast<uint64_t>(r) * P.lists + list) * P.nids;
+                    const uint32_t id = ids[k];
+                    const bool repeat = k > 0 && ids[k - 1] == id;
+                    // (a window of the whole context or more leaves from = first: no id counts)
+                    if (!repeat && id < static_cast<uint32_t>(min(sp.from, rq.limit)) && id >= static_cast<uint32_t>(sp.first))
+                        at = place_of(P, r, static_cast<int32_t>(id));
+                }
+                place[i] = at;
+            }
+            __syncthreads();
+
+            uint4 kr[2][STEPS], vr[2][STEPS];
+            bool held[2];
+            const auto load = [&](int32_t tile) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int2 at = place[tile * 32 + 16 * b + col];
+                    held[b] = at.x >= 0;
+                    const int64_t page = max(at.x, 0);
+                    const char *ks = kbase + page * P.cache.k_page + at.y * P.cache.k_token;
+                    const char *vs = vbase + page * P.cache.v_page + at.y * P.cache.v_token;
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s) {
+                        kr[b][s] = *reinterpret_cast<const uint4 *>(ks + 64 * s);
+                        vr[b][s] = *reinterpret_cast<const uint4 *>(vs + 64 * s);
+                    }
+                }
+            };
+            if (static_cast<int32_t>(wave) * 32 < n) load(wave);
+            for (int32_t tile = wave; tile * 32 < n; tile += 4) {
+                // scores: register i of s[b] is token 16 b + 4 quarter + i
+                f32x4 s[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    s[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) s[b] = T::mfma16(__builtin_bit_cast(vec, kr[b][k]), qv[k], s[b]);
+                }
+                const uint32_t held0 = static_cast<uint32_t>(__ballot(held[0])) & 0xFFFFu;
+                const uint32_t held1 = static_cast<uint32_t>(__ballot(held[1])) & 0xFFFFu;
+                bool special = false;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        // what no row may see can hold anything: 0 * inf would be NaN
+                        const uint4 v = held[b] ? vr[b][k] : uint4{0, 0, 0, 0};
+                        if (ragged) special |= any_special<T>(v);
+                        *reinterpret_cast<uint4 *>(vmine + (16 * b + col) * VROW + 64 * k + 16 * quarter) = v;
+                    }
+                if ((tile + 4) * 32 < n) load(tile + 4);
+
+                float p[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[i] = s[i / 4][i % 4] * P.scale2;
+                uint32_t see = ((held0 >> (4 * quarter)) & 15u) | (((held1 >> (4 * quarter)) & 15u) << 4);
+                if (ragged) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int32_t j = position_of(sp, c0 + tile * 32 + 16 * (i / 4) + 4 * static_cast<int32_t>(quarter) + i % 4);
+                        const int32_t back = pos - j;
+                        if (back < 0 || (static_cast<uint32_t>(back) >= P.window && static_cast<uint32_t>(j) >= P.sinks)) see &= ~(1u << i);
+                    }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    p[i] = (see >> i) & 1u ? p[i] : -INFINITY;
+                    top = fmaxf(top, p[i]);
+                }
+                top = fmaxf(m, max_other32(max_other16(top)));
+                const float base = top == -INFINITY ? 0.0f : top;
+                if (__any(top > m)) {
+                    const float shrink = __builtin_amdgcn_exp2f(m - base);
+                    l *= shrink;
+#pragma unroll
+                    for (int i = 0; i < DB; ++i) o[i] *= shrink;
+                    m = top;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    p[i] = __builtin_amdgcn_exp2f(p[i] - base);
+                    l += p[i];
+                }
+                // weights in the values' type: the matrix unit takes both alike, and
+                // the rounding of a weight is that of an output element
+                uint4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+                const vec pv = __builtin_bit_cast(vec, pk);
+                const char *vt = vmine + (4 * quarter + col / 4) * VROW + (col % 4) * 8;
+                if (!__any(special)) {
+#pragma unroll
+                    for (int i = 0; i < DB; ++i) {
+                        const s16x4 a0 = read_transposed(vt + 32 * i), a1 = read_transposed(vt + 16 * VROW + 32 * i);
+                        const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[i] = T::mfma16(__builtin_bit_cast(vec, a), pv, o[i]);
+                    }
+                } else {
+                    // infinities and NaNs reach the rows that see them and no others
+                    s16x8 ones;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ones[i] = (see >> i) & 1u ? static_cast<short>(T::kOne) : 0;
+                    const vec seen = __builtin_bit_cast(vec, ones);
+#pragma unroll
+                    for (int i = 0; i < DB; ++i) {
+                        const s16x4 a0 = read_transposed(vt + 32 * i), a1 = read_transposed(vt + 16 * VROW + 32 * i);
+                        s16x8 pos_a, neg_a;
+                        const s16x8 a = split_special<T>(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), &pos_a, &neg_a);
+                        o[i] = T::mfma16(__builtin_bit_cast(vec, a), pv, o[i]);
+                        const f32x4 up = T::mfma16(__builtin_bit_cast(vec, pos_a), seen, f32x4{0, 0, 0, 0});
+                        const f32x4 down = T::mfma16(__builtin_bit_cast(vec, neg_a), seen, f32x4{0, 0, 0, 0});
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if (up[k] > 0.0f) o[i][k] += INFINITY;
+                            if (down[k] > 0.0f) o[i][k] -= INFINITY;
+                        }
+                    }
+                }
+            }
+        }
+
+        // the four waves' softmaxes into one (each wave writes over its own tile of V)
+        l = add_other32(add_other16(l));
+        if (quarter == 0) {
+            wave_m[wave][col] = m;
+            wave_l[wave][col] = l;
+        }
+        float *omine = reinterpret_cast<float *>(vmine);
+#pragma unroll
+        for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4 *>(omine + col * OROW + 16 * i + 4 * quarter) = o[i];
+        __syncthreads();
+        {
+            const uint32_t orow = tid / 16, part = tid % 16;
+            float top = -INFINITY, sum = 0.0f, f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, wave_m[i][orow]);
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[i] = __builtin_amdgcn_exp2f(wave_m[i][orow] - base);
+                sum += f[i] * wave_l[i][orow];
+            }
+            const bool whole = u0 == 0 && u1 == rq.units;
+            const int32_t orow_all = row0 + static_cast<int32_t>(orow);
+            const int32_t otoken = P.group.div(orow_all);
+            const int64_t ohead = static_cast<int64_t>(list) * P.group.d + (orow_all - otoken * static_cast<int32_t>(P.group.d));
+            const int64_t qrow = rq.q0 + static_cast<int64_t>(otoken);
+            const uint32_t slot = 2 * w + (u0 == 0 ? 1 : 0);
+            if (orow_all < rq.rows) {
+                const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+#pragma unroll
+                for (int e = 0; e < D / 32; ++e) {
+                    const uint32_t d = 32 * e + 2 * part;
+                    float a = 0.0f, b = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 v = *reinterpret_cast<const float2 *>(reinterpret_cast<float *>(vbuf[i]) + orow * OROW + d);
+                        a = fmaf(f[i], v.x, a);
+                        b = fmaf(f[i], v.y, b);
+                    }
+                    if (whole)
+                        *reinterpret_cast<uint32_t *>(P.out + qrow * P.out_token + ohead * P.out_head + 2 * d) = T::pack(a * inv, b * inv);
+                    else
+                        *reinterpret_cast<float2 *>(P.part + (static_cast<uint64_t>(slot) * kRows + orow) * D + d) = float2{a, b};
+                }
+                if (part == 0) {
+                    if (!whole)
+                        P.part_ml[slot * kRows + orow] = float2{top, sum};
+                    else if (P.lse)
+                        P.lse[qrow * P.heads + ohead] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+                }
+            }
+            if (P.join && tid == 0 && u0 == 0 && u1 < rq.units) {
+                const uint64_t last = (x + rq.units - 1) / start.share;  // the workgroup that holds its last unit
+                P.joins[w] = Join{static_cast<uint32_t>(last - w + 1), static_cast<uint32_t>(row0), static_cast<uint32_t>(rq.rows),
+                                  static_cast<uint32_t>(rq.q0), list};
+            }
+        }
+        __syncthreads();
+        x += u1 - u0;
+    }
+}
+
+// The parts of an item into its rows: workgroup (w, row) of the item that
+// workgroup w of the attention kernel began and did not end.  Its parts are the
+// second of w and the first of w + 1, w + 2, ...
+template <class T, int D, uint32_t ROWS>
+__global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
+    constexpr uint32_t QUADS = D / 4, SETS = 256 / QUADS;  // threads across a row, sets of parts side by side
+    __shared__ float sum_m[4];
+    __shared__ float acc[SETS][D], acc_l[SETS];
+    const uint32_t w = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+    const Join j = P.joins[w];
+    if (j.pieces == 0 || j.row0 + row >= j.rows) return;
+    const auto slot_of = [&](uint32_t i) { return i == 0 ? 2 * w + 1 : 2 * (w + i); };
+
+    float top = -INFINITY;
+    for (uint32_t i = tid; i < j.pieces; i += 256) top = fmaxf(top, P.part_ml[slot_of(i) * ROWS + row].x);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (tid % 64 == 0) sum_m[tid / 64] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sum_m[0], sum_m[1]), fmaxf(sum_m[2], sum_m[3]));
+    const float base = top == -INFINITY ? 0.0f : top;
+
+    const uint32_t set = tid / QUADS, quad = tid % QUADS;
+    if (set < SETS) {
+        f32x4 a = {0, 0, 0, 0};
+        float l = 0.0f;
+#pragma unroll 4
+        for (uint32_t i = set; i < j.pieces; i += SETS) {
+            const uint32_t at = slot_of(i) * ROWS + row;
+            const float2 ml = P.part_ml[at];
+            const float f = __builtin_amdgcn_exp2f(ml.x - base);
+            a += f * *reinterpret_cast<const f32x4 *>(P.part + static_cast<uint64_t>(at) * D + 4 * quad);
+            l = fmaf(f, ml.y, l);
+        }
+        *reinterpret_cast<f32x4 *>(&acc[set][4 * quad]) = a;
+        if (quad == 0) acc_l[set] = l;
+    }
+    __syncthreads();
+    const uint32_t all = j.row0 + row, token = P.group.div(all), head = j.list * P.group.d + (all - token * P.group.d);
+    const int64_t qrow = static_cast<int64_t>(j.q0) + token;
+    float l = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < SETS; ++i) l += acc_l[i];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (tid < D / 2) {
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < SETS; ++i) {
+            a += acc[i][2 * tid];
+            b += acc[i][2 * tid + 1];
+        }
+        *reinterpret_cast<uint32_t *>(P.out + qrow * P.out_token + head * P.out_head + 4 * tid) = T::pack(a * inv, b * inv);
+    }
+    if (tid == 0 && P.lse) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+}
+
+// ---------------------------------------------------------------- host side
+
+struct Workspace {
+    uint64_t part, ml, joins, total;
+};
+
+Workspace workspace_of(uint32_t dim) {
+    Workspace s;
+    s.part = 0;
+    s.ml = s.part + 2ull * kWorkgroups * kRows * dim * 4;
+    s.joins = s.ml + 2ull * kWorkgroups * kRows * 8;
+    s.total = s.joins + kWorkgroups * sizeof(Join);
+    return s;
+}
+
+template <class T, int D, bool FOUND>
+int launch(AttendParams &P, uint64_t most_units, uint64_t item_units, hipStream_t st) {
+    const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(most_units, kWorkgroups));
+    // an item of one unit lies with one workgroup
+    P.join = item_units > 1;
+    hipLaunchKernelGGL((fg_rows_kernel<T, D, FOUND>), dim3(grid), dim3(256), 0, st, P);
+    if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, kRows>), dim3(grid, kRows), dim3(256), 0, st, P);
+    FG_HIP(hipGetLastError(), "attention launch");
+    return FG_OK;
+}
+
+template <class T, bool FOUND>
+int launch(AttendParams &P, uint32_t dim, uint64_t most_units, uint64_t item_units, hipStream_t st) {
+    switch (dim) {
+    case 64: return launch<T, 64, FOUND>(P, most_units, item_units, st);
+    case 96: return launch<T, 96, FOUND>(P, most_units, item_units, st);
+    case 128: return launch<T, 128, FOUND>(P, most_units, item_units, st);
+    default: return launch<T, 256, FOUND>(P, most_units, item_units, st);
+    }
+}
+
+template <bool FOUND>
+int attend(const fg_kv_cache *c, const fg_attention *a, void *stream) {
+    AttendParams P{};
+    if (int rc = check_cache(c, &P.cache)) return rc;
+    if (!a) return fail(FG_EINVAL, "attention arguments are NULL");
+    if (a->heads < 1 || a->heads > 1024 || a->heads % c->heads_kv)
+        return fail(FG_EINVAL, "heads must be a multiple of heads_kv, at most 1024");
+    if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return fail(FG_EINVAL, "scale must be positive and finite");
+    if (static_cast<uint64_t>(a->tokens) * a->heads > 0x7FFFFFFFull)
+        return fail(FG_EINVAL, "tokens * heads must be below 2^31");
+    if (a->table_width > 0x7FFFFFFFu || a->table_row < 0) return fail(FG_EINVAL, "table_width or table_row out of range");
+    if (a->sinks > 0x7FFFFFFFu) return fail(FG_EINVAL, "sinks must be below 2^31");
+    if (FOUND) {
+        if (a->window < 0) return fail(FG_EINVAL, "window must be >= 0");
+        if (a->lists < 1 || a->heads % a->lists || a->lists % c->heads_kv)
+            return fail(FG_EINVAL, "lists must be a multiple of heads_kv that divides heads");
+        if (a->nids > 0x3FFFFFFFu) return fail(FG_EINVAL, "ids of a list must be below 2^30");
+        if (a->requests != a->tokens) return fail(FG_EINVAL, "one query row a request");
+    } else if (a->window != -1 && a->window < 1) {
+        return fail(FG_EINVAL, "window must be >= 1, or -1 for none");
+    }
+    if (a->requests == 0 || a->tokens == 0) return FG_OK;
+    if (a->requests > 0x00FFFFFFu) return fail(FG_EINVAL, "requests must be below 2^24");
+    if (!a->q || !a->out || !a->kv_lens || (!FOUND && !a->q_starts) || (FOUND && a->nids && !a->ids) ||
+        (a->table_width && !a->table))
+        return fail(FG_EINVAL, "NULL device buffer");
+    if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
+        (a->q_token | a->q_head | a->out_token | a->out_head) % 8)
+        return fail(FG_EINVAL, "q and out must be 16-byte aligned, strides multiples of 8 elements");
+    const Workspace ws = workspace_of(c->dim);
+    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_bytes < ws.total)
+        return fail(FG_EINVAL, "workspace must be 16-byte aligned and hold " + std::to_string(ws.total) + " bytes");
+
+    P.q = static_cast<const char *>(a->q);
+    P.out = static_cast<char *>(a->out);
+    P.lse = a->lse;
+    P.q_token = 2 * a->q_token, P.q_head = 2 * a->q_head, P.out_token = 2 * a->out_token, P.out_head = 2 * a->out_head;
+    P.table = a->table;
+    P.table_row = a->table_row;
+    P.q_starts = a->q_starts;
+    P.kv_lens = a->kv_lens;
+    P.ids = a->ids;
+    P.table_width = a->table_width;
+    P.requests = a->requests;
+    P.tokens = a->tokens;
+    P.heads = a->heads;
+    P.lists = FOUND ? a->lists : c->heads_kv;
+    P.list_heads = P.lists / c->heads_kv;
+    P.nids = FOUND ? a->nids : 0;
+    P.window = static_cast<uint32_t>(a->window);
+    P.sinks = a->window == -1 ? 0 : a->sinks;
+    P.group = fast_div(a->heads / P.lists);
+    P.scale2 = a->scale * 1.44269504088896341f;
+    char *base = static_cast<char *>(a->workspace);
+    P.part = reinterpret_cast<float *>(base + ws.part);
+    P.part_ml = reinterpret_cast<float2 *>(base + ws.ml);
+    P.joins = reinterpret_cast<Join *>(base + ws.joins);
+
+    // what the host knows of the sizes: the table's room bounds a request's tokens
+    uint64_t seen = static_cast<uint64_t>(a->table_width) * c->page_size;
+    if (a->window != -1)
+        seen = std::min(seen, static_cast<uint64_t>(a->sinks) + static_cast<uint32_t>(a->window) + (kRows - 1) / P.group.d + 1);
+    seen += P.nids;
+    const uint64_t item_units = std::max<uint64_t>(1, (seen + kRowsUnit - 1) / kRowsUnit);
+    const uint64_t blocks = (static_cast<uint64_t>(a->tokens) * P.group.d + kRows - 1) / kRows + a->requests;
+    const uint64_t most_units = std::min<uint64_t>(blocks * P.lists, 1u << 20) * std::min<uint64_t>(item_units, 1u << 20);
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    return c->dtype == FG_BF16 ? launch<BF16, FOUND>(P, c->dim, most_units, item_units, st)
+                               : launch<F16, FOUND>(P, c->dim, most_units, item_units, st);
+}
+
+}  // namespace
+}  // namespace fgk
+
+extern "C" {
+
+uint64_t fg_attend_workspace_bytes(uint32_t dim) {
+    return dim == 64 || dim == 96 || dim == 128 || dim == 256 ? fgk::workspace_of(dim).total : 0;
+}
+
+int fg_attend(const fg_kv_cache *cache, const fg_attention *a, void *stream) { return fgk::attend<false>(cache, a, stream); }
+
+int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *stream) {
+    return fgk::attend<true>(cache, a, stream);
+}
+
+}  // extern "C"

@@ -39,6 +39,7 @@
 
 #include "../../include/flashgann.h"
 
+#include "fg_host.hpp"
 #include "fg_kernel.hpp"
 
 using namespace fgk;
@@ -615,19 +616,15 @@ struct fg_index {
 };
 
 namespace {
-
 thread_local std::string g_err;
+}  // namespace
 
-int fail(int code, const std::string &msg) {
+int fgk::fail(int code, const std::string &msg) {
     g_err = msg;
     return code;
 }
 
-#define FG_HIP(call, what)                                                                          \
-    do {                                                                                            \
-        hipError_t _e = (call);                                                                     \
-        if (_e != hipSuccess) return fail(FG_EDEVICE, std::string(what) + ": " + hipGetErrorString(_e)); \
-    } while (0)
+namespace {
 
 void compute_offsets(fg_index *ix) {
     uint32_t b = 1;

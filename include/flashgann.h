@@ -244,6 +244,116 @@ int fg_score_edges(fg_index *index, const float *queries, uint32_t nq, const uin
                    const uint32_t *parents, const uint32_t *slots, uint32_t n, float *est_lanes,
                    float *est_seq, float *exact);
 
+/* ------------------------------------------------------------------------
+ * A paged key/value cache and the attention that reads it.
+ *
+ * For programs that answer with what a search found: the tokens of a long
+ * context have their keys in an index (FG_METRIC_IP), a search with an
+ * attention query returns the positions that carry its weight, and
+ * fg_attend_retrieved attends to them, to the context's first tokens and to
+ * its last ones in one softmax.  fg_attend is the dense form (prompts, short
+ * contexts, layers with a sliding window).  The reference has no counterpart.
+ *
+ * All pointers are device memory; everything is enqueued on `stream` (a
+ * hipStream_t, NULL = default stream) of the current device, without
+ * synchronising, allocating or reading device memory from the host, so every
+ * call can be captured into a graph.  What depends on device values is checked
+ * on the device: lengths below zero count as zero, and a page id outside
+ * [0, pages), a position past the table or a slot outside the cache names
+ * nothing, its token is invisible or is not written. */
+
+#define FG_BF16 0
+#define FG_F16 1
+
+/* A cache of `pages` pages of page_size tokens, heads_kv x dim elements a
+ * token in two tensors.  Strides are in elements, those of dim are 1; every
+ * stride a multiple of 8 and both bases 16-byte aligned.  dim 64, 96, 128 or
+ * 256; page_size >= 1; pages * page_size < 2^31.  Slot s is token s mod
+ * page_size of page s div page_size. */
+typedef struct {
+    void *k, *v;
+    int64_t k_page, k_token, k_head;
+    int64_t v_page, v_token, v_head;
+    uint32_t pages, page_size, heads_kv, dim;
+    int32_t dtype; /* FG_BF16 or FG_F16 */
+    uint32_t reserved;
+} fg_kv_cache;
+
+/* Block tables and slot maps from request lengths, in one launch.  Request r
+ * holds d_lens[r] tokens and gets d_new[r] more; a request's page b (tokens
+ * b * page_size and on) is d_table[r * table_row + b].  Pages it lacks are
+ * taken from d_free[0 .. nfree), requests in order, and written into its row
+ * (-1 once the list is used up; other entries stay).  Outputs:
+ *   d_q_starts  requests + 1  exclusive sums of the new lengths
+ *   d_kv_lens   requests      lens + new
+ *   d_slots     max_tokens    slot of each new token, request after request;
+ *                             -1 where it has no page and past the last token
+ *   d_positions max_tokens    its position (0 past the last token)
+ *   d_used      1             pages needed; above nfree, the list was short
+ * Pages already held are read from the table, so no new page may be handed
+ * out twice: drop the first d_used entries from the free list.
+ * 1 <= requests <= 4096; the new tokens of all requests together < 2^31. */
+int fg_cache_plan(const int32_t *d_lens, const int32_t *d_new, uint32_t requests, int32_t *d_table, int64_t table_row,
+                  uint32_t table_width, const int32_t *d_free, uint32_t nfree, uint32_t page_size,
+                  uint32_t max_tokens, int32_t *d_q_starts, int32_t *d_kv_lens, int64_t *d_slots,
+                  int32_t *d_positions, int32_t *d_used, void *stream);
+
+/* Writes `tokens` rows of keys and values (heads_kv x dim each, strides in
+ * elements, as for the cache) into their slots; a slot outside the cache is
+ * skipped.  Two rows with the same slot leave either. */
+int fg_cache_append(const fg_kv_cache *cache, const void *k, const void *v, int64_t k_token, int64_t k_head,
+                    int64_t v_token, int64_t v_head, const int64_t *d_slots, uint32_t tokens, void *stream);
+
+/* One call of attention.  q and out: (tokens, heads, dim) in the cache's type,
+ * strides in elements, multiples of 8, bases 16-byte aligned; lse: (tokens,
+ * heads) float32, contiguous, may be NULL.  heads is a multiple of the cache's
+ * heads_kv; consecutive query heads share a key/value head.  lse is the natural
+ * logarithm of the sum of exponentials; a row that sees nothing gets 0 and
+ * -infinity.  Scores, softmax statistics and sums are 32-bit; weights are
+ * rounded to the cache's type for the product with the values.
+ * workspace: at least fg_attend_workspace_bytes(dim) bytes, 16-byte aligned,
+ * used until the call's work on `stream` ends; nothing is kept in it between
+ * calls. */
+typedef struct {
+    const void *q;
+    void *out;
+    float *lse;
+    int64_t q_token, q_head, out_token, out_head;
+    const int32_t *table; /* requests x table_width, rows table_row apart */
+    int64_t table_row;
+    const int32_t *q_starts; /* requests + 1 (fg_attend) */
+    const int32_t *kv_lens;  /* requests */
+    const uint32_t *ids;     /* requests x lists x nids, contiguous (fg_attend_retrieved) */
+    void *workspace;
+    uint64_t workspace_bytes;
+    uint32_t table_width, requests, tokens, heads;
+    uint32_t max_q; /* the longest chunk (fg_attend); a hint that picks the kernel */
+    int32_t window; /* -1: none (fg_attend) */
+    uint32_t sinks, lists, nids;
+    float scale; /* > 0 */
+} fg_attention;
+
+/* Attention of chunks of new tokens over the cache.  Request r's queries are
+ * rows q_starts[r] .. q_starts[r + 1) - 1 of q; the last is its token
+ * kv_lens[r] - 1, so the new tokens' own keys and values have to be in the
+ * cache.  The row at position p sees the tokens j <= p and, with a window >= 1,
+ * of those j > p - window and j < sinks.  Rows of q outside every request are
+ * left alone. */
+int fg_attend(const fg_kv_cache *cache, const fg_attention *a, void *stream);
+
+/* Attention of one token a request (q row r at position kv_lens[r] - 1) over
+ * the first `sinks` tokens, the last `window` tokens and the ids of a list.
+ * lists is a multiple of heads_kv that divides heads: the query heads
+ * l * heads/lists and on share list l.  An id counts if it lies below
+ * kv_lens[r], in neither of the first two sets, and differs from the id before
+ * it (a search whose beam is shorter than K repeats its last id); ids are
+ * token positions as fg_search_device writes them. */
+int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *stream);
+
+/* Bytes of workspace that both need at this head dimension; 0 for one that
+ * they do not take. */
+uint64_t fg_attend_workspace_bytes(uint32_t dim);
+
 const char *fg_last_error(void);
 const char *fg_version(void);
 
