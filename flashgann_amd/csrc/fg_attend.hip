@@ -100,28 +100,29 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
 
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, col = lane % 16, quarter = lane / 16;
     const uint32_t w = blockIdx.x, W = gridDim.x;
-    const Start start = find_start<FOUND, kRows, kRowsUnit>(P, w, W, 1);
+    const Start start = find_start<FOUND, kRows, 256>(P, w, W);
     if (P.join && tid == 0) P.joins[w].pieces = 0;
-    const uint64_t x1 = min((w + 1) * start.share, start.units);
+    const uint64_t x1 = min((w + 1) * start.share, start.all);
     uint64_t before = start.before;
     uint32_t r = start.request;
     char *const vmine = vbuf[wave];
 
     for (uint64_t x = w * start.share; x < x1;) {
-        const Request rq = request_of<FOUND, kRows, kRowsUnit>(P, r);
-        const uint64_t all = static_cast<uint64_t>(rq.blocks) * rq.units * P.lists;
+        const Request rq = request_of<FOUND, kRows>(P, r);
+        const uint64_t all = rq.weight_of(rq.blocks) * P.lists;
         if (x >= before + all) {
             before += all;
             ++r;
             continue;
         }
-        const uint64_t item = (x - before) / rq.units;
-        const uint32_t u0 = static_cast<uint32_t>((x - before) - item * rq.units);
-        const uint32_t u1 = static_cast<uint32_t>(min(static_cast<uint64_t>(rq.units), u0 + (x1 - x)));
-        const uint32_t list = static_cast<uint32_t>(item / rq.blocks), block = static_cast<uint32_t>(item - static_cast<uint64_t>(list) * rq.blocks);
-        const Span sp = span_of<FOUND, kRows>(P, rq, block);
-        const int32_t t_lo = static_cast<int32_t>(min(static_cast<uint64_t>(u0) * kRowsUnit, static_cast<uint64_t>(sp.total)));
-        const int32_t t_hi = static_cast<int32_t>(min(static_cast<uint64_t>(u1) * kRowsUnit, static_cast<uint64_t>(sp.total)));
+        Span sp;
+        const Piece pc = piece_of<FOUND, kRows, kRowsUnit>(P, rq, before, x, x1, &sp);
+        if (pc.none) {
+            x = x1;
+            continue;
+        }
+        const uint32_t list = pc.list, block = pc.block;
+        const int32_t t_lo = static_cast<int32_t>(pc.t_lo), t_hi = static_cast<int32_t>(pc.t_hi);
         const int32_t row0 = static_cast<int32_t>(block * kRows);
 
         // this lane's row: its query, and where its token stands
@@ -300,12 +301,12 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                 f[i] = __builtin_amdgcn_exp2f(wave_m[i][orow] - base);
                 sum += f[i] * wave_l[i][orow];
             }
-            const bool whole = u0 == 0 && u1 == rq.units;
+            const bool whole = pc.begins && pc.ends;
             const int32_t orow_all = row0 + static_cast<int32_t>(orow);
             const int32_t otoken = P.group.div(orow_all);
             const int64_t ohead = static_cast<int64_t>(list) * P.group.d + (orow_all - otoken * static_cast<int32_t>(P.group.d));
             const int64_t qrow = rq.q0 + static_cast<int64_t>(otoken);
-            const uint32_t slot = 2 * w + (u0 == 0 ? 1 : 0);
+            const uint32_t slot = 2 * w + (pc.begins ? 1 : 0);
             if (orow_all < rq.rows) {
                 const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
 #pragma unroll
@@ -330,14 +331,14 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                         P.lse[qrow * P.heads + ohead] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
                 }
             }
-            if (P.join && tid == 0 && u0 == 0 && u1 < rq.units) {
-                const uint64_t last = (x + rq.units - 1) / start.share;  // the workgroup that holds its last unit
+            if (P.join && tid == 0 && pc.begins && !pc.ends) {
+                const uint64_t last = (pc.end - 1) / start.share;  // the workgroup that holds its end
                 P.joins[w] = Join{static_cast<uint32_t>(last - w + 1), static_cast<uint32_t>(row0), static_cast<uint32_t>(rq.rows),
                                   static_cast<uint32_t>(rq.q0), list};
             }
         }
         __syncthreads();
-        x += u1 - u0;
+        x = min(pc.end, x1);
     }
 }
 
@@ -417,6 +418,7 @@ int launch(AttendParams &P, uint64_t most_units, uint64_t item_units, hipStream_
     const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(most_units, kWorkgroups));
     // an item of one unit lies with one workgroup
     P.join = item_units > 1;
+    P.least = kRowsUnit * P.group.d;
     hipLaunchKernelGGL((fg_rows_kernel<T, D, FOUND>), dim3(grid), dim3(256), 0, st, P);
     if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, kRows>), dim3(grid, kRows), dim3(256), 0, st, P);
     FG_HIP(hipGetLastError(), "attention launch");

@@ -2,10 +2,12 @@
 //
 // The work is a list of items.  An item is a block of query rows (rows of one
 // request that read the same keys and values: the query heads of a group, for
-// each new token) against its request's visible tokens; these are counted in
-// units, and the units of all items, laid end to end, are dealt out evenly:
-// workgroup w takes units [w * share, (w + 1) * share).  A ragged batch and one
-// long context fill the device the same way, and the host needs no lengths.
+// each new token) against its request's visible tokens.  Each item has a weight
+// near its cost, the weights of all items are laid end to end, and that length
+// is dealt out evenly: workgroup w takes [w * share, (w + 1) * share) of it, and
+// of an item that a cut goes through the tokens in proportion.  A ragged batch, a
+// causal triangle and one long context fill the device the same way, and the
+// host needs no lengths.
 // A workgroup writes the rows of an item that it holds whole; of one that it
 // holds in part it leaves the sum, the maximum and the weighted values in the
 // workspace, and the join kernel adds the parts in their order, so the result
@@ -38,6 +40,7 @@ struct AttendParams {
     uint32_t list_heads; // lists a key/value head
     uint32_t nids, window, sinks;  // window 0xFFFFFFFF: none
     uint32_t join;       // whether the join kernel follows
+    uint64_t least;      // weight that a workgroup takes at least
     FastDiv group;       // query heads that share a list
     float scale2;        // scale * log2(e)
 };
@@ -52,8 +55,17 @@ struct Request {
     int32_t q0, rows;     // first row of q, query rows of a list (new tokens * group)
     int32_t kv, limit;    // tokens of the request, and of those how many the table can name
     int32_t fresh;        // new tokens
-    uint32_t blocks, units;  // row blocks, units of each (enough for the longest)
+    uint32_t blocks;      // of rows
+    // Weight of the first b blocks of a list: b * base + b (b + 1) / 2 * step, in
+    // (token, query head of the group) pairs.  Without a window the tokens that
+    // block b sees grow by a block's tokens from block to block.
+    uint64_t base, step;
+    __device__ __forceinline__ uint64_t weight_of(uint64_t b) const { return b * base + b * (b + 1) / 2 * step; }
 };
+
+// An item's own cost beside its tokens: its prologue and its rows' output, in
+// tokens.  Not zero: an item without tokens still writes its rows.
+constexpr uint32_t kItemTokens = 32;
 
 // The tokens that the rows row0 .. of a block see between them: 0 .. first - 1, then
 // from `from` on, then the ids.  Token number t of them is at position_of(t).
@@ -82,7 +94,7 @@ __device__ __forceinline__ float add_other32(float x) {
 
 __device__ __forceinline__ int32_t clampi(int32_t v, int32_t lo, int32_t hi) { return min(max(v, lo), hi); }
 
-template <bool FOUND, uint32_t ROWS, uint32_t UNIT>
+template <bool FOUND, uint32_t ROWS>
 __device__ __forceinline__ Request request_of(const AttendParams &P, uint32_t r) {
     Request q;
     const int32_t T = static_cast<int32_t>(P.tokens);
@@ -98,12 +110,15 @@ __device__ __forceinline__ Request request_of(const AttendParams &P, uint32_t r)
     q.limit = static_cast<int32_t>(min(static_cast<uint64_t>(q.kv), room));
     q.rows = q.fresh * static_cast<int32_t>(P.group.d);
     q.blocks = (static_cast<uint32_t>(q.rows) + ROWS - 1) / ROWS;
-    // a block's window spans that many tokens more than one row's
-    uint64_t seen = q.limit;
-    if (P.window != 0xFFFFFFFFu)
-        seen = min(seen, static_cast<uint64_t>(P.sinks) + P.window + (ROWS - 1) / P.group.d + 1);
-    if constexpr (FOUND) seen += P.nids;
-    q.units = max(1u, static_cast<uint32_t>((seen + UNIT - 1) / UNIT));
+    q.base = static_cast<uint64_t>(kItemTokens + max(q.kv - q.fresh, 0)) * P.group.d;
+    q.step = ROWS;
+    if (FOUND || P.window != 0xFFFFFFFFu) {
+        // every block sees about as much (the first ones of a context less)
+        uint64_t seen = min(static_cast<uint64_t>(q.limit), static_cast<uint64_t>(P.sinks) + P.window + ROWS / P.group.d);
+        if constexpr (FOUND) seen += P.nids;
+        q.base = (kItemTokens + seen) * P.group.d;
+        q.step = 0;
+    }
     return q;
 }
 
@@ -136,27 +151,29 @@ __device__ __forceinline__ int2 place_of(const AttendParams &P, uint32_t r, int3
 
 // Where a workgroup's share begins.
 struct Start {
-    uint64_t units, share;  // of all items; of a workgroup
-    uint64_t before;        // units of the requests before `request`
+    uint64_t all, share;  // weight of all items; of a workgroup
+    uint64_t before;      // weight of the requests before `request`
     uint32_t request;
 };
 
-// Called by all 256 threads; every workgroup sums the requests' units itself.
-template <bool FOUND, uint32_t ROWS, uint32_t UNIT>
-__device__ Start find_start(const AttendParams &P, uint32_t w, uint32_t workgroups, uint64_t least) {
-    __shared__ uint64_t wave_sum[4];
+// Called by all THREADS threads; every workgroup sums the requests' weights itself.
+template <bool FOUND, uint32_t ROWS, uint32_t THREADS>
+__device__ Start find_start(const AttendParams &P, uint32_t w, uint32_t workgroups) {
+    constexpr uint32_t WAVES = THREADS / 64;
+    __shared__ uint64_t wave_sum[WAVES];
     __shared__ uint64_t found_before;
     __shared__ uint32_t found_request;
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const bool once = P.requests <= THREADS;  // one look at the requests gives the sum and the place
     Start s{0, 0, 0, 0};
-    for (int pass = 0; pass < 2; ++pass) {
+    for (int pass = once ? 1 : 0; pass < 2; ++pass) {
         uint64_t sum = 0;
-        for (uint32_t r0 = 0; r0 < P.requests; r0 += 256) {
+        for (uint32_t r0 = 0; r0 < P.requests; r0 += THREADS) {
             const uint32_t r = r0 + tid;
             uint64_t u = 0;
             if (r < P.requests) {
-                const Request q = request_of<FOUND, ROWS, UNIT>(P, r);
-                u = static_cast<uint64_t>(q.blocks) * q.units * P.lists;
+                const Request q = request_of<FOUND, ROWS>(P, r);
+                u = q.weight_of(q.blocks) * P.lists;
             }
             uint64_t v = u;
 #pragma unroll
@@ -168,35 +185,73 @@ __device__ Start find_start(const AttendParams &P, uint32_t w, uint32_t workgrou
             __syncthreads();
             uint64_t base = sum;
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
+            for (uint32_t i = 0; i < WAVES; ++i) {
                 if (i < wave) base += wave_sum[i];
                 sum += wave_sum[i];
             }
-            // one chunk of requests: the totals of the first pass serve the second
-            if (pass == 1 || P.requests <= 256) {
-                if (P.requests <= 256) {
-                    s.units = sum;
-                    s.share = max((sum + workgroups - 1) / workgroups, least);
-                }
-                const uint64_t x = w * s.share;
-                if (u && base + v - u <= x && x < base + v) {
-                    found_before = base + v - u;
-                    found_request = r;
-                }
+            if (once) {
+                s.all = sum;
+                s.share = max((sum + workgroups - 1) / workgroups, P.least);
+            }
+            const uint64_t x = w * s.share;
+            if (pass == 1 && u && base + v - u <= x && x < base + v) {
+                found_before = base + v - u;
+                found_request = r;
             }
             __syncthreads();
         }
-        if (P.requests <= 256) break;
         if (pass == 0) {
-            s.units = sum;
-            s.share = max((sum + workgroups - 1) / workgroups, least);
+            s.all = sum;
+            s.share = max((sum + workgroups - 1) / workgroups, P.least);
         }
     }
-    if (w * s.share < s.units) {
+    if (w * s.share < s.all) {
         s.before = found_before;
         s.request = found_request;
     }
     return s;
+}
+
+// What of an item a workgroup holds.
+struct Piece {
+    uint32_t list, block;
+    uint32_t t_lo, t_hi;      // token numbers of its span, cut between units of UNIT tokens
+    uint64_t end;             // where the item's weight ends
+    bool begins, ends;        // whether the item's first (last) unit is here
+    bool none;                // no unit is, and none came before: another workgroup begins the item
+};
+
+// The item that x lies in (x is inside request q, whose weight begins at
+// `before`), and its tokens up to x1.  Two neighbours work out the cut between
+// them from the same numbers.
+template <bool FOUND, uint32_t ROWS, uint32_t UNIT>
+__device__ __forceinline__ Piece piece_of(const AttendParams &P, const Request &q, uint64_t before, uint64_t x, uint64_t x1,
+                                          Span *span) {
+    Piece p;
+    const uint64_t list_weight = q.weight_of(q.blocks);
+    p.list = static_cast<uint32_t>((x - before) / list_weight);
+    const uint64_t start = before + p.list * list_weight, at = x - start;
+    uint32_t lo = 0, hi = q.blocks;  // the last block that begins at or before `at`
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (q.weight_of(mid) <= at) lo = mid;
+        else hi = mid;
+    }
+    p.block = lo;
+    const uint64_t begin = start + q.weight_of(lo), weight = q.weight_of(lo + 1) - q.weight_of(lo);
+    p.end = begin + weight;
+    *span = span_of<FOUND, ROWS>(P, q, lo);
+    const uint32_t total = span->total, units = max((total + UNIT - 1) / UNIT, 1u);
+    // x, and x1 inside the item, fall into units 0 .. units - 1: the workgroup that holds the
+    // item's end holds its last unit, and an item of one unit is never cut
+    const uint32_t u0 = static_cast<uint32_t>((x - begin) * units / weight);
+    const uint32_t u1 = x1 >= p.end ? units : static_cast<uint32_t>((x1 - begin) * units / weight);
+    p.begins = u0 == 0;
+    p.ends = u1 == units;
+    p.none = u1 == 0;
+    p.t_lo = min(u0 * UNIT, total);
+    p.t_hi = min(u1 * UNIT, total);
+    return p;
 }
 
 }  // namespace fgk
