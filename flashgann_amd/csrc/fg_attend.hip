@@ -14,78 +14,14 @@
 namespace fgk {
 namespace {
 
-typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-typedef __attribute__((ext_vector_type(4))) float f32x4;
-typedef __attribute__((ext_vector_type(4))) short s16x4;
-typedef __attribute__((ext_vector_type(8))) short s16x8;
-
-struct BF16 {
-    using vec = bf16x8;
-    static constexpr uint32_t kExponent = 0x7F80, kMantissa = 0x007F, kOne = 0x3F80;
-    static __device__ __forceinline__ f32x4 mfma16(vec a, vec b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
-        return __builtin_bit_cast(uint32_t, v);
-    }
-};
-struct F16 {
-    using vec = f16x8;
-    static constexpr uint32_t kExponent = 0x7C00, kMantissa = 0x03FF, kOne = 0x3C00;
-    static __device__ __forceinline__ f32x4 mfma16(vec a, vec b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
-        return __builtin_bit_cast(uint32_t, v);
-    }
-};
-
-// Four rows of one column each: lane i of 16 gets column i of the 4 x 16 block
-// whose row i / 4, columns 4 (i % 4) .. + 3 lie at lane i's address.
-__device__ __forceinline__ s16x4 read_transposed(const char *lds) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds));
-}
-
-template <class T>
-__device__ __forceinline__ bool any_special(uint4 w) {
-    bool s = false;
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        s |= (x[i] & T::kExponent) == T::kExponent || ((x[i] >> 16) & T::kExponent) == T::kExponent;
-    return s;
-}
-
-// a with its infinities and NaNs as zeros; ones in `pos` for +inf and NaN, in
-// `neg` for -inf and NaN.
-template <class T>
-__device__ __forceinline__ s16x8 split_special(s16x8 a, s16x8 *pos, s16x8 *neg) {
-    s16x8 fine;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t x = static_cast<uint16_t>(a[i]);
-        const bool special = (x & T::kExponent) == T::kExponent, nan = special && (x & T::kMantissa);
-        fine[i] = special ? 0 : a[i];
-        (*pos)[i] = nan || (special && !(x & 0x8000)) ? static_cast<short>(T::kOne) : 0;
-        (*neg)[i] = nan || (special && (x & 0x8000)) ? static_cast<short>(T::kOne) : 0;
-    }
-    return fine;
-}
-
 // ---------------------------------------------------------------- few rows
 //
 // Blocks of 16 query rows; each of the four waves takes every fourth tile of 32
 // tokens and keeps a softmax of its own, joined through LDS at the end.  Bound
 // by the cache's bytes: a tile is 32 x D keys and values against 16 rows.
-constexpr uint32_t kRows = 16;
 constexpr uint32_t kRowsUnit = 128;    // tokens a unit: one tile of each wave
 constexpr uint32_t kPlaces = 1024;     // token places resolved at a time
-constexpr uint32_t kWorkgroups = 512;  // at most: two a CU, two parts of the workspace each
+constexpr uint32_t kFewRows = 32;      // query rows of a list up to which this kernel serves
 
 template <class T, int D, bool FOUND>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendParams P) {
@@ -200,16 +136,28 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                 }
                 const uint32_t held0 = static_cast<uint32_t>(__ballot(held[0])) & 0xFFFFu;
                 const uint32_t held1 = static_cast<uint32_t>(__ballot(held[1])) & 0xFFFFu;
-                bool special = false;
+                uint32_t odd = 0;
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < 2; ++b) {
+                    bool special = false;
 #pragma unroll
                     for (int k = 0; k < STEPS; ++k) {
-                        // what no row may see can hold anything: 0 * inf would be NaN
-                        const uint4 v = held[b] ? vr[b][k] : uint4{0, 0, 0, 0};
-                        if (ragged) special |= any_special<T>(v);
+                        // (a token without a page: whatever was read instead)
+                        uint4 v = held[b] ? vr[b][k] : uint4{0, 0, 0, 0};
+                        if (ragged && any_special<T>(v)) {
+                            // 0 * inf is NaN: where not every row sees a token, infinities and NaNs
+                            // are taken out of the product and added to the rows that see them
+                            special = true;
+                            v = finite_part<T>(v);
+                        }
                         *reinterpret_cast<uint4 *>(vmine + (16 * b + col) * VROW + 64 * k + 16 * quarter) = v;
                     }
+                    if (ragged) {
+                        uint64_t any = __ballot(special);
+                        any |= any >> 32;
+                        odd |= static_cast<uint32_t>((any | any >> 16) & 0xFFFF) << (16 * b);
+                    }
+                }
                 if ((tile + 4) * 32 < n) load(tile + 4);
 
                 float p[8];
@@ -220,8 +168,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int32_t j = position_of(sp, c0 + tile * 32 + 16 * (i / 4) + 4 * static_cast<int32_t>(quarter) + i % 4);
-                        const int32_t back = pos - j;
-                        if (back < 0 || (static_cast<uint32_t>(back) >= P.window && static_cast<uint32_t>(j) >= P.sinks)) see &= ~(1u << i);
+                        see &= ~(static_cast<uint32_t>(!sees(P, pos, j)) << i);
                     }
                 }
                 float top = -INFINITY;
@@ -249,31 +196,25 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                 uint4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
                 const vec pv = __builtin_bit_cast(vec, pk);
                 const char *vt = vmine + (4 * quarter + col / 4) * VROW + (col % 4) * 8;
-                if (!__any(special)) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i) {
+                    const s16x4 a0 = read_transposed(vt + 32 * i), a1 = read_transposed(vt + 16 * VROW + 32 * i);
+                    const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[i] = T::mfma16(__builtin_bit_cast(vec, a), pv, o[i]);
+                }
+                for (; odd; odd &= odd - 1) {
+                    const int32_t at = tile * 32 + __ffs(odd) - 1;
+                    const int2 where = place[at];
+                    const char *src = vbase + where.x * P.cache.v_page + where.y * P.cache.v_token - quarter * 8;
+                    const bool shown = sees(P, pos, position_of(sp, c0 + at));
 #pragma unroll
                     for (int i = 0; i < DB; ++i) {
-                        const s16x4 a0 = read_transposed(vt + 32 * i), a1 = read_transposed(vt + 16 * VROW + 32 * i);
-                        const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-                        o[i] = T::mfma16(__builtin_bit_cast(vec, a), pv, o[i]);
-                    }
-                } else {
-                    // infinities and NaNs reach the rows that see them and no others
-                    s16x8 ones;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) ones[i] = (see >> i) & 1u ? static_cast<short>(T::kOne) : 0;
-                    const vec seen = __builtin_bit_cast(vec, ones);
-#pragma unroll
-                    for (int i = 0; i < DB; ++i) {
-                        const s16x4 a0 = read_transposed(vt + 32 * i), a1 = read_transposed(vt + 16 * VROW + 32 * i);
-                        s16x8 pos_a, neg_a;
-                        const s16x8 a = split_special<T>(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), &pos_a, &neg_a);
-                        o[i] = T::mfma16(__builtin_bit_cast(vec, a), pv, o[i]);
-                        const f32x4 up = T::mfma16(__builtin_bit_cast(vec, pos_a), seen, f32x4{0, 0, 0, 0});
-                        const f32x4 down = T::mfma16(__builtin_bit_cast(vec, neg_a), seen, f32x4{0, 0, 0, 0});
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if (up[k] > 0.0f) o[i][k] += INFINITY;
-                            if (down[k] > 0.0f) o[i][k] -= INFINITY;
+                        const uint2 v = *reinterpret_cast<const uint2 *>(src + 32 * i);
+                        if (shown) {
+                            o[i][0] += special_part<T>(v.x & 0xFFFF);
+                            o[i][1] += special_part<T>(v.x >> 16);
+                            o[i][2] += special_part<T>(v.y & 0xFFFF);
+                            o[i][3] += special_part<T>(v.y >> 16);
                         }
                     }
                 }
@@ -328,7 +269,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                     if (!whole)
                         P.part_ml[slot * kRows + orow] = float2{top, sum};
                     else if (P.lse)
-                        P.lse[qrow * P.heads + ohead] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+                        P.lse[qrow * P.heads + ohead] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
                 }
             }
             if (P.join && tid == 0 && pc.begins && !pc.ends) {
@@ -342,62 +283,6 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
     }
 }
 
-// The parts of an item into its rows: workgroup (w, row) of the item that
-// workgroup w of the attention kernel began and did not end.  Its parts are the
-// second of w and the first of w + 1, w + 2, ...
-template <class T, int D, uint32_t ROWS>
-__global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
-    constexpr uint32_t QUADS = D / 4, SETS = 256 / QUADS;  // threads across a row, sets of parts side by side
-    __shared__ float sum_m[4];
-    __shared__ float acc[SETS][D], acc_l[SETS];
-    const uint32_t w = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
-    const Join j = P.joins[w];
-    if (j.pieces == 0 || j.row0 + row >= j.rows) return;
-    const auto slot_of = [&](uint32_t i) { return i == 0 ? 2 * w + 1 : 2 * (w + i); };
-
-    float top = -INFINITY;
-    for (uint32_t i = tid; i < j.pieces; i += 256) top = fmaxf(top, P.part_ml[slot_of(i) * ROWS + row].x);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (tid % 64 == 0) sum_m[tid / 64] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(sum_m[0], sum_m[1]), fmaxf(sum_m[2], sum_m[3]));
-    const float base = top == -INFINITY ? 0.0f : top;
-
-    const uint32_t set = tid / QUADS, quad = tid % QUADS;
-    if (set < SETS) {
-        f32x4 a = {0, 0, 0, 0};
-        float l = 0.0f;
-#pragma unroll 4
-        for (uint32_t i = set; i < j.pieces; i += SETS) {
-            const uint32_t at = slot_of(i) * ROWS + row;
-            const float2 ml = P.part_ml[at];
-            const float f = __builtin_amdgcn_exp2f(ml.x - base);
-            a += f * *reinterpret_cast<const f32x4 *>(P.part + static_cast<uint64_t>(at) * D + 4 * quad);
-            l = fmaf(f, ml.y, l);
-        }
-        *reinterpret_cast<f32x4 *>(&acc[set][4 * quad]) = a;
-        if (quad == 0) acc_l[set] = l;
-    }
-    __syncthreads();
-    const uint32_t all = j.row0 + row, token = P.group.div(all), head = j.list * P.group.d + (all - token * P.group.d);
-    const int64_t qrow = static_cast<int64_t>(j.q0) + token;
-    float l = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < SETS; ++i) l += acc_l[i];
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (tid < D / 2) {
-        float a = 0.0f, b = 0.0f;
-#pragma unroll
-        for (uint32_t i = 0; i < SETS; ++i) {
-            a += acc[i][2 * tid];
-            b += acc[i][2 * tid + 1];
-        }
-        *reinterpret_cast<uint32_t *>(P.out + qrow * P.out_token + head * P.out_head + 4 * tid) = T::pack(a * inv, b * inv);
-    }
-    if (tid == 0 && P.lse) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
-}
-
 // ---------------------------------------------------------------- host side
 
 struct Workspace {
@@ -407,8 +292,9 @@ struct Workspace {
 Workspace workspace_of(uint32_t dim) {
     Workspace s;
     s.part = 0;
-    s.ml = s.part + 2ull * kWorkgroups * kRows * dim * 4;
-    s.joins = s.ml + 2ull * kWorkgroups * kRows * 8;
+    const uint64_t rows = 2ull * std::max(kWorkgroups * kRows, kTileRows);  // two parts a workgroup
+    s.ml = s.part + rows * dim * 4;
+    s.joins = s.ml + rows * 8;
     s.total = s.joins + kWorkgroups * sizeof(Join);
     return s;
 }
@@ -502,6 +388,8 @@ int attend(const fg_kv_cache *c, const fg_attention *a, void *stream) {
     const uint64_t blocks = (static_cast<uint64_t>(a->tokens) * P.group.d + kRows - 1) / kRows + a->requests;
     const uint64_t most_units = std::min<uint64_t>(blocks * P.lists, 1u << 20) * std::min<uint64_t>(item_units, 1u << 20);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    // many rows a list: blocks of them share their keys through LDS
+    if (!FOUND && static_cast<uint64_t>(a->max_q) * P.group.d > kFewRows) return launch_tiles(P, c->dtype, c->dim, st);
     return c->dtype == FG_BF16 ? launch<BF16, FOUND>(P, c->dim, most_units, item_units, st)
                                : launch<F16, FOUND>(P, c->dim, most_units, item_units, st);
 }

@@ -23,6 +23,78 @@
 
 namespace fgk {
 
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+struct BF16 {
+    using vec = bf16x8;
+    static constexpr uint32_t kExponent = 0x7F80, kMantissa = 0x007F;
+    static __device__ __forceinline__ f32x4 mfma16(vec a, vec b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(vec a, vec b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+};
+struct F16 {
+    using vec = f16x8;
+    static constexpr uint32_t kExponent = 0x7C00, kMantissa = 0x03FF;
+    static __device__ __forceinline__ f32x4 mfma16(vec a, vec b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(vec a, vec b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+};
+
+// Four rows of one column each: lane i of 16 gets column i of the 4 x 16 block
+// whose row i / 4, columns 4 (i % 4) .. + 3 lie at lane i's address.
+__device__ __forceinline__ s16x4 read_transposed(const char *lds) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds));
+}
+
+template <class T>
+__device__ __forceinline__ bool any_special(uint4 w) {
+    bool s = false;
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        s |= (x[i] & T::kExponent) == T::kExponent || ((x[i] >> 16) & T::kExponent) == T::kExponent;
+    return s;
+}
+
+// The same with its infinities and NaNs as zeros.
+template <class T>
+__device__ __forceinline__ uint4 finite_part(uint4 w) {
+    const auto part = [](uint32_t x) {
+        if ((x & T::kExponent) == T::kExponent) x &= 0xFFFF0000u;
+        if (((x >> 16) & T::kExponent) == T::kExponent) x &= 0x0000FFFFu;
+        return x;
+    };
+    return {part(w.x), part(w.y), part(w.z), part(w.w)};
+}
+
+// An infinity or NaN among a value's 16 bits as a float, 0 for any other.
+template <class T>
+__device__ __forceinline__ float special_part(uint32_t x) {
+    if ((x & T::kExponent) != T::kExponent) return 0.0f;
+    return x & T::kMantissa ? NAN : x & 0x8000 ? -INFINITY : INFINITY;
+}
+
 struct AttendParams {
     CacheView cache;
     const char *q;
@@ -149,6 +221,12 @@ __device__ __forceinline__ int2 place_of(const AttendParams &P, uint32_t r, int3
     return {static_cast<uint32_t>(page) < P.cache.pages ? page : -1, static_cast<int32_t>(j - b * P.cache.page_size.d)};
 }
 
+// Whether the row at `pos` sees the token at position j (pages aside).
+__device__ __forceinline__ bool sees(const AttendParams &P, int32_t pos, int32_t j) {
+    const int32_t back = pos - j;
+    return (back >= 0) & ((static_cast<uint32_t>(back) < P.window) | (static_cast<uint32_t>(j) < P.sinks));
+}
+
 // Where a workgroup's share begins.
 struct Start {
     uint64_t all, share;  // weight of all items; of a workgroup
@@ -253,6 +331,73 @@ __device__ __forceinline__ Piece piece_of(const AttendParams &P, const Request &
     p.t_hi = min(u1 * UNIT, total);
     return p;
 }
+
+constexpr uint32_t kRows = 16;         // query rows of a block of the few-rows kernel
+constexpr uint32_t kWorkgroups = 512;  // at most: two a CU
+constexpr float kLn2 = 0.69314718055994531f;
+
+// The parts of an item into its rows: workgroup (w, row) of the item that
+// workgroup w of the attention kernel began and did not end.  Its parts are the
+// second of w and the first of w + 1, w + 2, ...
+template <class T, int D, uint32_t ROWS>
+__global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
+    constexpr uint32_t QUADS = D / 4, SETS = 256 / QUADS;  // threads across a row, sets of parts side by side
+    __shared__ float sum_m[4];
+    __shared__ float acc[SETS][D], acc_l[SETS];
+    const uint32_t w = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+    const Join j = P.joins[w];
+    if (j.pieces == 0 || j.row0 + row >= j.rows) return;
+    const auto slot_of = [&](uint32_t i) { return i == 0 ? 2 * w + 1 : 2 * (w + i); };
+
+    float top = -INFINITY;
+    for (uint32_t i = tid; i < j.pieces; i += 256) top = fmaxf(top, P.part_ml[slot_of(i) * ROWS + row].x);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (tid % 64 == 0) sum_m[tid / 64] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sum_m[0], sum_m[1]), fmaxf(sum_m[2], sum_m[3]));
+    const float base = top == -INFINITY ? 0.0f : top;
+
+    const uint32_t set = tid / QUADS, quad = tid % QUADS;
+    if (set < SETS) {
+        f32x4 a = {0, 0, 0, 0};
+        float l = 0.0f;
+#pragma unroll 4
+        for (uint32_t i = set; i < j.pieces; i += SETS) {
+            const uint32_t at = slot_of(i) * ROWS + row;
+            const float2 ml = P.part_ml[at];
+            const float f = __builtin_amdgcn_exp2f(ml.x - base);
+            a += f * *reinterpret_cast<const f32x4 *>(P.part + static_cast<uint64_t>(at) * D + 4 * quad);
+            l = fmaf(f, ml.y, l);
+        }
+        *reinterpret_cast<f32x4 *>(&acc[set][4 * quad]) = a;
+        if (quad == 0) acc_l[set] = l;
+    }
+    __syncthreads();
+    const uint32_t all = j.row0 + row, token = P.group.div(all), head = j.list * P.group.d + (all - token * P.group.d);
+    const int64_t qrow = static_cast<int64_t>(j.q0) + token;
+    float l = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < SETS; ++i) l += acc_l[i];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (tid < D / 2) {
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < SETS; ++i) {
+            a += acc[i][2 * tid];
+            b += acc[i][2 * tid + 1];
+        }
+        *reinterpret_cast<uint32_t *>(P.out + qrow * P.out_token + head * P.out_head + 4 * tid) = T::pack(a * inv, b * inv);
+    }
+    if (tid == 0 && P.lse) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Rows of the tile kernel's blocks together over all workgroups: two parts of
+// the workspace each.
+constexpr uint32_t kTileRows = 256 * 256;
+
+// Blocks of many rows (fg_attend_tiles.hip): launches on `stream`.
+int launch_tiles(AttendParams &P, int dtype, uint32_t dim, hipStream_t stream);
 
 }  // namespace fgk
 

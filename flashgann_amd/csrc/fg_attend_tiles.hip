@@ -1,0 +1,333 @@
+// fg_attend_tiles.hip -- attention over the paged cache for blocks of many query
+// rows (chunks of prompts): bound by the matrix unit and the softmax beside it.
+//
+// A wave holds 32 query rows, one in each lane's column; the workgroup's waves
+// share tiles of 64 tokens, two of them in LDS, the next one's keys and values on
+// their way through registers.  Per tile a wave does 2 x D/16 products of 32 keys x
+// 16 dimensions for the scores and 4 x D/32 of 32 dimensions x 16 keys for the
+// output; rows of the same wave reuse what it reads from LDS.
+#include "fg_attend.hpp"
+
+namespace fgk {
+namespace {
+
+constexpr uint32_t kTile = 64;         // tokens
+constexpr uint32_t kTilesUnit = 256;   // tokens between cuts
+
+// The barrier that publishes LDS and nothing else: loads in flight from global
+// memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <class T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams P) {
+    using vec = typename T::vec;
+    constexpr uint32_t THREADS = 64 * NW, ROWS = 32 * NW;
+    constexpr int STEPS = D / 16, DB = D / 32, CHUNKS = D / 8;   // 16-byte pieces of a row
+    constexpr uint32_t PER = (kTile * CHUNKS + THREADS - 1) / THREADS;
+    // LDS rows are longer than the data: eight rows' 16-byte pieces of K, and eight
+    // rows' 64-byte pieces of V, then meet every bank equally often
+    constexpr uint32_t KROW = 2 * D + 16, VROW = 2 * D + (D == 96 ? 128 : 64);
+    __shared__ __attribute__((aligned(16))) char kbuf[2][kTile * KROW];
+    __shared__ __attribute__((aligned(16))) char vbuf[2][kTile * VROW];
+    // of tile i at i % 4: where its tokens lie (bytes from the head's first key and
+    // value), which of them there are, and in a tile that not every row sees which
+    // hold an infinite or NaN value: 0 * inf is NaN, so those are taken out of the
+    // product and added to the rows that see them
+    __shared__ longlong2 place[4][kTile];
+    __shared__ uint64_t held[4];
+    __shared__ unsigned long long special[4];
+
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, col = lane % 32, half = lane / 32;
+    const uint32_t W = gridDim.x;
+    // neighbours in weight, which read the same keys, on one die of eight (the
+    // grid is a multiple of 8)
+    const uint32_t w = blockIdx.x % 8 * (W / 8) + blockIdx.x / 8;
+    const Start start = find_start<false, ROWS, THREADS>(P, w, W);
+    if (tid == 0) P.joins[w].pieces = 0;
+    const uint64_t x1 = min((w + 1) * start.share, start.all);
+    uint64_t before = start.before;
+    uint32_t r = start.request;
+
+    for (uint64_t x = w * start.share; x < x1;) {
+        const Request rq = request_of<false, ROWS>(P, r);
+        const uint64_t all = rq.weight_of(rq.blocks) * P.lists;
+        if (x >= before + all) {
+            before += all;
+            ++r;
+            continue;
+        }
+        Span sp;
+        const Piece pc = piece_of<false, ROWS, kTilesUnit>(P, rq, before, x, x1, &sp);
+        if (pc.none) {
+            x = x1;
+            continue;
+        }
+        const int32_t t_lo = static_cast<int32_t>(pc.t_lo), t_hi = static_cast<int32_t>(pc.t_hi);
+        const int32_t tiles = (t_hi - t_lo + static_cast<int32_t>(kTile) - 1) / static_cast<int32_t>(kTile);
+
+        // this lane's row, and the positions that this wave's rows span
+        const int32_t row_first = static_cast<int32_t>(pc.block * ROWS + wave * 32);
+        const int32_t row = row_first + static_cast<int32_t>(col);
+        const int32_t token = P.group.div(row);
+        const int32_t pos = sp.pos0 + token;
+        const int32_t pos_lo = sp.pos0 + static_cast<int32_t>(P.group.div(row_first));
+        const int32_t pos_hi = sp.pos0 + static_cast<int32_t>(P.group.div(min(row_first + 31, max(rq.rows - 1, row_first))));
+        const int32_t block_lo = sp.pos0 + static_cast<int32_t>(P.group.div(pc.block * ROWS));
+        const int64_t head = static_cast<int64_t>(pc.list) * P.group.d + (row - token * static_cast<int32_t>(P.group.d));
+        const int64_t qrow = rq.q0 + static_cast<int64_t>(token);
+        vec qv[STEPS];
+        {
+            const char *src = P.q + qrow * P.q_token + head * P.q_head + half * 16;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                uint4 v = {0, 0, 0, 0};
+                if (row < rq.rows) v = *reinterpret_cast<const uint4 *>(src + 32 * s);
+                qv[s] = __builtin_bit_cast(vec, v);
+            }
+        }
+        const char *const kbase = P.cache.k + pc.list * P.cache.k_head;
+        const char *const vbase = P.cache.v + pc.list * P.cache.v_head;
+
+        // The places of tile i are looked up by wave i % NW: the table is read at
+        // tile i - 3 and the place written at tile i - 2, so nothing waits for it.
+        int32_t page = -1;
+        uint32_t offset = 0;
+        const auto look = [&](int32_t i) {
+            const int32_t t = t_lo + i * static_cast<int32_t>(kTile) + static_cast<int32_t>(lane);
+            page = -1;
+            if (t < t_hi) {
+                const int32_t j = position_of(sp, t);
+                const uint32_t b = P.cache.page_size.div(j);
+                offset = j - b * P.cache.page_size.d;
+                page = P.table[r * P.table_row + b];
+            }
+        };
+        const auto note = [&](int32_t i) {
+            const bool have = static_cast<uint32_t>(page) < P.cache.pages;
+            const int64_t p = have ? page : 0, o = have ? offset : 0;
+            place[i % 4][lane] = longlong2{p * P.cache.k_page + o * P.cache.k_token, p * P.cache.v_page + o * P.cache.v_token};
+            const uint64_t there = __ballot(have);
+            if (lane == 0) {
+                held[i % 4] = there;
+                special[i % 4] = 0;
+            }
+        };
+        // whether every row of the workgroup sees all tokens of tile i, pages aside
+        const auto whole_tile = [&](int32_t i, int32_t lo, int32_t hi) {
+            const int32_t t0 = t_lo + i * static_cast<int32_t>(kTile), t1 = min(t0 + static_cast<int32_t>(kTile), t_hi) - 1;
+            if (position_of(sp, t1) > lo) return false;
+            return P.window == 0xFFFFFFFFu || t1 < sp.first || hi - position_of(sp, t0) < static_cast<int64_t>(P.window);
+        };
+
+        uint4 kr[PER], vr[PER];
+        const auto load = [&](int32_t i) {
+#pragma unroll
+            for (uint32_t c = 0; c < PER; ++c) {
+                const uint32_t at = tid + c * THREADS, trow = at / CHUNKS, piece = at % CHUNKS;
+                if (kTile * CHUNKS % THREADS == 0 || at < kTile * CHUNKS) {
+                    const longlong2 o = place[i % 4][trow];
+                    kr[c] = *reinterpret_cast<const uint4 *>(kbase + o.x + piece * 16);
+                    vr[c] = *reinterpret_cast<const uint4 *>(vbase + o.y + piece * 16);
+                }
+            }
+        };
+        const int32_t block_hi = sp.pos0 + static_cast<int32_t>(P.group.div(min(pc.block * ROWS + ROWS, static_cast<uint32_t>(rq.rows)) - 1));
+        const auto store = [&](int32_t i) {
+            const uint64_t there = held[i % 4];
+            const bool edge = !whole_tile(i, block_lo, block_hi);
+#pragma unroll
+            for (uint32_t c = 0; c < PER; ++c) {
+                const uint32_t at = tid + c * THREADS, trow = at / CHUNKS, piece = at % CHUNKS;
+                if (kTile * CHUNKS % THREADS == 0 || at < kTile * CHUNKS) {
+                    uint4 v = vr[c];
+                    // (a token without a page: whatever was read instead)
+                    if (there != ~0ull && !((there >> trow) & 1)) v = uint4{0, 0, 0, 0};
+                    if (edge && any_special<T>(v)) {
+                        atomicOr(&special[i % 4], 1ull << trow);
+                        v = finite_part<T>(v);
+                    }
+                    *reinterpret_cast<uint4 *>(kbuf[i % 2] + trow * KROW + piece * 16) = kr[c];
+                    *reinterpret_cast<uint4 *>(vbuf[i % 2] + trow * VROW + piece * 16) = v;
+                }
+            }
+        };
+
+        float m = -INFINITY, l = 0.0f;  // m: of the scores before scaling
+        f32x16 o[DB];
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[i] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+
+        // (the last item's readers of LDS are past: see the barrier at the end)
+        if (tiles > 0) {
+            if (wave < 2) {
+                look(wave);
+                note(wave);
+            }
+            if (wave == 2 % NW) look(2);
+            lds_barrier();
+            load(0);
+            store(0);
+        }
+        for (int32_t i = 0; i < tiles; ++i) {
+            lds_barrier();
+            if (i + 1 < tiles) load(i + 1);
+            if (wave == static_cast<uint32_t>(i + 2) % NW) note(i + 2);
+            if (wave == static_cast<uint32_t>(i + 3) % NW) look(i + 3);
+
+            const int32_t t0 = t_lo + i * static_cast<int32_t>(kTile);
+            const uint64_t there = held[i % 4];
+            if (position_of(sp, t0) <= pos_hi && row_first < rq.rows) {
+                // scores: register i of s[b] is token 32 b + 8 (i / 4) + 4 half + i % 4
+                f32x16 s[2];
+                const char *kt = kbuf[i % 2] + col * KROW + half * 16;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    s[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        const uint4 a = *reinterpret_cast<const uint4 *>(kt + b * 32 * KROW + 32 * k);
+                        s[b] = T::mfma32(__builtin_bit_cast(vec, a), qv[k], s[b]);
+                    }
+                }
+                if (there != ~0ull || !whole_tile(i, pos_lo, pos_hi)) {
+                    uint32_t see = 0;  // bit 16 b + i: whether the row sees the token of s[b][i]
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        const int at = 32 * (k / 16) + 8 * (k % 16 / 4) + k % 4;
+                        see |= static_cast<uint32_t>(sees(P, pos, position_of(sp, t0 + at + 4 * static_cast<int32_t>(half)))) << k;
+                    }
+                    // the lane's tokens of each half of the tile, four of every eight
+                    const uint64_t mine = there >> (4 * half);
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        const uint32_t four = static_cast<uint32_t>(mine >> (8 * g)) & 15u;
+                        see &= (four << (4 * g)) | ~(15u << (4 * g));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) s[k / 16][k % 16] = (see >> k) & 1 ? s[k / 16][k % 16] : -INFINITY;
+                }
+                float top = s[0][0];
+#pragma unroll
+                for (int k = 1; k < 32; ++k) top = fmaxf(top, s[k / 16][k % 16]);
+                top = fmaxf(m, max_other32(top));
+                // the maximum follows when a row's grows by more than 2^8: weights stay
+                // below that, and the sums are no less exact for it
+                if (__any((top - m) * P.scale2 > 8.0f)) {
+                    const float from = m == -INFINITY ? top : m;
+                    const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((from - top) * P.scale2);
+                    l *= shrink;
+#pragma unroll
+                    for (int k = 0; k < DB; ++k) o[k] *= shrink;
+                    m = top;
+                }
+                const float base = m == -INFINITY ? 0.0f : -m * P.scale2;
+                vec pv[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float p[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        p[k] = __builtin_amdgcn_exp2f(fmaf(s[c / 2][8 * (c % 2) + k], P.scale2, base));
+                        l += p[k];
+                    }
+                    // weights in the values' type: the matrix unit takes both alike, and
+                    // the rounding of a weight is that of an output element
+                    const uint4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+                    pv[c] = __builtin_bit_cast(vec, pk);
+                }
+                const char *vt = vbuf[i % 2] + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const s16x4 a0 = read_transposed(vt + 16 * c * VROW + 64 * d), a1 = read_transposed(vt + (16 * c + 8) * VROW + 64 * d);
+                        const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[d] = T::mfma32(__builtin_bit_cast(vec, a), pv[c], o[d]);
+                    }
+                for (unsigned long long odd = special[i % 4]; odd; odd &= odd - 1) {
+                    const int at = __ffsll(odd) - 1;
+                    const char *src = vbase + place[i % 4][at].y + half * 8;
+                    const bool shown = sees(P, pos, position_of(sp, t0 + at));
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(src + 64 * d + 16 * k);
+                            if (shown) {
+                                o[d][4 * k] += special_part<T>(v.x & 0xFFFF);
+                                o[d][4 * k + 1] += special_part<T>(v.x >> 16);
+                                o[d][4 * k + 2] += special_part<T>(v.y & 0xFFFF);
+                                o[d][4 * k + 3] += special_part<T>(v.y >> 16);
+                            }
+                        }
+                }
+            }
+            if (i + 1 < tiles) store(i + 1);
+        }
+        lds_barrier();
+
+        l = add_other32(l);
+        const bool whole = pc.begins && pc.ends;
+        const float top = m == -INFINITY ? m : m * P.scale2;
+        if (row < rq.rows) {
+            if (whole) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                char *dst = P.out + qrow * P.out_token + head * P.out_head + half * 8;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<uint2 *>(dst + 64 * d + 16 * k) =
+                            uint2{T::pack(o[d][4 * k] * inv, o[d][4 * k + 1] * inv), T::pack(o[d][4 * k + 2] * inv, o[d][4 * k + 3] * inv)};
+                if (P.lse && half == 0) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
+            } else {
+                const uint32_t slot = 2 * w + (pc.begins ? 1 : 0);
+                const uint64_t at = static_cast<uint64_t>(slot) * ROWS + wave * 32 + col;
+                float *dst = P.part + at * D + half * 4;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<f32x4 *>(dst + 32 * d + 8 * k) = f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+                if (half == 0) P.part_ml[at] = float2{top, l};
+            }
+        }
+        if (tid == 0 && pc.begins && !pc.ends) {
+            const uint64_t last = (pc.end - 1) / start.share;  // the workgroup that holds its end
+            P.joins[w] = Join{static_cast<uint32_t>(last - w + 1), pc.block * ROWS, static_cast<uint32_t>(rq.rows), static_cast<uint32_t>(rq.q0), pc.list};
+        }
+        x = min(pc.end, x1);
+    }
+}
+
+template <class T, int D, int NW>
+int launch(AttendParams &P, hipStream_t st) {
+    constexpr uint32_t ROWS = 32 * NW, grid = 256;
+    P.least = static_cast<uint64_t>(kTilesUnit) * P.group.d;
+    hipLaunchKernelGGL((fg_tiles_kernel<T, D, NW>), dim3(grid), dim3(64 * NW), 0, st, P);
+    hipLaunchKernelGGL((fg_join_kernel<T, D, ROWS>), dim3(grid, ROWS), dim3(256), 0, st, P);
+    FG_HIP(hipGetLastError(), "attention launch");
+    return FG_OK;
+}
+
+template <class T>
+int launch(AttendParams &P, uint32_t dim, hipStream_t st) {
+    switch (dim) {
+    case 64: return launch<T, 64, 8>(P, st);
+    case 96: return launch<T, 96, 8>(P, st);
+    case 128: return launch<T, 128, 8>(P, st);
+    default: return launch<T, 256, 4>(P, st);
+    }
+}
+
+}  // namespace
+
+int launch_tiles(AttendParams &P, int dtype, uint32_t dim, hipStream_t stream) {
+    return dtype == FG_BF16 ? launch<BF16>(P, dim, stream) : launch<F16>(P, dim, stream);
+}
+
+}  // namespace fgk
