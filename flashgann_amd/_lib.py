@@ -94,10 +94,10 @@ def lib():
                                     vp, vp, vp, vp, vp, vp]
         # the structs arrive packed (flashgann_amd.attention)
         L.fg_cache_append.argtypes = [C.c_char_p, vp, vp, i64, i64, i64, i64, vp, C.c_uint32, vp]
-        L.fg_attend.argtypes = [C.c_char_p, C.c_char_p, vp]
+        L.fg_attend.argtypes = [C.c_char_p, C.c_char_p, vp, C.c_uint64, vp]
         L.fg_attend_retrieved.argtypes = L.fg_attend.argtypes
-        L.fg_attend_workspace_bytes.argtypes = [C.c_uint32]
-        L.fg_attend_workspace_bytes.restype = C.c_uint64
+        L.fg_attend_workspace_bytes.argtypes = [C.c_char_p, C.c_char_p]
+        L.fg_attend_workspace_bytes.restype = i64
         L.fg_last_error.restype = C.c_char_p
         L.fg_version.restype = C.c_char_p
         _lib = L

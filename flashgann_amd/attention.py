@@ -30,7 +30,11 @@ __all__ = ["CachePlan", "cache_plan", "cache_append", "attend", "attend_retrieve
 _DTYPES = {torch.bfloat16: FG_BF16, torch.float16: FG_F16}
 _IDS = (torch.int32, torch.uint32)
 _CACHE = struct.Struct("2Q6q4IiI")         # fg_kv_cache
-_ATTENTION = struct.Struct("3Q4qQq5Q5Ii3If")  # fg_attention
+_ATTENTION = struct.Struct("3Q4qQq3Q5Ii3If")  # fg_attention
+
+
+# the current stream's handle without a Stream object around it, a microsecond less a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
 
 
 class CachePlan(NamedTuple):
@@ -42,39 +46,39 @@ class CachePlan(NamedTuple):
     used: torch.Tensor       # (1,) int32
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
 def _stream(device: int) -> int:
-    _need(device >= 0 and device == torch.cuda.current_device(), "tensors must be on the current CUDA device")
-    return torch.cuda.current_stream(device).cuda_stream
+    if device < 0 or device != torch.cuda.current_device():
+        raise ValueError("tensors must be on the current CUDA device")
+    return _raw_stream(device)
 
 
-def _vector(t: torch.Tensor, n: int | None, dtype: torch.dtype, device: int, name: str) -> int:
-    _need(t.dtype == dtype and t.ndim == 1 and (n is None or t.shape[0] == n) and t.is_contiguous()
-          and t.get_device() == device,
-          f"{name} must be a contiguous {dtype} vector" + ("" if n is None else f" of {n}") + " on the same device")
+def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, device: int, name: str) -> int:
+    if t.shape != (n,) or t.dtype != dtype or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} on the same device")
     return t.data_ptr()
 
 
-def _cache(k: torch.Tensor, v: torch.Tensor, device: int) -> tuple[bytes, tuple]:
-    shape, ks, vs = k.shape, k.stride(), v.stride()
-    _need(len(shape) == 4 and v.shape == shape, "k_cache and v_cache must have shape (pages, page_size, heads_kv, dim)")
-    dtype = _DTYPES.get(k.dtype)
-    _need(dtype is not None and v.dtype == k.dtype, "k_cache and v_cache must be bfloat16 or float16")
-    _need(k.get_device() == device and v.get_device() == device, "k_cache and v_cache must be on the same device")
-    _need(ks[3] == 1 and vs[3] == 1, "the last dimension of k_cache and v_cache must be contiguous")
-    return _CACHE.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[0], shape[1],
-                       shape[2], shape[3], dtype, 0), shape
+def _cache(k: torch.Tensor, v: torch.Tensor, device: int) -> tuple[bytes, torch.Size]:
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 4 or v.shape != shape:
+        raise ValueError("k_cache and v_cache must have shape (pages, page_size, heads_kv, dim)")
+    if dtype not in _DTYPES or v.dtype != dtype:
+        raise ValueError("k_cache and v_cache must be bfloat16 or float16")
+    if k.get_device() != device or v.get_device() != device:
+        raise ValueError("k_cache and v_cache must be on the same device")
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3 = v.stride()
+    if k3 != 1 or v3 != 1:
+        raise ValueError("the last dimension of k_cache and v_cache must be contiguous")
+    return _CACHE.pack(k.data_ptr(), v.data_ptr(), k0, k1, k2, v0, v1, v2, *shape, _DTYPES[dtype], 0), shape
 
 
 def _table(t: torch.Tensor, requests: int, device: int) -> tuple[int, int, int]:
-    _need(t.dtype == torch.int32 and t.ndim == 2 and t.shape[0] == requests and t.get_device() == device
-          and (t.shape[1] <= 1 or t.stride(1) == 1) and t.stride(0) >= 0,
-          f"block_table must be int32 of shape ({requests}, width), its rows contiguous, on the same device")
-    return t.data_ptr(), t.stride(0), t.shape[1]
+    shape, stride = t.shape, t.stride()
+    if (t.dtype != torch.int32 or len(shape) != 2 or shape[0] != requests or t.get_device() != device
+            or (stride[1] != 1 and shape[1] > 1) or stride[0] < 0):
+        raise ValueError(f"block_table must be int32 of shape ({requests}, width), its rows contiguous, on the same device")
+    return t.data_ptr(), stride[0], shape[1]
 
 
 def cache_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, *,
@@ -88,21 +92,23 @@ def cache_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     every token to have an entry.  Entries past the last token hold slot -1.
     `used` is the number of pages taken: drop so many from free_pages."""
     device = lens.get_device()
-    requests = lens.shape[0]
     stream = _stream(device)
-    _need(0 <= max_tokens < 1 << 31, "max_tokens must be in [0, 2^31)")
-    _need(1 <= page_size < 1 << 31, "page_size must be in [1, 2^31)")
+    if lens.ndim != 1 or free_pages.ndim != 1:
+        raise ValueError("lens and free_pages must be vectors")
+    if not 0 <= max_tokens < 1 << 31 or not 1 <= page_size < 1 << 31:
+        raise ValueError("page_size must be in [1, 2^31), max_tokens in [0, 2^31)")
+    requests, nfree = lens.shape[0], free_pages.shape[0]
     table, row, width = _table(block_table, requests, device)
-    i32 = {"dtype": torch.int32, "device": lens.device}
-    out = CachePlan(torch.empty(requests + 1, **i32), torch.empty(requests, **i32),
-                    torch.empty(max_tokens, dtype=torch.int64, device=lens.device), torch.empty(max_tokens, **i32),
-                    torch.empty(1, **i32))
-    check(lib().fg_cache_plan(_vector(lens, None, torch.int32, device, "lens"),
+    # one allocation for the 32-bit outputs
+    q_starts, kv_lens, positions, used = torch.empty(2 * requests + max_tokens + 2, dtype=torch.int32, device=lens.device).split(
+        (requests + 1, requests, max_tokens, 1))
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=lens.device)
+    check(lib().fg_cache_plan(_vector(lens, requests, torch.int32, device, "lens"),
                               _vector(new_lens, requests, torch.int32, device, "new_lens"), requests, table, row, width,
-                              _vector(free_pages, None, torch.int32, device, "free_pages"), free_pages.shape[0],
-                              page_size, max_tokens, out.q_starts.data_ptr(), out.kv_lens.data_ptr(),
-                              out.slots.data_ptr(), out.positions.data_ptr(), out.used.data_ptr(), stream))
-    return out
+                              _vector(free_pages, nfree, torch.int32, device, "free_pages"), nfree, page_size, max_tokens,
+                              q_starts.data_ptr(), kv_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+                              used.data_ptr(), stream))
+    return CachePlan(q_starts, kv_lens, slots, positions, used)
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -111,56 +117,68 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     slot outside the cache, such as -1, is skipped."""
     device = k_cache.get_device()
     stream = _stream(device)
-    cache, shape = _cache(k_cache, v_cache, device)
+    cache, (_, _, heads_kv, dim) = _cache(k_cache, v_cache, device)
     tokens = slots.shape[0]
-    want = (tokens, shape[2], shape[3])
-    ks, vs = k.stride(), v.stride()
-    _need(k.shape == want and v.shape == want, f"k and v must have shape {want}")
-    _need(k.dtype == k_cache.dtype and v.dtype == k_cache.dtype, "k and v must have the cache's type")
-    _need(k.get_device() == device and v.get_device() == device, "k and v must be on the same device")
+    if k.shape != (tokens, heads_kv, dim) or v.shape != k.shape:
+        raise ValueError(f"k and v must have shape ({tokens}, {heads_kv}, {dim})")
+    if k.dtype != k_cache.dtype or v.dtype != k_cache.dtype:
+        raise ValueError("k and v must have the cache's type")
+    if k.get_device() != device or v.get_device() != device:
+        raise ValueError("k and v must be on the same device")
     if tokens == 0:
         return
-    _need(ks[2] == 1 and vs[2] == 1, "the last dimension of k and v must be contiguous")
-    check(lib().fg_cache_append(cache, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
+    k0, k1, k2 = k.stride()
+    v0, v1, v2 = v.stride()
+    if k2 != 1 or v2 != 1:
+        raise ValueError("the last dimension of k and v must be contiguous")
+    check(lib().fg_cache_append(cache, k.data_ptr(), v.data_ptr(), k0, k1, v0, v1,
                                 _vector(slots, tokens, torch.int64, device, "slots"), tokens, stream))
 
 
 def _attention(fn, q, k_cache, v_cache, block_table, q_starts, kv_lens, ids, max_q, scale, window, sinks, out, lse):
     device = q.get_device()
     stream = _stream(device)
-    cache, shape = _cache(k_cache, v_cache, device)
-    dim = shape[3]
-    _need(q.ndim == 3 and q.shape[2] == dim and q.dtype == k_cache.dtype,
-          f"q must have shape (tokens, heads, {dim}) and the cache's type")
-    tokens, heads, _ = q.shape
-    qs = q.stride()
-    _need(qs[2] == 1 or tokens == 0, "the last dimension of q must be contiguous")
-    requests = kv_lens.shape[0]
+    cache, (_, _, _, dim) = _cache(k_cache, v_cache, device)
+    shape, dtype, where = q.shape, q.dtype, q.device
+    if len(shape) != 3 or shape[2] != dim or dtype != k_cache.dtype:
+        raise ValueError(f"q must have shape (tokens, heads, {dim}) and the cache's type")
+    tokens, heads, _ = shape
+    q0, q1, q2 = q.stride()
+    if q2 != 1 and tokens:
+        raise ValueError("the last dimension of q must be contiguous")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty(tokens, heads, dim, dtype=dtype, device=where)
+        o0, o1 = heads * dim, dim
+    else:
+        o0, o1, o2 = out.stride()
+        if out.shape != shape or out.dtype != dtype or out.get_device() != device or (o2 != 1 and tokens):
+            raise ValueError("out must have q's shape and type, its last dimension contiguous, on the same device")
     if lse is None:
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
-    os_ = out.stride()
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.get_device() == device
-          and (os_[2] == 1 or tokens == 0),
-          "out must have q's shape and type, its last dimension contiguous, on the same device")
-    _need(lse.shape == (tokens, heads) and lse.dtype == torch.float32 and lse.is_contiguous()
-          and lse.get_device() == device, "lse must be contiguous float32 of shape (tokens, heads) on the same device")
-    _need(0 <= sinks < 1 << 31 and -1 <= window < 1 << 31, "window and sinks must be in [0, 2^31)")
+        lse = torch.empty(tokens, heads, dtype=torch.float32, device=where)
+    elif (lse.shape != (tokens, heads) or lse.dtype != torch.float32 or lse.get_device() != device
+          or not lse.is_contiguous()):
+        raise ValueError("lse must be contiguous float32 of shape (tokens, heads) on the same device")
+    if not 0 <= sinks < 1 << 31 or not -1 <= window < 1 << 31:
+        raise ValueError("window and sinks must be below 2^31, sinks not negative")
+    if kv_lens.ndim != 1:
+        raise ValueError("kv_lens must be a vector")
+    requests = kv_lens.shape[0]
     table, row, width = _table(block_table, requests, device)
-    starts = _vector(q_starts, requests + 1, torch.int32, device, "q_starts") if q_starts is not None else 0
-    lists = nids = ids_ptr = 0
-    if ids is not None:
-        _need(ids.ndim == 3 and ids.shape[0] == requests and ids.dtype in _IDS and ids.is_contiguous()
-              and ids.get_device() == device, f"ids must be contiguous int32 or uint32 of shape ({requests}, lists, K)")
+    starts = lists = nids = found = 0
+    if ids is None:
+        starts = _vector(q_starts, requests + 1, torch.int32, device, "q_starts")
+    else:
+        if (ids.ndim != 3 or ids.shape[0] != requests or ids.dtype not in _IDS or ids.get_device() != device
+                or not ids.is_contiguous()):
+            raise ValueError(f"ids must be contiguous int32 or uint32 of shape ({requests}, lists, K) on the same device")
         _, lists, nids = ids.shape
-        ids_ptr = ids.data_ptr()
-    need = lib().fg_attend_workspace_bytes(dim)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    check(fn(cache, _ATTENTION.pack(q.data_ptr(), out.data_ptr(), lse.data_ptr(), qs[0], qs[1], os_[0], os_[1], table, row,
-                                    starts, _vector(kv_lens, requests, torch.int32, device, "kv_lens"), ids_ptr,
-                                    work.data_ptr(), need, width, requests, tokens, heads, max_q, window, sinks, lists,
-                                    nids, scale if scale is not None else dim ** -0.5), stream))
+        found = ids.data_ptr()
+    args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), lse.data_ptr(), q0, q1, o0, o1, table, row, starts,
+                           _vector(kv_lens, requests, torch.int32, device, "kv_lens"), found, width, requests, tokens, heads,
+                           max_q, window, sinks, lists, nids, dim ** -0.5 if scale is None else scale)
+    need = lib().fg_attend_workspace_bytes(cache, args)
+    work = torch.empty(need, dtype=torch.uint8, device=where).data_ptr() if need > 0 else 0
+    check(fn(cache, args, work, need if need > 0 else 0, stream))
     return out, lse
 
 
@@ -178,9 +196,10 @@ def attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_
     p sees the tokens p - window + 1 .. p and the first `sinks`.
     Returns (out, lse): lse (tokens, heads) float32, the natural logarithm of the
     sum of exponentials.  A row that sees nothing gets 0 and -inf."""
-    _need(window is None or window >= 1, "window must be at least 1, or None")
-    _need(q_starts is not None, "q_starts is needed")
-    _need(0 <= max_q < 1 << 31, "max_q must be in [0, 2^31)")
+    if window is not None and window < 1:
+        raise ValueError("window must be at least 1, or None")
+    if q_starts is None or not 0 <= max_q < 1 << 31:
+        raise ValueError("q_starts is needed, and max_q in [0, 2^31)")
     return _attention(lib().fg_attend, q, k_cache, v_cache, block_table, q_starts, kv_lens, None, max_q, scale,
                       -1 if window is None else window, sinks, out, lse)
 
@@ -197,7 +216,7 @@ def attend_retrieved(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     each query head, for each key/value head, or between).  An id past the
     request's tokens, among the first or last ones, or equal to the id before it
     adds nothing.  Returns (out, lse) as `attend` does."""
-    _need(window >= 0, "window must be at least 0")
-    _need(ids is not None, "ids are needed")
+    if window < 0 or ids is None:
+        raise ValueError("ids are needed, and a window of at least 0")
     return _attention(lib().fg_attend_retrieved, q, k_cache, v_cache, block_table, None, kv_lens, ids, 1, scale, window,
                       sinks, out, lse)

@@ -35,8 +35,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
     __shared__ float wave_m[4][kRows], wave_l[4][kRows];
 
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, col = lane % 16, quarter = lane / 16;
-    const uint32_t w = blockIdx.x, W = gridDim.x;
-    const Start start = find_start<FOUND, kRows, 256>(P, w, W);
+    const uint32_t w = blockIdx.x;
+    const Start start = find_start<FOUND, kRows>(P, w);
     if (P.join && tid == 0) P.joins[w].pieces = 0;
     const uint64_t x1 = min((w + 1) * start.share, start.all);
     uint64_t before = start.before;
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
             continue;
         }
         Span sp;
-        const Piece pc = piece_of<FOUND, kRows, kRowsUnit>(P, rq, before, x, x1, &sp);
+        const Piece pc = piece_of<FOUND, kRows>(P, rq, before, x, x1, &sp);
         if (pc.none) {
             x = x1;
             continue;
@@ -223,61 +223,50 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
 
         // the four waves' softmaxes into one (each wave writes over its own tile of V)
         l = add_other32(add_other16(l));
-        if (quarter == 0) {
-            wave_m[wave][col] = m;
-            wave_l[wave][col] = l;
-        }
+        if (quarter == 0) wave_m[wave][col] = m;
+        __syncthreads();
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, wave_m[i][col]);
+        const float mine = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+        if (quarter == 0) wave_l[wave][col] = l * mine;
         float *omine = reinterpret_cast<float *>(vmine);
 #pragma unroll
-        for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4 *>(omine + col * OROW + 16 * i + 4 * quarter) = o[i];
+        for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4 *>(omine + col * OROW + 16 * i + 4 * quarter) = o[i] * mine;
         __syncthreads();
-        {
-            const uint32_t orow = tid / 16, part = tid % 16;
-            float top = -INFINITY, sum = 0.0f, f[4];
+        const bool whole = pc.begins && pc.ends;
+        const uint32_t slot = (2 * w + (pc.begins ? 1 : 0)) * kRows;
+        l = wave_l[0][col] + wave_l[1][col] + wave_l[2][col] + wave_l[3][col];
+        if (wave == 0 && quarter == 0 && row < rq.rows) {
+            if (!whole)
+                P.part_ml[slot + col] = float2{top, l};
+            else if (P.lse)
+                P.lse[(rq.q0 + static_cast<int64_t>(token)) * P.heads + list * P.group.d + (row - token * static_cast<int32_t>(P.group.d))] =
+                    (top + __builtin_amdgcn_logf(l)) * kLn2;
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, wave_m[i][orow]);
-            const float base = top == -INFINITY ? 0.0f : top;
+        for (uint32_t e = 0; e < kRows * D / 4; e += 256) {
+            const uint32_t at = e + tid, orow = at / (D / 4), quad = at % (D / 4);
+            const int32_t out_row = row0 + static_cast<int32_t>(orow);
+            if ((kRows * D / 4 % 256 == 0 || at < kRows * D / 4) && out_row < rq.rows) {
+                f32x4 a = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f[i] = __builtin_amdgcn_exp2f(wave_m[i][orow] - base);
-                sum += f[i] * wave_l[i][orow];
-            }
-            const bool whole = pc.begins && pc.ends;
-            const int32_t orow_all = row0 + static_cast<int32_t>(orow);
-            const int32_t otoken = P.group.div(orow_all);
-            const int64_t ohead = static_cast<int64_t>(list) * P.group.d + (orow_all - otoken * static_cast<int32_t>(P.group.d));
-            const int64_t qrow = rq.q0 + static_cast<int64_t>(otoken);
-            const uint32_t slot = 2 * w + (pc.begins ? 1 : 0);
-            if (orow_all < rq.rows) {
-                const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
-#pragma unroll
-                for (int e = 0; e < D / 32; ++e) {
-                    const uint32_t d = 32 * e + 2 * part;
-                    float a = 0.0f, b = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 v = *reinterpret_cast<const float2 *>(reinterpret_cast<float *>(vbuf[i]) + orow * OROW + d);
-                        a = fmaf(f[i], v.x, a);
-                        b = fmaf(f[i], v.y, b);
-                    }
-                    if (whole)
-                        *reinterpret_cast<uint32_t *>(P.out + qrow * P.out_token + ohead * P.out_head + 2 * d) = T::pack(a * inv, b * inv);
-                    else
-                        *reinterpret_cast<float2 *>(P.part + (static_cast<uint64_t>(slot) * kRows + orow) * D + d) = float2{a, b};
+                for (int i = 0; i < 4; ++i) a += *reinterpret_cast<const f32x4 *>(reinterpret_cast<float *>(vbuf[i]) + orow * OROW + 4 * quad);
+                if (whole) {
+                    const float sum = wave_l[0][orow] + wave_l[1][orow] + wave_l[2][orow] + wave_l[3][orow];
+                    a *= sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const int32_t t = P.group.div(out_row);
+                    char *dst = P.out + (rq.q0 + static_cast<int64_t>(t)) * P.out_token +
+                                static_cast<int64_t>(list * P.group.d + (out_row - t * P.group.d)) * P.out_head;
+                    *reinterpret_cast<uint2 *>(dst + 8 * quad) = uint2{T::pack(a[0], a[1]), T::pack(a[2], a[3])};
+                } else {
+                    *reinterpret_cast<f32x4 *>(P.part + static_cast<uint64_t>(slot + orow) * D + 4 * quad) = a;
                 }
-                if (part == 0) {
-                    if (!whole)
-                        P.part_ml[slot * kRows + orow] = float2{top, sum};
-                    else if (P.lse)
-                        P.lse[qrow * P.heads + ohead] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
-                }
-            }
-            if (P.join && tid == 0 && pc.begins && !pc.ends) {
-                const uint64_t last = (pc.end - 1) / start.share;  // the workgroup that holds its end
-                P.joins[w] = Join{static_cast<uint32_t>(last - w + 1), static_cast<uint32_t>(row0), static_cast<uint32_t>(rq.rows),
-                                  static_cast<uint32_t>(rq.q0), list};
             }
         }
+        if (P.join && tid == 0 && pc.begins && !pc.ends)
+            P.joins[w] = Join{workgroup_at(pc.end - 1, start.share) - w + 1, static_cast<uint32_t>(row0), static_cast<uint32_t>(rq.rows),
+                              static_cast<uint32_t>(rq.q0), list};
         __syncthreads();
         x = min(pc.end, x1);
     }
@@ -285,45 +274,28 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
 
 // ---------------------------------------------------------------- host side
 
-struct Workspace {
-    uint64_t part, ml, joins, total;
-};
-
-Workspace workspace_of(uint32_t dim) {
-    Workspace s;
-    s.part = 0;
-    const uint64_t rows = 2ull * std::max(kWorkgroups * kRows, kTileRows);  // two parts a workgroup
-    s.ml = s.part + rows * dim * 4;
-    s.joins = s.ml + rows * 8;
-    s.total = s.joins + kWorkgroups * sizeof(Join);
-    return s;
-}
-
 template <class T, int D, bool FOUND>
-int launch(AttendParams &P, uint64_t most_units, uint64_t item_units, hipStream_t st) {
-    const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(most_units, kWorkgroups));
-    // an item of one unit lies with one workgroup
-    P.join = item_units > 1;
-    P.least = kRowsUnit * P.group.d;
-    hipLaunchKernelGGL((fg_rows_kernel<T, D, FOUND>), dim3(grid), dim3(256), 0, st, P);
-    if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, kRows>), dim3(grid, kRows), dim3(256), 0, st, P);
+int launch(AttendParams &P, hipStream_t st) {
+    hipLaunchKernelGGL((fg_rows_kernel<T, D, FOUND>), dim3(P.workgroups), dim3(256), 0, st, P);
+    if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, kRows>), dim3(kJoinWorkgroups), dim3(256), 0, st, P);
     FG_HIP(hipGetLastError(), "attention launch");
     return FG_OK;
 }
 
 template <class T, bool FOUND>
-int launch(AttendParams &P, uint32_t dim, uint64_t most_units, uint64_t item_units, hipStream_t st) {
+int launch(AttendParams &P, uint32_t dim, hipStream_t st) {
     switch (dim) {
-    case 64: return launch<T, 64, FOUND>(P, most_units, item_units, st);
-    case 96: return launch<T, 96, FOUND>(P, most_units, item_units, st);
-    case 128: return launch<T, 128, FOUND>(P, most_units, item_units, st);
-    default: return launch<T, 256, FOUND>(P, most_units, item_units, st);
+    case 64: return launch<T, 64, FOUND>(P, st);
+    case 96: return launch<T, 96, FOUND>(P, st);
+    case 128: return launch<T, 128, FOUND>(P, st);
+    default: return launch<T, 256, FOUND>(P, st);
     }
 }
 
+// Checks the arguments and fills all of P but the workspace's addresses.
 template <bool FOUND>
-int attend(const fg_kv_cache *c, const fg_attention *a, void *stream) {
-    AttendParams P{};
+int prepare(const fg_kv_cache *c, const fg_attention *a, AttendParams *out) {
+    AttendParams &P = *out;
     if (int rc = check_cache(c, &P.cache)) return rc;
     if (!a) return fail(FG_EINVAL, "attention arguments are NULL");
     if (a->heads < 1 || a->heads > 1024 || a->heads % c->heads_kv)
@@ -332,28 +304,27 @@ int attend(const fg_kv_cache *c, const fg_attention *a, void *stream) {
     if (static_cast<uint64_t>(a->tokens) * a->heads > 0x7FFFFFFFull)
         return fail(FG_EINVAL, "tokens * heads must be below 2^31");
     if (a->table_width > 0x7FFFFFFFu || a->table_row < 0) return fail(FG_EINVAL, "table_width or table_row out of range");
+    if (static_cast<uint64_t>(a->table_width) * c->page_size > 0x3FFFFFFFull)
+        return fail(FG_EINVAL, "table_width * page_size must be below 2^30");
     if (a->sinks > 0x7FFFFFFFu) return fail(FG_EINVAL, "sinks must be below 2^31");
     if (FOUND) {
         if (a->window < 0) return fail(FG_EINVAL, "window must be >= 0");
         if (a->lists < 1 || a->heads % a->lists || a->lists % c->heads_kv)
             return fail(FG_EINVAL, "lists must be a multiple of heads_kv that divides heads");
-        if (a->nids > 0x3FFFFFFFu) return fail(FG_EINVAL, "ids of a list must be below 2^30");
+        if (a->nids > 0x1FFFFFFFu) return fail(FG_EINVAL, "ids of a list must be below 2^29");
         if (a->requests != a->tokens) return fail(FG_EINVAL, "one query row a request");
-    } else if (a->window != -1 && a->window < 1) {
-        return fail(FG_EINVAL, "window must be >= 1, or -1 for none");
+    } else {
+        if (a->window != -1 && a->window < 1) return fail(FG_EINVAL, "window must be >= 1, or -1 for none");
+        if (a->lists) return fail(FG_EINVAL, "lists are for retrieved tokens");
     }
-    if (a->requests == 0 || a->tokens == 0) return FG_OK;
     if (a->requests > 0x00FFFFFFu) return fail(FG_EINVAL, "requests must be below 2^24");
-    if (!a->q || !a->out || !a->kv_lens || (!FOUND && !a->q_starts) || (FOUND && a->nids && !a->ids) ||
-        (a->table_width && !a->table))
+    if (a->requests && a->tokens &&
+        (!a->q || !a->out || !a->kv_lens || (!FOUND && !a->q_starts) || (FOUND && a->nids && !a->ids) ||
+         (a->table_width && !a->table)))
         return fail(FG_EINVAL, "NULL device buffer");
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
         (a->q_token | a->q_head | a->out_token | a->out_head) % 8)
         return fail(FG_EINVAL, "q and out must be 16-byte aligned, strides multiples of 8 elements");
-    const Workspace ws = workspace_of(c->dim);
-    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_bytes < ws.total)
-        return fail(FG_EINVAL, "workspace must be 16-byte aligned and hold " + std::to_string(ws.total) + " bytes");
-
     P.q = static_cast<const char *>(a->q);
     P.out = static_cast<char *>(a->out);
     P.lse = a->lse;
@@ -374,24 +345,57 @@ int attend(const fg_kv_cache *c, const fg_attention *a, void *stream) {
     P.sinks = a->window == -1 ? 0 : a->sinks;
     P.group = fast_div(a->heads / P.lists);
     P.scale2 = a->scale * 1.44269504088896341f;
-    char *base = static_cast<char *>(a->workspace);
-    P.part = reinterpret_cast<float *>(base + ws.part);
-    P.part_ml = reinterpret_cast<float2 *>(base + ws.ml);
-    P.joins = reinterpret_cast<Join *>(base + ws.joins);
 
-    // what the host knows of the sizes: the table's room bounds a request's tokens
+    // What the host knows of the sizes: the table's room bounds a request's tokens.
+    P.tiles = !FOUND && static_cast<uint64_t>(a->max_q) * P.group.d > kFewRows;
+    if (P.tiles) {
+        plan_tiles(P, c->dim);
+        return FG_OK;
+    }
     uint64_t seen = static_cast<uint64_t>(a->table_width) * c->page_size;
     if (a->window != -1)
         seen = std::min(seen, static_cast<uint64_t>(a->sinks) + static_cast<uint32_t>(a->window) + (kRows - 1) / P.group.d + 1);
     seen += P.nids;
-    const uint64_t item_units = std::max<uint64_t>(1, (seen + kRowsUnit - 1) / kRowsUnit);
+    // Cutting an item of up to 512 tokens (four tiles a wave) gains less than the
+    // join kernel takes.
+    const uint32_t unit = seen <= 512 ? 512 : kRowsUnit;
     const uint64_t blocks = (static_cast<uint64_t>(a->tokens) * P.group.d + kRows - 1) / kRows + a->requests;
-    const uint64_t most_units = std::min<uint64_t>(blocks * P.lists, 1u << 20) * std::min<uint64_t>(item_units, 1u << 20);
+    const uint64_t items = std::min<uint64_t>(blocks * P.lists, 1u << 20);
+    const uint64_t pieces = items * std::max<uint64_t>(1, std::min<uint64_t>((seen + unit - 1) / unit, kWorkgroups));
+    P.rows = kRows;
+    P.unit = fast_div(unit);
+    P.join = seen > unit;
+    P.workgroups = 8;
+    while (P.workgroups < pieces && P.workgroups < kWorkgroups) P.workgroups *= 2;
+    P.least = static_cast<uint64_t>(kRowsUnit) * P.group.d;
+    return FG_OK;
+}
+
+// Two parts a workgroup, their maxima and sums, and a join record each.
+struct Workspace {
+    uint64_t ml, joins, total;
+};
+Workspace workspace_of(const AttendParams &P, uint32_t dim) {
+    if (!P.join) return {0, 0, 0};
+    const uint64_t rows = 2ull * P.workgroups * P.rows;
+    return {rows * dim * 4, rows * (dim * 4 + 8), rows * (dim * 4 + 8) + P.workgroups * sizeof(Join)};
+}
+
+template <bool FOUND>
+int attend(const fg_kv_cache *c, const fg_attention *a, void *workspace, uint64_t workspace_bytes, void *stream) {
+    AttendParams P{};
+    if (int rc = prepare<FOUND>(c, a, &P)) return rc;
+    if (a->requests == 0 || a->tokens == 0) return FG_OK;
+    const Workspace ws = workspace_of(P, c->dim);
+    if (ws.total && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < ws.total))
+        return fail(FG_EINVAL, "workspace must be 16-byte aligned and hold " + std::to_string(ws.total) + " bytes");
+    char *base = static_cast<char *>(workspace);
+    P.part = reinterpret_cast<float *>(base);
+    P.part_ml = reinterpret_cast<float2 *>(base + ws.ml);
+    P.joins = reinterpret_cast<Join *>(base + ws.joins);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    // many rows a list: blocks of them share their keys through LDS
-    if (!FOUND && static_cast<uint64_t>(a->max_q) * P.group.d > kFewRows) return launch_tiles(P, c->dtype, c->dim, st);
-    return c->dtype == FG_BF16 ? launch<BF16, FOUND>(P, c->dim, most_units, item_units, st)
-                               : launch<F16, FOUND>(P, c->dim, most_units, item_units, st);
+    if (P.tiles) return launch_tiles(P, c->dtype, c->dim, st);
+    return c->dtype == FG_BF16 ? launch<BF16, FOUND>(P, c->dim, st) : launch<F16, FOUND>(P, c->dim, st);
 }
 
 }  // namespace
@@ -399,14 +403,19 @@ int attend(const fg_kv_cache *c, const fg_attention *a, void *stream) {
 
 extern "C" {
 
-uint64_t fg_attend_workspace_bytes(uint32_t dim) {
-    return dim == 64 || dim == 96 || dim == 128 || dim == 256 ? fgk::workspace_of(dim).total : 0;
+int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a) {
+    fgk::AttendParams P{};
+    const int rc = a && a->lists ? fgk::prepare<true>(cache, a, &P) : fgk::prepare<false>(cache, a, &P);
+    return rc ? rc : static_cast<int64_t>(a->requests && a->tokens ? fgk::workspace_of(P, cache->dim).total : 0);
 }
 
-int fg_attend(const fg_kv_cache *cache, const fg_attention *a, void *stream) { return fgk::attend<false>(cache, a, stream); }
+int fg_attend(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes, void *stream) {
+    return fgk::attend<false>(cache, a, workspace, workspace_bytes, stream);
+}
 
-int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *stream) {
-    return fgk::attend<true>(cache, a, stream);
+int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes,
+                        void *stream) {
+    return fgk::attend<true>(cache, a, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -112,8 +112,11 @@ struct AttendParams {
     uint32_t list_heads; // lists a key/value head
     uint32_t nids, window, sinks;  // window 0xFFFFFFFF: none
     uint32_t join;       // whether the join kernel follows
+    uint32_t tiles, rows;  // whether the tile kernel runs; query rows of a block
+    uint32_t workgroups; // of the attention kernel, a power of two
     uint64_t least;      // weight that a workgroup takes at least
     FastDiv group;       // query heads that share a list
+    FastDiv unit;        // tokens between cuts through an item, a multiple of a tile
     float scale2;        // scale * log2(e)
 };
 
@@ -221,6 +224,14 @@ __device__ __forceinline__ int2 place_of(const AttendParams &P, uint32_t r, int3
     return {static_cast<uint32_t>(page) < P.cache.pages ? page : -1, static_cast<int32_t>(j - b * P.cache.page_size.d)};
 }
 
+// The workgroup that weight x falls to.
+__device__ __forceinline__ uint32_t workgroup_at(uint64_t x, uint64_t share) {
+    uint64_t w = static_cast<uint64_t>(static_cast<double>(x) / static_cast<double>(share));
+    w -= w * share > x;
+    w += (w + 1) * share <= x;
+    return static_cast<uint32_t>(w);
+}
+
 // Whether the row at `pos` sees the token at position j (pages aside).
 __device__ __forceinline__ bool sees(const AttendParams &P, int32_t pos, int32_t j) {
     const int32_t back = pos - j;
@@ -231,69 +242,43 @@ __device__ __forceinline__ bool sees(const AttendParams &P, int32_t pos, int32_t
 struct Start {
     uint64_t all, share;  // weight of all items; of a workgroup
     uint64_t before;      // weight of the requests before `request`
-    uint32_t request;
+    uint32_t request;     // at most a few requests before the first one of the share
 };
 
-// Called by all THREADS threads; every workgroup sums the requests' weights itself.
-template <bool FOUND, uint32_t ROWS, uint32_t THREADS>
-__device__ Start find_start(const AttendParams &P, uint32_t w, uint32_t workgroups) {
-    constexpr uint32_t WAVES = THREADS / 64;
-    __shared__ uint64_t wave_sum[WAVES];
-    __shared__ uint64_t found_before;
-    __shared__ uint32_t found_request;
-    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-    const bool once = P.requests <= THREADS;  // one look at the requests gives the sum and the place
-    Start s{0, 0, 0, 0};
-    for (int pass = once ? 1 : 0; pass < 2; ++pass) {
-        uint64_t sum = 0;
-        for (uint32_t r0 = 0; r0 < P.requests; r0 += THREADS) {
-            const uint32_t r = r0 + tid;
-            uint64_t u = 0;
-            if (r < P.requests) {
-                const Request q = request_of<FOUND, ROWS>(P, r);
-                u = q.weight_of(q.blocks) * P.lists;
-            }
-            uint64_t v = u;
-#pragma unroll
-            for (uint32_t d = 1; d < 64; d <<= 1) {
-                const uint64_t o = __shfl_up(v, d);
-                if (lane >= d) v += o;
-            }
-            if (lane == 63) wave_sum[wave] = v;
-            __syncthreads();
-            uint64_t base = sum;
-#pragma unroll
-            for (uint32_t i = 0; i < WAVES; ++i) {
-                if (i < wave) base += wave_sum[i];
-                sum += wave_sum[i];
-            }
-            if (once) {
-                s.all = sum;
-                s.share = max((sum + workgroups - 1) / workgroups, P.least);
-            }
-            const uint64_t x = w * s.share;
-            if (pass == 1 && u && base + v - u <= x && x < base + v) {
-                found_before = base + v - u;
-                found_request = r;
-            }
-            __syncthreads();
-        }
-        if (pass == 0) {
-            s.all = sum;
-            s.share = max((sum + workgroups - 1) / workgroups, P.least);
+// Every wave sums the requests' weights itself, a lane a run of them: nothing is
+// waited for but the lengths.  workgroups is a power of two.
+template <bool FOUND, uint32_t ROWS>
+__device__ __forceinline__ Start find_start(const AttendParams &P, uint32_t w) {
+    const uint32_t lane = threadIdx.x % 64, run = (P.requests + 63) / 64;
+    uint64_t mine = 0;
+    for (uint32_t i = 0; i < run; ++i) {
+        const uint32_t r = lane * run + i;
+        if (r < P.requests) {
+            const Request q = request_of<FOUND, ROWS>(P, r);
+            mine += q.weight_of(q.blocks) * P.lists;
         }
     }
-    if (w * s.share < s.all) {
-        s.before = found_before;
-        s.request = found_request;
+    uint64_t upto = mine;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint64_t o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
     }
+    Start s;
+    s.all = __shfl(upto, 63);
+    s.share = max((s.all + P.workgroups - 1) >> __builtin_ctz(P.workgroups), P.least);
+    const uint64_t x = w * s.share;
+    const uint64_t at = __ballot(upto > x && upto - mine <= x);
+    const uint32_t owner = at ? __ffsll(static_cast<unsigned long long>(at)) - 1 : 0;
+    s.before = __shfl(upto - mine, owner);
+    s.request = owner * run;
     return s;
 }
 
 // What of an item a workgroup holds.
 struct Piece {
     uint32_t list, block;
-    uint32_t t_lo, t_hi;      // token numbers of its span, cut between units of UNIT tokens
+    uint32_t t_lo, t_hi;      // token numbers of its span, cut between units
     uint64_t end;             // where the item's weight ends
     bool begins, ends;        // whether the item's first (last) unit is here
     bool none;                // no unit is, and none came before: another workgroup begins the item
@@ -302,33 +287,45 @@ struct Piece {
 // The item that x lies in (x is inside request q, whose weight begins at
 // `before`), and its tokens up to x1.  Two neighbours work out the cut between
 // them from the same numbers.
-template <bool FOUND, uint32_t ROWS, uint32_t UNIT>
+template <bool FOUND, uint32_t ROWS>
 __device__ __forceinline__ Piece piece_of(const AttendParams &P, const Request &q, uint64_t before, uint64_t x, uint64_t x1,
                                           Span *span) {
     Piece p;
+    const uint32_t lane = threadIdx.x % 64;
+    // the list and the block by 64 guesses at a time (a division of 64-bit numbers is
+    // a hundred instructions in a row)
     const uint64_t list_weight = q.weight_of(q.blocks);
-    p.list = static_cast<uint32_t>((x - before) / list_weight);
-    const uint64_t start = before + p.list * list_weight, at = x - start;
-    uint32_t lo = 0, hi = q.blocks;  // the last block that begins at or before `at`
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (q.weight_of(mid) <= at) lo = mid;
-        else hi = mid;
+    uint32_t list = 0;
+    for (uint32_t n = 64; n == 64; list += 64) {
+        const uint32_t guess = list + lane;
+        n = __popcll(__ballot(guess < P.lists && guess * list_weight <= x - before));
+        if (n < 64) list += n - 1;
+        if (n < 64) break;
+    }
+    p.list = list;
+    const uint64_t start = before + list * list_weight, at = x - start;
+    uint32_t lo = 0;  // the last block that begins at or before `at`
+    for (uint32_t len = q.blocks; len > 1;) {
+        const uint32_t stride = (len + 63) / 64, guess = lane * stride;
+        const uint32_t n = __popcll(__ballot(guess < len && q.weight_of(lo + guess) <= at)) - 1;
+        lo += n * stride;
+        len = min(stride, len - n * stride);
     }
     p.block = lo;
     const uint64_t begin = start + q.weight_of(lo), weight = q.weight_of(lo + 1) - q.weight_of(lo);
     p.end = begin + weight;
     *span = span_of<FOUND, ROWS>(P, q, lo);
-    const uint32_t total = span->total, units = max((total + UNIT - 1) / UNIT, 1u);
+    const uint32_t total = span->total, units = max(P.unit.div(total + P.unit.d - 1), 1u);
     // x, and x1 inside the item, fall into units 0 .. units - 1: the workgroup that holds the
     // item's end holds its last unit, and an item of one unit is never cut
-    const uint32_t u0 = static_cast<uint32_t>((x - begin) * units / weight);
-    const uint32_t u1 = x1 >= p.end ? units : static_cast<uint32_t>((x1 - begin) * units / weight);
+    const float per = static_cast<float>(units) * __builtin_amdgcn_rcpf(static_cast<float>(weight));
+    const uint32_t u0 = min(static_cast<uint32_t>(static_cast<float>(x - begin) * per), units - 1);
+    const uint32_t u1 = x1 >= p.end ? units : min(static_cast<uint32_t>(static_cast<float>(x1 - begin) * per), units - 1);
     p.begins = u0 == 0;
     p.ends = u1 == units;
     p.none = u1 == 0;
-    p.t_lo = min(u0 * UNIT, total);
-    p.t_hi = min(u1 * UNIT, total);
+    p.t_lo = min(u0 * P.unit.d, total);
+    p.t_hi = u1 == units ? total : u1 * P.unit.d;
     return p;
 }
 
@@ -336,67 +333,111 @@ constexpr uint32_t kRows = 16;         // query rows of a block of the few-rows 
 constexpr uint32_t kWorkgroups = 512;  // at most: two a CU
 constexpr float kLn2 = 0.69314718055994531f;
 
-// The parts of an item into its rows: workgroup (w, row) of the item that
-// workgroup w of the attention kernel began and did not end.  Its parts are the
-// second of w and the first of w + 1, w + 2, ...
+// The parts of items into their rows.  Workgroup w of the attention kernel began an
+// item and did not end it where joins[w] says so; its parts are the second of w and
+// the first of w + 1, w + 2, ...  Every workgroup here lists the rows of all such
+// items; few rows (one long context, its parts by the hundred) take a workgroup
+// each, many (a part or two each) the lanes of one row.  Bound by latency: a part is
+// read once, without a look at the maximum before.
 template <class T, int D, uint32_t ROWS>
 __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
-    constexpr uint32_t QUADS = D / 4, SETS = 256 / QUADS;  // threads across a row, sets of parts side by side
-    __shared__ float sum_m[4];
-    __shared__ float acc[SETS][D], acc_l[SETS];
-    const uint32_t w = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
-    const Join j = P.joins[w];
-    if (j.pieces == 0 || j.row0 + row >= j.rows) return;
-    const auto slot_of = [&](uint32_t i) { return i == 0 ? 2 * w + 1 : 2 * (w + i); };
-
-    float top = -INFINITY;
-    for (uint32_t i = tid; i < j.pieces; i += 256) top = fmaxf(top, P.part_ml[slot_of(i) * ROWS + row].x);
+    constexpr uint32_t QUADS = D / 4, LANES = D <= 64 ? 16 : D <= 128 ? 32 : 64, SETS = 256 / LANES;
+    __shared__ uint32_t first[kWorkgroups + 1], wave_sum[4];
+    __shared__ f32x4 acc[256];
+    __shared__ float2 acc_ml[SETS];
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, W = P.workgroups;
+    uint32_t mine[kWorkgroups / 256], sum = 0;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (tid % 64 == 0) sum_m[tid / 64] = top;
+    for (uint32_t i = 0; i < kWorkgroups / 256; ++i) {  // consecutive workgroups in one thread
+        const uint32_t w = tid * (kWorkgroups / 256) + i;
+        mine[i] = 0;
+        if (w < W) {
+            const Join j = P.joins[w];
+            if (j.pieces) mine[i] = min(ROWS, j.rows - j.row0);
+        }
+        sum += mine[i];
+    }
+    uint32_t upto = sum;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 63) wave_sum[wave] = upto;
     __syncthreads();
-    top = fmaxf(fmaxf(sum_m[0], sum_m[1]), fmaxf(sum_m[2], sum_m[3]));
-    const float base = top == -INFINITY ? 0.0f : top;
+    upto -= sum;
+    uint32_t all = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        if (i < wave) upto += wave_sum[i];
+        all += wave_sum[i];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kWorkgroups / 256; ++i) {
+        first[tid * (kWorkgroups / 256) + i] = upto;
+        upto += mine[i];
+    }
+    __syncthreads();
 
-    const uint32_t set = tid / QUADS, quad = tid % QUADS;
-    if (set < SETS) {
+    const bool few = all <= gridDim.x;
+    const uint32_t set = tid / LANES, quad = tid % LANES, step = few ? SETS : 1;
+    for (uint32_t at = blockIdx.x * (few ? 1 : SETS); at < all; at += gridDim.x * (few ? 1 : SETS)) {
+        const uint32_t task = at + (few ? 0 : set);
+        uint32_t lo = 0, hi = W;  // the last workgroup whose rows begin at or before `task`
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (first[mid] <= task) lo = mid;
+            else hi = mid;
+        }
+        const uint32_t w = lo, row = task - first[w];
+        const Join j = P.joins[w];
+        float top = -INFINITY, l = 0.0f;
         f32x4 a = {0, 0, 0, 0};
-        float l = 0.0f;
-#pragma unroll 4
-        for (uint32_t i = set; i < j.pieces; i += SETS) {
-            const uint32_t at = slot_of(i) * ROWS + row;
-            const float2 ml = P.part_ml[at];
-            const float f = __builtin_amdgcn_exp2f(ml.x - base);
-            a += f * *reinterpret_cast<const f32x4 *>(P.part + static_cast<uint64_t>(at) * D + 4 * quad);
-            l = fmaf(f, ml.y, l);
+        if (task < all && quad < QUADS) {
+#pragma unroll 8
+            for (uint32_t i = few ? set : 0; i < j.pieces; i += step) {
+                const uint32_t p = (i == 0 ? 2 * w + 1 : 2 * (w + i)) * ROWS + row;
+                const float2 ml = P.part_ml[p];
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(P.part + static_cast<uint64_t>(p) * D + 4 * quad);
+                const float next = fmaxf(top, ml.x), base = next == -INFINITY ? 0.0f : next;
+                const float f = __builtin_amdgcn_exp2f(top - base), g = __builtin_amdgcn_exp2f(ml.x - base);
+                a = a * f + v * g;
+                l = fmaf(g, ml.y, l * f);
+                top = next;
+            }
         }
-        *reinterpret_cast<f32x4 *>(&acc[set][4 * quad]) = a;
-        if (quad == 0) acc_l[set] = l;
-    }
-    __syncthreads();
-    const uint32_t all = j.row0 + row, token = P.group.div(all), head = j.list * P.group.d + (all - token * P.group.d);
-    const int64_t qrow = static_cast<int64_t>(j.q0) + token;
-    float l = 0.0f;
+        if (few) {
+            acc[tid] = a;
+            if (quad == 0) acc_ml[set] = float2{top, l};
+            __syncthreads();
+            if (set == 0) {
+                for (uint32_t i = 0; i < SETS; ++i) top = fmaxf(top, acc_ml[i].x);
+                const float base = top == -INFINITY ? 0.0f : top;
+                a = f32x4{0, 0, 0, 0};
+                l = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < SETS; ++i) l += acc_l[i];
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (tid < D / 2) {
-        float a = 0.0f, b = 0.0f;
-#pragma unroll
-        for (uint32_t i = 0; i < SETS; ++i) {
-            a += acc[i][2 * tid];
-            b += acc[i][2 * tid + 1];
+                for (uint32_t i = 0; i < SETS; ++i) {
+                    const float f = __builtin_amdgcn_exp2f(acc_ml[i].x - base);
+                    a += acc[tid + i * LANES] * f;
+                    l = fmaf(f, acc_ml[i].y, l);
+                }
+            }
         }
-        *reinterpret_cast<uint32_t *>(P.out + qrow * P.out_token + head * P.out_head + 4 * tid) = T::pack(a * inv, b * inv);
+        if (task < all && quad < QUADS && (!few || set == 0)) {
+            const uint32_t r = j.row0 + row, token = P.group.div(r), head = j.list * P.group.d + (r - token * P.group.d);
+            const int64_t qrow = static_cast<int64_t>(j.q0) + token;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            *reinterpret_cast<uint2 *>(P.out + qrow * P.out_token + head * P.out_head + 8 * quad) = uint2{T::pack(a[0] * inv, a[1] * inv), T::pack(a[2] * inv, a[3] * inv)};
+            if (quad == 0 && P.lse) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
+        }
+        if (few) __syncthreads();
     }
-    if (tid == 0 && P.lse) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
+constexpr uint32_t kJoinWorkgroups = 1024;
 
-// Rows of the tile kernel's blocks together over all workgroups: two parts of
-// the workspace each.
-constexpr uint32_t kTileRows = 256 * 256;
-
-// Blocks of many rows (fg_attend_tiles.hip): launches on `stream`.
+// Blocks of many rows (fg_attend_tiles.hip): sets rows, unit, least, workgroups and
+// join; launches.
+void plan_tiles(AttendParams &P, uint32_t dim);
 int launch_tiles(AttendParams &P, int dtype, uint32_t dim, hipStream_t stream);
 
 }  // namespace fgk

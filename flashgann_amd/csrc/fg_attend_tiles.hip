@@ -46,7 +46,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
     // neighbours in weight, which read the same keys, on one die of eight (the
     // grid is a multiple of 8)
     const uint32_t w = blockIdx.x % 8 * (W / 8) + blockIdx.x / 8;
-    const Start start = find_start<false, ROWS, THREADS>(P, w, W);
+    const Start start = find_start<false, ROWS>(P, w);
     if (tid == 0) P.joins[w].pieces = 0;
     const uint64_t x1 = min((w + 1) * start.share, start.all);
     uint64_t before = start.before;
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
             continue;
         }
         Span sp;
-        const Piece pc = piece_of<false, ROWS, kTilesUnit>(P, rq, before, x, x1, &sp);
+        const Piece pc = piece_of<false, ROWS>(P, rq, before, x, x1, &sp);
         if (pc.none) {
             x = x1;
             continue;
@@ -297,19 +297,19 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
             }
         }
         if (tid == 0 && pc.begins && !pc.ends) {
-            const uint64_t last = (pc.end - 1) / start.share;  // the workgroup that holds its end
-            P.joins[w] = Join{static_cast<uint32_t>(last - w + 1), pc.block * ROWS, static_cast<uint32_t>(rq.rows), static_cast<uint32_t>(rq.q0), pc.list};
+            P.joins[w] = Join{workgroup_at(pc.end - 1, start.share) - w + 1, pc.block * ROWS, static_cast<uint32_t>(rq.rows), static_cast<uint32_t>(rq.q0), pc.list};
         }
         x = min(pc.end, x1);
     }
 }
 
-template <class T, int D, int NW>
+constexpr int waves_of(int dim) { return dim > 128 ? 4 : 8; }
+
+template <class T, int D>
 int launch(AttendParams &P, hipStream_t st) {
-    constexpr uint32_t ROWS = 32 * NW, grid = 256;
-    P.least = static_cast<uint64_t>(kTilesUnit) * P.group.d;
-    hipLaunchKernelGGL((fg_tiles_kernel<T, D, NW>), dim3(grid), dim3(64 * NW), 0, st, P);
-    hipLaunchKernelGGL((fg_join_kernel<T, D, ROWS>), dim3(grid, ROWS), dim3(256), 0, st, P);
+    constexpr int NW = waves_of(D);
+    hipLaunchKernelGGL((fg_tiles_kernel<T, D, NW>), dim3(P.workgroups), dim3(64 * NW), 0, st, P);
+    hipLaunchKernelGGL((fg_join_kernel<T, D, 32 * NW>), dim3(kJoinWorkgroups), dim3(256), 0, st, P);
     FG_HIP(hipGetLastError(), "attention launch");
     return FG_OK;
 }
@@ -317,14 +317,22 @@ int launch(AttendParams &P, hipStream_t st) {
 template <class T>
 int launch(AttendParams &P, uint32_t dim, hipStream_t st) {
     switch (dim) {
-    case 64: return launch<T, 64, 8>(P, st);
-    case 96: return launch<T, 96, 8>(P, st);
-    case 128: return launch<T, 128, 8>(P, st);
-    default: return launch<T, 256, 4>(P, st);
+    case 64: return launch<T, 64>(P, st);
+    case 96: return launch<T, 96>(P, st);
+    case 128: return launch<T, 128>(P, st);
+    default: return launch<T, 256>(P, st);
     }
 }
 
 }  // namespace
+
+void plan_tiles(AttendParams &P, uint32_t dim) {
+    P.rows = 32 * waves_of(dim);
+    P.unit = fast_div(kTilesUnit);
+    P.least = static_cast<uint64_t>(kTilesUnit) * P.group.d;
+    P.workgroups = 256;
+    P.join = 1;
+}
 
 int launch_tiles(AttendParams &P, int dtype, uint32_t dim, hipStream_t stream) {
     return dtype == FG_BF16 ? launch<BF16>(P, dim, stream) : launch<F16>(P, dim, stream);

@@ -307,13 +307,11 @@ int fg_cache_append(const fg_kv_cache *cache, const void *k, const void *v, int6
 /* One call of attention.  q and out: (tokens, heads, dim) in the cache's type,
  * strides in elements, multiples of 8, bases 16-byte aligned; lse: (tokens,
  * heads) float32, contiguous, may be NULL.  heads is a multiple of the cache's
- * heads_kv; consecutive query heads share a key/value head.  lse is the natural
+ * heads_kv; consecutive query heads share a key/value head.  The table names
+ * fewer than 2^30 tokens a request (table_width * page_size).  lse is the natural
  * logarithm of the sum of exponentials; a row that sees nothing gets 0 and
  * -infinity.  Scores, softmax statistics and sums are 32-bit; weights are
- * rounded to the cache's type for the product with the values.
- * workspace: at least fg_attend_workspace_bytes(dim) bytes, 16-byte aligned,
- * used until the call's work on `stream` ends; nothing is kept in it between
- * calls. */
+ * rounded to the cache's type for the product with the values. */
 typedef struct {
     const void *q;
     void *out;
@@ -324,8 +322,6 @@ typedef struct {
     const int32_t *q_starts; /* requests + 1 (fg_attend) */
     const int32_t *kv_lens;  /* requests */
     const uint32_t *ids;     /* requests x lists x nids, contiguous (fg_attend_retrieved) */
-    void *workspace;
-    uint64_t workspace_bytes;
     uint32_t table_width, requests, tokens, heads;
     uint32_t max_q; /* the longest chunk (fg_attend); a hint that picks the kernel */
     int32_t window; /* -1: none (fg_attend) */
@@ -339,7 +335,8 @@ typedef struct {
  * cache.  The row at position p sees the tokens j <= p and, with a window >= 1,
  * of those j > p - window and j < sinks.  Rows of q outside every request are
  * left alone. */
-int fg_attend(const fg_kv_cache *cache, const fg_attention *a, void *stream);
+int fg_attend(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes,
+              void *stream);
 
 /* Attention of one token a request (q row r at position kv_lens[r] - 1) over
  * the first `sinks` tokens, the last `window` tokens and the ids of a list.
@@ -348,11 +345,15 @@ int fg_attend(const fg_kv_cache *cache, const fg_attention *a, void *stream);
  * kv_lens[r], in neither of the first two sets, and differs from the id before
  * it (a search whose beam is shorter than K repeats its last id); ids are
  * token positions as fg_search_device writes them. */
-int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *stream);
+int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes,
+                        void *stream);
 
-/* Bytes of workspace that both need at this head dimension; 0 for one that
- * they do not take. */
-uint64_t fg_attend_workspace_bytes(uint32_t dim);
+/* Bytes of workspace (16-byte aligned, used until the call's work on `stream`
+ * ends, nothing kept in it between calls) that such a call needs at most, from
+ * the sizes alone: 0 where no item's tokens can be split over workgroups.  `a` is
+ * fg_attend_retrieved's if its lists are not 0.  Negative FG_E* on arguments that
+ * the call would refuse. */
+int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
 
 const char *fg_last_error(void);
 const char *fg_version(void);

@@ -12,8 +12,8 @@ AT = 1 << 20  # an aligned address of nothing
 CACHE = dict(k=AT, v=AT, k_page=4096, k_token=256, k_head=128, v_page=4096, v_token=256, v_head=128, pages=10, page_size=16,
              heads_kv=2, dim=128, dtype=0, reserved=0)
 ATTENTION = dict(q=AT, out=AT, lse=AT, q_token=1024, q_head=128, out_token=1024, out_head=128, table=AT, table_row=5,
-                 q_starts=AT, kv_lens=AT, ids=AT, workspace=AT, workspace_bytes=1 << 40, table_width=5, requests=3, tokens=3,
-                 heads=8, max_q=1, window=-1, sinks=0, lists=2, nids=7, scale=0.1)
+                 q_starts=AT, kv_lens=AT, ids=AT, table_width=500, requests=3, tokens=3,
+                 heads=8, max_q=1, window=-1, sinks=0, lists=0, nids=7, scale=0.1)
 
 
 def refused(rc, word):
@@ -29,6 +29,17 @@ def attention_bytes(**kw):
     return attention._ATTENTION.pack(*{**ATTENTION, **kw}.values())
 
 
+def dense(cache, a, work=AT, bytes_=1 << 40):
+    return _lib.lib().fg_attend(cache, a, work, bytes_, None)
+
+
+def found(cache, a, work=AT, bytes_=1 << 40):
+    return _lib.lib().fg_attend_retrieved(cache, a, work, bytes_, None)
+
+
+FOUND = dict(window=3, lists=2)
+
+
 BAD_CACHES = ((dict(dim=80), "dim"), (dict(dim=0), "dim"), (dict(dtype=2), "dtype"), (dict(heads_kv=0), "heads_kv"),
               (dict(pages=0), "tokens"), (dict(page_size=0), "tokens"), (dict(pages=1 << 20, page_size=1 << 11), "tokens"),
               (dict(k=0), "NULL"), (dict(v=AT + 8), "aligned"), (dict(k_token=100), "strides"), (dict(v_page=4), "strides"))
@@ -37,8 +48,9 @@ BAD_CACHES = ((dict(dim=80), "dim"), (dict(dim=0), "dim"), (dict(dtype=2), "dtyp
 @pytest.mark.parametrize("bad,word", BAD_CACHES)
 def test_caches(bad, word):
     L = _lib.lib()
-    refused(L.fg_attend(cache_bytes(**bad), attention_bytes(), None), word)
-    refused(L.fg_attend_retrieved(cache_bytes(**bad), attention_bytes(window=3), None), word)
+    refused(dense(cache_bytes(**bad), attention_bytes()), word)
+    refused(found(cache_bytes(**bad), attention_bytes(**FOUND)), word)
+    assert L.fg_attend_workspace_bytes(cache_bytes(**bad), attention_bytes()) == _lib.FG_EINVAL
     refused(L.fg_cache_append(cache_bytes(**bad), AT, AT, 256, 128, 256, 128, AT, 4, None), word)
 
 
@@ -47,27 +59,40 @@ def test_caches(bad, word):
     (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(tokens=1 << 30, requests=1 << 30), "tokens"), (dict(table_row=-1), "table"), (dict(table_width=1 << 31), "table"),
     (dict(sinks=1 << 31), "sinks"), (dict(q=0), "NULL"), (dict(out=0), "NULL"), (dict(table=0), "NULL"), (dict(kv_lens=0), "NULL"),
-    (dict(q=AT + 2), "aligned"), (dict(q_head=130), "strides"), (dict(out_token=4), "strides"), (dict(workspace=0), "workspace"),
-    (dict(workspace=AT + 4), "workspace"), (dict(workspace_bytes=100), "workspace")))
+    (dict(q=AT + 2), "aligned"), (dict(q_head=130), "strides"), (dict(out_token=4), "strides"),
+    (dict(table_width=1 << 27), "table_width")))
 def test_attention(bad, word):
-    L = _lib.lib()
-    refused(L.fg_attend(cache_bytes(), attention_bytes(**bad), None), word)
-    refused(L.fg_attend_retrieved(cache_bytes(), attention_bytes(**{"window": 3, **bad}), None), word)
+    refused(dense(cache_bytes(), attention_bytes(**bad)), word)
+    refused(found(cache_bytes(), attention_bytes(**{**FOUND, **bad})), word)
 
 
 def test_attention_of_one_kind():
-    L = _lib.lib()
-    refused(L.fg_attend(cache_bytes(), attention_bytes(window=0), None), "window")
-    refused(L.fg_attend(cache_bytes(), attention_bytes(window=-2), None), "window")
-    refused(L.fg_attend(cache_bytes(), attention_bytes(q_starts=0), None), "NULL")
-    refused(L.fg_attend_retrieved(cache_bytes(), attention_bytes(window=-1), None), "window")
+    refused(dense(cache_bytes(), attention_bytes(window=0)), "window")
+    refused(dense(cache_bytes(), attention_bytes(window=-2)), "window")
+    refused(dense(cache_bytes(), attention_bytes(q_starts=0)), "NULL")
+    refused(dense(cache_bytes(), attention_bytes(lists=2)), "lists")
+    refused(found(cache_bytes(), attention_bytes(window=-1, lists=2)), "window")
     for lists in (0, 1, 3, 16):
-        refused(L.fg_attend_retrieved(cache_bytes(), attention_bytes(window=3, lists=lists), None), "lists")
-    refused(L.fg_attend_retrieved(cache_bytes(), attention_bytes(window=3, tokens=4), None), "row")
-    refused(L.fg_attend_retrieved(cache_bytes(), attention_bytes(window=3, ids=0), None), "NULL")
-    refused(L.fg_attend_retrieved(cache_bytes(), attention_bytes(window=3, nids=1 << 30), None), "ids")
-    refused(L.fg_attend(None, attention_bytes(), None), "NULL")
-    refused(L.fg_attend(cache_bytes(), None, None), "NULL")
+        refused(found(cache_bytes(), attention_bytes(window=3, lists=lists)), "lists")
+    refused(found(cache_bytes(), attention_bytes(**FOUND, tokens=4)), "row")
+    refused(found(cache_bytes(), attention_bytes(**FOUND, ids=0)), "NULL")
+    refused(found(cache_bytes(), attention_bytes(**FOUND, nids=1 << 29)), "ids")
+    refused(dense(None, attention_bytes()), "NULL")
+    refused(dense(cache_bytes(), None), "NULL")
+
+
+def test_workspace():
+    """What a call needs: nothing where no item is cut, and a smaller, absent or odd one is refused."""
+    L = _lib.lib()
+    for a, call in ((attention_bytes(), dense), (attention_bytes(max_q=1000), dense),
+                    (attention_bytes(window=900, lists=2, sinks=4), found)):
+        need = L.fg_attend_workspace_bytes(cache_bytes(), a)
+        assert need > 0
+        for work, n in ((None, need), (AT + 4, need), (AT, need - 1)):
+            refused(call(cache_bytes(), a, work, n), "workspace")
+    assert L.fg_attend_workspace_bytes(cache_bytes(), attention_bytes(window=3, lists=2)) == 0
+    assert L.fg_attend_workspace_bytes(cache_bytes(), attention_bytes(table_width=20)) == 0
+    assert L.fg_attend_workspace_bytes(cache_bytes(), attention_bytes(tokens=0)) == 0
 
 
 def test_plan():
@@ -97,17 +122,10 @@ def test_append():
     assert L.fg_cache_append(cache_bytes(), None, None, 256, 128, 256, 128, None, 0, None) == _lib.FG_OK
 
 
-def test_workspace_sizes():
-    L = _lib.lib()
-    sizes = [L.fg_attend_workspace_bytes(d) for d in (64, 96, 128, 256)]
-    assert sizes == sorted(sizes) and sizes[0] > 0
-    assert [L.fg_attend_workspace_bytes(d) for d in (0, 32, 80, 512)] == [0] * 4
-
-
 def test_struct_sizes():
     """The packed structs are the header's: no padding between the fields or at the end."""
     assert attention._CACHE.size == 2 * 8 + 6 * 8 + 6 * 4
-    assert attention._ATTENTION.size == 14 * 8 + 10 * 4
+    assert attention._ATTENTION.size == 12 * 8 + 10 * 4
     assert C.sizeof(C.c_void_p) == 8
 
 
