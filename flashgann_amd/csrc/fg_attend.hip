@@ -72,8 +72,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
             const char *src = P.q + (rq.q0 + static_cast<int64_t>(token)) * P.q_token + head * P.q_head + quarter * 16;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
-                uint4 v = {0, 0, 0, 0};
-                if (row < rq.rows) v = *reinterpret_cast<const uint4 *>(src + 64 * s);
+                u32x4 v = {0, 0, 0, 0};
+                if (row < rq.rows) v = *reinterpret_cast<const u32x4 *>(src + 64 * s);
                 qv[s] = __builtin_bit_cast(vec, v);
             }
         }
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
             }
             __syncthreads();
 
-            uint4 kr[2][STEPS], vr[2][STEPS];
+            u32x4 kr[2][STEPS], vr[2][STEPS];
             bool held[2];
             const auto load = [&](int32_t tile) {
 #pragma unroll
@@ -119,8 +119,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                     const char *vs = vbase + page * P.cache.v_page + at.y * P.cache.v_token;
 #pragma unroll
                     for (int s = 0; s < STEPS; ++s) {
-                        kr[b][s] = *reinterpret_cast<const uint4 *>(ks + 64 * s);
-                        vr[b][s] = *reinterpret_cast<const uint4 *>(vs + 64 * s);
+                        kr[b][s] = *reinterpret_cast<const u32x4 *>(ks + 64 * s);
+                        vr[b][s] = *reinterpret_cast<const u32x4 *>(vs + 64 * s);
                     }
                 }
             };
@@ -143,14 +143,14 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
 #pragma unroll
                     for (int k = 0; k < STEPS; ++k) {
                         // (a token without a page: whatever was read instead)
-                        uint4 v = held[b] ? vr[b][k] : uint4{0, 0, 0, 0};
+                        u32x4 v = held[b] ? vr[b][k] : u32x4{0, 0, 0, 0};
                         if (ragged && any_special<T>(v)) {
                             // 0 * inf is NaN: where not every row sees a token, infinities and NaNs
                             // are taken out of the product and added to the rows that see them
                             special = true;
                             v = finite_part<T>(v);
                         }
-                        *reinterpret_cast<uint4 *>(vmine + (16 * b + col) * VROW + 64 * k + 16 * quarter) = v;
+                        *reinterpret_cast<u32x4 *>(vmine + (16 * b + col) * VROW + 64 * k + 16 * quarter) = v;
                     }
                     if (ragged) {
                         uint64_t any = __ballot(special);
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                 }
                 // weights in the values' type: the matrix unit takes both alike, and
                 // the rounding of a weight is that of an output element
-                uint4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+                u32x4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
                 const vec pv = __builtin_bit_cast(vec, pk);
                 const char *vt = vmine + (4 * quarter + col / 4) * VROW + (col % 4) * 8;
 #pragma unroll
@@ -210,12 +210,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
 #pragma unroll
                     for (int i = 0; i < DB; ++i) {
                         const uint2 v = *reinterpret_cast<const uint2 *>(src + 32 * i);
-                        if (shown) {
-                            o[i][0] += special_part<T>(v.x & 0xFFFF);
-                            o[i][1] += special_part<T>(v.x >> 16);
-                            o[i][2] += special_part<T>(v.y & 0xFFFF);
-                            o[i][3] += special_part<T>(v.y >> 16);
-                        }
+                        o[i][0] += shown ? special_part<T>(v.x & 0xFFFF) : 0.0f;
+                        o[i][1] += shown ? special_part<T>(v.x >> 16) : 0.0f;
+                        o[i][2] += shown ? special_part<T>(v.y & 0xFFFF) : 0.0f;
+                        o[i][3] += shown ? special_part<T>(v.y >> 16) : 0.0f;
                     }
                 }
             }

@@ -29,6 +29,7 @@ typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 
@@ -68,31 +69,30 @@ __device__ __forceinline__ s16x4 read_transposed(const char *lds) {
 }
 
 template <class T>
-__device__ __forceinline__ bool any_special(uint4 w) {
+__device__ __forceinline__ bool any_special(u32x4 w) {
     bool s = false;
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        s |= (x[i] & T::kExponent) == T::kExponent || ((x[i] >> 16) & T::kExponent) == T::kExponent;
+        s |= ((w[i] & T::kExponent) == T::kExponent) | (((w[i] >> 16) & T::kExponent) == T::kExponent);
     return s;
 }
 
 // The same with its infinities and NaNs as zeros.
 template <class T>
-__device__ __forceinline__ uint4 finite_part(uint4 w) {
-    const auto part = [](uint32_t x) {
-        if ((x & T::kExponent) == T::kExponent) x &= 0xFFFF0000u;
-        if (((x >> 16) & T::kExponent) == T::kExponent) x &= 0x0000FFFFu;
-        return x;
-    };
-    return {part(w.x), part(w.y), part(w.z), part(w.w)};
+__device__ __forceinline__ u32x4 finite_part(u32x4 w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & T::kExponent) == T::kExponent) w[i] &= 0xFFFF0000u;
+        if (((w[i] >> 16) & T::kExponent) == T::kExponent) w[i] &= 0x0000FFFFu;
+    }
+    return w;
 }
 
 // An infinity or NaN among a value's 16 bits as a float, 0 for any other.
 template <class T>
 __device__ __forceinline__ float special_part(uint32_t x) {
-    if ((x & T::kExponent) != T::kExponent) return 0.0f;
-    return x & T::kMantissa ? NAN : x & 0x8000 ? -INFINITY : INFINITY;
+    const float inf = x & 0x8000 ? -INFINITY : INFINITY;
+    return (x & T::kExponent) != T::kExponent ? 0.0f : x & T::kMantissa ? NAN : inf;
 }
 
 struct AttendParams {

@@ -84,8 +84,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
             const char *src = P.q + qrow * P.q_token + head * P.q_head + half * 16;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
-                uint4 v = {0, 0, 0, 0};
-                if (row < rq.rows) v = *reinterpret_cast<const uint4 *>(src + 32 * s);
+                u32x4 v = {0, 0, 0, 0};
+                if (row < rq.rows) v = *reinterpret_cast<const u32x4 *>(src + 32 * s);
                 qv[s] = __builtin_bit_cast(vec, v);
             }
         }
@@ -123,15 +123,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
             return P.window == 0xFFFFFFFFu || t1 < sp.first || hi - position_of(sp, t0) < static_cast<int64_t>(P.window);
         };
 
-        uint4 kr[PER], vr[PER];
+        u32x4 kr[PER], vr[PER];
         const auto load = [&](int32_t i) {
 #pragma unroll
             for (uint32_t c = 0; c < PER; ++c) {
                 const uint32_t at = tid + c * THREADS, trow = at / CHUNKS, piece = at % CHUNKS;
                 if (kTile * CHUNKS % THREADS == 0 || at < kTile * CHUNKS) {
                     const longlong2 o = place[i % 4][trow];
-                    kr[c] = *reinterpret_cast<const uint4 *>(kbase + o.x + piece * 16);
-                    vr[c] = *reinterpret_cast<const uint4 *>(vbase + o.y + piece * 16);
+                    kr[c] = *reinterpret_cast<const u32x4 *>(kbase + o.x + piece * 16);
+                    vr[c] = *reinterpret_cast<const u32x4 *>(vbase + o.y + piece * 16);
                 }
             }
         };
@@ -143,15 +143,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
             for (uint32_t c = 0; c < PER; ++c) {
                 const uint32_t at = tid + c * THREADS, trow = at / CHUNKS, piece = at % CHUNKS;
                 if (kTile * CHUNKS % THREADS == 0 || at < kTile * CHUNKS) {
-                    uint4 v = vr[c];
+                    u32x4 v = vr[c];
                     // (a token without a page: whatever was read instead)
-                    if (there != ~0ull && !((there >> trow) & 1)) v = uint4{0, 0, 0, 0};
+                    if (there != ~0ull && !((there >> trow) & 1)) v = u32x4{0, 0, 0, 0};
                     if (edge && any_special<T>(v)) {
                         atomicOr(&special[i % 4], 1ull << trow);
                         v = finite_part<T>(v);
                     }
-                    *reinterpret_cast<uint4 *>(kbuf[i % 2] + trow * KROW + piece * 16) = kr[c];
-                    *reinterpret_cast<uint4 *>(vbuf[i % 2] + trow * VROW + piece * 16) = v;
+                    *reinterpret_cast<u32x4 *>(kbuf[i % 2] + trow * KROW + piece * 16) = kr[c];
+                    *reinterpret_cast<u32x4 *>(vbuf[i % 2] + trow * VROW + piece * 16) = v;
                 }
             }
         };
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
                     s[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
                     for (int k = 0; k < STEPS; ++k) {
-                        const uint4 a = *reinterpret_cast<const uint4 *>(kt + b * 32 * KROW + 32 * k);
+                        const u32x4 a = *reinterpret_cast<const u32x4 *>(kt + b * 32 * KROW + 32 * k);
                         s[b] = T::mfma32(__builtin_bit_cast(vec, a), qv[k], s[b]);
                     }
                 }
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
                     }
                     // weights in the values' type: the matrix unit takes both alike, and
                     // the rounding of a weight is that of an output element
-                    const uint4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+                    const u32x4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
                     pv[c] = __builtin_bit_cast(vec, pk);
                 }
                 const char *vt = vbuf[i % 2] + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
@@ -257,12 +257,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uint2 v = *reinterpret_cast<const uint2 *>(src + 64 * d + 16 * k);
-                            if (shown) {
-                                o[d][4 * k] += special_part<T>(v.x & 0xFFFF);
-                                o[d][4 * k + 1] += special_part<T>(v.x >> 16);
-                                o[d][4 * k + 2] += special_part<T>(v.y & 0xFFFF);
-                                o[d][4 * k + 3] += special_part<T>(v.y >> 16);
-                            }
+                            o[d][4 * k] += shown ? special_part<T>(v.x & 0xFFFF) : 0.0f;
+                            o[d][4 * k + 1] += shown ? special_part<T>(v.x >> 16) : 0.0f;
+                            o[d][4 * k + 2] += shown ? special_part<T>(v.y & 0xFFFF) : 0.0f;
+                            o[d][4 * k + 3] += shown ? special_part<T>(v.y >> 16) : 0.0f;
                         }
                 }
             }
