@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
     __shared__ int2 place[kPlaces];
     __shared__ float wave_m[4][kRows], wave_l[4][kRows];
 
-    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, col = lane % 16, quarter = lane / 16;
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 16, quarter = lane / 16;
     const uint32_t w = blockIdx.x;
     const Start start = find_start<FOUND, kRows>(P, w);
     if (P.join && tid == 0) P.joins[w].pieces = 0;
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
     char *const vmine = vbuf[wave];
 
     for (uint64_t x = w * start.share; x < x1;) {
-        const Request rq = request_of<FOUND, kRows>(P, r);
+        const Request rq = uniform_request<FOUND, kRows>(P, r);
         const uint64_t all = rq.weight_of(rq.blocks) * P.lists;
         if (x >= before + all) {
             before += all;

@@ -167,6 +167,21 @@ __device__ __forceinline__ float add_other32(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// A value that all lanes hold alike, into scalar registers: what describes an item
+// lives through its whole loop.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x));
+}
+
+// The same value, as far as the compiler knows another: what follows from it is
+// worked out again instead of being kept in registers.
+__device__ __forceinline__ int32_t renewed(int32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ int32_t clampi(int32_t v, int32_t lo, int32_t hi) { return min(max(v, lo), hi); }
 
 template <bool FOUND, uint32_t ROWS>
@@ -200,7 +215,7 @@ __device__ __forceinline__ Request request_of(const AttendParams &P, uint32_t r)
 template <bool FOUND, uint32_t ROWS>
 __device__ __forceinline__ Span span_of(const AttendParams &P, const Request &q, uint32_t block) {
     const int32_t row0 = static_cast<int32_t>(block * ROWS), row1 = min(row0 + static_cast<int32_t>(ROWS), q.rows) - 1;
-    const int32_t t0 = P.group.div(row0), t1 = P.group.div(row1);
+    const int32_t t0 = uniform(static_cast<int32_t>(P.group.div(row0))), t1 = uniform(static_cast<int32_t>(P.group.div(row1)));
     Span s;
     s.pos0 = q.kv - q.fresh;
     const int32_t end = clampi(s.pos0 + t1 + 1, 0, q.limit);
@@ -238,6 +253,20 @@ __device__ __forceinline__ bool sees(const AttendParams &P, int32_t pos, int32_t
     return (back >= 0) & ((static_cast<uint32_t>(back) < P.window) | (static_cast<uint32_t>(j) < P.sinks));
 }
 
+// The request of every lane's `r`, which is the same.
+template <bool FOUND, uint32_t ROWS>
+__device__ __forceinline__ Request uniform_request(const AttendParams &P, uint32_t r) {
+    Request q = request_of<FOUND, ROWS>(P, r);
+    q.q0 = uniform(q.q0);
+    q.fresh = uniform(q.fresh);
+    q.rows = uniform(q.rows);
+    q.kv = uniform(q.kv);
+    q.limit = uniform(q.limit);
+    q.blocks = uniform(q.blocks);
+    q.base = uniform(q.base);
+    return q;
+}
+
 // Where a workgroup's share begins.
 struct Start {
     uint64_t all, share;  // weight of all items; of a workgroup
@@ -265,13 +294,13 @@ __device__ __forceinline__ Start find_start(const AttendParams &P, uint32_t w) {
         if (lane >= d) upto += o;
     }
     Start s;
-    s.all = __shfl(upto, 63);
+    s.all = uniform(static_cast<uint64_t>(__shfl(upto, 63)));
     s.share = max((s.all + P.workgroups - 1) >> __builtin_ctz(P.workgroups), P.least);
     const uint64_t x = w * s.share;
     const uint64_t at = __ballot(upto > x && upto - mine <= x);
     const uint32_t owner = at ? __ffsll(static_cast<unsigned long long>(at)) - 1 : 0;
-    s.before = __shfl(upto - mine, owner);
-    s.request = owner * run;
+    s.before = uniform(static_cast<uint64_t>(__shfl(upto - mine, owner)));
+    s.request = uniform(owner * run);
     return s;
 }
 
@@ -315,12 +344,12 @@ __device__ __forceinline__ Piece piece_of(const AttendParams &P, const Request &
     const uint64_t begin = start + q.weight_of(lo), weight = q.weight_of(lo + 1) - q.weight_of(lo);
     p.end = begin + weight;
     *span = span_of<FOUND, ROWS>(P, q, lo);
-    const uint32_t total = span->total, units = max(P.unit.div(total + P.unit.d - 1), 1u);
+    const uint32_t total = span->total, units = uniform(max(P.unit.div(total + P.unit.d - 1), 1u));
     // x, and x1 inside the item, fall into units 0 .. units - 1: the workgroup that holds the
     // item's end holds its last unit, and an item of one unit is never cut
     const float per = static_cast<float>(units) * __builtin_amdgcn_rcpf(static_cast<float>(weight));
-    const uint32_t u0 = min(static_cast<uint32_t>(static_cast<float>(x - begin) * per), units - 1);
-    const uint32_t u1 = x1 >= p.end ? units : min(static_cast<uint32_t>(static_cast<float>(x1 - begin) * per), units - 1);
+    const uint32_t u0 = uniform(min(static_cast<uint32_t>(static_cast<float>(x - begin) * per), units - 1));
+    const uint32_t u1 = x1 >= p.end ? units : uniform(min(static_cast<uint32_t>(static_cast<float>(x1 - begin) * per), units - 1));
     p.begins = u0 == 0;
     p.ends = u1 == units;
     p.none = u1 == 0;

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
     __shared__ uint64_t held[4];
     __shared__ unsigned long long special[4];
 
-    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, col = lane % 32, half = lane / 32;
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 32, half = lane / 32;
     const uint32_t W = gridDim.x;
     // neighbours in weight, which read the same keys, on one die of eight (the
     // grid is a multiple of 8)
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
     uint32_t r = start.request;
 
     for (uint64_t x = w * start.share; x < x1;) {
-        const Request rq = request_of<false, ROWS>(P, r);
+        const Request rq = uniform_request<false, ROWS>(P, r);
         const uint64_t all = rq.weight_of(rq.blocks) * P.lists;
         if (x >= before + all) {
             before += all;
@@ -74,13 +74,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
         const int32_t row = row_first + static_cast<int32_t>(col);
         const int32_t token = P.group.div(row);
         const int32_t pos = sp.pos0 + token;
-        const int32_t pos_lo = sp.pos0 + static_cast<int32_t>(P.group.div(row_first));
-        const int32_t pos_hi = sp.pos0 + static_cast<int32_t>(P.group.div(min(row_first + 31, max(rq.rows - 1, row_first))));
-        const int32_t block_lo = sp.pos0 + static_cast<int32_t>(P.group.div(pc.block * ROWS));
-        const int64_t head = static_cast<int64_t>(pc.list) * P.group.d + (row - token * static_cast<int32_t>(P.group.d));
-        const int64_t qrow = rq.q0 + static_cast<int64_t>(token);
+        const int32_t pos_lo = uniform(sp.pos0 + static_cast<int32_t>(P.group.div(row_first)));
+        const int32_t pos_hi = uniform(sp.pos0 + static_cast<int32_t>(P.group.div(min(row_first + 31, max(rq.rows - 1, row_first)))));
+        const int32_t block_lo = uniform(sp.pos0 + static_cast<int32_t>(P.group.div(pc.block * ROWS)));
         vec qv[STEPS];
         {
+            const int64_t head = static_cast<int64_t>(pc.list) * P.group.d + (row - token * static_cast<int32_t>(P.group.d));
+            const int64_t qrow = rq.q0 + static_cast<int64_t>(token);
             const char *src = P.q + qrow * P.q_token + head * P.q_head + half * 16;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
@@ -135,9 +135,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
                 }
             }
         };
-        const int32_t block_hi = sp.pos0 + static_cast<int32_t>(P.group.div(min(pc.block * ROWS + ROWS, static_cast<uint32_t>(rq.rows)) - 1));
+        const int32_t block_hi = uniform(sp.pos0 + static_cast<int32_t>(P.group.div(min(pc.block * ROWS + ROWS, static_cast<uint32_t>(rq.rows)) - 1)));
         const auto store = [&](int32_t i) {
-            const uint64_t there = held[i % 4];
+            const uint64_t there = uniform(held[i % 4]);
             const bool edge = !whole_tile(i, block_lo, block_hi);
 #pragma unroll
             for (uint32_t c = 0; c < PER; ++c) {
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
             if (wave == static_cast<uint32_t>(i + 3) % NW) look(i + 3);
 
             const int32_t t0 = t_lo + i * static_cast<int32_t>(kTile);
-            const uint64_t there = held[i % 4];
+            const uint64_t there = uniform(held[i % 4]);
             if (position_of(sp, t0) <= pos_hi && row_first < rq.rows) {
                 // scores: register i of s[b] is token 32 b + 8 (i / 4) + 4 half + i % 4
                 f32x16 s[2];
@@ -193,6 +193,14 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
                         s[b] = T::mfma32(__builtin_bit_cast(vec, a), qv[k], s[b]);
                     }
                 }
+                // LDS reads run four products ahead
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+                for (int k = 0; k < 2 * STEPS - 4; ++k) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
                 if (there != ~0ull || !whole_tile(i, pos_lo, pos_hi)) {
                     uint32_t see = 0;  // bit 16 b + i: whether the row sees the token of s[b][i]
 #pragma unroll
@@ -225,9 +233,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
                     m = top;
                 }
                 const float base = m == -INFINITY ? 0.0f : -m * P.scale2;
-                vec pv[4];
+                const char *vt = vbuf[i % 2] + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
+                    s16x8 a[DB];
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        const s16x4 a0 = read_transposed(vt + 16 * c * VROW + 64 * d), a1 = read_transposed(vt + (16 * c + 8) * VROW + 64 * d);
+                        a[d] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    }
                     float p[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
@@ -237,19 +251,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
                     // weights in the values' type: the matrix unit takes both alike, and
                     // the rounding of a weight is that of an output element
                     const u32x4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
-                    pv[c] = __builtin_bit_cast(vec, pk);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) o[d] = T::mfma32(__builtin_bit_cast(vec, a[d]), __builtin_bit_cast(vec, pk), o[d]);
                 }
-                const char *vt = vbuf[i % 2] + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const s16x4 a0 = read_transposed(vt + 16 * c * VROW + 64 * d), a1 = read_transposed(vt + (16 * c + 8) * VROW + 64 * d);
-                        const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-                        o[d] = T::mfma32(__builtin_bit_cast(vec, a), pv[c], o[d]);
-                    }
-                for (unsigned long long odd = special[i % 4]; odd; odd &= odd - 1) {
-                    const int at = __ffsll(odd) - 1;
+                for (uint64_t odd = uniform(static_cast<uint64_t>(special[i % 4])); odd; odd &= odd - 1) {
+                    const int at = __ffsll(static_cast<unsigned long long>(odd)) - 1;
                     const char *src = vbase + place[i % 4][at].y + half * 8;
                     const bool shown = sees(P, pos, position_of(sp, t0 + at));
 #pragma unroll
@@ -271,7 +277,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
         l = add_other32(l);
         const bool whole = pc.begins && pc.ends;
         const float top = m == -INFINITY ? m : m * P.scale2;
-        if (row < rq.rows) {
+        const int32_t out_row = renewed(row);
+        if (out_row < rq.rows) {
+            const int32_t t = P.group.div(out_row);
+            const int64_t head = static_cast<int64_t>(pc.list) * P.group.d + (out_row - t * static_cast<int32_t>(P.group.d));
+            const int64_t qrow = rq.q0 + static_cast<int64_t>(t);
             if (whole) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 char *dst = P.out + qrow * P.out_token + head * P.out_head + half * 8;
@@ -284,7 +294,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
                 if (P.lse && half == 0) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
             } else {
                 const uint32_t slot = 2 * w + (pc.begins ? 1 : 0);
-                const uint64_t at = static_cast<uint64_t>(slot) * ROWS + wave * 32 + col;
+                const uint64_t at = static_cast<uint64_t>(slot) * ROWS + (out_row - static_cast<int32_t>(pc.block * ROWS));
                 float *dst = P.part + at * D + half * 4;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
