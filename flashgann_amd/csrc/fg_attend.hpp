@@ -175,6 +175,11 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
     return static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x));
 }
 
+// Waits for every load from global memory.  Where loads on one path into a loop are
+// not known to have landed, the compiler waits for all of them inside it, those
+// under way for the next tile with them.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // The same value, as far as the compiler knows another: what follows from it is
 // worked out again instead of being kept in registers.
 __device__ __forceinline__ int32_t renewed(int32_t x) {

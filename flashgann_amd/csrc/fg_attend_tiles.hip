@@ -23,7 +23,7 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 template <class T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams P) {
+__global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void fg_tiles_kernel(AttendParams P) {
     using vec = typename T::vec;
     constexpr uint32_t THREADS = 64 * NW, ROWS = 32 * NW;
     constexpr int STEPS = D / 16, DB = D / 32, CHUNKS = D / 8;   // 16-byte pieces of a row
@@ -172,11 +172,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
             load(0);
             store(0);
         }
+        wait_loads();
         for (int32_t i = 0; i < tiles; ++i) {
             lds_barrier();
-            if (i + 1 < tiles) load(i + 1);
+            // (places first: what waits for the table must not wait for the tile)
             if (wave == static_cast<uint32_t>(i + 2) % NW) note(i + 2);
             if (wave == static_cast<uint32_t>(i + 3) % NW) look(i + 3);
+            if (i + 1 < tiles) load(i + 1);
 
             const int32_t t0 = t_lo + i * static_cast<int32_t>(kTile);
             const uint64_t there = uniform(held[i % 4]);
@@ -268,6 +270,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void fg_tiles_kernel(AttendParams 
                             o[d][4 * k + 2] += shown ? special_part<T>(v.y & 0xFFFF) : 0.0f;
                             o[d][4 * k + 3] += shown ? special_part<T>(v.y >> 16) : 0.0f;
                         }
+                    wait_loads();
                 }
             }
             if (i + 1 < tiles) store(i + 1);
