@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             }
         };
 
-        float m = -INFINITY, l = 0.0f;  // m: of the scores before scaling
+        float m = -INFINITY, l = 0.0f, l2 = 0.0f;  // m: of the scores before scaling; the sum is l + l2
         f32x16 o[DB];
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -186,23 +186,21 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 // scores: register i of s[b] is token 32 b + 8 (i / 4) + 4 half + i % 4
                 f32x16 s[2];
                 const char *kt = kbuf[i % 2] + col * KROW + half * 16;
+                // (the compiler would read for one product at a time: reads run AHEAD products
+                // ahead, held there by the barriers for its scheduler)
+                constexpr int AHEAD = 4;
+                u32x4 kq[AHEAD];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    s[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                for (int k = 0; k < AHEAD; ++k) kq[k] = *reinterpret_cast<const u32x4 *>(kt + 32 * k);
+                s[0] = s[1] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int k = 0; k < STEPS; ++k) {
-                        const u32x4 a = *reinterpret_cast<const u32x4 *>(kt + b * 32 * KROW + 32 * k);
-                        s[b] = T::mfma32(__builtin_bit_cast(vec, a), qv[k], s[b]);
-                    }
+                for (int k = 0; k < 2 * STEPS; ++k) {
+                    s[k / STEPS] = T::mfma32(__builtin_bit_cast(vec, kq[k % AHEAD]), qv[k % STEPS], s[k / STEPS]);
+                    const int n = k + AHEAD;
+                    if (n < 2 * STEPS) kq[k % AHEAD] = *reinterpret_cast<const u32x4 *>(kt + n / STEPS * 32 * KROW + 32 * (n % STEPS));
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                // LDS reads run four products ahead
-                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-                for (int k = 0; k < 2 * STEPS - 4; ++k) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
                 if (there != ~0ull || !whole_tile(i, pos_lo, pos_hi)) {
                     uint32_t see = 0;  // bit 16 b + i: whether the row sees the token of s[b][i]
 #pragma unroll
@@ -230,31 +228,47 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                     const float from = m == -INFINITY ? top : m;
                     const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((from - top) * P.scale2);
                     l *= shrink;
+                    l2 *= shrink;
 #pragma unroll
                     for (int k = 0; k < DB; ++k) o[k] *= shrink;
                     m = top;
                 }
                 const float base = m == -INFINITY ? 0.0f : -m * P.scale2;
                 const char *vt = vbuf[i % 2] + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
+                // product d of step c adds 16 tokens to 32 dimensions; while the matrix unit is at
+                // it, two weights of the next step are worked out and its values read
+                s16x8 a[2][DB];
+                u32x4 pk[2];
+                const auto read = [&](int c, int d) {
+                    const s16x4 a0 = read_transposed(vt + 16 * c * VROW + 64 * d), a1 = read_transposed(vt + (16 * c + 8) * VROW + 64 * d);
+                    a[c % 2][d] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                };
+                // weights in the values' type: the matrix unit takes both alike, and the
+                // rounding of a weight is that of an output element
+                const auto weigh = [&](int c, int k) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[c / 2][8 * (c % 2) + 2 * k], P.scale2, base));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[c / 2][8 * (c % 2) + 2 * k + 1], P.scale2, base));
+                    l += p0;
+                    l2 += p1;
+                    pk[c % 2][k] = T::pack(p0, p1);
+                };
+#pragma unroll
+                for (int d = 0; d < DB; ++d) read(0, d);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) weigh(0, k);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    s16x8 a[DB];
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
-                        const s16x4 a0 = read_transposed(vt + 16 * c * VROW + 64 * d), a1 = read_transposed(vt + (16 * c + 8) * VROW + 64 * d);
-                        a[d] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    }
-                    float p[8];
+                        o[d] = T::mfma32(__builtin_bit_cast(vec, a[c % 2][d]), __builtin_bit_cast(vec, pk[c % 2]), o[d]);
+                        if (c < 3) {
+                            read(c + 1, d);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        p[k] = __builtin_amdgcn_exp2f(fmaf(s[c / 2][8 * (c % 2) + k], P.scale2, base));
-                        l += p[k];
+                            for (int k = d * 4 / DB; k < (d + 1) * 4 / DB; ++k) weigh(c + 1, k);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    // weights in the values' type: the matrix unit takes both alike, and
-                    // the rounding of a weight is that of an output element
-                    const u32x4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) o[d] = T::mfma32(__builtin_bit_cast(vec, a[d]), __builtin_bit_cast(vec, pk), o[d]);
                 }
                 for (uint64_t odd = uniform(static_cast<uint64_t>(special[i % 4])); odd; odd &= odd - 1) {
                     const int at = __ffsll(static_cast<unsigned long long>(odd)) - 1;
@@ -277,7 +291,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         }
         lds_barrier();
 
-        l = add_other32(l);
+        l = add_other32(l + l2);
         const bool whole = pc.begins && pc.ends;
         const float top = m == -INFINITY ? m : m * P.scale2;
         const int32_t out_row = renewed(row);
