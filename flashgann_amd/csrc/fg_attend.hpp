@@ -252,6 +252,17 @@ __device__ __forceinline__ uint32_t workgroup_at(uint64_t x, uint64_t share) {
     return static_cast<uint32_t>(w);
 }
 
+// The n lowest bits; none below 0, all from 64 on.
+__device__ __forceinline__ uint64_t bits_below(int32_t n) {
+    return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+}
+
+// x where bit `at` of `bits` is set, else -infinity.
+__device__ __forceinline__ float keep_if(uint32_t bits, int at, float x) {
+    const uint32_t all = static_cast<int32_t>(bits << (31 - at)) >> 31;
+    return __uint_as_float((__float_as_uint(x) & all) | (0xFF800000u & ~all));
+}
+
 // Whether the row at `pos` sees the token at position j (pages aside).
 __device__ __forceinline__ bool sees(const AttendParams &P, int32_t pos, int32_t j) {
     const int32_t back = pos - j;

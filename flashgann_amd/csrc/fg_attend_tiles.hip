@@ -2,10 +2,15 @@
 // rows (chunks of prompts): bound by the matrix unit and the softmax beside it.
 //
 // A wave holds 32 query rows, one in each lane's column; the workgroup's waves
-// share tiles of 64 tokens, two of them in LDS, the next one's keys and values on
+// share tiles of 64 tokens in LDS, two of keys and two of values, the next ones on
 // their way through registers.  Per tile a wave does 2 x D/16 products of 32 keys x
 // 16 dimensions for the scores and 4 x D/32 of 32 dimensions x 16 keys for the
 // output; rows of the same wave reuse what it reads from LDS.
+//
+// The matrix unit and the softmax take about as long (at dim 128 and a tile 1024 and
+// 960 cycles a wave), and one wave issues a vector instruction every eight cycles at
+// best.  So a wave works out the weights of one tile between its products for the
+// scores of the next.
 #include "fg_attend.hpp"
 
 namespace fgk {
@@ -33,13 +38,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
     constexpr uint32_t KROW = 2 * D + 16, VROW = 2 * D + (D == 96 ? 128 : 64);
     __shared__ __attribute__((aligned(16))) char kbuf[2][kTile * KROW];
     __shared__ __attribute__((aligned(16))) char vbuf[2][kTile * VROW];
-    // of tile i at i % 4: where its tokens lie (bytes from the head's first key and
+    // of tile i at i % 8: where its tokens lie (bytes from the head's first key and
     // value), which of them there are, and in a tile that not every row sees which
     // hold an infinite or NaN value: 0 * inf is NaN, so those are taken out of the
     // product and added to the rows that see them
-    __shared__ longlong2 place[4][kTile];
-    __shared__ uint64_t held[4];
-    __shared__ unsigned long long special[4];
+    __shared__ longlong2 place[8][kTile];
+    __shared__ uint64_t held[8];
+    __shared__ unsigned long long special[8];
 
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 32, half = lane / 32;
     const uint32_t W = gridDim.x;
@@ -93,7 +98,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         const char *const vbase = P.cache.v + pc.list * P.cache.v_head;
 
         // The places of tile i are looked up by wave i % NW: the table is read at
-        // tile i - 3 and the place written at tile i - 2, so nothing waits for it.
+        // step i - 5 and the place written at step i - 4, so nothing waits for it.
         int32_t page = -1;
         uint32_t offset = 0;
         const auto look = [&](int32_t i) {
@@ -109,13 +114,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         const auto note = [&](int32_t i) {
             const bool have = static_cast<uint32_t>(page) < P.cache.pages;
             const int64_t p = have ? page : 0, o = have ? offset : 0;
-            place[i % 4][lane] = longlong2{p * P.cache.k_page + o * P.cache.k_token, p * P.cache.v_page + o * P.cache.v_token};
+            place[i % 8][lane] = longlong2{p * P.cache.k_page + o * P.cache.k_token, p * P.cache.v_page + o * P.cache.v_token};
             const uint64_t there = __ballot(have);
             if (lane == 0) {
-                held[i % 4] = there;
-                special[i % 4] = 0;
+                held[i % 8] = there;
+                special[i % 8] = 0;
             }
         };
+        const int32_t shift = sp.from - sp.first;  // position less token number past the first ones
+        const int32_t window = static_cast<int32_t>(min(P.window, 0x7FFFFFFFu));
         // whether every row of the workgroup sees all tokens of tile i, pages aside
         const auto whole_tile = [&](int32_t i, int32_t lo, int32_t hi) {
             const int32_t t0 = t_lo + i * static_cast<int32_t>(kTile), t1 = min(t0 + static_cast<int32_t>(kTile), t_hi) - 1;
@@ -124,34 +131,49 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         };
 
         u32x4 kr[PER], vr[PER];
-        const auto load = [&](int32_t i) {
+        // where this thread's pieces of a tile's keys (values) lie
+        int64_t k_at[PER], v_at[PER];
+        const auto find_k = [&](int32_t i) {
+#pragma unroll
+            for (uint32_t c = 0; c < PER; ++c) k_at[c] = place[i % 8][min((tid + c * THREADS) / CHUNKS, kTile - 1)].x + (tid + c * THREADS) % CHUNKS * 16;
+        };
+        const auto find_v = [&](int32_t i) {
+#pragma unroll
+            for (uint32_t c = 0; c < PER; ++c) v_at[c] = place[i % 8][min((tid + c * THREADS) / CHUNKS, kTile - 1)].y + (tid + c * THREADS) % CHUNKS * 16;
+        };
+        const auto load_k = [&]() {
+#pragma unroll
+            for (uint32_t c = 0; c < PER; ++c)
+                if (kTile * CHUNKS % THREADS == 0 || tid + c * THREADS < kTile * CHUNKS) kr[c] = *reinterpret_cast<const u32x4 *>(kbase + k_at[c]);
+        };
+        const auto load_v = [&]() {
+#pragma unroll
+            for (uint32_t c = 0; c < PER; ++c)
+                if (kTile * CHUNKS % THREADS == 0 || tid + c * THREADS < kTile * CHUNKS) vr[c] = *reinterpret_cast<const u32x4 *>(vbase + v_at[c]);
+        };
+        const auto store_k = [&](int32_t i) {
 #pragma unroll
             for (uint32_t c = 0; c < PER; ++c) {
-                const uint32_t at = tid + c * THREADS, trow = at / CHUNKS, piece = at % CHUNKS;
-                if (kTile * CHUNKS % THREADS == 0 || at < kTile * CHUNKS) {
-                    const longlong2 o = place[i % 4][trow];
-                    kr[c] = *reinterpret_cast<const u32x4 *>(kbase + o.x + piece * 16);
-                    vr[c] = *reinterpret_cast<const u32x4 *>(vbase + o.y + piece * 16);
-                }
+                const uint32_t at = tid + c * THREADS;
+                if (kTile * CHUNKS % THREADS == 0 || at < kTile * CHUNKS)
+                    *reinterpret_cast<u32x4 *>(kbuf[i % 2] + at / CHUNKS * KROW + at % CHUNKS * 16) = kr[c];
             }
         };
         const int32_t block_hi = uniform(sp.pos0 + static_cast<int32_t>(P.group.div(min(pc.block * ROWS + ROWS, static_cast<uint32_t>(rq.rows)) - 1)));
-        const auto store = [&](int32_t i) {
-            const uint64_t there = uniform(held[i % 4]);
+        const auto store_v = [&](int32_t i, uint64_t there) {
             const bool edge = !whole_tile(i, block_lo, block_hi);
 #pragma unroll
             for (uint32_t c = 0; c < PER; ++c) {
-                const uint32_t at = tid + c * THREADS, trow = at / CHUNKS, piece = at % CHUNKS;
+                const uint32_t at = tid + c * THREADS, trow = at / CHUNKS;
                 if (kTile * CHUNKS % THREADS == 0 || at < kTile * CHUNKS) {
                     u32x4 v = vr[c];
                     // (a token without a page: whatever was read instead)
                     if (there != ~0ull && !((there >> trow) & 1)) v = u32x4{0, 0, 0, 0};
                     if (edge && any_special<T>(v)) {
-                        atomicOr(&special[i % 4], 1ull << trow);
+                        atomicOr(&special[i % 8], 1ull << trow);
                         v = finite_part<T>(v);
                     }
-                    *reinterpret_cast<u32x4 *>(kbuf[i % 2] + trow * KROW + piece * 16) = kr[c];
-                    *reinterpret_cast<u32x4 *>(vbuf[i % 2] + trow * VROW + piece * 16) = v;
+                    *reinterpret_cast<u32x4 *>(vbuf[i % 2] + trow * VROW + at % CHUNKS * 16) = v;
                 }
             }
         };
@@ -161,122 +183,118 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
-        // (the last item's readers of LDS are past: see the barrier at the end)
-        if (tiles > 0) {
-            if (wave < 2) {
-                look(wave);
-                note(wave);
-            }
-            if (wave == 2 % NW) look(2);
-            lds_barrier();
-            load(0);
-            store(0);
-        }
-        wait_loads();
-        for (int32_t i = 0; i < tiles; ++i) {
-            lds_barrier();
-            // (places first: what waits for the table must not wait for the tile)
-            if (wave == static_cast<uint32_t>(i + 2) % NW) note(i + 2);
-            if (wave == static_cast<uint32_t>(i + 3) % NW) look(i + 3);
-            if (i + 1 < tiles) load(i + 1);
+        // Scores: register i of s[b] is that of token 32 b + 8 (i / 4) + 4 half + i % 4.
+        // Two tiles': one's are weighed while the other's are worked out.
+        f32x16 s_even[2], s_odd[2];
+        float top = -INFINITY;  // the largest of the next tile to be weighed
+        uint64_t there = 0;     // its tokens
+        u32x4 pk[4];            // the weights of 16 tokens each
+        // Two weights of 32.  In the values' type: the matrix unit takes both alike, and
+        // the rounding of a weight is that of an output element.
+        const auto weigh = [&](const f32x16 *s, int k, float base) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[k / 8][2 * (k % 8)], P.scale2, base));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[k / 8][2 * (k % 8) + 1], P.scale2, base));
+            l += p0;
+            l2 += p1;
+            asm volatile("" : "+v"(l), "+v"(l2));  // here, not when the sums are next looked at
+            pk[k / 4][k % 4] = T::pack(p0, p1);
+        };
+        const auto read_key = [&](int32_t i, int n) {
+            return *reinterpret_cast<const u32x4 *>(kbuf[i % 2] + (n / STEPS * 32 + col) * KROW + half * 16 + 32 * (n % STEPS));
+        };
+        // (the compiler would read for one product at a time and gather the rest: LDS
+        // reads run AHEAD products ahead, held there by the barriers for its scheduler)
+        constexpr int AHEAD = 4;
 
+        // An even number of steps: the last may find no token.
+        const int32_t steps = (tiles + 1) & ~1;
+        const auto step = [&](int32_t i, f32x16 *s, f32x16 *next) {
+            lds_barrier();
+            if (wave == static_cast<uint32_t>(i + 4) % NW) note(i + 4);
+            if (wave == static_cast<uint32_t>(i + 5) % NW) look(i + 5);
+            // LDS gets the next tile's values and the keys of the one after (past the last
+            // tile what lies in page 0), whose places in it are read.  No branch among
+            // the products below: the compiler would gather the weights behind it.
+            find_v(i + 2);
+            const uint64_t there_next = uniform(held[(i + 1) % 8]);
+            store_v(i + 1, there_next);
             const int32_t t0 = t_lo + i * static_cast<int32_t>(kTile);
-            const uint64_t there = uniform(held[i % 4]);
-            if (position_of(sp, t0) <= pos_hi && row_first < rq.rows) {
-                // scores: register i of s[b] is token 32 b + 8 (i / 4) + 4 half + i % 4
-                f32x16 s[2];
-                const char *kt = kbuf[i % 2] + col * KROW + half * 16;
-                // (the compiler would read for one product at a time: reads run AHEAD products
-                // ahead, held there by the barriers for its scheduler)
-                constexpr int AHEAD = 4;
-                u32x4 kq[AHEAD];
+            if (there != ~0ull || !whole_tile(i, pos_lo, pos_hi)) {
+                // the tile's tokens that the row sees, then the lane's: four of every eight
+                const uint64_t seen = there & (bits_below(sp.first - t0) & bits_below(pos + 1 - t0) |
+                                               bits_below(pos + 1 - shift - t0) & ~bits_below(max(pos - window, -1) + 1 - shift - t0) & ~bits_below(sp.first - t0));
+                const uint64_t mine = seen >> (4 * half);
+                top = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) kq[k] = *reinterpret_cast<const u32x4 *>(kt + 32 * k);
-                s[0] = s[1] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                for (int k = 0; k < 32; ++k) {
+                    const int at = 8 * (k % 16 / 4) + k % 4;  // in its half of the tile
+                    s[k / 16][k % 16] = keep_if(static_cast<uint32_t>(mine >> (k / 16 * 32)), at, s[k / 16][k % 16]);
+                    top = fmaxf(top, s[k / 16][k % 16]);
+                }
+            }
+            top = fmaxf(m, max_other32(top));
+            // the maximum follows when a row's grows by more than 2^8: weights stay
+            // below that, and the sums are no less exact for it
+            if (__any((top - m) * P.scale2 > 8.0f)) {
+                const float from = m == -INFINITY ? top : m;
+                const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((from - top) * P.scale2);
+                l *= shrink;
+                l2 *= shrink;
+#pragma unroll
+                for (int k = 0; k < DB; ++k) o[k] *= shrink;
+                m = top;
+            }
+            const float base = m == -INFINITY ? 0.0f : -m * P.scale2;
+
+            // the scores of the next tile (after the last one, of what LDS holds: unused), the
+            // weights of this one between the products
+            u32x4 kq[AHEAD];
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) kq[n] = read_key(i + 1, n);
+            next[0] = next[1] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2 * STEPS; ++k) {
+                next[k / STEPS] = T::mfma32(__builtin_bit_cast(vec, kq[k % AHEAD]), qv[k % STEPS], next[k / STEPS]);
+                if (k + AHEAD < 2 * STEPS) kq[k % AHEAD] = read_key(i + 1, k + AHEAD);
+#pragma unroll
+                for (int j = k * 16 / (2 * STEPS); j < (k + 1) * 16 / (2 * STEPS); ++j) weigh(s, j, base);
+                if (k == 1) load_v();
+                if (k == 2) store_k(i + 2);
+                if (k == 3) find_k(i + 3);
+                if (k == 7) load_k();
                 __builtin_amdgcn_sched_barrier(0);
+            }
+
+            // this tile's values: product n adds 16 tokens, n / DB, to 32 dimensions; the
+            // next scores' maximum between the products
+            const char *vt = vbuf[i % 2] + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
+            constexpr int N = 4 * DB;
+            s16x8 a[AHEAD];
+            const auto read_values = [&](int n) {
+                const char *at = vt + 16 * (n / DB) * VROW + 64 * (n % DB);
+                return __builtin_shufflevector(read_transposed(at), read_transposed(at + 8 * VROW), 0, 1, 2, 3, 4, 5, 6, 7);
+            };
 #pragma unroll
-                for (int k = 0; k < 2 * STEPS; ++k) {
-                    s[k / STEPS] = T::mfma32(__builtin_bit_cast(vec, kq[k % AHEAD]), qv[k % STEPS], s[k / STEPS]);
-                    const int n = k + AHEAD;
-                    if (n < 2 * STEPS) kq[k % AHEAD] = *reinterpret_cast<const u32x4 *>(kt + n / STEPS * 32 * KROW + 32 * (n % STEPS));
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (there != ~0ull || !whole_tile(i, pos_lo, pos_hi)) {
-                    uint32_t see = 0;  // bit 16 b + i: whether the row sees the token of s[b][i]
+            for (int n = 0; n < AHEAD; ++n) a[n] = read_values(n);
+            top = -INFINITY;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const int at = 32 * (k / 16) + 8 * (k % 16 / 4) + k % 4;
-                        see |= static_cast<uint32_t>(sees(P, pos, position_of(sp, t0 + at + 4 * static_cast<int32_t>(half)))) << k;
-                    }
-                    // the lane's tokens of each half of the tile, four of every eight
-                    const uint64_t mine = there >> (4 * half);
+            for (int n = 0; n < N; ++n) {
+                o[n % DB] = T::mfma32(__builtin_bit_cast(vec, a[n % AHEAD]), __builtin_bit_cast(vec, pk[n / DB]), o[n % DB]);
+                if (n + AHEAD < N) a[n % AHEAD] = read_values(n + AHEAD);
 #pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        const uint32_t four = static_cast<uint32_t>(mine >> (8 * g)) & 15u;
-                        see &= (four << (4 * g)) | ~(15u << (4 * g));
-                    }
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) s[k / 16][k % 16] = (see >> k) & 1 ? s[k / 16][k % 16] : -INFINITY;
-                }
-                float top = s[0][0];
-#pragma unroll
-                for (int k = 1; k < 32; ++k) top = fmaxf(top, s[k / 16][k % 16]);
-                top = fmaxf(m, max_other32(top));
-                // the maximum follows when a row's grows by more than 2^8: weights stay
-                // below that, and the sums are no less exact for it
-                if (__any((top - m) * P.scale2 > 8.0f)) {
-                    const float from = m == -INFINITY ? top : m;
-                    const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((from - top) * P.scale2);
-                    l *= shrink;
-                    l2 *= shrink;
-#pragma unroll
-                    for (int k = 0; k < DB; ++k) o[k] *= shrink;
-                    m = top;
-                }
-                const float base = m == -INFINITY ? 0.0f : -m * P.scale2;
-                const char *vt = vbuf[i % 2] + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
-                // product d of step c adds 16 tokens to 32 dimensions; while the matrix unit is at
-                // it, two weights of the next step are worked out and its values read
-                s16x8 a[2][DB];
-                u32x4 pk[2];
-                const auto read = [&](int c, int d) {
-                    const s16x4 a0 = read_transposed(vt + 16 * c * VROW + 64 * d), a1 = read_transposed(vt + (16 * c + 8) * VROW + 64 * d);
-                    a[c % 2][d] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-                };
-                // weights in the values' type: the matrix unit takes both alike, and the
-                // rounding of a weight is that of an output element
-                const auto weigh = [&](int c, int k) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[c / 2][8 * (c % 2) + 2 * k], P.scale2, base));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[c / 2][8 * (c % 2) + 2 * k + 1], P.scale2, base));
-                    l += p0;
-                    l2 += p1;
-                    pk[c % 2][k] = T::pack(p0, p1);
-                };
-#pragma unroll
-                for (int d = 0; d < DB; ++d) read(0, d);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) weigh(0, k);
+                for (int j = n * 32 / N; j < (n + 1) * 32 / N; ++j) top = fmaxf(top, next[j / 16][j % 16]);
                 __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        o[d] = T::mfma32(__builtin_bit_cast(vec, a[c % 2][d]), __builtin_bit_cast(vec, pk[c % 2]), o[d]);
-                        if (c < 3) {
-                            read(c + 1, d);
-#pragma unroll
-                            for (int k = d * 4 / DB; k < (d + 1) * 4 / DB; ++k) weigh(c + 1, k);
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-                for (uint64_t odd = uniform(static_cast<uint64_t>(special[i % 4])); odd; odd &= odd - 1) {
+            }
+            if (there != ~0ull || !whole_tile(i, block_lo, block_hi))
+                for (uint64_t odd = uniform(static_cast<uint64_t>(special[i % 8])); odd; odd &= odd - 1) {
                     const int at = __ffsll(static_cast<unsigned long long>(odd)) - 1;
-                    const char *src = vbase + place[i % 4][at].y + half * 8;
+                    const char *src = vbase + place[i % 8][at].y + half * 8;
                     const bool shown = sees(P, pos, position_of(sp, t0 + at));
-#pragma unroll
+    #pragma unroll
                     for (int d = 0; d < DB; ++d)
-#pragma unroll
+    #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uint2 v = *reinterpret_cast<const uint2 *>(src + 64 * d + 16 * k);
                             o[d][4 * k] += shown ? special_part<T>(v.x & 0xFFFF) : 0.0f;
@@ -286,14 +304,49 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                         }
                     wait_loads();
                 }
+            there = there_next;
+        };
+
+        // (the last item's readers of LDS are past: see the barrier at the end)
+        if (tiles > 0) {
+            if (wave < 4) {
+                look(wave);
+                note(wave);
             }
-            if (i + 1 < tiles) store(i + 1);
+            if (wave == 4 % NW) look(4);
+            lds_barrier();
+            find_k(0);
+            find_v(0);
+            load_k();
+            load_v();
+            there = uniform(held[0]);
+            find_k(1);
+            find_v(1);
+            store_k(0);
+            load_k();
+            store_v(0, there);
+            load_v();
+            find_k(2);
+            store_k(1);
+            load_k();
+            lds_barrier();
+            wait_loads();
+            s_even[0] = s_even[1] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < 2 * STEPS; ++k)
+                s_even[k / STEPS] = T::mfma32(__builtin_bit_cast(vec, read_key(0, k)), qv[k % STEPS], s_even[k / STEPS]);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) top = fmaxf(top, s_even[k / 16][k % 16]);
+        }
+        for (int32_t i = 0; i < steps; i += 2) {
+            step(i, s_even, s_odd);
+            step(i + 1, s_odd, s_even);
         }
         lds_barrier();
 
         l = add_other32(l + l2);
         const bool whole = pc.begins && pc.ends;
-        const float top = m == -INFINITY ? m : m * P.scale2;
+        top = m == -INFINITY ? m : m * P.scale2;
         const int32_t out_row = renewed(row);
         if (out_row < rq.rows) {
             const int32_t t = P.group.div(out_row);
