@@ -2,7 +2,7 @@
 // rows (chunks of prompts): bound by the matrix unit and the softmax beside it.
 //
 // A wave holds 32 query rows, one in each lane's column; the workgroup's waves
-// share tiles of 64 tokens in LDS, two of keys and two of values, the next ones on
+// share tiles of 64 tokens (32 at dim 256) in LDS, two of keys and two of values, the next ones on
 // their way through registers.  Per tile a wave does 2 x D/16 products of 32 keys x
 // 16 dimensions for the scores and 4 x D/32 of 32 dimensions x 16 keys for the
 // output; rows of the same wave reuse what it reads from LDS.
@@ -16,7 +16,7 @@
 namespace fgk {
 namespace {
 
-constexpr uint32_t kTile = 64;         // tokens
+constexpr uint32_t kRing = 16;         // tiles whose places are known at a time
 constexpr uint32_t kTilesUnit = 256;   // tokens between cuts
 
 // The barrier that publishes LDS and nothing else: loads in flight from global
@@ -27,24 +27,26 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <class T, int D, int NW>
+template <class T, int D, int NW, uint32_t kTile>
 __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void fg_tiles_kernel(AttendParams P) {
     using vec = typename T::vec;
     constexpr uint32_t THREADS = 64 * NW, ROWS = 32 * NW;
     constexpr int STEPS = D / 16, DB = D / 32, CHUNKS = D / 8;   // 16-byte pieces of a row
+    constexpr int BLOCKS = kTile / 32, SCORES = 16 * BLOCKS;     // of 32 tokens; a lane's
+    constexpr uint64_t ALL = kTile == 64 ? ~0ull : (1ull << kTile) - 1;
     constexpr uint32_t PER = (kTile * CHUNKS + THREADS - 1) / THREADS;
     // LDS rows are longer than the data: eight rows' 16-byte pieces of K, and eight
     // rows' 64-byte pieces of V, then meet every bank equally often
     constexpr uint32_t KROW = 2 * D + 16, VROW = 2 * D + (D == 96 ? 128 : 64);
     __shared__ __attribute__((aligned(16))) char kbuf[2][kTile * KROW];
     __shared__ __attribute__((aligned(16))) char vbuf[2][kTile * VROW];
-    // of tile i at i % 8: where its tokens lie (bytes from the head's first key and
+    // of tile i at i % kRing: where its tokens lie (bytes from the head's first key and
     // value), which of them there are, and in a tile that not every row sees which
     // hold an infinite or NaN value: 0 * inf is NaN, so those are taken out of the
     // product and added to the rows that see them
-    __shared__ longlong2 place[8][kTile];
-    __shared__ uint64_t held[8];
-    __shared__ unsigned long long special[8];
+    __shared__ longlong2 place[kRing][kTile];
+    __shared__ uint64_t held[kRing];
+    __shared__ unsigned long long special[kRing];
 
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 32, half = lane / 32;
     const uint32_t W = gridDim.x;
@@ -56,13 +58,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
     const uint64_t x1 = min((w + 1) * start.share, start.all);
     uint64_t before = start.before;
     uint32_t r = start.request;
+    uint64_t x = w * start.share;
+    if (x >= x1) return;
+    Request rq = uniform_request<false, ROWS>(P, r);
 
-    for (uint64_t x = w * start.share; x < x1;) {
-        const Request rq = uniform_request<false, ROWS>(P, r);
+    while (x < x1) {
         const uint64_t all = rq.weight_of(rq.blocks) * P.lists;
         if (x >= before + all) {
             before += all;
-            ++r;
+            rq = uniform_request<false, ROWS>(P, ++r);
             continue;
         }
         Span sp;
@@ -97,14 +101,16 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         const char *const kbase = P.cache.k + pc.list * P.cache.k_head;
         const char *const vbase = P.cache.v + pc.list * P.cache.v_head;
 
-        // The places of tile i are looked up by wave i % NW: the table is read at
-        // step i - 5 and the place written at step i - 4, so nothing waits for it.
+        // The places of NW tiles are looked up at a time, one by each wave, every NW steps
+        // (one wave at every step would hold up the others every time): the table is
+        // read eight steps ahead or more, the places are written one step later, so nothing
+        // waits for it.
         int32_t page = -1;
         uint32_t offset = 0;
         const auto look = [&](int32_t i) {
             const int32_t t = t_lo + i * static_cast<int32_t>(kTile) + static_cast<int32_t>(lane);
             page = -1;
-            if (t < t_hi) {
+            if (t < t_hi && lane < kTile) {
                 const int32_t j = position_of(sp, t);
                 const uint32_t b = P.cache.page_size.div(j);
                 offset = j - b * P.cache.page_size.d;
@@ -114,11 +120,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         const auto note = [&](int32_t i) {
             const bool have = static_cast<uint32_t>(page) < P.cache.pages;
             const int64_t p = have ? page : 0, o = have ? offset : 0;
-            place[i % 8][lane] = longlong2{p * P.cache.k_page + o * P.cache.k_token, p * P.cache.v_page + o * P.cache.v_token};
+            if (lane < kTile) place[i % kRing][lane] = longlong2{p * P.cache.k_page + o * P.cache.k_token, p * P.cache.v_page + o * P.cache.v_token};
             const uint64_t there = __ballot(have);
             if (lane == 0) {
-                held[i % 8] = there;
-                special[i % 8] = 0;
+                held[i % kRing] = there;
+                special[i % kRing] = 0;
             }
         };
         const int32_t shift = sp.from - sp.first;  // position less token number past the first ones
@@ -135,11 +141,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         int64_t k_at[PER], v_at[PER];
         const auto find_k = [&](int32_t i) {
 #pragma unroll
-            for (uint32_t c = 0; c < PER; ++c) k_at[c] = place[i % 8][min((tid + c * THREADS) / CHUNKS, kTile - 1)].x + (tid + c * THREADS) % CHUNKS * 16;
+            for (uint32_t c = 0; c < PER; ++c) k_at[c] = place[i % kRing][min((tid + c * THREADS) / CHUNKS, kTile - 1)].x + (tid + c * THREADS) % CHUNKS * 16;
         };
         const auto find_v = [&](int32_t i) {
 #pragma unroll
-            for (uint32_t c = 0; c < PER; ++c) v_at[c] = place[i % 8][min((tid + c * THREADS) / CHUNKS, kTile - 1)].y + (tid + c * THREADS) % CHUNKS * 16;
+            for (uint32_t c = 0; c < PER; ++c) v_at[c] = place[i % kRing][min((tid + c * THREADS) / CHUNKS, kTile - 1)].y + (tid + c * THREADS) % CHUNKS * 16;
         };
         const auto load_k = [&]() {
 #pragma unroll
@@ -168,9 +174,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 if (kTile * CHUNKS % THREADS == 0 || at < kTile * CHUNKS) {
                     u32x4 v = vr[c];
                     // (a token without a page: whatever was read instead)
-                    if (there != ~0ull && !((there >> trow) & 1)) v = u32x4{0, 0, 0, 0};
+                    if (there != ALL && !((there >> trow) & 1)) v = u32x4{0, 0, 0, 0};
                     if (edge && any_special<T>(v)) {
-                        atomicOr(&special[i % 8], 1ull << trow);
+                        atomicOr(&special[i % kRing], 1ull << trow);
                         v = finite_part<T>(v);
                     }
                     *reinterpret_cast<u32x4 *>(vbuf[i % 2] + trow * VROW + at % CHUNKS * 16) = v;
@@ -185,10 +191,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
 
         // Scores: register i of s[b] is that of token 32 b + 8 (i / 4) + 4 half + i % 4.
         // Two tiles': one's are weighed while the other's are worked out.
-        f32x16 s_even[2], s_odd[2];
+        f32x16 s_even[BLOCKS], s_odd[BLOCKS];
         float top = -INFINITY;  // the largest of the next tile to be weighed
         uint64_t there = 0;     // its tokens
-        u32x4 pk[4];            // the weights of 16 tokens each
+        uint64_t raw_there = 0; // those of the tile after, as read from LDS
+        u32x4 pk[2 * BLOCKS];   // the weights of 16 tokens each
         // Two weights of 32.  In the values' type: the matrix unit takes both alike, and
         // the rounding of a weight is that of an output element.
         const auto weigh = [&](const f32x16 *s, int k, float base) {
@@ -200,7 +207,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             pk[k / 4][k % 4] = T::pack(p0, p1);
         };
         const auto read_key = [&](int32_t i, int n) {
-            return *reinterpret_cast<const u32x4 *>(kbuf[i % 2] + (n / STEPS * 32 + col) * KROW + half * 16 + 32 * (n % STEPS));
+            return __builtin_bit_cast(vec, *reinterpret_cast<const u32x4 *>(kbuf[i % 2] + (n / STEPS * 32 + col) * KROW + half * 16 + 32 * (n % STEPS)));
+        };
+        const uint32_t v_lane = (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
+        const auto read_values = [&](int32_t i, int n) {
+            const char *at = vbuf[i % 2] + v_lane + 16 * (n / DB) * VROW + 64 * (n % DB);
+            return __builtin_bit_cast(vec, __builtin_shufflevector(read_transposed(at), read_transposed(at + 8 * VROW), 0, 1, 2, 3, 4, 5, 6, 7));
         };
         // (the compiler would read for one product at a time and gather the rest: LDS
         // reads run AHEAD products ahead, held there by the barriers for its scheduler)
@@ -210,29 +222,33 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         const int32_t steps = (tiles + 1) & ~1;
         const auto step = [&](int32_t i, f32x16 *s, f32x16 *next) {
             lds_barrier();
-            if (wave == static_cast<uint32_t>(i + 4) % NW) note(i + 4);
-            if (wave == static_cast<uint32_t>(i + 5) % NW) look(i + 5);
+            // the products' operands from LDS: K of the next tile, then V of this one
+            vec ring[AHEAD];
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) ring[n] = read_key(i + 1, n);
+            if (i % NW == 0) look(i + 8 + wave);
+            if (i % NW == 1) note(i + 7 + wave);
             // LDS gets the next tile's values and the keys of the one after (past the last
             // tile what lies in page 0), whose places in it are read.  No branch among
             // the products below: the compiler would gather the weights behind it.
-            find_v(i + 2);
-            const uint64_t there_next = uniform(held[(i + 1) % 8]);
+            const uint64_t there_next = uniform(raw_there);
             store_v(i + 1, there_next);
             const int32_t t0 = t_lo + i * static_cast<int32_t>(kTile);
-            if (there != ~0ull || !whole_tile(i, pos_lo, pos_hi)) {
+            if (there != ALL || !whole_tile(i, pos_lo, pos_hi)) {
                 // the tile's tokens that the row sees, then the lane's: four of every eight
                 const uint64_t seen = there & (bits_below(sp.first - t0) & bits_below(pos + 1 - t0) |
                                                bits_below(pos + 1 - shift - t0) & ~bits_below(max(pos - window, -1) + 1 - shift - t0) & ~bits_below(sp.first - t0));
                 const uint64_t mine = seen >> (4 * half);
                 top = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
+                for (int k = 0; k < SCORES; ++k) {
                     const int at = 8 * (k % 16 / 4) + k % 4;  // in its half of the tile
                     s[k / 16][k % 16] = keep_if(static_cast<uint32_t>(mine >> (k / 16 * 32)), at, s[k / 16][k % 16]);
                     top = fmaxf(top, s[k / 16][k % 16]);
                 }
+                top = max_other32(top);
             }
-            top = fmaxf(m, max_other32(top));
+            top = fmaxf(m, top);
             // the maximum follows when a row's grows by more than 2^8: weights stay
             // below that, and the sums are no less exact for it
             if (__any((top - m) * P.scale2 > 8.0f)) {
@@ -246,19 +262,19 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             }
             const float base = m == -INFINITY ? 0.0f : -m * P.scale2;
 
-            // the scores of the next tile (after the last one, of what LDS holds: unused), the
-            // weights of this one between the products
-            u32x4 kq[AHEAD];
+            // the scores of the next tile (after the last one, of what LDS holds: unused), three
+            // quarters of this one's weights between the products
 #pragma unroll
-            for (int n = 0; n < AHEAD; ++n) kq[n] = read_key(i + 1, n);
-            next[0] = next[1] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            for (int b = 0; b < BLOCKS; ++b) next[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            constexpr int M = BLOCKS * STEPS, N = 2 * BLOCKS * DB;  // products for the scores, for the output
+            static_assert(M % AHEAD == 0);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < 2 * STEPS; ++k) {
-                next[k / STEPS] = T::mfma32(__builtin_bit_cast(vec, kq[k % AHEAD]), qv[k % STEPS], next[k / STEPS]);
-                if (k + AHEAD < 2 * STEPS) kq[k % AHEAD] = read_key(i + 1, k + AHEAD);
+            for (int k = 0; k < M; ++k) {
+                next[k / STEPS] = T::mfma32(ring[k % AHEAD], qv[k % STEPS], next[k / STEPS]);
+                ring[k % AHEAD] = k + AHEAD < M ? read_key(i + 1, k + AHEAD) : read_values(i, k + AHEAD - M);
 #pragma unroll
-                for (int j = k * 16 / (2 * STEPS); j < (k + 1) * 16 / (2 * STEPS); ++j) weigh(s, j, base);
+                for (int j = k * 6 * BLOCKS / M; j < (k + 1) * 6 * BLOCKS / M; ++j) weigh(s, j, base);
                 if (k == 1) load_v();
                 if (k == 2) store_k(i + 2);
                 if (k == 3) find_k(i + 3);
@@ -266,31 +282,27 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 __builtin_amdgcn_sched_barrier(0);
             }
 
-            // this tile's values: product n adds 16 tokens, n / DB, to 32 dimensions; the
-            // next scores' maximum between the products
-            const char *vt = vbuf[i % 2] + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
-            constexpr int N = 4 * DB;
-            s16x8 a[AHEAD];
-            const auto read_values = [&](int n) {
-                const char *at = vt + 16 * (n / DB) * VROW + 64 * (n % DB);
-                return __builtin_shufflevector(read_transposed(at), read_transposed(at + 8 * VROW), 0, 1, 2, 3, 4, 5, 6, 7);
-            };
-#pragma unroll
-            for (int n = 0; n < AHEAD; ++n) a[n] = read_values(n);
+            // this tile's values: product n adds 16 tokens, n / DB, to 32 dimensions; between
+            // the products the last quarter's weights and the next scores' maximum
             top = -INFINITY;
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                o[n % DB] = T::mfma32(__builtin_bit_cast(vec, a[n % AHEAD]), __builtin_bit_cast(vec, pk[n / DB]), o[n % DB]);
-                if (n + AHEAD < N) a[n % AHEAD] = read_values(n + AHEAD);
+                o[n % DB] = T::mfma32(ring[n % AHEAD], __builtin_bit_cast(vec, pk[n / DB]), o[n % DB]);
+                if (n + AHEAD < N) ring[n % AHEAD] = read_values(i, n + AHEAD);
 #pragma unroll
-                for (int j = n * 32 / N; j < (n + 1) * 32 / N; ++j) top = fmaxf(top, next[j / 16][j % 16]);
+                for (int j = n * SCORES / N; j < (n + 1) * SCORES / N; ++j) top = fmaxf(top, next[j / 16][j % 16]);
+#pragma unroll
+                for (int j = 6 * BLOCKS + n * 2 * BLOCKS / (N - DB); j < min(6 * BLOCKS + (n + 1) * 2 * BLOCKS / (N - DB), 8 * BLOCKS); ++j) weigh(s, j, base);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (there != ~0ull || !whole_tile(i, block_lo, block_hi))
-                for (uint64_t odd = uniform(static_cast<uint64_t>(special[i % 8])); odd; odd &= odd - 1) {
+            find_v(i + 3);
+            raw_there = held[(i + 2) % kRing];
+            top = max_other32(top);
+            if (there != ALL || !whole_tile(i, block_lo, block_hi))
+                for (uint64_t odd = uniform(static_cast<uint64_t>(special[i % kRing])); odd; odd &= odd - 1) {
                     const int at = __ffsll(static_cast<unsigned long long>(odd)) - 1;
-                    const char *src = vbase + place[i % 8][at].y + half * 8;
+                    const char *src = vbase + place[i % kRing][at].y + half * 8;
                     const bool shown = sees(P, pos, position_of(sp, t0 + at));
     #pragma unroll
                     for (int d = 0; d < DB; ++d)
@@ -309,34 +321,44 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
 
         // (the last item's readers of LDS are past: see the barrier at the end)
         if (tiles > 0) {
-            if (wave < 4) {
-                look(wave);
-                note(wave);
+#pragma unroll
+            for (int32_t i = 0; i < 8; i += NW) {
+                look(i + wave);
+                note(i + wave);
             }
-            if (wave == 4 % NW) look(4);
             lds_barrier();
+            // the first tile's keys and values and the second one's keys, all under way at once
             find_k(0);
+            load_k();
+            u32x4 first[PER];
+#pragma unroll
+            for (uint32_t c = 0; c < PER; ++c) first[c] = kr[c];
             find_v(0);
-            load_k();
             load_v();
-            there = uniform(held[0]);
             find_k(1);
-            find_v(1);
-            store_k(0);
             load_k();
+            there = uniform(held[0]);
+            find_v(1);
+            find_k(2);
+#pragma unroll
+            for (uint32_t c = 0; c < PER; ++c)
+                if (kTile * CHUNKS % THREADS == 0 || tid + c * THREADS < kTile * CHUNKS)
+                    *reinterpret_cast<u32x4 *>(kbuf[0] + (tid + c * THREADS) / CHUNKS * KROW + (tid + c * THREADS) % CHUNKS * 16) = first[c];
             store_v(0, there);
             load_v();
-            find_k(2);
             store_k(1);
             load_k();
             lds_barrier();
             wait_loads();
-            s_even[0] = s_even[1] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-            for (int k = 0; k < 2 * STEPS; ++k)
-                s_even[k / STEPS] = T::mfma32(__builtin_bit_cast(vec, read_key(0, k)), qv[k % STEPS], s_even[k / STEPS]);
+            for (int b = 0; b < BLOCKS; ++b) s_even[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-            for (int k = 0; k < 32; ++k) top = fmaxf(top, s_even[k / 16][k % 16]);
+            for (int k = 0; k < BLOCKS * STEPS; ++k) s_even[k / STEPS] = T::mfma32(read_key(0, k), qv[k % STEPS], s_even[k / STEPS]);
+#pragma unroll
+            for (int k = 0; k < SCORES; ++k) top = fmaxf(top, s_even[k / 16][k % 16]);
+            top = max_other32(top);
+            find_v(2);
+            raw_there = held[1];
         }
         for (int32_t i = 0; i < steps; i += 2) {
             step(i, s_even, s_odd);
@@ -386,7 +408,7 @@ constexpr int waves_of(int dim) { return dim > 128 ? 4 : 8; }
 template <class T, int D>
 int launch(AttendParams &P, hipStream_t st) {
     constexpr int NW = waves_of(D);
-    hipLaunchKernelGGL((fg_tiles_kernel<T, D, NW>), dim3(P.workgroups), dim3(64 * NW), 0, st, P);
+    hipLaunchKernelGGL((fg_tiles_kernel<T, D, NW, (D > 128 ? 32 : 64)>), dim3(P.workgroups), dim3(64 * NW), 0, st, P);
     hipLaunchKernelGGL((fg_join_kernel<T, D, 32 * NW>), dim3(kJoinWorkgroups), dim3(256), 0, st, P);
     FG_HIP(hipGetLastError(), "attention launch");
     return FG_OK;
