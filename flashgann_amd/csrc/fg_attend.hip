@@ -43,12 +43,12 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
     uint32_t r = start.request;
     char *const vmine = vbuf[wave];
 
+    Request rq = start.first;
     for (uint64_t x = w * start.share; x < x1;) {
-        const Request rq = uniform_request<FOUND, kRows>(P, r);
         const uint64_t all = rq.weight_of(rq.blocks) * P.lists;
         if (x >= before + all) {
             before += all;
-            ++r;
+            rq = uniform_request<FOUND, kRows>(P, ++r);
             continue;
         }
         Span sp;
@@ -354,11 +354,12 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, AttendParams *out) {
     if (a->window != -1)
         seen = std::min(seen, static_cast<uint64_t>(a->sinks) + static_cast<uint32_t>(a->window) + (kRows - 1) / P.group.d + 1);
     seen += P.nids;
-    // Cutting an item of up to 512 tokens (four tiles a wave) gains less than the
-    // join kernel takes.
-    const uint32_t unit = seen <= 512 ? 512 : kRowsUnit;
     const uint64_t blocks = (static_cast<uint64_t>(a->tokens) * P.group.d + kRows - 1) / kRows + a->requests;
     const uint64_t items = std::min<uint64_t>(blocks * P.lists, 1u << 20);
+    // Cutting an item of up to 512 tokens (four tiles a wave) gains less than the
+    // join kernel takes: one token over 168 tokens a list, 32 lists, took 19.4 us cut
+    // and 11.7 whole.  784 tokens a list, 256 lists: 28.7 cut, 31.2 whole.
+    const uint32_t unit = seen <= 512 ? 512 : kRowsUnit;
     const uint64_t pieces = items * std::max<uint64_t>(1, std::min<uint64_t>((seen + unit - 1) / unit, kWorkgroups));
     P.rows = kRows;
     P.unit = fast_div(unit);

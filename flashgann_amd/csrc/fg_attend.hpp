@@ -175,6 +175,13 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
     return static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x));
 }
 
+// Lane `from`'s value; `from` is the same in all lanes.
+__device__ __forceinline__ int32_t of_lane(int32_t x, uint32_t from) { return __builtin_amdgcn_readlane(x, from); }
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, uint32_t from) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int32_t>(x >> 32), from))) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int32_t>(x), from));
+}
+
 // Waits for every load from global memory.  Where loads on one path into a loop are
 // not known to have landed, the compiler waits for all of them inside it, those
 // under way for the next tile with them.
@@ -288,6 +295,7 @@ struct Start {
     uint64_t all, share;  // weight of all items; of a workgroup
     uint64_t before;      // weight of the requests before `request`
     uint32_t request;     // at most a few requests before the first one of the share
+    Request first;        // what that request is
 };
 
 // Every wave sums the requests' weights itself, a lane a run of them: nothing is
@@ -296,10 +304,11 @@ template <bool FOUND, uint32_t ROWS>
 __device__ __forceinline__ Start find_start(const AttendParams &P, uint32_t w) {
     const uint32_t lane = threadIdx.x % 64, run = (P.requests + 63) / 64;
     uint64_t mine = 0;
-    for (uint32_t i = 0; i < run; ++i) {
+    Request q{};  // the first of the lane's run
+    for (uint32_t i = run; i-- > 0;) {
         const uint32_t r = lane * run + i;
         if (r < P.requests) {
-            const Request q = request_of<FOUND, ROWS>(P, r);
+            q = request_of<FOUND, ROWS>(P, r);
             mine += q.weight_of(q.blocks) * P.lists;
         }
     }
@@ -310,13 +319,21 @@ __device__ __forceinline__ Start find_start(const AttendParams &P, uint32_t w) {
         if (lane >= d) upto += o;
     }
     Start s;
-    s.all = uniform(static_cast<uint64_t>(__shfl(upto, 63)));
+    s.all = of_lane(upto, 63);
     s.share = max((s.all + P.workgroups - 1) >> __builtin_ctz(P.workgroups), P.least);
     const uint64_t x = w * s.share;
     const uint64_t at = __ballot(upto > x && upto - mine <= x);
     const uint32_t owner = at ? __ffsll(static_cast<unsigned long long>(at)) - 1 : 0;
-    s.before = uniform(static_cast<uint64_t>(__shfl(upto - mine, owner)));
-    s.request = uniform(owner * run);
+    s.before = of_lane(upto - mine, owner);
+    s.request = owner * run;
+    s.first.q0 = of_lane(q.q0, owner);
+    s.first.rows = of_lane(q.rows, owner);
+    s.first.kv = of_lane(q.kv, owner);
+    s.first.limit = of_lane(q.limit, owner);
+    s.first.fresh = of_lane(q.fresh, owner);
+    s.first.blocks = of_lane(static_cast<int32_t>(q.blocks), owner);
+    s.first.base = of_lane(q.base, owner);
+    s.first.step = FOUND || P.window != 0xFFFFFFFFu ? 0 : ROWS;
     return s;
 }
 
@@ -381,7 +398,7 @@ constexpr float kLn2 = 0.69314718055994531f;
 // The parts of items into their rows.  Workgroup w of the attention kernel began an
 // item and did not end it where joins[w] says so; its parts are the second of w and
 // the first of w + 1, w + 2, ...  Every workgroup here lists the rows of all such
-// items; few rows (one long context, its parts by the hundred) take a workgroup
+// items; few rows (one long context, its parts by the hundred) take several workgroups
 // each, many (a part or two each) the lanes of one row.  Bound by latency: a part is
 // read once, without a look at the maximum before.
 template <class T, int D, uint32_t ROWS>
@@ -389,7 +406,7 @@ __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
     constexpr uint32_t QUADS = D / 4, LANES = D <= 64 ? 16 : D <= 128 ? 32 : 64, SETS = 256 / LANES;
     __shared__ uint32_t first[kWorkgroups + 1], wave_sum[4];
     __shared__ f32x4 acc[256];
-    __shared__ float2 acc_ml[SETS];
+    __shared__ float2 acc_ml[32];
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, W = P.workgroups;
     uint32_t mine[kWorkgroups / 256], sum = 0;
 #pragma unroll
@@ -424,10 +441,14 @@ __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
     }
     __syncthreads();
 
-    const bool few = all <= gridDim.x;
-    const uint32_t set = tid / LANES, quad = tid % LANES, step = few ? SETS : 1;
-    for (uint32_t at = blockIdx.x * (few ? 1 : SETS); at < all; at += gridDim.x * (few ? 1 : SETS)) {
-        const uint32_t task = at + (few ? 0 : set);
+    // a workgroup for every 32 values of a row, for a row, or for every SETS rows
+    constexpr uint32_t SLICES = D / 32;
+    const bool few = all <= gridDim.x, least = all <= 64;
+    const uint32_t lanes = least ? 8 : LANES, sets = 256 / lanes, step = few ? sets : 1;
+    const uint32_t tasks = least ? all * SLICES : all;
+    for (uint32_t at = blockIdx.x * (few ? 1 : SETS); at < tasks; at += gridDim.x * (few ? 1 : SETS)) {
+        const uint32_t set = tid / lanes, quad = (least ? at % SLICES * 8 : 0) + tid % lanes;
+        const uint32_t task = least ? at / SLICES : few ? at : at + set;
         uint32_t lo = 0, hi = W;  // the last workgroup whose rows begin at or before `task`
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) / 2;
@@ -453,17 +474,17 @@ __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
         }
         if (few) {
             acc[tid] = a;
-            if (quad == 0) acc_ml[set] = float2{top, l};
+            if (tid % lanes == 0) acc_ml[set] = float2{top, l};
             __syncthreads();
             if (set == 0) {
-                for (uint32_t i = 0; i < SETS; ++i) top = fmaxf(top, acc_ml[i].x);
+                for (uint32_t i = 0; i < sets; ++i) top = fmaxf(top, acc_ml[i].x);
                 const float base = top == -INFINITY ? 0.0f : top;
                 a = f32x4{0, 0, 0, 0};
                 l = 0.0f;
-#pragma unroll
-                for (uint32_t i = 0; i < SETS; ++i) {
+#pragma unroll 4
+                for (uint32_t i = 0; i < sets; ++i) {
                     const float f = __builtin_amdgcn_exp2f(acc_ml[i].x - base);
-                    a += acc[tid + i * LANES] * f;
+                    a += acc[tid + i * lanes] * f;
                     l = fmaf(f, acc_ml[i].y, l);
                 }
             }

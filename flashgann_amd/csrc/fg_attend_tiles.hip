@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
     uint32_t r = start.request;
     uint64_t x = w * start.share;
     if (x >= x1) return;
-    Request rq = uniform_request<false, ROWS>(P, r);
+    Request rq = start.first;
 
     while (x < x1) {
         const uint64_t all = rq.weight_of(rq.blocks) * P.lists;
