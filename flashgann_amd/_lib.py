@@ -92,7 +92,7 @@ def lib():
         i64 = C.c_int64
         L.fg_cache_plan.argtypes = [vp, vp, C.c_uint32, vp, i64, C.c_uint32, vp, C.c_uint32, C.c_uint32, C.c_uint32,
                                     vp, vp, vp, vp, vp, vp]
-        # the structs arrive packed (flashgann_amd.attention)
+        # (their structs as packed bytes; torch tensors go through _attention)
         L.fg_cache_append.argtypes = [C.c_char_p, vp, vp, i64, i64, i64, i64, vp, C.c_uint32, vp]
         L.fg_attend.argtypes = [C.c_char_p, C.c_char_p, vp, C.c_uint64, vp]
         L.fg_attend_retrieved.argtypes = L.fg_attend.argtypes
