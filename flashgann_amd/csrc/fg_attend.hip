@@ -21,7 +21,6 @@ namespace {
 // by the cache's bytes: a tile is 32 x D keys and values against 16 rows.
 constexpr uint32_t kRowsUnit = 128;    // tokens a unit: one tile of each wave
 constexpr uint32_t kPlaces = 1024;     // token places resolved at a time
-constexpr uint32_t kFewRows = 32;      // query rows of a list up to which this kernel serves
 
 template <class T, int D, bool FOUND>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendParams P) {
@@ -345,15 +344,19 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, AttendParams *out) {
     P.scale2 = a->scale * 1.44269504088896341f;
 
     // What the host knows of the sizes: the table's room bounds a request's tokens.
-    P.tiles = !FOUND && static_cast<uint64_t>(a->max_q) * P.group.d > kFewRows;
-    if (P.tiles) {
-        plan_tiles(P, c->dim);
-        return FG_OK;
-    }
     uint64_t seen = static_cast<uint64_t>(a->table_width) * c->page_size;
     if (a->window != -1)
         seen = std::min(seen, static_cast<uint64_t>(a->sinks) + static_cast<uint32_t>(a->window) + (kRows - 1) / P.group.d + 1);
     seen += P.nids;
+    // Rows of a list: past one block the few-rows kernel reads the keys again for each,
+    // the tile kernel once.  20 rows over 8 x 9,000 tokens: 118 us against 87; 40 rows:
+    // 173 against 87.  Over short contexts it has no parts to join: 32 rows over 64 x
+    // 150 tokens 16.4 us against 30.8, 64 rows 47.5 against 35.2.
+    P.tiles = !FOUND && static_cast<uint64_t>(a->max_q) * P.group.d > (seen <= 512 ? 2 * kRows : kRows);
+    if (P.tiles) {
+        plan_tiles(P, c->dim, seen);
+        return FG_OK;
+    }
     const uint64_t blocks = (static_cast<uint64_t>(a->tokens) * P.group.d + kRows - 1) / kRows + a->requests;
     const uint64_t items = std::min<uint64_t>(blocks * P.lists, 1u << 20);
     // Cutting an item of up to 512 tokens (four tiles a wave) gains less than the

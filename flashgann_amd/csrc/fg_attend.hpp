@@ -502,8 +502,8 @@ __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
 constexpr uint32_t kJoinWorkgroups = 1024;
 
 // Blocks of many rows (fg_attend_tiles.hip): sets rows, unit, least, workgroups and
-// join; launches.
-void plan_tiles(AttendParams &P, uint32_t dim);
+// join for items of up to `seen` tokens; launches.
+void plan_tiles(AttendParams &P, uint32_t dim, uint64_t seen);
 int launch_tiles(AttendParams &P, int dtype, uint32_t dim, hipStream_t stream);
 
 }  // namespace fgk

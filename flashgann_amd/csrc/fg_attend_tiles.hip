@@ -54,7 +54,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
     // grid is a multiple of 8)
     const uint32_t w = blockIdx.x % 8 * (W / 8) + blockIdx.x / 8;
     const Start start = find_start<false, ROWS>(P, w);
-    if (tid == 0) P.joins[w].pieces = 0;
+    if (P.join && tid == 0) P.joins[w].pieces = 0;
     const uint64_t x1 = min((w + 1) * start.share, start.all);
     uint64_t before = start.before;
     uint32_t r = start.request;
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 if (half == 0) P.part_ml[at] = float2{top, l};
             }
         }
-        if (tid == 0 && pc.begins && !pc.ends) {
+        if (P.join && tid == 0 && pc.begins && !pc.ends) {
             P.joins[w] = Join{workgroup_at(pc.end - 1, start.share) - w + 1, pc.block * ROWS, static_cast<uint32_t>(rq.rows), static_cast<uint32_t>(rq.q0), pc.list};
         }
         x = min(pc.end, x1);
@@ -409,7 +409,7 @@ template <class T, int D>
 int launch(AttendParams &P, hipStream_t st) {
     constexpr int NW = waves_of(D);
     hipLaunchKernelGGL((fg_tiles_kernel<T, D, NW, (D > 128 ? 32 : 64)>), dim3(P.workgroups), dim3(64 * NW), 0, st, P);
-    hipLaunchKernelGGL((fg_join_kernel<T, D, 32 * NW>), dim3(kJoinWorkgroups), dim3(256), 0, st, P);
+    if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, 32 * NW>), dim3(kJoinWorkgroups), dim3(256), 0, st, P);
     FG_HIP(hipGetLastError(), "attention launch");
     return FG_OK;
 }
@@ -426,12 +426,15 @@ int launch(AttendParams &P, uint32_t dim, hipStream_t st) {
 
 }  // namespace
 
-void plan_tiles(AttendParams &P, uint32_t dim) {
+void plan_tiles(AttendParams &P, uint32_t dim, uint64_t seen) {
     P.rows = 32 * waves_of(dim);
-    P.unit = fast_div(kTilesUnit);
+    if (P.window != 0xFFFFFFFFu) seen += P.rows / P.group.d;  // a block's rows span so many tokens more
+    // (cutting up to 512 tokens gains less than the join kernel takes)
+    const uint32_t unit = seen <= 512 ? 512 : kTilesUnit;
+    P.unit = fast_div(unit);
     P.least = static_cast<uint64_t>(kTilesUnit) * P.group.d;
     P.workgroups = 256;
-    P.join = 1;
+    P.join = seen > unit;
 }
 
 int launch_tiles(AttendParams &P, int dtype, uint32_t dim, hipStream_t stream) {
