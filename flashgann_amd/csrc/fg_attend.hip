@@ -314,7 +314,7 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, AttendParams *out) {
         if (a->window != -1 && a->window < 1) return fail(FG_EINVAL, "window must be >= 1, or -1 for none");
         if (a->lists) return fail(FG_EINVAL, "lists are for retrieved tokens");
     }
-    if (a->requests > 0x00FFFFFFu) return fail(FG_EINVAL, "requests must be below 2^24");
+    if (a->requests > 65536) return fail(FG_EINVAL, "requests must be at most 65,536");
     if (a->requests && a->tokens &&
         (!a->q || !a->out || !a->kv_lens || (!FOUND && !a->q_starts) || (FOUND && a->nids && !a->ids) ||
          (a->table_width && !a->table)))
@@ -406,18 +406,20 @@ int attend(const fg_kv_cache *c, const fg_attention *a, void *workspace, uint64_
 extern "C" {
 
 int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a) {
-    fgk::AttendParams P{};
-    const int rc = a && a->lists ? fgk::prepare<true>(cache, a, &P) : fgk::prepare<false>(cache, a, &P);
-    return rc ? rc : static_cast<int64_t>(a->requests && a->tokens ? fgk::workspace_of(P, cache->dim).total : 0);
+    return fgk::guarded<int64_t>([&]() -> int64_t {
+        fgk::AttendParams P{};
+        const int rc = a && a->lists ? fgk::prepare<true>(cache, a, &P) : fgk::prepare<false>(cache, a, &P);
+        return rc ? rc : static_cast<int64_t>(a->requests && a->tokens ? fgk::workspace_of(P, cache->dim).total : 0);
+    });
 }
 
 int fg_attend(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes, void *stream) {
-    return fgk::attend<false>(cache, a, workspace, workspace_bytes, stream);
+    return fgk::guarded<int>([&] { return fgk::attend<false>(cache, a, workspace, workspace_bytes, stream); });
 }
 
 int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes,
                         void *stream) {
-    return fgk::attend<true>(cache, a, workspace, workspace_bytes, stream);
+    return fgk::guarded<int>([&] { return fgk::attend<true>(cache, a, workspace, workspace_bytes, stream); });
 }
 
 }  // extern "C"

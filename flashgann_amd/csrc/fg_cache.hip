@@ -187,45 +187,51 @@ int fg_cache_plan(const int32_t *d_lens, const int32_t *d_new, uint32_t requests
                   uint32_t table_width, const int32_t *d_free, uint32_t nfree, uint32_t page_size,
                   uint32_t max_tokens, int32_t *d_q_starts, int32_t *d_kv_lens, int64_t *d_slots,
                   int32_t *d_positions, int32_t *d_used, void *stream) {
-    if (requests < 1 || requests > kMaxRequests) return fail(FG_EINVAL, "requests must be in [1, 4096]");
-    if (page_size < 1 || page_size > 0x7FFFFFFFu) return fail(FG_EINVAL, "page_size must be in [1, 2^31)");
-    if (max_tokens > 0x7FFFFFFFu) return fail(FG_EINVAL, "max_tokens must be below 2^31");
-    if (table_width > 0x7FFFFFFFu / requests) return fail(FG_EINVAL, "requests * table_width must be below 2^31");
-    if (!d_lens || !d_new || !d_q_starts || !d_kv_lens || !d_used || (table_width && !d_table) ||
-        (nfree && !d_free) || (max_tokens && (!d_slots || !d_positions)))
-        return fail(FG_EINVAL, "NULL device buffer");
-    const PlanParams P{d_lens, d_new, d_table, d_free, d_q_starts, d_kv_lens, d_slots, d_positions, d_used, table_row,
-                       requests, table_width, nfree, max_tokens, fast_div(page_size)};
-    const uint32_t grid = max_tokens ? (max_tokens + kPlanTokens - 1) / kPlanTokens : 1;
-    hipLaunchKernelGGL(fg_cache_plan_kernel, dim3(grid), dim3(kPlanThreads), requests * 12, reinterpret_cast<hipStream_t>(stream), P);
-    FG_HIP(hipGetLastError(), "cache plan launch");
-    return FG_OK;
+    return guarded<int>([&]() -> int {
+        if (requests < 1 || requests > kMaxRequests) return fail(FG_EINVAL, "requests must be in [1, 4096]");
+        if (page_size < 1 || page_size > 0x7FFFFFFFu) return fail(FG_EINVAL, "page_size must be in [1, 2^31)");
+        if (max_tokens > 0x7FFFFFFFu) return fail(FG_EINVAL, "max_tokens must be below 2^31");
+        if (table_width > 0x7FFFFFFFu / requests) return fail(FG_EINVAL, "requests * table_width must be below 2^31");
+        if (!d_lens || !d_new || !d_q_starts || !d_kv_lens || !d_used || (table_width && !d_table) ||
+            (nfree && !d_free) || (max_tokens && (!d_slots || !d_positions)))
+            return fail(FG_EINVAL, "NULL device buffer");
+        const PlanParams P{d_lens, d_new, d_table, d_free, d_q_starts, d_kv_lens, d_slots, d_positions, d_used,
+                           table_row, requests, table_width, nfree, max_tokens, fast_div(page_size)};
+        const uint32_t grid = max_tokens ? (max_tokens + kPlanTokens - 1) / kPlanTokens : 1;
+        hipLaunchKernelGGL(fg_cache_plan_kernel, dim3(grid), dim3(kPlanThreads), requests * 12,
+                           reinterpret_cast<hipStream_t>(stream), P);
+        FG_HIP(hipGetLastError(), "cache plan launch");
+        return FG_OK;
+    });
 }
 
 int fg_cache_append(const fg_kv_cache *cache, const void *k, const void *v, int64_t k_token, int64_t k_head,
                     int64_t v_token, int64_t v_head, const int64_t *d_slots, uint32_t tokens, void *stream) {
-    AppendParams P;
-    if (int rc = check_cache(cache, &P.cache)) return rc;
-    if (tokens > 0x7FFFFFFFu) return fail(FG_EINVAL, "tokens must be below 2^31");
-    if (tokens == 0) return FG_OK;
-    if (!k || !v || !d_slots) return fail(FG_EINVAL, "NULL device buffer");
-    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 ||
-        (k_token | k_head | v_token | v_head) % 8)
-        return fail(FG_EINVAL, "keys and values must be 16-byte aligned, strides multiples of 8 elements");
-    P.k = static_cast<const char *>(k);
-    P.v = static_cast<const char *>(v);
-    P.k_token = 2 * k_token, P.k_head = 2 * k_head, P.v_token = 2 * v_token, P.v_head = 2 * v_head;
-    P.slots = d_slots;
-    P.tokens = tokens;
-    P.limit = cache->pages * cache->page_size;
-    P.head_chunks = fast_div(cache->dim / 8);
-    P.chunks = fast_div(cache->heads_kv * (cache->dim / 8));
-    // one piece a thread, whole tokens a workgroup
-    P.per_block = P.chunks.d >= kAppendThreads ? 1 : kAppendThreads / P.chunks.d;
-    const uint32_t grid = (tokens + P.per_block - 1) / P.per_block;
-    hipLaunchKernelGGL(fg_cache_append_kernel, dim3(grid), dim3(kAppendThreads), 0, reinterpret_cast<hipStream_t>(stream), P);
-    FG_HIP(hipGetLastError(), "cache append launch");
-    return FG_OK;
+    return guarded<int>([&]() -> int {
+        AppendParams P;
+        if (int rc = check_cache(cache, &P.cache)) return rc;
+        if (tokens > 0x7FFFFFFFu) return fail(FG_EINVAL, "tokens must be below 2^31");
+        if (tokens == 0) return FG_OK;
+        if (!k || !v || !d_slots) return fail(FG_EINVAL, "NULL device buffer");
+        if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 ||
+            (k_token | k_head | v_token | v_head) % 8)
+            return fail(FG_EINVAL, "keys and values must be 16-byte aligned, strides multiples of 8 elements");
+        P.k = static_cast<const char *>(k);
+        P.v = static_cast<const char *>(v);
+        P.k_token = 2 * k_token, P.k_head = 2 * k_head, P.v_token = 2 * v_token, P.v_head = 2 * v_head;
+        P.slots = d_slots;
+        P.tokens = tokens;
+        P.limit = cache->pages * cache->page_size;
+        P.head_chunks = fast_div(cache->dim / 8);
+        P.chunks = fast_div(cache->heads_kv * (cache->dim / 8));
+        // one piece a thread, whole tokens a workgroup
+        P.per_block = P.chunks.d >= kAppendThreads ? 1 : kAppendThreads / P.chunks.d;
+        const uint32_t grid = (tokens + P.per_block - 1) / P.per_block;
+        hipLaunchKernelGGL(fg_cache_append_kernel, dim3(grid), dim3(kAppendThreads), 0,
+                           reinterpret_cast<hipStream_t>(stream), P);
+        FG_HIP(hipGetLastError(), "cache append launch");
+        return FG_OK;
+    });
 }
 
 }  // extern "C"

@@ -11,6 +11,17 @@
 namespace fgk {
 // Sets the calling thread's fg_last_error() text and returns `code`.
 int fail(int code, const std::string &msg);
+
+// body(), for a C entry point: no C++ exception (a message that found no memory)
+// leaves it.
+template <class R, class F>
+R guarded(F body) noexcept {
+    try {
+        return body();
+    } catch (...) {
+        return FG_ENOMEM;
+    }
+}
 }  // namespace fgk
 
 #define FG_HIP(call, what)                                                                          \

@@ -308,7 +308,8 @@ int fg_cache_append(const fg_kv_cache *cache, const void *k, const void *v, int6
  * strides in elements, multiples of 8, bases 16-byte aligned; lse: (tokens,
  * heads) float32, contiguous, may be NULL.  heads is a multiple of the cache's
  * heads_kv; consecutive query heads share a key/value head.  The table names
- * fewer than 2^30 tokens a request (table_width * page_size).  lse is the natural
+ * fewer than 2^30 tokens a request (table_width * page_size); a call takes at
+ * most 65,536 requests and 2^31 - 1 query rows (tokens * heads).  lse is the natural
  * logarithm of the sum of exponentials; a row that sees nothing gets 0 and
  * -infinity.  Scores, softmax statistics and sums are 32-bit; weights are
  * rounded to the cache's type for the product with the values. */

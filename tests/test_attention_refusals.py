@@ -59,7 +59,8 @@ def test_caches(bad, word):
 @pytest.mark.parametrize("bad,word", (
     (dict(heads=7), "heads"), (dict(heads=0), "heads"), (dict(heads=2048), "heads"), (dict(scale=0.0), "scale"),
     (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
-    (dict(tokens=1 << 30, requests=1 << 30), "tokens"), (dict(table_row=-1), "table"), (dict(table_width=1 << 31), "table"),
+    (dict(tokens=1 << 30, requests=1 << 30), "tokens"), (dict(tokens=65537, requests=65537), "requests"),
+    (dict(table_row=-1), "table"), (dict(table_width=1 << 31), "table"),
     (dict(sinks=1 << 31), "sinks"), (dict(q=0), "NULL"), (dict(out=0), "NULL"), (dict(table=0), "NULL"), (dict(kv_lens=0), "NULL"),
     (dict(q=AT + 2), "aligned"), (dict(q_head=130), "strides"), (dict(out_token=4), "strides"),
     (dict(table_width=1 << 27), "table_width")))
