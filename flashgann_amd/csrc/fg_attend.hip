@@ -349,9 +349,10 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, AttendParams *out) {
         seen = std::min(seen, static_cast<uint64_t>(a->sinks) + static_cast<uint32_t>(a->window) + (kRows - 1) / P.group.d + 1);
     seen += P.nids;
     // Rows of a list: past one block the few-rows kernel reads the keys again for each,
-    // the tile kernel once.  20 rows over 8 x 9,000 tokens: 118 us against 87; 40 rows:
-    // 173 against 87.  Over short contexts it has no parts to join: 32 rows over 64 x
-    // 150 tokens 16.4 us against 30.8, 64 rows 47.5 against 35.2.
+    // the tile kernel once.  At dim 128, 8 key/value heads: 20 rows over 8 x 9,000 tokens
+    // 118 us against 85; 40 rows 171 against 88.  Over short contexts the second reading
+    // is from the caches and an item is cheaper: 32 rows over 64 x 100 tokens 19.8 us
+    // against 22.5, 40 rows 26.5 against 23.2.
     P.tiles = !FOUND && static_cast<uint64_t>(a->max_q) * P.group.d > (seen <= 512 ? 2 * kRows : kRows);
     if (P.tiles) {
         plan_tiles(P, c->dim, seen);
@@ -369,7 +370,6 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, AttendParams *out) {
     P.join = seen > unit;
     P.workgroups = 8;
     while (P.workgroups < pieces && P.workgroups < kWorkgroups) P.workgroups *= 2;
-    P.least = static_cast<uint64_t>(kRowsUnit) * P.group.d;
     return FG_OK;
 }
 

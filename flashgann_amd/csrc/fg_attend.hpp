@@ -114,7 +114,6 @@ struct AttendParams {
     uint32_t join;       // whether the join kernel follows
     uint32_t tiles, rows;  // whether the tile kernel runs; query rows of a block
     uint32_t workgroups; // of the attention kernel, a power of two
-    uint64_t least;      // weight that a workgroup takes at least
     FastDiv group;       // query heads that share a list
     FastDiv unit;        // tokens between cuts through an item, a multiple of a tile
     float scale2;        // scale * log2(e)
@@ -139,8 +138,13 @@ struct Request {
 };
 
 // An item's own cost beside its tokens: its prologue and its rows' output, in
-// tokens.  Not zero: an item without tokens still writes its rows.
-constexpr uint32_t kItemTokens = 32;
+// tokens.  It is also the weight that a workgroup takes at least.  With 32 of both
+// (and 256 at least) four items of few tokens shared a workgroup while most had
+// none: 7 requests of up to 24 tokens took 43.7 us against 13.0, 24 mixed chunks 127
+// against 107; few rows, 4 requests of 200 to 1,500 tokens, 16.4 against 13.5 (and
+// 64 of 500 to 16,000, 475 against 480).
+template <uint32_t ROWS>
+constexpr uint32_t kItemTokens = ROWS > 16 ? 256 : 128;
 
 // The tokens that the rows row0 .. of a block see between them: 0 .. first - 1, then
 // from `from` on, then the ids.  Token number t of them is at position_of(t).
@@ -212,13 +216,13 @@ __device__ __forceinline__ Request request_of(const AttendParams &P, uint32_t r)
     q.limit = static_cast<int32_t>(min(static_cast<uint64_t>(q.kv), room));
     q.rows = q.fresh * static_cast<int32_t>(P.group.d);
     q.blocks = (static_cast<uint32_t>(q.rows) + ROWS - 1) / ROWS;
-    q.base = static_cast<uint64_t>(kItemTokens + max(q.kv - q.fresh, 0)) * P.group.d;
+    q.base = static_cast<uint64_t>(kItemTokens<ROWS> + max(q.kv - q.fresh, 0)) * P.group.d;
     q.step = ROWS;
     if (FOUND || P.window != 0xFFFFFFFFu) {
         // every block sees about as much (the first ones of a context less)
         uint64_t seen = min(static_cast<uint64_t>(q.limit), static_cast<uint64_t>(P.sinks) + P.window + ROWS / P.group.d);
         if constexpr (FOUND) seen += P.nids;
-        q.base = (kItemTokens + seen) * P.group.d;
+        q.base = (kItemTokens<ROWS> + seen) * P.group.d;
         q.step = 0;
     }
     return q;
@@ -320,7 +324,7 @@ __device__ __forceinline__ Start find_start(const AttendParams &P, uint32_t w) {
     }
     Start s;
     s.all = of_lane(upto, 63);
-    s.share = max((s.all + P.workgroups - 1) >> __builtin_ctz(P.workgroups), P.least);
+    s.share = max((s.all + P.workgroups - 1) >> __builtin_ctz(P.workgroups), static_cast<uint64_t>(kItemTokens<ROWS>) * P.group.d);
     const uint64_t x = w * s.share;
     const uint64_t at = __ballot(upto > x && upto - mine <= x);
     const uint32_t owner = at ? __ffsll(static_cast<unsigned long long>(at)) - 1 : 0;
@@ -501,8 +505,7 @@ __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
 }
 constexpr uint32_t kJoinWorkgroups = 1024;
 
-// Blocks of many rows (fg_attend_tiles.hip): sets rows, unit, least, workgroups and
-// join for items of up to `seen` tokens; launches.
+// Blocks of many rows (fg_attend_tiles.hip): sets rows, unit, workgroups and join for items of up to `seen` tokens; launches.
 void plan_tiles(AttendParams &P, uint32_t dim, uint64_t seen);
 int launch_tiles(AttendParams &P, int dtype, uint32_t dim, hipStream_t stream);
 

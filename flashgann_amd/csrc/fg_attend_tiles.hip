@@ -218,8 +218,6 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         // reads run AHEAD products ahead, held there by the barriers for its scheduler)
         constexpr int AHEAD = 4;
 
-        // An even number of steps: the last may find no token.
-        const int32_t steps = (tiles + 1) & ~1;
         const auto step = [&](int32_t i, f32x16 *s, f32x16 *next) {
             lds_barrier();
             // the products' operands from LDS: K of the next tile, then V of this one
@@ -360,8 +358,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             find_v(2);
             raw_there = held[1];
         }
-        for (int32_t i = 0; i < steps; i += 2) {
+        for (int32_t i = 0; i < tiles; i += 2) {
             step(i, s_even, s_odd);
+            if (i + 1 == tiles) break;
             step(i + 1, s_odd, s_even);
         }
         lds_barrier();
@@ -432,7 +431,6 @@ void plan_tiles(AttendParams &P, uint32_t dim, uint64_t seen) {
     // (cutting up to 512 tokens gains less than the join kernel takes)
     const uint32_t unit = seen <= 512 ? 512 : kTilesUnit;
     P.unit = fast_div(unit);
-    P.least = static_cast<uint64_t>(kTilesUnit) * P.group.d;
     P.workgroups = 256;
     P.join = seen > unit;
 }
