@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
     constexpr uint32_t QUADS = D / 4, LANES = D <= 64 ? 16 : D <= 128 ? 32 : 64, SETS = 256 / LANES;
     __shared__ uint32_t first[kWorkgroups + 1], wave_sum[4];
     __shared__ f32x4 acc[256];
-    __shared__ float2 acc_ml[32];
+    __shared__ float2 acc_ml[4];
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, W = P.workgroups;
     uint32_t mine[kWorkgroups / 256], sum = 0;
 #pragma unroll
@@ -476,19 +476,31 @@ __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
                 top = next;
             }
         }
-        if (few) {
-            acc[tid] = a;
-            if (tid % lanes == 0) acc_ml[set] = float2{top, l};
+        if (few) {  // the sets of a wave, then the four waves
+            for (uint32_t d = lanes; d < 64; d <<= 1) {
+                const float next = fmaxf(top, __shfl_xor(top, d)), f = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.0f : next));
+                l *= f;
+                a *= f;
+                l += __shfl_xor(l, d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] += __shfl_xor(a[i], d);
+                top = next;
+            }
+            if (lane < lanes) {
+                acc[wave * 64 + lane] = a;
+                if (lane == 0) acc_ml[wave] = float2{top, l};
+            }
             __syncthreads();
             if (set == 0) {
-                for (uint32_t i = 0; i < sets; ++i) top = fmaxf(top, acc_ml[i].x);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) top = fmaxf(top, acc_ml[i].x);
                 const float base = top == -INFINITY ? 0.0f : top;
                 a = f32x4{0, 0, 0, 0};
                 l = 0.0f;
-#pragma unroll 4
-                for (uint32_t i = 0; i < sets; ++i) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
                     const float f = __builtin_amdgcn_exp2f(acc_ml[i].x - base);
-                    a += acc[tid + i * lanes] * f;
+                    a += acc[lane + i * 64] * f;
                     l = fmaf(f, acc_ml[i].y, l);
                 }
             }
