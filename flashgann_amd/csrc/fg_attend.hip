@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
 template <class T, int D, bool FOUND>
 int launch(AttendParams &P, hipStream_t st) {
     hipLaunchKernelGGL((fg_rows_kernel<T, D, FOUND>), dim3(P.workgroups), dim3(256), 0, st, P);
-    if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, kRows>), dim3(kJoinWorkgroups), dim3(256), 0, st, P);
+    if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, kRows>), dim3(kJoinWorkgroups<kRows>), dim3(256), 0, st, P);
     FG_HIP(hipGetLastError(), "attention launch");
     return FG_OK;
 }

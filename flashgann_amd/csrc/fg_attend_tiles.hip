@@ -429,7 +429,7 @@ template <class T, int D>
 int launch(AttendParams &P, hipStream_t st) {
     constexpr int NW = waves_of(D);
     hipLaunchKernelGGL((fg_tiles_kernel<T, D, NW, (D > 128 ? 32 : 64)>), dim3(P.workgroups), dim3(64 * NW), 0, st, P);
-    if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, 32 * NW>), dim3(kJoinWorkgroups), dim3(256), 0, st, P);
+    if (P.join) hipLaunchKernelGGL((fg_join_kernel<T, D, 32 * NW>), dim3(kJoinWorkgroups<32 * NW>), dim3(256), 0, st, P);
     FG_HIP(hipGetLastError(), "attention launch");
     return FG_OK;
 }
