@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "fg_cache.hpp"
 
@@ -192,7 +193,7 @@ __device__ __forceinline__ uint64_t of_lane(uint64_t x, uint32_t from) {
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 // The same value, as far as the compiler knows another: what follows from it is
-// worked out again instead of being kept in registers.
+// worked out again instead of being kept in registers through the products.
 __device__ __forceinline__ int32_t renewed(int32_t x) {
     asm volatile("" : "+v"(x));
     return x;

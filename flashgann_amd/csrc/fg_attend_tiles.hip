@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         int32_t page = -1;
         uint32_t offset = 0;
         const auto look = [&](int32_t i) {
-            const int32_t t = t_lo + i * static_cast<int32_t>(kTile) + static_cast<int32_t>(lane);
+            const int32_t t = t_lo + i * static_cast<int32_t>(kTile) + renewed(static_cast<int32_t>(lane));
             page = -1;
             if (t < t_hi && lane < kTile) {
                 const int32_t j = position_of(sp, t);
@@ -121,7 +121,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         const auto note = [&](int32_t i) {
             const bool have = static_cast<uint32_t>(page) < P.cache.pages;
             const int64_t p = have ? page : 0, o = have ? offset : 0;
-            if (lane < kTile) place[i % kRing][lane] = longlong2{p * P.cache.k_page + o * P.cache.k_token, p * P.cache.v_page + o * P.cache.v_token};
+            const uint32_t at = renewed(static_cast<int32_t>(lane));
+            if (at < kTile) place[i % kRing][at] = longlong2{p * P.cache.k_page + o * P.cache.k_token, p * P.cache.v_page + o * P.cache.v_token};
             const uint64_t there = __ballot(have);
             if (lane == 0) {
                 held[i % kRing] = there;
@@ -219,6 +220,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         // reads run AHEAD products ahead, held there by the barriers for its scheduler)
         constexpr int AHEAD = 4;
 
+        // Of two waves on a SIMD the one among its products issues first, the one among
+        // those for the scores before the other: they fall out of step, one's matrix work
+        // beside the other's vector work (a window of 1,000 over 12,000 tokens 115.4 us
+        // against 111.7, the chunk of 8,192 1,667 against 1,650).
+        const auto first_in_line = [](auto level) {
+            if constexpr (NW > 4) __builtin_amdgcn_s_setprio(level.value);
+        };
         const auto step = [&](int32_t i, f32x16 *s, f32x16 *next) {
             lds_barrier();
             // the products' operands from LDS: K of the next tile, then V of this one
@@ -267,6 +275,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             for (int b = 0; b < BLOCKS; ++b) next[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
             constexpr int M = BLOCKS * STEPS, N = 2 * BLOCKS * DB;  // products for the scores, for the output
             static_assert(M % AHEAD == 0);
+            first_in_line(std::integral_constant<int, 2>{});
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < M; ++k) {
@@ -284,6 +293,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             // this tile's values: product n adds 16 tokens, n / DB, to 32 dimensions; between
             // the products the last quarter's weights and the next scores' maximum
             top = -INFINITY;
+            first_in_line(std::integral_constant<int, 1>{});
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int n = 0; n < N; ++n) {
@@ -295,13 +305,14 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 for (int j = 6 * BLOCKS + n * 2 * BLOCKS / (N - DB); j < min(6 * BLOCKS + (n + 1) * 2 * BLOCKS / (N - DB), 8 * BLOCKS); ++j) weigh(s, j, base);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            first_in_line(std::integral_constant<int, 0>{});
             find_v(i + 3);
             raw_there = held[(i + 2) % kRing];
             top = max_other32(top);
             if (there != ALL || !whole_tile(i, block_lo, block_hi))
                 for (uint64_t odd = uniform(static_cast<uint64_t>(special[i % kRing])); odd; odd &= odd - 1) {
                     const int at = __ffsll(static_cast<unsigned long long>(odd)) - 1;
-                    const char *src = vbase + place[i % kRing][at].y + half * 8;
+                    const char *src = vbase + place[i % kRing][at].y + renewed(static_cast<int32_t>(half)) * 8;
                     const bool shown = sees(P, pos, position_of(sp, t0 + at));
     #pragma unroll
                     for (int d = 0; d < DB; ++d)
@@ -389,31 +400,32 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         l = add_other32(l + l2);
         const bool whole = pc.begins && pc.ends;
         top = m == -INFINITY ? m : m * P.scale2;
-        const int32_t out_row = renewed(row);
+        const int32_t again = renewed(static_cast<int32_t>(tid));
+        const int32_t out_row = row_first + again % 32, out_half = again / 32 % 2;
         if (out_row < rq.rows) {
             const int32_t t = P.group.div(out_row);
             const int64_t head = static_cast<int64_t>(pc.list) * P.group.d + (out_row - t * static_cast<int32_t>(P.group.d));
             const int64_t qrow = rq.q0 + static_cast<int64_t>(t);
             if (whole) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                char *dst = P.out + qrow * P.out_token + head * P.out_head + half * 8;
+                char *dst = P.out + qrow * P.out_token + head * P.out_head + out_half * 8;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         *reinterpret_cast<uint2 *>(dst + 64 * d + 16 * k) =
                             uint2{T::pack(o[d][4 * k] * inv, o[d][4 * k + 1] * inv), T::pack(o[d][4 * k + 2] * inv, o[d][4 * k + 3] * inv)};
-                if (P.lse && half == 0) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
+                if (P.lse && out_half == 0) P.lse[qrow * P.heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
             } else {
                 const uint32_t slot = 2 * w + (pc.begins ? 1 : 0);
                 const uint64_t at = static_cast<uint64_t>(slot) * ROWS + (out_row - static_cast<int32_t>(pc.block * ROWS));
-                float *dst = P.part + at * D + half * 4;
+                float *dst = P.part + at * D + out_half * 4;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         *reinterpret_cast<f32x4 *>(dst + 32 * d + 8 * k) = f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
-                if (half == 0) P.part_ml[at] = float2{top, l};
+                if (out_half == 0) P.part_ml[at] = float2{top, l};
             }
         }
         if (P.join && tid == 0 && pc.begins && !pc.ends) {
