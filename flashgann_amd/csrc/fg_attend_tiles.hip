@@ -232,6 +232,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         // those for the scores before the other: they fall out of step, one's matrix work
         // beside the other's vector work (a window of 1,000 over 12,000 tokens 115.4 us
         // against 111.7, the chunk of 8,192 1,667 against 1,650).
+        // With a SIMD's 512 registers the compiler moved the output from the matrix unit's
+        // half to the other and back at every step, in case the maximum grows; told where
+        // it stays, only then (dim 256: a chunk of 4,000 after 4,000 651 us against 570).
+        const auto settle = [&] {
+            if constexpr (NW == 4) {
+#pragma unroll
+                for (int k = 0; k < DB; ++k) asm volatile("" : "+a"(o[k]));
+            }
+        };
         const auto first_in_line = [](auto level) {
             if constexpr (NW > 4) __builtin_amdgcn_s_setprio(level.value);
         };
@@ -266,6 +275,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             top = fmaxf(m, top);
             // the maximum follows when a row's grows by more than 2^8: weights stay
             // below that, and the sums are no less exact for it
+            settle();
             if (__any((top - m) * P.scale2 > 8.0f)) {
                 const float from = m == -INFINITY ? top : m;
                 const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((from - top) * P.scale2);
@@ -273,6 +283,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 l2 *= shrink;
 #pragma unroll
                 for (int k = 0; k < DB; ++k) o[k] *= shrink;
+                settle();
                 m = top;
             }
             const float base = m == -INFINITY ? 0.0f : -m * P.scale2;
