@@ -18,7 +18,7 @@
 // the card, 950 to 1,030 TFLOP/s, where a library product of 8,192^3 reaches 1,226; the
 // matrix unit is busy 47% of the cycles and vector instructions issue in 46%, at 1.96
 // GHz.  At dim 64 the softmax is twice as much for the same products: 560 TFLOP/s.  At
-// dim 256 nothing runs beside a SIMD's one wave: 600.
+// dim 256 nothing runs beside a SIMD's one wave: 690.
 #include "fg_attend.hpp"
 
 namespace fgk {
@@ -390,10 +390,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             wait_loads();
         }
         // A wave without rows takes its share of the loads and leaves the matrix unit and LDS
-        // to the others: 40 rows a list over 8 x 9,000 tokens (8 lists, dim 128) took 67 us
-        // against 91, 128 rows 76 against 98, 256 rows 108 either way.  (At dim 256 a wave
-        // has its SIMD to itself; the second loop cost the first one 5%.)
-        if (D <= 128 && idle) {
+        // to the others: 40 rows a list over 8 x 9,000 tokens (8 lists) took 67 us against 91
+        // at dim 128 and 125 against 140 at dim 256; 128 rows (dim 128) 76 against 98, 256
+        // rows 108 either way.
+        if (idle) {
             for (int32_t i = 0; i < tiles; ++i) {
                 lds_barrier();
                 if (i % NW == 0) look(i + 8 + wave);
