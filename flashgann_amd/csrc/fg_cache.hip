@@ -11,6 +11,7 @@ namespace {
 constexpr uint32_t kPlanThreads = 256;
 constexpr uint32_t kPlanTokens = 1024;   // tokens of a workgroup
 constexpr uint32_t kMaxRequests = 4096;  // three LDS words each, 48 KB
+constexpr uint32_t kMaxLength = 0x7FFFFFFFu;  // tokens of a request: what int32 and FastDiv hold
 
 struct PlanParams {
     const int32_t *lens, *fresh;
@@ -74,7 +75,7 @@ __global__ __launch_bounds__(kPlanThreads) void fg_cache_plan_kernel(PlanParams 
             const uint32_t n = max(P.lens[r], 0), fresh = max(P.fresh[r], 0), pages = pages_of(P, n);
             start[r] = m, base[r] = e, held[r] = n;
             m += fresh;
-            e += pages_of(P, n + fresh) - pages;
+            e += pages_of(P, min(n + fresh, kMaxLength)) - pages;
         }
     }
     const uint32_t ms = wave_scan(m, lane), es = wave_scan(e, lane);
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(kPlanThreads) void fg_cache_plan_kernel(PlanParams 
     const uint32_t threads = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + tid;
     for (uint32_t r = first; r < B; r += threads) {
         P.q_starts[r] = start[r];
-        P.kv_lens[r] = held[r] + max(P.fresh[r], 0);
+        P.kv_lens[r] = min(held[r] + max(P.fresh[r], 0), kMaxLength);
     }
     if (first == 0) P.q_starts[B] = tokens, P.used[0] = pages;
     for (uint32_t p = first; p < pages; p += threads) {
@@ -116,9 +117,9 @@ __global__ __launch_bounds__(kPlanThreads) void fg_cache_plan_kernel(PlanParams 
         uint32_t pos = 0;
         if (x[k] < tokens) {
             const uint32_t n = held[r[k]];
-            pos = n + x[k] - start[r[k]];
+            pos = min(n + x[k] - start[r[k]], kMaxLength);  // (the last of them: past the end)
             const uint32_t b = P.page_size.div(pos), own = pages_of(P, n);
-            if (b < P.table_width) {
+            if (b < P.table_width && pos < kMaxLength) {
                 const uint32_t p = base[r[k]] + b - own;
                 const int32_t page = b < own ? P.table[r[k] * P.table_row + b] : p < P.nfree ? P.free_list[p] : -1;
                 if (page >= 0) slot = static_cast<int64_t>(page) * P.page_size.d + (pos - b * P.page_size.d);

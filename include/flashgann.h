@@ -292,7 +292,9 @@ typedef struct {
  *   d_used      1             pages needed; above nfree, the list was short
  * Pages already held are read from the table, so no new page may be handed
  * out twice: drop the first d_used entries from the free list.
- * 1 <= requests <= 4096; the new tokens of all requests together < 2^31. */
+ * 1 <= requests <= 4096; the new tokens of all requests together < 2^31.  A
+ * request ends at 2^31 - 1 tokens: its kv_len stays there, and new tokens past it
+ * get slot -1 and position 2^31 - 1. */
 int fg_cache_plan(const int32_t *d_lens, const int32_t *d_new, uint32_t requests, int32_t *d_table, int64_t table_row,
                   uint32_t table_width, const int32_t *d_free, uint32_t nfree, uint32_t page_size,
                   uint32_t max_tokens, int32_t *d_q_starts, int32_t *d_kv_lens, int64_t *d_slots,
