@@ -4,7 +4,8 @@
 // (scale2 = scale * log2 e, so that weights are powers of two), maximum m:
 //   out = sum 2^(s_j - m) v_j / l,  l = sum 2^(s_j - m),  lse = ln 2 (m + log2 l)
 // in one pass over the tokens: a new maximum m' multiplies what is summed so far
-// by 2^(m - m').  Products run on the matrix unit, transposed: S' = K Q', then
+// by 2^(m - m').  Weights and so sums may carry a common power of two (kTopWeight), taken
+// out, exactly, with the sums.  Products run on the matrix unit, transposed: S' = K Q', then
 // O' = V' P', so that a query row is a lane's column in both.  Its weights leave
 // the first product in the lanes where the second wants them, once the second's
 // contraction takes the tokens in the order that the first leaves them, and V is
@@ -33,6 +34,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
     constexpr int STEPS = D / 32, DB = D / 16;
     constexpr uint32_t VROW = 2 * D + 32;  // bytes of a row of V in LDS: 16 rows' 32-byte pieces meet each bank twice
     constexpr uint32_t OROW = D + 4;       // floats of a row of O in LDS
+    constexpr float UP = T::kTopWeight, DOWN = 1.0f / (1 << T::kTopWeight);  // what is added to a weight's exponent, what takes it out
     static_assert(kRows * OROW * 4 <= 32 * VROW);
     __shared__ __attribute__((aligned(16))) char vbuf[4][32 * VROW];
     __shared__ int2 place[kPlaces];
@@ -190,9 +192,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                     for (int i = 0; i < DB; ++i) o[i] *= shrink;
                     m = top;
                 }
+                const float zero = base - UP;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    p[i] = __builtin_amdgcn_exp2f(p[i] - base);
+                    p[i] = __builtin_amdgcn_exp2f(p[i] - zero);
                     l += p[i];
                 }
                 // weights in the values' type: the matrix unit takes both alike, and
@@ -230,7 +233,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, wave_m[i][col]);
-        const float mine = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+        const float mine = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top)) * DOWN;
         if (quarter == 0) wave_l[wave][col] = l * mine;
         float *omine = reinterpret_cast<float *>(vmine);
 #pragma unroll

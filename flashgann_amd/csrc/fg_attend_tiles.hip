@@ -41,6 +41,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
     constexpr uint32_t THREADS = 64 * NW, ROWS = 32 * NW;
     constexpr int STEPS = D / 16, DB = D / 32, CHUNKS = D / 8;   // 16-byte pieces of a row
     constexpr int BLOCKS = kTile / 32, SCORES = 16 * BLOCKS;     // of 32 tokens; a lane's
+    // The maximum that weights are relative to follows when a row's grows past it by more
+    // than 2^8, so they go up to there; what their exponents are raised by for the product, out
+    // of the sums at the end.
+    constexpr int LAG = 8;
+    constexpr float UP = T::kTopWeight > LAG ? T::kTopWeight - LAG : 0, DOWN = 1.0f / (1 << static_cast<int>(UP));
     constexpr uint64_t ALL = kTile == 64 ? ~0ull : (1ull << kTile) - 1;
     constexpr uint32_t PER = (kTile * CHUNKS + THREADS - 1) / THREADS;
     // LDS rows are longer than the data: eight rows' 16-byte pieces of K, and eight
@@ -273,10 +278,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 top = max_other32(top);
             }
             top = fmaxf(m, top);
-            // the maximum follows when a row's grows by more than 2^8: weights stay
-            // below that, and the sums are no less exact for it
+            // (the sums are no less exact for a maximum that lags)
             settle();
-            if (__any((top - m) * P.scale2 > 8.0f)) {
+            if (__any((top - m) * P.scale2 > static_cast<float>(LAG))) {
                 const float from = m == -INFINITY ? top : m;
                 const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((from - top) * P.scale2);
                 l *= shrink;
@@ -286,7 +290,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 settle();
                 m = top;
             }
-            const float base = m == -INFINITY ? 0.0f : -m * P.scale2;
+            const float base = m == -INFINITY ? 0.0f : fmaf(-m, P.scale2, UP);
 
             // the scores of the next tile (after the last one, of what LDS holds: unused), three
             // quarters of this one's weights between the products
@@ -416,7 +420,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         }
         lds_barrier();
 
-        l = add_other32(l + l2);
+        l = add_other32(l + l2) * DOWN;
         const bool whole = pc.begins && pc.ends;
         top = m == -INFINITY ? m : m * P.scale2;
         const int32_t again = renewed(static_cast<int32_t>(tid));
@@ -426,7 +430,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             const int64_t head = static_cast<int64_t>(pc.list) * P.group.d + (out_row - t * static_cast<int32_t>(P.group.d));
             const int64_t qrow = rq.q0 + static_cast<int64_t>(t);
             if (whole) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const float inv = l == 0.0f ? 0.0f : DOWN / l;
                 char *dst = P.out + qrow * P.out_token + head * P.out_head + out_half * 8;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -443,7 +447,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        *reinterpret_cast<f32x4 *>(dst + 32 * d + 8 * k) = f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+                        *reinterpret_cast<f32x4 *>(dst + 32 * d + 8 * k) = f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * DOWN;
                 if (out_half == 0) P.part_ml[at] = float2{top, l};
             }
         }

@@ -314,8 +314,9 @@ int fg_cache_append(const fg_kv_cache *cache, const void *k, const void *v, int6
  * most 65,536 requests and 2^31 - 1 query rows (tokens * heads).  lse is the natural
  * logarithm of the sum of exponentials; a row that sees nothing gets 0 and
  * -infinity.  Scores, softmax statistics and sums are 32-bit; weights are
- * rounded to the cache's type for the product with the values (an infinite value
- * under a weight that rounds to 0 gives NaN). */
+ * rounded to the cache's type for the product with the values (in float16 those
+ * below 2^-32 of the row's largest are lost; an infinite value under a weight that
+ * rounds to 0 gives NaN). */
 typedef struct {
     const void *q;
     void *out;
