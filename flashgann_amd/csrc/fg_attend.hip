@@ -194,10 +194,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_rows_kernel(AttendPar
                 }
                 const float zero = base - UP;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    p[i] = __builtin_amdgcn_exp2f(p[i] - zero);
-                    l += p[i];
-                }
+                for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(p[i] - zero);
+                // (a tile's first: one by one, those below the last place of a long row's sum are lost)
+                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
                 // weights in the values' type: the matrix unit takes both alike, and
                 // the rounding of a weight is that of an output element
                 u32x4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};

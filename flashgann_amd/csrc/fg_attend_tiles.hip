@@ -162,15 +162,18 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
             for (uint32_t c = 0; c < PER; ++c) v_at[c] = place[i % kRing][min((tid + c * THREADS) / CHUNKS, kTile - 1)].y + (tid + c * THREADS) % CHUNKS * 16;
         };
+        // (at dim 96 a tile is one and a half pieces a thread: the threads past its end load its
+        // last row once more.  A branch there instead had the compiler wait for all loads
+        // under way at every step: 24 mixed chunks 106 us against 87)
         const auto load_k = [&]() {
 #pragma unroll
             for (uint32_t c = 0; c < PER; ++c)
-                if (kTile * CHUNKS % THREADS == 0 || tid + c * THREADS < kTile * CHUNKS) kr[c] = *reinterpret_cast<const u32x4 *>(kbase + k_at[c]);
+                kr[c] = *reinterpret_cast<const u32x4 *>(kbase + k_at[c]);
         };
         const auto load_v = [&]() {
 #pragma unroll
             for (uint32_t c = 0; c < PER; ++c)
-                if (kTile * CHUNKS % THREADS == 0 || tid + c * THREADS < kTile * CHUNKS) vr[c] = *reinterpret_cast<const u32x4 *>(vbase + v_at[c]);
+                vr[c] = *reinterpret_cast<const u32x4 *>(vbase + v_at[c]);
         };
         const auto store_k = [&](int32_t i) {
 #pragma unroll
@@ -199,7 +202,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
             }
         };
 
-        float m = -INFINITY, l = 0.0f, l2 = 0.0f;  // m: of the scores before scaling; the sum is l + l2
+        // m: of the scores before scaling; l: of the tiles that are done, l_tile: of this one
+        // (one by one, weights below the last place of a long row's sum are lost)
+        float m = -INFINITY, l = 0.0f, l_tile = 0.0f;
         f32x16 o[DB];
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -216,9 +221,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         const auto weigh = [&](const f32x16 *s, int k, float base) {
             const float p0 = __builtin_amdgcn_exp2f(fmaf(s[k / 8][2 * (k % 8)], P.scale2, base));
             const float p1 = __builtin_amdgcn_exp2f(fmaf(s[k / 8][2 * (k % 8) + 1], P.scale2, base));
-            l += p0;
-            l2 += p1;
-            asm volatile("" : "+v"(l), "+v"(l2));  // here, not when the sums are next looked at
+            l_tile = k ? l_tile + (p0 + p1) : p0 + p1;
+            asm volatile("" : "+v"(l_tile));  // here, not when the sum is next looked at
             pk[k / 4][k % 4] = T::pack(p0, p1);
         };
         const auto read_key = [&](int32_t i, int n) {
@@ -284,7 +288,6 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 const float from = m == -INFINITY ? top : m;
                 const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((from - top) * P.scale2);
                 l *= shrink;
-                l2 *= shrink;
 #pragma unroll
                 for (int k = 0; k < DB; ++k) o[k] *= shrink;
                 settle();
@@ -329,6 +332,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
                 __builtin_amdgcn_sched_barrier(0);
             }
             first_in_line(std::integral_constant<int, 0>{});
+            l += l_tile;
             find_v(i + 3);
             raw_there = held[(i + 2) % kRing];
             top = max_other32(top);
@@ -420,7 +424,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) __attribute__((amdgpu_waves_per_eu
         }
         lds_barrier();
 
-        l = add_other32(l + l2) * DOWN;
+        l = add_other32(l) * DOWN;
         const bool whole = pc.begins && pc.ends;
         top = m == -INFINITY ? m : m * P.scale2;
         const int32_t again = renewed(static_cast<int32_t>(tid));

@@ -81,3 +81,13 @@ def test_many_small_weights(form, dim):
     tol = n[:, None, None] * 2.0 ** -32 + want * ((n[:, None, None] + 8) * 2.0 ** -22 + 18.1 * (dim + 8) * 2.0 ** -23 + 2.0 ** -11)
     off = np.abs(out - want)
     assert (off <= tol).all(), (float(off.max()), float(tol.max()), float(want.max()))
+
+
+@pytest.mark.parametrize("form", ("rows", "tiles", "retrieved"))
+@pytest.mark.parametrize("dim", (64, 96, 128, 256))
+def test_many_small_weights_in_the_sum(form, dim):
+    """Nor may they get lost in the denominator, next to 1."""
+    _, lse, n, w = small_weights(form, dim)
+    want = (4.2421875 * 4.25 + np.log1p(w))[:, None]
+    off = np.abs(lse - want)
+    assert (off <= 18.1 * (dim + 8) * 2.0 ** -24 + 2.0 ** -21 * 20 + (n[:, None] + 8) * 2.0 ** -24 * w[:, None]).all(), float(off.max())
