@@ -15,7 +15,8 @@ stream and return without synchronising.  A cache is two tensors of shape
 any order in memory whose last dimension is contiguous serves, such as
 (pages, heads_kv, page_size, dim) permuted.  All compute goes through
 libflashgann.so; there is no fallback.  Wrong types, shapes or devices raise
-ValueError, what the library refuses FlashGannError.
+ValueError, what the library refuses FlashGannError.  Nothing here has a gradient:
+with autograd on, a tensor that requires one is refused (ValueError).
 """
 from __future__ import annotations
 

@@ -10,6 +10,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -37,6 +38,14 @@ void need(bool ok, const char *what) {
 const at::Tensor &tensor(PyObject *o, const char *name) {
     if (!THPVariable_Check(o)) throw Refused(std::string(name) + " must be a tensor");
     return THPVariable_Unpack(o);
+}
+
+// No operator here has a gradient: one that autograd would have to pass on is not
+// dropped in silence.
+void no_gradient(std::initializer_list<const at::Tensor *> ts) {
+    if (!c10::GradMode::is_enabled()) return;
+    for (const at::Tensor *t : ts)
+        need(!t->requires_grad(), "cache_append and attention have no gradient: detach their tensors or call them under torch.no_grad()");
 }
 
 int64_t integer(PyObject *o, const char *name, int64_t lo, int64_t hi) {
@@ -172,6 +181,7 @@ PyObject *cache_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
         need(n == 5, "cache_append takes 5 arguments");
         const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &kc = tensor(a[2], "k_cache"), &vc = tensor(a[3], "v_cache");
+        no_gradient({&k, &v, &kc, &vc});
         const Call c(kc);
         const fg_kv_cache cache = cache_of(c, kc, vc);
         const at::Tensor &slots = tensor(a[4], "slots");
@@ -195,6 +205,7 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return guarded([&] {
         need(n == 13, "attend takes 13 arguments");
         const at::Tensor &q = tensor(a[0], "q"), &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache");
+        no_gradient({&q, &kc, &vc});
         const Call c(q);
         const fg_kv_cache cache = cache_of(c, kc, vc);
         need(q.dim() == 3 && q.size(2) == kc.size(3) && q.scalar_type() == kc.scalar_type(), "q must have shape (tokens, heads, dim) and the cache's type");
@@ -202,9 +213,11 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
         need(tokens <= kMost && heads <= kMost, "q is too large");
         need(q.stride(2) == 1 || !tokens, "the last dimension of q must be contiguous");
         at::Tensor out = a[11] == Py_None ? c.empty({tokens, heads, dim}, q.scalar_type()) : tensor(a[11], "out");
+        no_gradient({&out});
         need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && c.has(out) && (out.stride(2) == 1 || !tokens),
              "out must have q's shape and type, its last dimension contiguous, on the same device");
         at::Tensor lse = a[12] == Py_None ? c.empty({tokens, heads}, at::kFloat) : tensor(a[12], "lse");
+        no_gradient({&lse});
         need(lse.dim() == 2 && lse.size(0) == tokens && lse.size(1) == heads && lse.scalar_type() == at::kFloat && c.has(lse) && lse.is_contiguous(),
              "lse must be contiguous float32 of shape (tokens, heads) on the same device");
         const at::Tensor &kv_lens = tensor(a[5], "kv_lens");
