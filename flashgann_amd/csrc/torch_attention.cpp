@@ -48,6 +48,12 @@ void no_gradient(std::initializer_list<const at::Tensor *> ts) {
         need(!t->requires_grad(), "cache_append and attention have no gradient: detach their tensors or call them under torch.no_grad()");
 }
 
+// What a call writes in place: autograd has to see it where it saved the tensor.
+void written(std::initializer_list<const at::Tensor *> ts) {
+    for (const at::Tensor *t : ts)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 int64_t integer(PyObject *o, const char *name, int64_t lo, int64_t hi) {
     const int64_t v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) {
@@ -172,6 +178,7 @@ PyObject *cache_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
                             static_cast<int32_t *>(q_starts.data_ptr()), static_cast<int32_t *>(kv_lens.data_ptr()),
                             static_cast<int64_t *>(slots.data_ptr()), static_cast<int32_t *>(positions.data_ptr()),
                             static_cast<int32_t *>(used.data_ptr()), c.stream));
+        written({&tensor(a[2], "block_table")});
         return pack({q_starts, kv_lens, slots, positions, used});
     });
 }
@@ -195,6 +202,7 @@ PyObject *cache_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (tokens) {
             need(k.stride(2) == 1 && v.stride(2) == 1, "the last dimension of k and v must be contiguous");
             check(fg_cache_append(&cache, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), at, u32(tokens), c.stream));
+            written({&kc, &vc});
         }
         Py_RETURN_NONE;
     });
@@ -262,6 +270,8 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
         at::Tensor work;
         if (bytes) work = c.empty({bytes}, at::kByte);
         check((found ? fg_attend_retrieved : fg_attend)(&cache, &p, bytes ? work.data_ptr() : nullptr, static_cast<uint64_t>(bytes), c.stream));
+        if (a[11] != Py_None) written({&out});
+        if (a[12] != Py_None) written({&lse});
         return pack({out, lse});
     });
 }

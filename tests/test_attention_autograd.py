@@ -46,3 +46,26 @@ def test_without_autograd(gpu_available):
     for name, like in (("out", maybe["q"]), ("lse", torch.zeros((3, 4), device="cuda"))):
         with pytest.raises(ValueError, match="gradient"):
             attend(**maybe, **rest, **{name: like.clone().requires_grad_()})
+
+
+@pytest.mark.gpu
+def test_writes_in_place_are_counted(gpu_available):
+    """What autograd saved and a call then overwrote is found out, as with torch's own writes."""
+    (attend, maybe, rest), _, (append, rows, slots) = tensors("cuda")
+    out, lse = torch.zeros_like(maybe["q"]), torch.zeros((3, 4), device="cuda")
+    saved = [rows["k_cache"], rows["v_cache"], out, lse, rest["block_table"]]
+    before = [t._version for t in saved]
+    append(**rows, **slots)
+    assert [t._version for t in saved] == [before[0] + 1, before[1] + 1, *before[2:]]
+    attend(**maybe, **rest, out=out, lse=lse)
+    attention.cache_plan(rest["kv_lens"], rest["kv_lens"], rest["block_table"], rest["kv_lens"], page_size=16, max_tokens=0)
+    assert [t._version for t in saved] == [v + 1 for v in before]
+    weight = torch.ones((), device="cuda", requires_grad=True)
+    loss = (weight * rows["k_cache"]).sum()
+    append(**rows, **slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # such tensors have no counter
+        held = torch.zeros_like(rows["k_cache"])
+        append(rows["k"], rows["v"], held, held.clone(), **slots)
+    append(rows["k"], rows["v"], held, held, **slots)
