@@ -14,7 +14,8 @@ go into an index (inner product).  Every step then
 
 and compares with attention over the whole context (attend): the share of the
 softmax's weight that the retrieved tokens carry, exp(lse - lse of all), and how
-far the outputs lie apart.  Tokens newer than the index are the window's.
+far the outputs lie apart.  Tokens newer than the index are the window's, so there
+are as many steps as it has tokens at most: past them build the indexes again.
 
 Trained keys cluster and their queries look for few of them; so do these: keys
 around shared directions, queries near a key of the past.
@@ -49,7 +50,10 @@ class LongContext:
 
     def __init__(self, tokens: int, steps: int, heads: int = 8, heads_kv: int = 2, dim: int = 128, k: int = 128,
                  beam: int = 256, window: int = 256, sinks: int = 4, dtype: torch.dtype = torch.bfloat16, seed: int = 1):
+        if steps > window:  # a token would leave the window that no index holds
+            raise ValueError(f"steps ({steps}) must be at most window ({window})")
         self.heads, self.heads_kv, self.dim, self.k, self.beam = heads, heads_kv, dim, k, beam
+        self.steps_left = steps
         self.window, self.sinks, self.dtype = window, sinks, dtype
         self.g = torch.Generator(device="cuda")
         self.g.manual_seed(seed)
@@ -88,6 +92,9 @@ class LongContext:
         return plan
 
     def step(self) -> Step:
+        if self.steps_left == 0:
+            raise RuntimeError("no step is left: the cache and the window are planned for `steps`")
+        self.steps_left -= 1
         group = self.heads // self.heads_kv
         near = torch.randint(self.keys.shape[0], (self.heads,), generator=self.g, device="cuda")
         head = torch.arange(self.heads, device="cuda") // group
@@ -110,6 +117,8 @@ def main(argv: list[str] | None = None) -> int:
                         ("window", 256), ("sinks", 4)):
         ap.add_argument("--" + name, type=int, default=value)
     args = vars(ap.parse_args(argv))
+    if args["steps"] > args["window"]:
+        ap.error("--steps must be at most --window")
     if not torch.cuda.is_available():
         raise SystemExit("no GPU is visible")
     ctx = LongContext(**args)
