@@ -20,6 +20,7 @@ with autograd on, a tensor that requires one is refused (ValueError).
 """
 from __future__ import annotations
 
+import sys
 from typing import NamedTuple
 
 import torch
@@ -27,7 +28,11 @@ import torch
 from . import _lib
 
 _lib.lib()  # its message where the library is missing
-from . import _attention  # noqa: E402  (csrc/torch_attention.cpp)
+try:
+    from . import _attention  # (csrc/torch_attention.cpp)
+except ImportError as e:
+    raise ImportError(f"flashgann_amd._attention is not built for {sys.executable}: make -C flashgann_amd/csrc "
+                      f"PYTHON={sys.executable} ({e})") from e
 
 __all__ = ["CachePlan", "cache_plan", "cache_append", "attend", "attend_retrieved"]
 
