@@ -55,14 +55,15 @@ def cache_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     a page (-1 once free_pages is used up); free_pages: (n,) int32;
     max_tokens: the length of the slot map, at least the sum of new_lens for
     every token to have an entry.  Entries past the last token hold slot -1.
-    `used` is the number of pages taken: drop so many from free_pages."""
+    `used` is the number of pages taken: drop so many from free_pages.  1 to 4,096
+    requests a call."""
     return CachePlan(*_attention.cache_plan(lens, new_lens, block_table, free_pages, page_size, max_tokens))
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  slots: torch.Tensor) -> None:
     """Writes rows k, v (tokens, heads_kv, dim) to the cache's slots (int64); a
-    slot outside the cache, such as -1, is skipped."""
+    slot outside the cache, such as -1, is skipped; no two rows may share a slot."""
     _attention.cache_append(k, v, k_cache, v_cache, slots)
 
 
@@ -79,7 +80,13 @@ def attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_
     depend on it).  scale: dim ** -0.5 unless given.  window: the row at position
     p sees the tokens p - window + 1 .. p and the first `sinks`.
     Returns (out, lse): lse (tokens, heads) float32, the natural logarithm of the
-    sum of exponentials.  A row that sees nothing gets 0 and -inf."""
+    sum of exponentials.  A row that sees nothing gets 0 and -inf; rows outside every
+    request, such as a padded batch's last ones, are left as they are, uninitialised
+    unless out and lse are given.  0 to 65,536 requests a call.
+
+    The host does not know the lengths: a block_table (and window) with room for up to 512
+    tokens a request spares the call its second kernel, 3 to 6 us, and a workspace of up
+    to 68 MB, so pass the columns in use, block_table[:, :n]."""
     return _attention.attend(q, k_cache, v_cache, block_table, q_starts, kv_lens, None, max_q, scale, window, sinks, out, lse)
 
 
@@ -88,13 +95,14 @@ def attend_retrieved(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      scale: float | None = None, out: torch.Tensor | None = None,
                      lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of one token a request over its first `sinks` tokens, its last
-    `window` and the positions in a list, each token once.
+    `window` and the positions in a list.
 
     q: (requests, heads, dim), at position kv_lens - 1; ids: (requests, lists, K)
     int32 or uint32, lists a multiple of heads_kv that divides heads (one list for
     each query head, for each key/value head, or between).  An id past the
     request's tokens, among the first or last ones, or equal to the id before it
-    adds nothing.  Returns (out, lse) as `attend` does."""
+    adds nothing; other repeats count again, so sort a list merged of several searches.
+    Returns (out, lse) as `attend` does."""
     if ids is None:
         raise ValueError("ids are needed")
     return _attention.attend(q, k_cache, v_cache, block_table, None, kv_lens, ids, 1, scale, window, sinks, out, lse)

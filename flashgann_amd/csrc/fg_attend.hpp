@@ -112,8 +112,8 @@ struct AttendParams {
     const int32_t *table, *q_starts, *kv_lens;
     const uint32_t *ids;
     int64_t table_row;
-    float *part;         // kParts x rows x dim
-    float2 *part_ml;     // kParts x rows: maximum (base 2), sum
+    float *part;         // two a workgroup x rows x dim
+    float2 *part_ml;     // two a workgroup x rows: maximum (base 2), sum
     struct Join *joins;  // one a workgroup
     uint32_t table_width, requests, tokens, heads;
     uint32_t lists;      // items side by side: key/value heads, or id lists
@@ -148,8 +148,8 @@ struct Request {
 // An item's own cost beside its tokens: its prologue and its rows' output, in
 // tokens.  It is also the weight that a workgroup takes at least.  With 32 of both
 // (and 256 at least) four items of few tokens shared a workgroup while most had
-// none: 7 requests of up to 24 tokens took 43.7 us against 13.0, 24 mixed chunks 127
-// against 107; few rows, 4 requests of 200 to 1,500 tokens, 16.4 against 13.5 (and
+// none: 7 requests of up to 24 tokens took 43.7 us against 13.0, 24 mixed chunks 105
+// against 85; few rows, 4 requests of 200 to 1,500 tokens, 16.4 against 13.5 (and
 // 64 of 500 to 16,000, 475 against 480).
 template <uint32_t ROWS>
 constexpr uint32_t kItemTokens = ROWS > 16 ? 256 : 128;
@@ -306,12 +306,15 @@ __device__ __forceinline__ Request uniform_request(const AttendParams &P, uint32
 struct Start {
     uint64_t all, share;  // weight of all items; of a workgroup
     uint64_t before;      // weight of the requests before `request`
-    uint32_t request;     // at most a few requests before the first one of the share
+    uint32_t request;     // the first of the lane's run that the share begins in: up to requests / 64 before its own
     Request first;        // what that request is
 };
 
 // Every wave sums the requests' weights itself, a lane a run of them: nothing is
-// waited for but the lengths.  workgroups is a power of two.
+// waited for but the lengths.  The run that the share begins in is then walked a request
+// at a time (65,536 requests: up to 1,023).  One token each over 10, 8 heads over 2: 64
+// requests 8 us, 4,096 135 us, 65,536 2,160 us, most of it their items.  workgroups is a
+// power of two.
 template <bool FOUND, uint32_t ROWS>
 __device__ __forceinline__ Start find_start(const AttendParams &P, uint32_t w) {
     const uint32_t lane = threadIdx.x % 64, run = (P.requests + 63) / 64;
@@ -525,7 +528,7 @@ __global__ __launch_bounds__(256) void fg_join_kernel(AttendParams P) {
     }
 }
 // Eight a CU for blocks of many rows, whose tasks wait for their loads (of 512: 24 mixed
-// chunks 113.6 us, 1,024: 106.5, 2,048: 104.6); fewer for few rows, where every one
+// chunks 94.5 us, 1,024: 87.9, 2,048: 85.4); fewer for few rows, where every one
 // sums the list (1,024: 28.1 us for 32 requests with 256 ids, 512: 27.6).
 template <uint32_t ROWS>
 constexpr uint32_t kJoinWorkgroups = ROWS > 16 ? 2048 : 512;

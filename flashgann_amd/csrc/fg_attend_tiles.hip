@@ -17,8 +17,9 @@
 // A chunk of 8,192 tokens after 8,192 (32 heads over 8, dim 128): 1,600 to 1,740 us by
 // the card, 950 to 1,030 TFLOP/s, where a library product of 8,192^3 reaches 1,226; the
 // matrix unit is busy 47% of the cycles and vector instructions issue in 46%, at 1.96
-// GHz.  At dim 64 the softmax is twice as much for the same products: 560 TFLOP/s.  At
-// dim 256 nothing runs beside a SIMD's one wave: 690.
+// GHz.  A chunk of 4,096 after 4,096 (the same heads): dim 128 909 TFLOP/s, 96 755 (matrix
+// unit 37%, vector issue 48%), 64 621 (the softmax is twice as much for the same
+// products), 256 725 (29% and 28%: neither is near its limit, and a SIMD has one wave).
 #include "fg_attend.hpp"
 
 namespace fgk {

@@ -302,7 +302,7 @@ int fg_cache_plan(const int32_t *d_lens, const int32_t *d_new, uint32_t requests
 
 /* Writes `tokens` rows of keys and values (heads_kv x dim each, strides in
  * elements, as for the cache) into their slots; a slot outside the cache is
- * skipped.  Two rows with the same slot leave either. */
+ * skipped.  Rows with the same slot leave an unspecified mix of themselves there. */
 int fg_cache_append(const fg_kv_cache *cache, const void *k, const void *v, int64_t k_token, int64_t k_head,
                     int64_t v_token, int64_t v_head, const int64_t *d_slots, uint32_t tokens, void *stream);
 
@@ -355,9 +355,13 @@ int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *w
 
 /* Bytes of workspace (16-byte aligned, used until the call's work on `stream`
  * ends, nothing kept in it between calls) that such a call needs at most, from
- * the sizes alone: 0 where no item's tokens can be split over workgroups.  `a` is
- * fg_attend_retrieved's if its lists are not 0.  Negative FG_E* on arguments that
- * the call would refuse. */
+ * the sizes alone: 0 where no item's tokens can be split over workgroups, that is where
+ * the table has room for 512 tokens a request at most, or window, sinks and ids come to
+ * no more.  Lengths are not known here: a table wider than its contexts costs a join
+ * kernel (3 to 6 us) and this workspace, which depends on the kernel and dim and not on
+ * the rows: up to 68 MB for chunks (35 at dim 64, 51 at 96), 17 MB for few rows.
+ * `a` is fg_attend_retrieved's if its lists are not 0.  Negative FG_E* on arguments that the
+ * call would refuse. */
 int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
 
 const char *fg_last_error(void);
