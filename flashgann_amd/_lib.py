@@ -28,6 +28,8 @@ EXPORTED = (
     "fg_index_create", "fg_index_load", "fg_index_destroy", "fg_index_get_info", "fg_search", "fg_search_noalloc",
     "fg_search_device", "fg_search_stream", "fg_search_profile", "fg_lds_bytes", "fg_search_waves", "fg_search_launches", "fg_search_geometry", "fg_encode_rows", "fg_query_prepare", "fg_score_edges", "fg_last_error",
     "fg_version", "fg_cache_plan", "fg_cache_append", "fg_attend", "fg_attend_retrieved", "fg_attend_workspace_bytes",
+    "fg_cache_bounds", "fg_select_blocks", "fg_select_blocks_workspace_bytes", "fg_attend_blocks", "fg_attend_blocks_workspace_bytes",
+    "fg_cache_weigh", "fg_cache_evict", "fg_cache_evict_workspace_bytes",
 )
 
 
@@ -98,6 +100,16 @@ def lib():
         L.fg_attend_retrieved.argtypes = L.fg_attend.argtypes
         L.fg_attend_workspace_bytes.argtypes = [C.c_char_p, C.c_char_p]
         L.fg_attend_workspace_bytes.restype = i64
+        L.fg_cache_bounds.argtypes = [C.c_char_p, vp, C.c_uint32, vp, vp, vp]
+        L.fg_select_blocks.argtypes = [C.c_char_p, C.c_char_p, vp, vp, vp, vp, C.c_uint64, vp]
+        L.fg_attend_blocks.argtypes = L.fg_attend.argtypes
+        for f in (L.fg_select_blocks_workspace_bytes, L.fg_attend_blocks_workspace_bytes):
+            f.argtypes, f.restype = L.fg_attend_workspace_bytes.argtypes, i64
+        L.fg_cache_weigh.argtypes = [C.c_char_p, C.c_char_p, vp, vp, vp]
+        u32 = C.c_uint32
+        L.fg_cache_evict.argtypes = [C.c_char_p, vp, vp, i64, u32, vp, u32, u32, u32, u32, vp, vp, vp, vp, C.c_uint64, vp]
+        L.fg_cache_evict_workspace_bytes.argtypes = [C.c_char_p, u32, u32, u32]
+        L.fg_cache_evict_workspace_bytes.restype = i64
         L.fg_last_error.restype = C.c_char_p
         L.fg_version.restype = C.c_char_p
         _lib = L

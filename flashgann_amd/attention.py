@@ -8,6 +8,12 @@ programs that answer with what a search found.
                     that stay visible
   attend_retrieved  one token a request over the first tokens, the last ones
                     and the ids that `Index.search_device` returned
+  cache_bounds      bounds of the keys of each page that new tokens filled
+  select_blocks     the pages whose bounds promise each query the most: the search
+                    of a context that no index is built for
+  attend_blocks     new tokens over the selected pages, the first and the last ones
+  cache_weigh       the attention weight that each cached token has drawn
+  cache_evict       requests back to a budget of tokens, the heaviest kept
 
 Tensors are torch tensors on the current device; calls are queued on its current
 stream and return without synchronising.  A cache is two tensors of shape
@@ -34,7 +40,8 @@ except ImportError as e:
     raise ImportError(f"flashgann_amd._attention is not built for {sys.executable}: make -C flashgann_amd/csrc "
                       f"PYTHON={sys.executable} ({e})") from e
 
-__all__ = ["CachePlan", "cache_plan", "cache_append", "attend", "attend_retrieved"]
+__all__ = ["CacheEviction", "CachePlan", "attend", "attend_blocks", "attend_retrieved", "cache_append", "cache_bounds", "cache_evict",
+           "cache_plan", "cache_weigh", "select_blocks"]
 
 
 class CachePlan(NamedTuple):
@@ -106,3 +113,80 @@ def attend_retrieved(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if ids is None:
         raise ValueError("ids are needed")
     return _attention.attend(q, k_cache, v_cache, block_table, None, kv_lens, ids, 1, scale, window, sinks, out, lse)
+
+
+def cache_bounds(k_cache: torch.Tensor, slots: torch.Tensor, bounds: torch.Tensor, scales: torch.Tensor) -> None:
+    """Bounds of the keys of each page whose last slot is among `slots` (int64), such as
+    those that `cache_append` has just written: call it after with the same slots.
+
+    bounds: (pages, heads_kv, 2, dim) int8, scales: (pages, heads_kv) float32, contiguous.
+    bounds[p, h, 0] * scales[p, h] is no less than any key of the page, bounds[p, h, 1] *
+    scales[p, h] no more; scales are powers of two, the least of which 127 reach the
+    largest key.  A page with an infinity or NaN gets scale infinity.  Where keys are written
+    again or moved (`cache_evict`), pass their pages' last slots once more."""
+    _attention.cache_bounds(k_cache, slots, bounds, scales)
+
+
+def select_blocks(q: torch.Tensor, bounds: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, q_starts: torch.Tensor,
+                  kv_lens: torch.Tensor, *, page_size: int, k: int, lists: int | None = None, first_blocks: int = 1,
+                  last_blocks: int = 1) -> torch.Tensor:
+    """The k pages that promise each row of q the most: (tokens, lists, k) int32, page
+    numbers within the request (its block b holds tokens b * page_size and on), ascending,
+    -1 behind them where fewer can be selected.
+
+    q, q_starts and kv_lens as for `attend`.  The row at position p, in block c, selects
+    from first_blocks <= b <= c - last_blocks, the blocks that `attend_blocks` does not
+    read anyway.  lists: a multiple of heads_kv that divides heads, heads_kv unless given; the
+    query heads of a list select together, by the sum over them of the most that the bounds
+    leave for q . key, with the summed queries in 8 bits too.  Scores are exact, and equal
+    ones go to the lower block.  1 to 4,096 pages a list; up to 4,194,304 rows a call."""
+    return _attention.select_blocks(q, bounds, scales, block_table, q_starts, kv_lens, page_size, k, lists, first_blocks, last_blocks)
+
+
+def attend_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, q_starts: torch.Tensor,
+                  kv_lens: torch.Tensor, ids: torch.Tensor, *, first_blocks: int = 1, last_blocks: int = 1,
+                  scale: float | None = None, out: torch.Tensor | None = None,
+                  lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Causal attention of each request's new tokens over the pages on a list, the
+    first `first_blocks` of its context and the last `last_blocks` (the row's own among them).
+
+    ids: (tokens, lists, k) int32 as `select_blocks` returns them, a list for each row; an
+    id that is not above all before it in its list, or names one of the first or last blocks
+    or one after them, adds nothing.  Everything else, and (out, lse), as for `attend`."""
+    return _attention.attend_blocks(q, k_cache, v_cache, block_table, q_starts, kv_lens, ids, first_blocks, last_blocks, scale, out, lse)
+
+
+def cache_weigh(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor,
+                lse: torch.Tensor, weights: torch.Tensor, known: torch.Tensor, *, scale: float | None = None) -> None:
+    """Adds to each cached token's weight what these rows of q gave it: the sum over the
+    rows that see it and the query heads of its key/value head of exp(scale q . k - lse).
+
+    q, q_starts, kv_lens: as for `attend` (all new tokens, or a request's last ones only);
+    lse: what `attend` returned for them, without a window.  weights: (pages, heads_kv,
+    page_size) float32, contiguous, written in place.  known: (requests,) int32, the tokens
+    that have a weight already (the length before this step, say): those from there on are
+    set instead of added to.  Pages shared by requests of the call add up."""
+    _attention.cache_weigh(q, k_cache, block_table, q_starts, kv_lens, lse, weights, known, scale)
+
+
+class CacheEviction(NamedTuple):
+    """What `cache_evict` returns."""
+    kv_lens: torch.Tensor   # (requests,) int32
+    freed: torch.Tensor     # (requests * width,) int32
+    released: torch.Tensor  # (1,) int32
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                *, budget: int, window: int, sinks: int = 0) -> CacheEviction:
+    """Takes each request of more than `budget` tokens back to it: its first `sinks` and last
+    `window` tokens stay, and for each key/value head those of largest weight between them
+    (equal ones: the earlier).
+
+    Kept tokens below place budget - window stay where they are, those above it move into the
+    places that became free there, the last `window` behind them: keys, values and
+    weights, in place.  So a place's heads may hold different tokens, and the cache is for
+    `attend` without a window from then on; keys hold their own positions.  Returns the
+    new lengths, the pages that are free now (the first `released` entries of `freed`, -1
+    behind them) and their number; block_table keeps its entries, which `cache_plan` writes
+    over as the request grows.  Pages may not be shared.  1 to 4,096 requests a call."""
+    return CacheEviction(*_attention.cache_evict(k_cache, v_cache, weights, block_table, kv_lens, budget, window, sinks))

@@ -1,0 +1,481 @@
+// fg_blocks.hip -- which pages of a cache a query should read: bounds of a page's keys in
+// 8 bits, and the pages that promise a query the most.
+//
+// For a page, u and l its keys' largest and smallest value of each channel, a query q gives
+// a key of it at most  sum_d max(q_d, 0) u_d + min(q_d, 0) l_d,  and the sum of that over
+// the query heads of a list is the same with q+ = sum_h max(q_h, 0), q- = sum_h min(q_h, 0):
+// one product of 2 dim terms a list, however many heads share it.  u and l are kept as 8-bit
+// codes with a power-of-two scale, rounded outwards, so they stay bounds; q+ and q- are
+// coded the same way for the product.  Integers below 2^24 times a power of two are exact
+// in 32 bits: scores, and so the pages, do not depend on how the work is split.
+#include "fg_blocks.hpp"
+#include "fg_pick.hpp"
+
+namespace fgk {
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+
+// 2^s as the bits of a float: the least power of two of which 127 reach `most` (not
+// negative, finite), not below 2^-126.  127 = 1.984375 * 2^6.
+__device__ __forceinline__ uint32_t scale_bits(float most) {
+    const uint32_t e = (__float_as_uint(most) + 0x01FFFFu) >> 23;
+    return max(static_cast<int32_t>(e) - 6, 1) << 23;
+}
+__device__ __forceinline__ float inverse(uint32_t scale_bits) { return __uint_as_float((254u << 23) - scale_bits); }
+
+__device__ __forceinline__ uint32_t pack4(const int (&c)[4]) {
+    return (c[0] & 0xFF) | (c[1] & 0xFF) << 8 | (c[2] & 0xFF) << 16 | static_cast<uint32_t>(c[3]) << 24;
+}
+
+template <class T>
+__device__ __forceinline__ float as_float(uint32_t bits16);
+template <>
+__device__ __forceinline__ float as_float<BF16>(uint32_t x) { return __uint_as_float(x << 16); }
+template <>
+__device__ __forceinline__ float as_float<F16>(uint32_t x) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x)));
+}
+
+// ---------------------------------------------------------------- bounds
+
+constexpr uint32_t kBoundsThreads = 256, kBoundsTokens = 256;
+
+struct BoundsParams {
+    const char *k;
+    int64_t k_page, k_token, k_head;  // bytes
+    const int64_t *slots;
+    int8_t *bounds;
+    float *scales;
+    uint32_t tokens, limit, heads;
+    FastDiv page_size;
+};
+
+// A workgroup looks through 256 slots for those that end a page; each wave then takes a page
+// of its head at a time, D / 8 lanes a row.  Bound by the keys' bytes, or by a launch.
+template <class T, int D>
+__global__ __launch_bounds__(kBoundsThreads) void fg_cache_bounds_kernel(BoundsParams P) {
+    constexpr uint32_t LANES = D <= 64 ? 8 : D <= 128 ? 16 : 32, ROWS = 64 / LANES;  // (dim 96: 12 of 16 lanes work)
+    __shared__ uint32_t full[kBoundsTokens], count;
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, head = blockIdx.y;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    const uint32_t t = blockIdx.x * kBoundsTokens + tid;
+    if (t < P.tokens) {
+        const int64_t slot = P.slots[t];
+        if (slot >= 0 && slot < static_cast<int64_t>(P.limit)) {
+            const uint32_t page = P.page_size.div(static_cast<uint32_t>(slot));
+            if (static_cast<uint32_t>(slot) - page * P.page_size.d == P.page_size.d - 1) full[atomicAdd(&count, 1u)] = page;
+        }
+    }
+    __syncthreads();
+    const uint32_t piece = lane % LANES, sub = lane / LANES;
+    const bool works = piece * 8 < D;
+    for (uint32_t i = wave; i < count; i += kBoundsThreads / 64) {
+        const int64_t page = full[i];
+        const char *src = P.k + page * P.k_page + head * P.k_head + piece * 16;
+        float hi[8], lo[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) hi[c] = -INFINITY, lo[c] = INFINITY;
+        bool special = false;
+        if (works) {
+#pragma unroll 4
+            for (uint32_t row = sub; row < P.page_size.d; row += ROWS) {
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(src + row * P.k_token);
+                special |= any_special<T>(w);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float a = as_float<T>(w[c] & 0xFFFF), b = as_float<T>(w[c] >> 16);
+                    hi[2 * c] = fmaxf(hi[2 * c], a), lo[2 * c] = fminf(lo[2 * c], a);
+                    hi[2 * c + 1] = fmaxf(hi[2 * c + 1], b), lo[2 * c + 1] = fminf(lo[2 * c + 1], b);
+                }
+            }
+        }
+        float most = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+#pragma unroll
+            for (uint32_t d = LANES; d < 64; d <<= 1) {
+                hi[c] = fmaxf(hi[c], __shfl_xor(hi[c], d));
+                lo[c] = fminf(lo[c], __shfl_xor(lo[c], d));
+            }
+            if (works) most = fmaxf(most, fmaxf(fabsf(hi[c]), fabsf(lo[c])));
+        }
+#pragma unroll
+        for (uint32_t d = 1; d < LANES; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+        const bool finite = !__any(special);
+        const uint32_t scale = finite ? scale_bits(most) : 0x7F800000u;
+        const int64_t at = page * P.heads + head;
+        if (lane == 0) P.scales[at] = __uint_as_float(scale);
+        if (sub < 2 && works) {  // (two rows at least in a wave: one writes the upper bounds, one the lower)
+            const float inv = finite ? inverse(scale) : 0.0f;
+            int c[2][4];
+#pragma unroll
+            for (int i8 = 0; i8 < 8; ++i8) {
+                const float x = sub ? floorf(lo[i8] * inv) : ceilf(hi[i8] * inv);
+                c[i8 / 4][i8 % 4] = finite ? static_cast<int>(x) : 0;
+            }
+            *reinterpret_cast<uint2 *>(P.bounds + (at * 2 + sub) * D + piece * 8) = uint2{pack4(c[0]), pack4(c[1])};
+        }
+    }
+}
+
+// ---------------------------------------------------------------- selection
+
+constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kSelectRows = 16;
+constexpr uint32_t kSelectLds = 128 * 1024;  // bytes of keys that a workgroup holds
+
+struct SelectParams {
+    const char *q;
+    int64_t q_token, q_head;  // bytes
+    const int8_t *bounds;
+    const float *scales;
+    const int32_t *table, *q_starts, *kv_lens;
+    int64_t table_row;
+    int32_t *ids;
+    uint32_t *keys;     // where LDS does not hold them, or they are made and picked from by different kernels
+    uint32_t table_width, requests, tokens, heads_kv, lists, list_heads, pages;
+    uint32_t group;     // query heads of a list
+    uint32_t count, first, last;
+    FastDiv rows;       // query rows of a tile
+    uint32_t stride;    // keys of a row
+    uint32_t parts;     // workgroups that share a tile's blocks
+    FastDiv page_size;
+};
+
+// One past the last block that the row at `pos` selects from.
+__device__ __forceinline__ int32_t end_of(const SelectParams &P, int32_t pos) {
+    if (pos < 0) return 0;
+    const int64_t end = static_cast<int64_t>(P.page_size.div(pos)) - P.last + 1;
+    return static_cast<int32_t>(min(max(end, static_cast<int64_t>(0)), static_cast<int64_t>(P.table_width)));
+}
+
+// The codes of a tile's queries, 2 D bytes a row, into LDS; a wave a row.
+template <class T, int D>
+__device__ __forceinline__ void code_queries(const SelectParams &P, const Tile &t, uint32_t list, char *codes, uint32_t row_bytes) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    constexpr uint32_t PAIRS = D / 2, N = (PAIRS + 63) / 64;  // two channels a lane at a time
+    for (uint32_t row = wave; row < kSelectRows; row += kSelectWaves) {
+        float up[N][2] = {}, down[N][2] = {};
+        if (row < static_cast<uint32_t>(t.rows)) {
+            const char *src = P.q + (t.q0 + static_cast<int64_t>(row)) * P.q_token + static_cast<int64_t>(list) * P.group * P.q_head;
+#pragma unroll 4
+            for (uint32_t h = 0; h < P.group; ++h) {
+#pragma unroll
+                for (uint32_t n = 0; n < N; ++n) {
+                    const uint32_t pair = n * 64 + lane;
+                    if (PAIRS % 64 == 0 || pair < PAIRS) {
+                        const uint32_t w = *reinterpret_cast<const uint32_t *>(src + h * P.q_head + pair * 4);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float x = as_float<T>(c ? w >> 16 : w & 0xFFFF);
+                            // (not fmaxf: a NaN has to stay one)
+                            up[n][c] += x < 0.0f ? 0.0f : x;
+                            down[n][c] += x > 0.0f ? 0.0f : x;
+                        }
+                    }
+                }
+            }
+        }
+        float most = 0.0f;
+        bool special = false;
+#pragma unroll
+        for (uint32_t n = 0; n < N; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                special |= !(fabsf(up[n][c]) < INFINITY) | !(fabsf(down[n][c]) < INFINITY);
+                most = fmaxf(most, fmaxf(fabsf(up[n][c]), fabsf(down[n][c])));
+            }
+#pragma unroll
+        for (uint32_t d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+        const bool finite = !__any(special);
+        const float inv = finite ? inverse(scale_bits(most)) : 0.0f;
+#pragma unroll
+        for (uint32_t n = 0; n < N; ++n) {
+            const uint32_t pair = n * 64 + lane;
+            if (PAIRS % 64 == 0 || pair < PAIRS) {
+                const auto code = [&](float x) { return finite ? static_cast<int>(rintf(x * inv)) & 0xFF : 0; };
+                *reinterpret_cast<uint16_t *>(codes + row * row_bytes + 2 * pair) = static_cast<uint16_t>(code(up[n][0]) | code(up[n][1]) << 8);
+                *reinterpret_cast<uint16_t *>(codes + row * row_bytes + D + 2 * pair) = static_cast<uint16_t>(code(down[n][0]) | code(down[n][1]) << 8);
+            }
+        }
+    }
+}
+
+// The P.count largest of n keys (0: none) by their places, ascending, -1 behind them.
+template <uint32_t WAVES, class Keys>
+__device__ __forceinline__ void pick(Keys keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, Picking<WAVES> &S) {
+    const uint32_t lane = threadIdx.x % 64, wave = WAVES > 1 ? uniform(threadIdx.x / 64) : 0;
+    const Border B = border_of<WAVES>(keys, n, count, S);
+    const Run run = run_of<WAVES>(n);
+    uint32_t at = 0, equal = 0;  // ids written, and keys equal to the border, before this wave's run
+    if constexpr (WAVES > 1) {
+        uint32_t above = 0, same = 0;
+#pragma unroll 4
+        for (uint32_t i = run.begin + lane; i < run.end; i += 64) {
+            const uint32_t x = keys[i];
+            above += x > B.border, same += x == B.border;
+        }
+        above = wave_sum(above), same = wave_sum(same);
+        if (lane == 0) S.count[0][wave] = above, S.count[1][wave] = same;
+        __syncthreads();
+        for (uint32_t w = 0; w < wave; ++w) {
+            at += S.count[0][w] + min(S.count[1][w], B.ties - min(B.ties, equal));
+            equal += S.count[1][w];
+        }
+    }
+    for (uint32_t i0 = run.begin; B.valid && i0 < run.end; i0 += 64) {
+        const uint32_t i = i0 + lane, x = i < run.end ? static_cast<uint32_t>(keys[i]) : 0;
+        const bool take = taken(B, x, equal);
+        const uint64_t all = __ballot(take);
+        if (take) ids[at + __popcll(all & ((1ull << lane) - 1))] = static_cast<int32_t>(first + i);
+        at += __popcll(all);
+    }
+    for (uint32_t i = min(B.valid, count) + (WAVES > 1 ? threadIdx.x : lane); i < count; i += 64 * WAVES) ids[i] = -1;
+}
+
+enum { kFused, kScratch, kScore, kPick };  // keys in LDS; in a scratch of the workgroup; made only; picked from only
+
+// A workgroup takes a tile of rows of one list: queries coded once, then each wave a group
+// of 16 blocks at a time through the matrix unit, rows against blocks.
+template <class T, int D, int MODE, bool TEAM>
+__global__ __launch_bounds__(kSelectThreads) void fg_select_kernel(SelectParams P) {
+    constexpr int STEPS = 2 * D / 64;
+    constexpr uint32_t QROW = 2 * D + 16;  // bytes of a row's codes in LDS
+    extern __shared__ uint32_t held[];
+    __shared__ __attribute__((aligned(16))) char codes[kSelectRows * QROW];
+    constexpr uint32_t WAVES = TEAM ? kSelectWaves : 1;
+    __shared__ Picking<WAVES> picking[TEAM ? 1 : kSelectRows];
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 16, quarter = lane / 16;
+    const uint32_t list = blockIdx.y, part = MODE == kScore ? blockIdx.z : 0;
+    const uint32_t tiles = P.rows.div(P.tokens) + P.requests;
+    const uint64_t scratch = MODE == kScratch ? static_cast<uint64_t>(blockIdx.y) * gridDim.x + blockIdx.x : 0;
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const Tile t = tile_of(P.q_starts, P.kv_lens, P.requests, P.tokens, P.rows, tile);
+        if (t.rows == 0) continue;
+        const int32_t first = static_cast<int32_t>(min(P.first, P.table_width)), end = end_of(P, t.pos + t.rows - 1);
+        const uint32_t n = static_cast<uint32_t>(max(end - first, 0));
+        uint32_t *const stored = MODE == kScratch ? P.keys + scratch * P.rows.d * P.stride
+                                                  : P.keys + (static_cast<uint64_t>(list) * tiles + tile) * P.rows.d * P.stride;
+        const auto put = [&](uint32_t row, uint32_t i, uint32_t key) {
+            if constexpr (MODE == kFused) held[row * P.stride + i] = key;
+            else stored[static_cast<uint64_t>(row) * P.stride + i] = key;
+        };
+        if constexpr (MODE != kPick) {
+            code_queries<T, D>(P, t, list, codes, QROW);
+            __syncthreads();
+            i32x4 qv[STEPS];
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) qv[s] = *reinterpret_cast<const i32x4 *>(codes + col * QROW + 64 * s + 16 * quarter);
+            int32_t ends[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ends[i] = end_of(P, t.pos + static_cast<int32_t>(4 * quarter) + i);
+            const uint32_t kv_head = list / P.list_heads;
+            const int32_t *row = P.table + t.request * P.table_row;
+            const uint32_t groups = (n + 15) / 16, step = kSelectWaves * (MODE == kScore ? P.parts : 1);
+            uint32_t g = wave + kSelectWaves * part;
+            int32_t page = g < groups && g * 16 + col < n ? row[first + g * 16 + col] : -1;
+            for (; g < groups; g += step) {
+                const bool real = static_cast<uint32_t>(page) < P.pages;
+                const int64_t at = static_cast<int64_t>(real ? page : 0) * P.heads_kv + kv_head;
+                const int8_t *src = P.bounds + at * (2 * D) + 16 * quarter;
+                i32x4 b[STEPS];
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) b[s] = *reinterpret_cast<const i32x4 *>(src + 64 * s);
+                const float scale = P.scales[at];
+                const uint32_t i16 = g * 16 + col, next = g + step;
+                page = next < groups && next * 16 + col < n ? row[first + next * 16 + col] : -1;
+                i32x4 s4 = {0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) s4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(qv[s], b[s], s4, 0, 0, 0);
+                if (i16 < n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t r = 4 * quarter + i;
+                        if (r < static_cast<uint32_t>(t.rows)) {
+                            const float score = scale == INFINITY ? INFINITY : static_cast<float>(s4[i]) * scale;
+                            put(r, i16, real && first + static_cast<int32_t>(i16) < ends[i] ? key_of(score) : 0u);
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if constexpr (MODE != kScore) {
+            for (uint32_t r = TEAM ? 0 : wave; r < static_cast<uint32_t>(t.rows); r += TEAM ? 1 : kSelectWaves) {
+                int32_t *out = P.ids + ((t.q0 + static_cast<uint64_t>(r)) * P.lists + list) * P.count;
+                if constexpr (MODE == kFused) pick<WAVES>(held + r * P.stride, n, P.count, first, out, picking[TEAM ? 0 : r]);
+                else pick<WAVES>(static_cast<const uint32_t *>(stored) + static_cast<uint64_t>(r) * P.stride, n, P.count, first, out, picking[TEAM ? 0 : r]);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+template <class T, int D>
+int launch_select(const SelectParams &P, int mode, dim3 grid, uint32_t lds, hipStream_t st) {
+    const auto go = [&](auto kernel, dim3 g, uint32_t bytes) -> int {
+        if (bytes > 32 * 1024) FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kSelectLds), "selection LDS");
+        hipLaunchKernelGGL(kernel, g, dim3(kSelectThreads), bytes, st, P);
+        return FG_OK;
+    };
+    int rc = FG_OK;
+    if (mode == kFused) rc = P.rows.d == 1 ? go(fg_select_kernel<T, D, kFused, true>, grid, lds) : go(fg_select_kernel<T, D, kFused, false>, grid, lds);
+    else if (mode == kScratch) rc = go(fg_select_kernel<T, D, kScratch, true>, grid, 0);
+    else {
+        rc = go(fg_select_kernel<T, D, kScore, true>, dim3(grid.x, grid.y, P.parts), 0);
+        if (rc == FG_OK) rc = go(fg_select_kernel<T, D, kPick, true>, grid, 0);
+    }
+    if (rc != FG_OK) return rc;
+    FG_HIP(hipGetLastError(), "selection launch");
+    return FG_OK;
+}
+
+// How a call is run.
+struct SelectPlan {
+    int mode;
+    dim3 grid;
+    uint32_t lds;
+    uint64_t workspace;
+};
+
+int prepare_select(const fg_kv_cache *c, const fg_attention *a, SelectParams *out, SelectPlan *plan) {
+    SelectParams &P = *out;
+    if (int rc = check_cache_shape(c)) return rc;
+    if (!a) return fail(FG_EINVAL, "selection arguments are NULL");
+    if (a->heads < 1 || a->heads > 1024 || a->heads % c->heads_kv) return fail(FG_EINVAL, "heads must be a multiple of heads_kv, at most 1024");
+    if (a->lists < 1 || a->heads % a->lists || a->lists % c->heads_kv) return fail(FG_EINVAL, "lists must be a multiple of heads_kv that divides heads");
+    if (a->nids < 1 || a->nids > kMostBlocks) return fail(FG_EINVAL, "blocks of a list must be in [1, 4096]");
+    if (a->tokens > kMostTokens) return fail(FG_EINVAL, "tokens must be at most 4,194,304");
+    if (static_cast<uint64_t>(a->tokens) * a->heads > 0x7FFFFFFFull) return fail(FG_EINVAL, "tokens * heads must be below 2^31");
+    if (static_cast<uint64_t>(a->tokens) * a->lists * a->nids > 0x7FFFFFFFull) return fail(FG_EINVAL, "tokens * lists * blocks of a list must be below 2^31");
+    if (a->table_width > 0x7FFFFFFFu || a->table_row < 0) return fail(FG_EINVAL, "table_width or table_row out of range");
+    if (static_cast<uint64_t>(a->table_width) * c->page_size > 0x3FFFFFFFull) return fail(FG_EINVAL, "table_width * page_size must be below 2^30");
+    if (a->sinks > 0x7FFFFFFFu) return fail(FG_EINVAL, "first blocks (sinks) must be below 2^31");
+    if (a->window < 1) return fail(FG_EINVAL, "last blocks (window) must be >= 1");
+    if (a->requests > 65536) return fail(FG_EINVAL, "requests must be at most 65,536");
+    if (a->requests && a->tokens && (!a->q || !a->kv_lens || !a->q_starts || (a->table_width && !a->table))) return fail(FG_EINVAL, "NULL device buffer");
+    if (reinterpret_cast<uintptr_t>(a->q) % 16 || (a->q_token | a->q_head) % 8) return fail(FG_EINVAL, "q must be 16-byte aligned, strides multiples of 8 elements");
+    P.q = static_cast<const char *>(a->q);
+    P.q_token = 2 * a->q_token, P.q_head = 2 * a->q_head;
+    P.table = a->table;
+    P.q_starts = a->q_starts;
+    P.kv_lens = a->kv_lens;
+    P.table_row = a->table_row;
+    P.table_width = a->table_width;
+    P.requests = a->requests;
+    P.tokens = a->tokens;
+    P.heads_kv = c->heads_kv;
+    P.lists = a->lists;
+    P.list_heads = a->lists / c->heads_kv;
+    P.pages = c->pages;
+    P.group = a->heads / a->lists;
+    P.count = a->nids;
+    P.first = a->sinks;
+    P.last = static_cast<uint32_t>(a->window);
+    P.page_size = fast_div(c->page_size);
+
+    // Keys of a tile's rows are held in LDS: 16 rows where they fit, fewer over longer tables.
+    const uint32_t most = std::max(1u, a->table_width - std::min(a->table_width, P.first));
+    P.stride = most | 1;  // (odd: the rows of a tile lie in different banks)
+    uint32_t rows = kSelectRows;
+    while (rows > 1 && (static_cast<uint64_t>(rows) * P.stride * 4 > kSelectLds || a->tokens <= 2 * static_cast<uint64_t>(a->requests))) rows /= 2;
+    P.rows = fast_div(rows);
+    const uint64_t tiles = a->tokens / rows + static_cast<uint64_t>(a->requests), items = tiles * a->lists;
+    P.parts = 1;
+    plan->grid = dim3(static_cast<uint32_t>(std::min<uint64_t>(tiles, 1u << 20)), a->lists);
+    plan->lds = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(rows) * P.stride * 4, 0xFFFFFFFFu));
+    plan->workspace = 0;
+    plan->mode = kFused;
+    if (plan->lds > kSelectLds) {
+        plan->mode = kScratch;
+        plan->grid.x = static_cast<uint32_t>(std::min<uint64_t>(tiles, std::max(1u, 512 / a->lists)));
+        plan->workspace = static_cast<uint64_t>(plan->grid.x) * a->lists * P.stride * 4;
+    }
+    // Few rows over many blocks: several workgroups make a row's keys, and one picks from them.
+    if (rows == 1 && items < 128 && most >= 2048) {
+        plan->mode = kScore;
+        plan->grid.x = static_cast<uint32_t>(tiles);
+        P.parts = std::min<uint32_t>((most + 16 * kSelectWaves - 1) / (16 * kSelectWaves), static_cast<uint32_t>(std::max<uint64_t>(1, 512 / items)));
+        plan->workspace = items * P.stride * 4;
+    }
+    return FG_OK;
+}
+
+template <class T>
+int launch_select(const SelectParams &P, const SelectPlan &plan, uint32_t dim, hipStream_t st) {
+    switch (dim) {
+    case 64: return launch_select<T, 64>(P, plan.mode, plan.grid, plan.lds, st);
+    case 96: return launch_select<T, 96>(P, plan.mode, plan.grid, plan.lds, st);
+    case 128: return launch_select<T, 128>(P, plan.mode, plan.grid, plan.lds, st);
+    default: return launch_select<T, 256>(P, plan.mode, plan.grid, plan.lds, st);
+    }
+}
+
+template <class T>
+void launch_bounds(const BoundsParams &P, uint32_t dim, dim3 grid, hipStream_t st) {
+    switch (dim) {
+    case 64: hipLaunchKernelGGL((fg_cache_bounds_kernel<T, 64>), grid, dim3(kBoundsThreads), 0, st, P); break;
+    case 96: hipLaunchKernelGGL((fg_cache_bounds_kernel<T, 96>), grid, dim3(kBoundsThreads), 0, st, P); break;
+    case 128: hipLaunchKernelGGL((fg_cache_bounds_kernel<T, 128>), grid, dim3(kBoundsThreads), 0, st, P); break;
+    default: hipLaunchKernelGGL((fg_cache_bounds_kernel<T, 256>), grid, dim3(kBoundsThreads), 0, st, P); break;
+    }
+}
+
+}  // namespace
+}  // namespace fgk
+
+using namespace fgk;
+
+extern "C" {
+
+int fg_cache_bounds(const fg_kv_cache *cache, const int64_t *d_slots, uint32_t tokens, int8_t *d_bounds, float *d_scales,
+                    void *stream) {
+    return guarded<int>([&]() -> int {
+        CacheView view;
+        if (int rc = check_cache(cache, &view)) return rc;
+        if (tokens > 0x7FFFFFFFu) return fail(FG_EINVAL, "tokens must be below 2^31");
+        if (tokens == 0) return FG_OK;
+        if (!d_slots || !d_bounds || !d_scales) return fail(FG_EINVAL, "NULL device buffer");
+        if (reinterpret_cast<uintptr_t>(d_bounds) % 16) return fail(FG_EINVAL, "bounds must be 16-byte aligned");
+        const BoundsParams P{view.k, view.k_page, view.k_token, view.k_head, d_slots, d_bounds, d_scales, tokens,
+                             cache->pages * cache->page_size, cache->heads_kv, view.page_size};
+        const dim3 grid((tokens + kBoundsTokens - 1) / kBoundsTokens, cache->heads_kv);
+        hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+        if (cache->dtype == FG_BF16) launch_bounds<BF16>(P, cache->dim, grid, st);
+        else launch_bounds<F16>(P, cache->dim, grid, st);
+        FG_HIP(hipGetLastError(), "bounds launch");
+        return FG_OK;
+    });
+}
+
+int64_t fg_select_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a) {
+    return guarded<int64_t>([&]() -> int64_t {
+        SelectParams P{};
+        SelectPlan plan;
+        if (int rc = prepare_select(cache, a, &P, &plan)) return rc;
+        return static_cast<int64_t>(a->requests && a->tokens ? plan.workspace : 0);
+    });
+}
+
+int fg_select_blocks(const fg_kv_cache *cache, const fg_attention *a, const int8_t *d_bounds, const float *d_scales,
+                     int32_t *d_ids, void *workspace, uint64_t workspace_bytes, void *stream) {
+    return guarded<int>([&]() -> int {
+        SelectParams P{};
+        SelectPlan plan;
+        if (int rc = prepare_select(cache, a, &P, &plan)) return rc;
+        if (a->requests == 0 || a->tokens == 0) return FG_OK;
+        if (!d_bounds || !d_scales || !d_ids) return fail(FG_EINVAL, "NULL device buffer");
+        if (reinterpret_cast<uintptr_t>(d_bounds) % 16) return fail(FG_EINVAL, "bounds must be 16-byte aligned");
+        if (plan.workspace && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < plan.workspace))
+            return fail(FG_EINVAL, "workspace must be 16-byte aligned and hold " + std::to_string(plan.workspace) + " bytes");
+        P.bounds = d_bounds;
+        P.scales = d_scales;
+        P.ids = d_ids;
+        P.keys = static_cast<uint32_t *>(workspace);
+        hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+        return cache->dtype == FG_BF16 ? launch_select<BF16>(P, plan, cache->dim, st) : launch_select<F16>(P, plan, cache->dim, st);
+    });
+}
+
+}  // extern "C"

@@ -163,13 +163,18 @@ __global__ __launch_bounds__(kAppendThreads) void fg_cache_append_kernel(AppendP
 
 }  // namespace
 
-int check_cache(const fg_kv_cache *c, CacheView *view) {
+int check_cache_shape(const fg_kv_cache *c) {
     if (!c) return fail(FG_EINVAL, "cache is NULL");
     if (c->dtype != FG_BF16 && c->dtype != FG_F16) return fail(FG_EINVAL, "cache dtype must be FG_BF16 or FG_F16");
     if (c->dim != 64 && c->dim != 96 && c->dim != 128 && c->dim != 256) return fail(FG_EINVAL, "dim must be 64, 96, 128 or 256");
     if (c->heads_kv < 1 || c->heads_kv > 1024) return fail(FG_EINVAL, "heads_kv must be in [1, 1024]");
     if (c->page_size < 1 || c->pages < 1 || static_cast<uint64_t>(c->pages) * c->page_size > 0x7FFFFFFFull)
         return fail(FG_EINVAL, "the cache must hold 1 to 2^31 - 1 tokens");
+    return FG_OK;
+}
+
+int check_cache(const fg_kv_cache *c, CacheView *view) {
+    if (int rc = check_cache_shape(c)) return rc;
     if (!c->k || !c->v) return fail(FG_EINVAL, "NULL cache buffer");
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16)
         return fail(FG_EINVAL, "cache buffers must be 16-byte aligned");

@@ -29,6 +29,9 @@ struct CacheView {
     FastDiv page_size;
 };
 
+// Checks a cache's sizes and type, its pointers and strides aside; FG_OK or a reported failure.
+int check_cache_shape(const fg_kv_cache *c);
+
 // Checks the cache and fills its view; FG_OK or a reported failure.
 int check_cache(const fg_kv_cache *c, CacheView *view);
 

@@ -1,0 +1,490 @@
+// fg_evict.hip -- a paged cache held to a budget: the attention weight that each token has
+// drawn, and which tokens stay.
+//
+// Weights: for token j the sum over rows of exp(scale q . k_j - lse), the column sums of the
+// matrix that attention takes row by row.  With lse known there is no maximum to follow.
+// Eviction: of n tokens the heaviest H stay, those below place H where they are; each hole
+// there takes a token from above, so only rows that have to move are read and written.
+#include "fg_blocks.hpp"
+#include "fg_pick.hpp"
+
+namespace fgk {
+namespace {
+
+// ---------------------------------------------------------------- weights
+
+constexpr uint32_t kWeighTokens = 256, kWeighRows = 64;  // tokens of a workgroup; rows in LDS at a time
+
+struct WeighParams {
+    CacheView cache;
+    const char *q;
+    int64_t q_token, q_head;  // bytes
+    const float *lse;
+    const int32_t *table, *q_starts, *kv_lens, *known;
+    int64_t table_row;
+    float *weights;
+    uint32_t table_width, requests, tokens, heads, heads_kv;
+    uint32_t spread;  // workgroups side by side over a request's tokens
+    FastDiv group;
+    float scale2;  // scale * log2(e)
+};
+
+// Each of the four waves holds the keys of 64 tokens in registers and goes through the rows,
+// which all share from LDS, 16 at a time on the matrix unit: a lane's column is a token, so
+// its sum stays in one register till the end.
+template <class T, int D>
+__global__ __launch_bounds__(256) void fg_weigh_kernel(WeighParams P) {
+    using vec = typename T::vec;
+    constexpr int STEPS = D / 32;
+    constexpr uint32_t QROW = 2 * D + 16;  // bytes of a row in LDS
+    __shared__ __attribute__((aligned(16))) char rows_of[kWeighRows * QROW];
+    __shared__ __attribute__((aligned(16))) float lse2[kWeighRows];
+    __shared__ __attribute__((aligned(16))) int32_t row_pos[kWeighRows];  // INT_MIN: the row counts nowhere
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 16, quarter = lane / 16;
+    const uint64_t items = static_cast<uint64_t>(P.requests) * P.heads_kv * P.spread;
+    for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t x = item % P.spread, rh = static_cast<uint32_t>(item / P.spread), r = rh / P.heads_kv, h = rh - r * P.heads_kv;
+        const int32_t cap = static_cast<int32_t>(P.tokens);
+        const int32_t q0 = clampi(P.q_starts[r], 0, cap), fresh = clampi(P.q_starts[r + 1], q0, cap) - q0;
+        const int32_t kv = max(P.kv_lens[r], 0), known = P.known[r], pos0 = kv - fresh;
+        const int32_t limit = static_cast<int32_t>(min(static_cast<uint64_t>(kv), static_cast<uint64_t>(P.table_width) * P.cache.page_size.d));
+        const int32_t nrows = fresh * static_cast<int32_t>(P.group.d);
+        const char *const kbase = P.cache.k + h * P.cache.k_head + quarter * 16;
+        for (int32_t j0 = static_cast<int32_t>(x * kWeighTokens); j0 < limit; j0 += static_cast<int32_t>(P.spread * kWeighTokens)) {
+            // this lane's token of the wave's 64
+            const int32_t jw = j0 + static_cast<int32_t>(wave * 64), j = jw + static_cast<int32_t>(lane);
+            int2 at = {-1, 0};
+            if (j < limit) {
+                const uint32_t b = P.cache.page_size.div(j);
+                const int32_t page = P.table[r * P.table_row + b];
+                at = {static_cast<uint32_t>(page) < P.cache.pages ? page : -1, static_cast<int32_t>(j - b * P.cache.page_size.d)};
+            }
+            vec kf[4][STEPS];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int64_t page = max(__shfl(at.x, 16 * c + static_cast<int>(col)), 0);
+                const char *src = kbase + page * P.cache.k_page + __shfl(at.y, 16 * c + static_cast<int>(col)) * P.cache.k_token;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) kf[c][s] = *reinterpret_cast<const vec *>(src + 64 * s);
+            }
+            float sum[4] = {0, 0, 0, 0};
+            // rows before position j0 see none of these tokens
+            const int32_t begin = max(j0 - pos0, 0) < fresh ? max(j0 - pos0, 0) * static_cast<int32_t>(P.group.d) : nrows;
+            for (int32_t base = begin; base < nrows; base += kWeighRows) {
+                __syncthreads();
+#pragma unroll
+                for (uint32_t e0 = 0; e0 < kWeighRows * (D / 8); e0 += 256) {
+                    const uint32_t e = e0 + tid, i = e / (D / 8), piece = e % (D / 8);
+                    const int32_t row = base + static_cast<int32_t>(i), token = P.group.div(min(row, nrows - 1));
+                    u32x4 v = {0, 0, 0, 0};
+                    if (row < nrows)
+                        v = *reinterpret_cast<const u32x4 *>(P.q + (q0 + static_cast<int64_t>(token)) * P.q_token +
+                                                             (static_cast<int64_t>(h) * P.group.d + (row - token * static_cast<int32_t>(P.group.d))) * P.q_head + piece * 16);
+                    *reinterpret_cast<u32x4 *>(rows_of + i * QROW + piece * 16) = v;
+                }
+                if (tid < kWeighRows) {
+                    const int32_t row = base + static_cast<int32_t>(tid), token = P.group.div(min(row, nrows - 1));
+                    float z = 0.0f;
+                    int32_t pos = INT32_MIN;
+                    if (row < nrows) {
+                        z = P.lse[(q0 + static_cast<int64_t>(token)) * P.heads + h * P.group.d + (row - token * static_cast<int32_t>(P.group.d))];
+                        if (z != -INFINITY) pos = pos0 + token;
+                        else z = 0.0f;
+                    }
+                    lse2[tid] = z * 1.44269504088896341f;
+                    row_pos[tid] = pos;
+                }
+                __syncthreads();
+                const int32_t here = min(nrows - base, static_cast<int32_t>(kWeighRows));
+                for (int32_t i0 = 0; i0 < here; i0 += 16) {
+                    const int32_t tail = base + min(i0 + 15, here - 1);
+                    if (pos0 + static_cast<int32_t>(P.group.div(tail)) < jw) continue;
+                    vec qf[STEPS];
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s) qf[s] = *reinterpret_cast<const vec *>(rows_of + (i0 + col) * QROW + 64 * s + 16 * quarter);
+                    const f32x4 z = *reinterpret_cast<const f32x4 *>(lse2 + i0 + 4 * quarter);
+                    const s32x4 pos = *reinterpret_cast<const s32x4 *>(row_pos + i0 + 4 * quarter);
+                    const bool all = __all(min(min(pos[0], pos[1]), min(pos[2], pos[3])) >= jw + 63);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+                        for (int k = 0; k < STEPS; ++k) s = T::mfma16(qf[k], kf[c][k], s);
+                        float p[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.scale2, -z[i]));
+                        if (!all) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) p[i] = pos[i] >= jw + 16 * c + static_cast<int32_t>(col) ? p[i] : 0.0f;
+                        }
+                        sum[c] += (p[0] + p[1]) + (p[2] + p[3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] = add_other32(add_other16(sum[c]));
+            const float mine = quarter < 2 ? (quarter == 0 ? sum[0] : sum[1]) : (quarter == 2 ? sum[2] : sum[3]);
+            if (at.x >= 0) {
+                float *to = P.weights + (static_cast<int64_t>(at.x) * P.heads_kv + h) * P.cache.page_size.d + at.y;
+                if (j >= known) *to = mine;
+                else unsafeAtomicAdd(to, mine);  // (requests that share the page add too)
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- eviction
+
+constexpr uint32_t kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
+constexpr uint32_t kChooseKeys = 32768;     // weights that a workgroup holds in LDS
+constexpr uint32_t kChooseWorkgroups = 512; // at most, where it does not
+constexpr uint32_t kEvictRequests = 4096;
+constexpr uint32_t kMoveThreads = 256, kMovePieces = 4;  // 16-byte pieces of a row that a workgroup moves
+
+struct EvictParams {
+    CacheView cache;
+    float *weights;
+    const int32_t *table, *kv_lens;
+    int64_t table_row;
+    int32_t *new_lens, *freed, *released;
+    int32_t *from, *to;  // slots, `most` for each request and head: places above H, and below
+    uint32_t *counts;    // how many
+    uint32_t *keys;      // where LDS does not hold them: `room` for each workgroup
+    uint32_t table_width, requests, heads_kv, budget, window, sinks;
+    uint32_t room;       // tokens that the table names
+    uint32_t most;       // min(budget, room)
+    uint32_t choosers;   // workgroups that choose; the others list the pages that go
+};
+
+__device__ __forceinline__ int32_t slot_of(const EvictParams &P, uint32_t r, uint32_t j) {
+    const uint32_t b = P.cache.page_size.div(j);
+    const int32_t page = P.table[r * P.table_row + b];
+    return static_cast<uint32_t>(page) < P.cache.pages ? static_cast<int32_t>(page * P.cache.page_size.d + (j - b * P.cache.page_size.d)) : -1;
+}
+__device__ __forceinline__ int64_t weight_at(const EvictParams &P, uint32_t h, int32_t slot) {
+    const uint32_t page = P.cache.page_size.div(slot);
+    return (static_cast<int64_t>(page) * P.heads_kv + h) * P.cache.page_size.d + (slot - page * P.cache.page_size.d);
+}
+__device__ __forceinline__ uint32_t length_of(const EvictParams &P, uint32_t r) { return min(static_cast<uint32_t>(max(P.kv_lens[r], 0)), P.room); }
+__device__ __forceinline__ uint32_t pages_of(const EvictParams &P, uint32_t n) {
+    const uint32_t whole = P.cache.page_size.div(n);
+    return whole + (whole * P.cache.page_size.d != n ? 1 : 0);
+}
+
+// The new lengths, and the pages that go one after another: every workgroup sums the lengths itself.
+__device__ __forceinline__ void list_freed(const EvictParams &P, uint32_t w, uint32_t workgroups, uint32_t *first, uint32_t *sums) {
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, run = (P.requests + kChooseThreads - 1) / kChooseThreads;
+    uint32_t mine = 0;
+    for (uint32_t i = 0; i < run; ++i) {
+        const uint32_t r = tid * run + i;
+        if (r >= P.requests) break;
+        const uint32_t n = length_of(P, r), left = min(n, P.budget);
+        first[r] = mine;
+        mine += pages_of(P, n) - pages_of(P, left);
+        if (w == 0) P.new_lens[r] = static_cast<int32_t>(left);
+    }
+    uint32_t upto = mine;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    uint32_t before = upto - mine, all = 0;
+    for (uint32_t i = 0; i < kChooseWaves; ++i) {
+        if (i < wave) before += sums[i];
+        all += sums[i];
+    }
+    for (uint32_t i = 0; i < run && tid * run + i < P.requests; ++i) first[tid * run + i] += before;
+    __syncthreads();
+    if (w == 0 && tid == 0) P.released[0] = static_cast<int32_t>(all);
+    const uint32_t entries = P.requests * P.table_width;
+    for (uint32_t f = w * kChooseThreads + tid; f < entries; f += workgroups * kChooseThreads) {
+        int32_t page = -1;
+        if (f < all) {
+            uint32_t r = 0;  // the last request whose pages begin at or before f
+            for (uint32_t step = 1u << (31 - __clz(P.requests)); step; step >>= 1)
+                if (r + step < P.requests && first[r + step] <= f) r += step;
+            page = P.table[r * P.table_row + pages_of(P, min(length_of(P, r), P.budget)) + (f - first[r])];
+        }
+        P.freed[f] = page;
+    }
+}
+
+// A workgroup for a request and head: weights as ordered integers, the border of the heaviest,
+// then which slots move where.
+template <bool HELD>
+__global__ __launch_bounds__(kChooseThreads) void fg_evict_choose_kernel(EvictParams P) {
+    extern __shared__ uint32_t dynamic[];
+    __shared__ Picking<kChooseWaves> S;
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64);
+    if (blockIdx.x >= P.choosers) {
+        list_freed(P, blockIdx.x - P.choosers, gridDim.x - P.choosers, dynamic, S.least);
+        return;
+    }
+    uint32_t *const keys = HELD ? dynamic : P.keys + static_cast<uint64_t>(blockIdx.x) * P.room;
+    for (uint32_t rh = blockIdx.x; rh < P.requests * P.heads_kv; rh += P.choosers) {
+        const uint32_t r = rh / P.heads_kv, h = rh - r * P.heads_kv, n = length_of(P, r);
+        if (n <= P.budget) {
+            if (tid == 0) P.counts[rh] = 0;
+            continue;
+        }
+        // tokens sinks .. end - 1 are chosen from: `want` of them, so that `keep` stand before the last ones
+        const uint32_t end = n - P.window, keep = P.budget - P.window, want = keep - P.sinks, span = end - P.sinks;
+#pragma unroll 4
+        for (uint32_t i = tid; i < span; i += kChooseThreads) {
+            const int32_t slot = slot_of(P, r, P.sinks + i);
+            uint32_t key = 1;
+            if (slot >= 0) {
+                const float x = P.weights[weight_at(P, h, slot)];
+                key = x != x ? key_of(INFINITY) : key_of(x + 0.0f);  // (-0 as 0)
+            }
+            keys[i] = key;
+        }
+        __syncthreads();
+        Border B{0xFFFFFFFFu, 0, 0};
+        if (want) B = border_of<kChooseWaves>(static_cast<const uint32_t *>(keys), span, want, S);
+        const Run run = run_of<kChooseWaves>(span);
+        uint32_t same = 0;
+#pragma unroll 4
+        for (uint32_t i = run.begin + lane; i < run.end; i += 64) same += keys[i] == B.border;
+        same = wave_sum(same);
+        if (lane == 0) S.count[0][wave] = same;
+        __syncthreads();
+        uint32_t equal = 0;
+        for (uint32_t w = 0; w < wave; ++w) equal += S.count[0][w];
+        __syncthreads();
+        const uint32_t equal0 = equal, low = keep - P.sinks;  // places from `low` on are above
+        uint32_t holes = 0, late = 0;
+        for (uint32_t i0 = run.begin; i0 < run.end; i0 += 64) {
+            const uint32_t i = i0 + lane;
+            const bool in = i < run.end, take = taken(B, in ? keys[i] : 0u, equal) && want;
+            holes += __popcll(__ballot(in && i < low && !take));
+            late += __popcll(__ballot(in && i >= low && take));
+        }
+        if (lane == 0) S.count[0][wave] = holes, S.count[1][wave] = late;
+        __syncthreads();
+        uint32_t at_hole = 0, at_late = 0, moved = 0;
+        for (uint32_t w = 0; w < kChooseWaves; ++w) {
+            if (w < wave) at_hole += S.count[0][w], at_late += S.count[1][w];
+            moved += S.count[0][w];
+        }
+        int32_t *const to = P.to + static_cast<uint64_t>(rh) * P.most, *const from = P.from + static_cast<uint64_t>(rh) * P.most;
+        equal = equal0;
+        for (uint32_t i0 = run.begin; i0 < run.end; i0 += 64) {
+            const uint32_t i = i0 + lane;
+            const bool in = i < run.end, take = taken(B, in ? keys[i] : 0u, equal) && want;
+            const bool hole = in && i < low && !take, above = in && i >= low && take;
+            const uint64_t hs = __ballot(hole), as = __ballot(above), below = (1ull << lane) - 1;
+            if (hole) to[at_hole + __popcll(hs & below)] = slot_of(P, r, P.sinks + i);
+            if (above) from[at_late + __popcll(as & below)] = slot_of(P, r, P.sinks + i);
+            at_hole += __popcll(hs), at_late += __popcll(as);
+        }
+        if (tid == 0) P.counts[rh] = moved;
+        __syncthreads();
+    }
+}
+
+// A workgroup moves 64 bytes of every row of a request and head: the chosen ones, from above
+// into the holes below, which no other move touches; then the last `window` in order.  Those may
+// go to places that others of them leave, but never to one that a later step reads, so a step
+// loads all of its rows before it writes any.
+__global__ __launch_bounds__(kMoveThreads) void fg_evict_move_kernel(EvictParams P, uint32_t pieces) {
+    constexpr uint32_t ROWS = kMoveThreads / kMovePieces, U = 4;
+    const uint32_t tid = threadIdx.x, slice = blockIdx.x, h = blockIdx.y, r = blockIdx.z, rh = r * P.heads_kv + h;
+    const uint32_t n = length_of(P, r);
+    if (n <= P.budget) return;
+    const uint32_t piece = slice * kMovePieces + tid % kMovePieces, row = tid / kMovePieces;  // pieces of keys, then of values
+    const bool value = piece >= pieces, works = piece < 2 * pieces, weighs = piece == 0;
+    char *const base = const_cast<char *>(value ? P.cache.v + h * P.cache.v_head : P.cache.k + h * P.cache.k_head) + (value ? piece - pieces : piece) * 16;
+    const int64_t page_step = value ? P.cache.v_page : P.cache.k_page, token_step = value ? P.cache.v_token : P.cache.k_token;
+    const auto place = [&](int32_t slot) {
+        const uint32_t page = P.cache.page_size.div(slot);
+        return base + page * page_step + (slot - page * P.cache.page_size.d) * token_step;
+    };
+    const auto move = [&](uint32_t count, auto source, auto target) {
+        for (uint32_t i0 = 0; i0 < count; i0 += ROWS * U) {
+            int32_t from[U], to[U];
+            u32x4 x[U];
+            float w[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t i = i0 + u * ROWS + row;
+                const bool in = works && i < count;
+                from[u] = in ? source(i) : -1;
+                to[u] = in ? target(i) : -1;
+                if (from[u] < 0) to[u] = -1;
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                x[u] = u32x4{0, 0, 0, 0};
+                w[u] = 0.0f;
+                if (to[u] >= 0) x[u] = *reinterpret_cast<const u32x4 *>(place(from[u]));
+                if (to[u] >= 0 && weighs) w[u] = P.weights[weight_at(P, h, from[u])];
+            }
+            wait_loads();
+            __syncthreads();
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                if (to[u] >= 0) *reinterpret_cast<u32x4 *>(place(to[u])) = x[u];
+                if (to[u] >= 0 && weighs) P.weights[weight_at(P, h, to[u])] = w[u];
+            }
+        }
+    };
+    const int32_t *const from = P.from + static_cast<uint64_t>(rh) * P.most, *const to = P.to + static_cast<uint64_t>(rh) * P.most;
+    move(P.counts[rh], [&](uint32_t i) { return from[i]; }, [&](uint32_t i) { return to[i]; });
+    __syncthreads();
+    move(P.window, [&](uint32_t i) { return slot_of(P, r, n - P.window + i); }, [&](uint32_t i) { return slot_of(P, r, P.budget - P.window + i); });
+}
+
+// ---------------------------------------------------------------- host side
+
+template <class T>
+void launch_weigh(const WeighParams &P, uint32_t dim, uint32_t grid, hipStream_t st) {
+    switch (dim) {
+    case 64: hipLaunchKernelGGL((fg_weigh_kernel<T, 64>), dim3(grid), dim3(256), 0, st, P); break;
+    case 96: hipLaunchKernelGGL((fg_weigh_kernel<T, 96>), dim3(grid), dim3(256), 0, st, P); break;
+    case 128: hipLaunchKernelGGL((fg_weigh_kernel<T, 128>), dim3(grid), dim3(256), 0, st, P); break;
+    default: hipLaunchKernelGGL((fg_weigh_kernel<T, 256>), dim3(grid), dim3(256), 0, st, P); break;
+    }
+}
+
+int weigh(const fg_kv_cache *c, const fg_attention *a, float *weights, const int32_t *known, void *stream) {
+    WeighParams P{};
+    if (int rc = check_cache(c, &P.cache)) return rc;
+    if (!a) return fail(FG_EINVAL, "attention arguments are NULL");
+    if (a->heads < 1 || a->heads > 1024 || a->heads % c->heads_kv) return fail(FG_EINVAL, "heads must be a multiple of heads_kv, at most 1024");
+    if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return fail(FG_EINVAL, "scale must be positive and finite");
+    if (static_cast<uint64_t>(a->tokens) * a->heads > 0x7FFFFFFFull) return fail(FG_EINVAL, "tokens * heads must be below 2^31");
+    if (a->table_width > 0x7FFFFFFFu || a->table_row < 0) return fail(FG_EINVAL, "table_width or table_row out of range");
+    if (static_cast<uint64_t>(a->table_width) * c->page_size > 0x3FFFFFFFull) return fail(FG_EINVAL, "table_width * page_size must be below 2^30");
+    if (a->requests > 65536) return fail(FG_EINVAL, "requests must be at most 65,536");
+    if (a->requests == 0) return FG_OK;
+    if (!a->kv_lens || !a->q_starts || !known || !weights || (a->tokens && (!a->q || !a->lse)) || (a->table_width && !a->table))
+        return fail(FG_EINVAL, "NULL device buffer");
+    if (reinterpret_cast<uintptr_t>(a->q) % 16 || (a->q_token | a->q_head) % 8) return fail(FG_EINVAL, "q must be 16-byte aligned, strides multiples of 8 elements");
+    P.q = static_cast<const char *>(a->q);
+    P.q_token = 2 * a->q_token, P.q_head = 2 * a->q_head;
+    P.lse = a->lse;
+    P.table = a->table;
+    P.q_starts = a->q_starts;
+    P.kv_lens = a->kv_lens;
+    P.known = known;
+    P.table_row = a->table_row;
+    P.weights = weights;
+    P.table_width = a->table_width;
+    P.requests = a->requests;
+    P.tokens = a->tokens;
+    P.heads = a->heads;
+    P.heads_kv = c->heads_kv;
+    P.group = fast_div(a->heads / c->heads_kv);
+    P.scale2 = a->scale * 1.44269504088896341f;
+    const uint64_t pairs = static_cast<uint64_t>(a->requests) * c->heads_kv;
+    const uint64_t tiles = (static_cast<uint64_t>(a->table_width) * c->page_size + kWeighTokens - 1) / kWeighTokens;
+    if (tiles == 0) return FG_OK;
+    // a workgroup a tile, up to 16,384 of them
+    P.spread = static_cast<uint32_t>(std::min<uint64_t>(tiles, std::max<uint64_t>(1, 16384 / pairs)));
+    const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(pairs * P.spread, 65536));
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (c->dtype == FG_BF16) launch_weigh<BF16>(P, c->dim, grid, st);
+    else launch_weigh<F16>(P, c->dim, grid, st);
+    FG_HIP(hipGetLastError(), "weigh launch");
+    return FG_OK;
+}
+
+struct EvictPlan {
+    bool held;
+    uint64_t from, counts, keys, workspace;
+};
+
+int plan_evict(const fg_kv_cache *c, uint32_t table_width, uint32_t requests, uint32_t budget, EvictParams *out, EvictPlan *plan) {
+    EvictParams &P = *out;
+    if (int rc = check_cache_shape(c)) return rc;
+    if (requests < 1 || requests > kEvictRequests) return fail(FG_EINVAL, "requests must be in [1, 4096]");
+    if (budget < 1 || budget > 0x7FFFFFFFu) return fail(FG_EINVAL, "budget must be in [1, 2^31)");
+    if (static_cast<uint64_t>(table_width) * c->page_size > 0x3FFFFFFFull) return fail(FG_EINVAL, "table_width * page_size must be below 2^30");
+    if (table_width > 0x7FFFFFFFu / requests) return fail(FG_EINVAL, "requests * table_width must be below 2^31");
+    P.table_width = table_width;
+    P.requests = requests;
+    P.heads_kv = c->heads_kv;
+    P.budget = budget;
+    P.room = table_width * c->page_size;
+    P.most = std::min(budget, P.room);
+    const uint64_t pairs = static_cast<uint64_t>(requests) * c->heads_kv, slots = pairs * P.most;
+    plan->held = P.room <= kChooseKeys;
+    P.choosers = static_cast<uint32_t>(plan->held ? pairs : std::min<uint64_t>(pairs, kChooseWorkgroups));
+    plan->from = slots * 4;
+    plan->counts = slots * 8;
+    plan->keys = plan->counts + (pairs * 4 + 15) / 16 * 16;
+    plan->workspace = plan->keys + (plan->held ? 0 : static_cast<uint64_t>(P.choosers) * P.room * 4);
+    return FG_OK;
+}
+
+}  // namespace
+}  // namespace fgk
+
+using namespace fgk;
+
+extern "C" {
+
+int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_weights, const int32_t *d_known, void *stream) {
+    return guarded<int>([&] { return weigh(cache, a, d_weights, d_known, stream); });
+}
+
+int64_t fg_cache_evict_workspace_bytes(const fg_kv_cache *cache, uint32_t table_width, uint32_t requests, uint32_t budget) {
+    return guarded<int64_t>([&]() -> int64_t {
+        EvictParams P{};
+        EvictPlan plan;
+        if (int rc = plan_evict(cache, table_width, requests, budget, &P, &plan)) return rc;
+        return static_cast<int64_t>(plan.workspace);
+    });
+}
+
+int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_table, int64_t table_row, uint32_t table_width,
+                   const int32_t *d_kv_lens, uint32_t requests, uint32_t budget, uint32_t window, uint32_t sinks,
+                   int32_t *d_new_lens, int32_t *d_freed, int32_t *d_released, void *workspace, uint64_t workspace_bytes,
+                   void *stream) {
+    return guarded<int>([&]() -> int {
+        EvictParams P{};
+        EvictPlan plan;
+        if (int rc = plan_evict(cache, table_width, requests, budget, &P, &plan)) return rc;
+        if (int rc = check_cache(cache, &P.cache)) return rc;
+        if (static_cast<uint64_t>(window) + sinks > budget) return fail(FG_EINVAL, "window + sinks must be at most budget");
+        if (table_row < 0) return fail(FG_EINVAL, "table_row out of range");
+        if (!d_weights || !d_kv_lens || !d_new_lens || !d_released || (table_width && (!d_table || !d_freed))) return fail(FG_EINVAL, "NULL device buffer");
+        if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < plan.workspace)
+            return fail(FG_EINVAL, "workspace must be 16-byte aligned and hold " + std::to_string(plan.workspace) + " bytes");
+        char *base = static_cast<char *>(workspace);
+        P.weights = d_weights;
+        P.table = d_table;
+        P.kv_lens = d_kv_lens;
+        P.table_row = table_row;
+        P.new_lens = d_new_lens;
+        P.freed = d_freed;
+        P.released = d_released;
+        P.to = reinterpret_cast<int32_t *>(base);
+        P.from = reinterpret_cast<int32_t *>(base + plan.from);
+        P.counts = reinterpret_cast<uint32_t *>(base + plan.counts);
+        P.keys = reinterpret_cast<uint32_t *>(base + plan.keys);
+        P.window = window;
+        P.sinks = sinks;
+        hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+        const uint64_t entries = static_cast<uint64_t>(requests) * table_width;
+        const uint32_t listers = static_cast<uint32_t>(std::min<uint64_t>(64, 1 + entries / (4 * kChooseThreads)));
+        const uint32_t lds = std::max<uint32_t>(plan.held ? P.room * 4 : 0, requests * 4);
+        if (plan.held) {
+            FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(fg_evict_choose_kernel<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kChooseKeys * 4), "eviction LDS");
+            hipLaunchKernelGGL(fg_evict_choose_kernel<true>, dim3(P.choosers + listers), dim3(kChooseThreads), lds, st, P);
+        } else {
+            hipLaunchKernelGGL(fg_evict_choose_kernel<false>, dim3(P.choosers + listers), dim3(kChooseThreads), lds, st, P);
+        }
+        const uint32_t pieces = cache->dim / 8, slices = (2 * pieces + kMovePieces - 1) / kMovePieces;
+        if (P.room > budget)
+            hipLaunchKernelGGL(fg_evict_move_kernel, dim3(slices, cache->heads_kv, requests), dim3(kMoveThreads), 0, st, P, pieces);
+        FG_HIP(hipGetLastError(), "eviction launch");
+        return FG_OK;
+    });
+}
+
+}  // extern "C"

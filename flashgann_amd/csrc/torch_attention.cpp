@@ -276,10 +276,197 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
-PyMethodDef kMethods[] = {{"cache_plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_plan)), METH_FASTCALL, nullptr},
-                          {"cache_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_append)), METH_FASTCALL, nullptr},
-                          {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
-                          {nullptr, nullptr, 0, nullptr}};
+// What calls over rows of q share: q, its requests and their table.
+struct Rows {
+    int64_t tokens, heads, requests;
+    fg_attention p{};
+};
+Rows rows_of(const Call &c, const at::Tensor &q, int64_t dim, PyObject *table, PyObject *q_starts, PyObject *lens) {
+    Rows w;
+    need(q.dim() == 3 && q.size(2) == dim && c.has(q), "q must have shape (tokens, heads, dim), on the same device");
+    w.tokens = q.size(0), w.heads = q.size(1);
+    need(w.tokens <= kMost && w.heads <= kMost, "q is too large");
+    need(q.stride(2) == 1 || !w.tokens, "the last dimension of q must be contiguous");
+    const at::Tensor &kv_lens = tensor(lens, "kv_lens");
+    need(kv_lens.dim() == 1 && kv_lens.size(0) <= kMost, "kv_lens must be a vector");
+    w.requests = kv_lens.size(0);
+    const Table t = table_of(c, table, w.requests);
+    w.p.q = q.data_ptr();
+    w.p.q_token = q.stride(0), w.p.q_head = q.stride(1);
+    w.p.table = t.at, w.p.table_row = t.row, w.p.table_width = t.width;
+    w.p.kv_lens = static_cast<int32_t *>(vector_of(c, lens, w.requests, at::kInt, "kv_lens"));
+    w.p.q_starts = static_cast<int32_t *>(vector_of(c, q_starts, w.requests + 1, at::kInt, "q_starts"));
+    w.p.requests = u32(w.requests);
+    w.p.tokens = u32(w.tokens);
+    w.p.heads = u32(w.heads);
+    return w;
+}
+
+float scale_of(PyObject *o, int64_t dim) {
+    const float s = static_cast<float>(o == Py_None ? 1.0 / std::sqrt(static_cast<double>(dim)) : PyFloat_AsDouble(o));
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        throw Refused("scale must be a number");
+    }
+    return s;
+}
+
+at::Tensor workspace(const Call &c, int64_t bytes) {
+    if (bytes < 0) throw Failed{static_cast<int>(bytes)};
+    return bytes ? c.empty({bytes}, at::kByte) : at::Tensor();
+}
+void *start_of(const at::Tensor &work) { return work.defined() ? work.data_ptr() : nullptr; }
+
+// (codes, scales) of a cache's pages
+void bounds_of(const Call &c, const at::Tensor &bounds, const at::Tensor &scales) {
+    need(bounds.dim() == 4 && bounds.size(2) == 2 && bounds.scalar_type() == at::kChar && c.has(bounds) && bounds.is_contiguous(),
+         "bounds must be contiguous int8 of shape (pages, heads_kv, 2, dim) on the same device");
+    need(scales.dim() == 2 && scales.size(0) == bounds.size(0) && scales.size(1) == bounds.size(1) && scales.scalar_type() == at::kFloat &&
+             c.has(scales) && scales.is_contiguous(),
+         "scales must be contiguous float32 of shape (pages, heads_kv) on the same device");
+}
+
+// (k_cache, slots, bounds, scales)
+PyObject *cache_bounds(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        need(n == 4, "cache_bounds takes 4 arguments");
+        const at::Tensor &k = tensor(a[0], "k_cache"), &slots = tensor(a[1], "slots"), &bounds = tensor(a[2], "bounds"), &scales = tensor(a[3], "scales");
+        no_gradient({&k, &scales});
+        const Call c(k);
+        const fg_kv_cache cache = cache_of(c, k, k);
+        bounds_of(c, bounds, scales);
+        need(bounds.size(0) == k.size(0) && bounds.size(1) == k.size(2) && bounds.size(3) == k.size(3), "bounds must have shape (pages, heads_kv, 2, dim)");
+        need(slots.dim() == 1 && slots.size(0) <= kMost, "slots must be a vector");
+        const int64_t tokens = slots.size(0);
+        const auto *at = static_cast<int64_t *>(vector_of(c, a[1], tokens, at::kLong, "slots"));
+        check(fg_cache_bounds(&cache, at, u32(tokens), static_cast<int8_t *>(bounds.data_ptr()), static_cast<float *>(scales.data_ptr()), c.stream));
+        if (tokens) written({&bounds, &scales});
+        Py_RETURN_NONE;
+    });
+}
+
+// (q, bounds, scales, block_table, q_starts, kv_lens, page_size, k, lists | None, first_blocks, last_blocks) -> ids
+PyObject *select_blocks(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&] {
+        need(n == 11, "select_blocks takes 11 arguments");
+        const at::Tensor &q = tensor(a[0], "q"), &bounds = tensor(a[1], "bounds"), &scales = tensor(a[2], "scales");
+        no_gradient({&q, &scales});
+        const Call c(q);
+        bounds_of(c, bounds, scales);
+        need(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "q must be bfloat16 or float16");
+        for (int i = 0; i < 4; ++i) need(bounds.size(i) <= kMost, "bounds are too large");
+        fg_kv_cache cache{};
+        cache.pages = u32(bounds.size(0)), cache.heads_kv = u32(bounds.size(1)), cache.dim = u32(bounds.size(3));
+        cache.page_size = u32(integer(a[6], "page_size", 1, kMost));
+        cache.dtype = q.scalar_type() == at::kBFloat16 ? FG_BF16 : FG_F16;
+        Rows w = rows_of(c, q, bounds.size(3), a[3], a[4], a[5]);
+        w.p.nids = u32(integer(a[7], "k", 1, kMost));
+        w.p.lists = a[8] == Py_None ? cache.heads_kv : u32(integer(a[8], "lists", 1, kMost));
+        w.p.sinks = u32(integer(a[9], "first_blocks", 0, kMost));
+        w.p.window = static_cast<int32_t>(integer(a[10], "last_blocks", 1, kMost));
+        const int64_t bytes = fg_select_blocks_workspace_bytes(&cache, &w.p);
+        const at::Tensor work = workspace(c, bytes);
+        at::Tensor ids = c.empty({w.tokens, static_cast<int64_t>(w.p.lists), static_cast<int64_t>(w.p.nids)}, at::kInt);
+        check(fg_select_blocks(&cache, &w.p, static_cast<int8_t *>(bounds.data_ptr()), static_cast<float *>(scales.data_ptr()),
+                               static_cast<int32_t *>(ids.data_ptr()), start_of(work), static_cast<uint64_t>(bytes), c.stream));
+        return wrap(ids);
+    });
+}
+
+// (q, k_cache, v_cache, block_table, q_starts, kv_lens, ids, first_blocks, last_blocks, scale | None, out | None, lse | None) -> (out, lse)
+PyObject *attend_blocks(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&] {
+        need(n == 12, "attend_blocks takes 12 arguments");
+        const at::Tensor &q = tensor(a[0], "q"), &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache"), &ids = tensor(a[6], "ids");
+        no_gradient({&q, &kc, &vc});
+        const Call c(q);
+        const fg_kv_cache cache = cache_of(c, kc, vc);
+        need(q.scalar_type() == kc.scalar_type(), "q must have the cache's type");
+        Rows w = rows_of(c, q, kc.size(3), a[3], a[4], a[5]);
+        need(ids.dim() == 3 && ids.size(0) == w.tokens && ids.scalar_type() == at::kInt && c.has(ids) && ids.is_contiguous() && ids.size(1) <= kMost &&
+                 ids.size(2) <= kMost,
+             "ids must be contiguous int32 of shape (tokens, lists, k) on the same device");
+        at::Tensor out = a[10] == Py_None ? c.empty({w.tokens, w.heads, q.size(2)}, q.scalar_type()) : tensor(a[10], "out");
+        at::Tensor lse = a[11] == Py_None ? c.empty({w.tokens, w.heads}, at::kFloat) : tensor(a[11], "lse");
+        no_gradient({&out, &lse});
+        need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && c.has(out) && (out.stride(2) == 1 || !w.tokens),
+             "out must have q's shape and type, its last dimension contiguous, on the same device");
+        need(lse.dim() == 2 && lse.size(0) == w.tokens && lse.size(1) == w.heads && lse.scalar_type() == at::kFloat && c.has(lse) && lse.is_contiguous(),
+             "lse must be contiguous float32 of shape (tokens, heads) on the same device");
+        w.p.out = out.data_ptr();
+        w.p.out_token = out.stride(0), w.p.out_head = out.stride(1);
+        w.p.lse = static_cast<float *>(lse.data_ptr());
+        w.p.ids = reinterpret_cast<uint32_t *>(ids.data_ptr());
+        w.p.lists = u32(ids.size(1)), w.p.nids = u32(ids.size(2));
+        w.p.sinks = u32(integer(a[7], "first_blocks", 0, kMost));
+        w.p.window = static_cast<int32_t>(integer(a[8], "last_blocks", 1, kMost));
+        w.p.scale = scale_of(a[9], q.size(2));
+        const int64_t bytes = fg_attend_blocks_workspace_bytes(&cache, &w.p);
+        const at::Tensor work = workspace(c, bytes);
+        check(fg_attend_blocks(&cache, &w.p, start_of(work), static_cast<uint64_t>(bytes), c.stream));
+        if (a[10] != Py_None) written({&out});
+        if (a[11] != Py_None) written({&lse});
+        return pack({out, lse});
+    });
+}
+
+void weights_of(const Call &c, const at::Tensor &weights, const at::Tensor &k) {
+    need(weights.dim() == 3 && weights.size(0) == k.size(0) && weights.size(1) == k.size(2) && weights.size(2) == k.size(1) &&
+             weights.scalar_type() == at::kFloat && c.has(weights) && weights.is_contiguous(),
+         "weights must be contiguous float32 of shape (pages, heads_kv, page_size) on the same device");
+}
+
+// (q, k_cache, block_table, q_starts, kv_lens, lse, weights, known, scale | None)
+PyObject *cache_weigh(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        need(n == 9, "cache_weigh takes 9 arguments");
+        const at::Tensor &q = tensor(a[0], "q"), &kc = tensor(a[1], "k_cache"), &lse = tensor(a[5], "lse"), &weights = tensor(a[6], "weights");
+        no_gradient({&q, &kc, &lse, &weights});
+        const Call c(q);
+        const fg_kv_cache cache = cache_of(c, kc, kc);
+        need(q.scalar_type() == kc.scalar_type(), "q must have the cache's type");
+        Rows w = rows_of(c, q, kc.size(3), a[2], a[3], a[4]);
+        need(lse.dim() == 2 && lse.size(0) == w.tokens && lse.size(1) == w.heads && lse.scalar_type() == at::kFloat && c.has(lse) && lse.is_contiguous(),
+             "lse must be contiguous float32 of shape (tokens, heads) on the same device");
+        weights_of(c, weights, kc);
+        const auto *known = static_cast<int32_t *>(vector_of(c, a[7], w.requests, at::kInt, "known"));
+        w.p.lse = static_cast<float *>(lse.data_ptr());
+        w.p.scale = scale_of(a[8], q.size(2));
+        check(fg_cache_weigh(&cache, &w.p, static_cast<float *>(weights.data_ptr()), known, c.stream));
+        written({&weights});
+        Py_RETURN_NONE;
+    });
+}
+
+// (k_cache, v_cache, weights, block_table, kv_lens, budget, window, sinks) -> (kv_lens, freed, released)
+PyObject *cache_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&] {
+        need(n == 8, "cache_evict takes 8 arguments");
+        const at::Tensor &kc = tensor(a[0], "k_cache"), &vc = tensor(a[1], "v_cache"), &weights = tensor(a[2], "weights");
+        no_gradient({&kc, &vc, &weights});
+        const Call c(kc);
+        const fg_kv_cache cache = cache_of(c, kc, vc);
+        weights_of(c, weights, kc);
+        const at::Tensor &kv_lens = tensor(a[4], "kv_lens");
+        need(kv_lens.dim() == 1 && kv_lens.size(0) <= kMost, "kv_lens must be a vector");
+        const int64_t requests = kv_lens.size(0);
+        const Table t = table_of(c, a[3], requests);
+        const auto *lens = static_cast<int32_t *>(vector_of(c, a[4], requests, at::kInt, "kv_lens"));
+        const uint32_t budget = u32(integer(a[5], "budget", 1, kMost)), window = u32(integer(a[6], "window", 0, kMost)), sinks = u32(integer(a[7], "sinks", 0, kMost));
+        const int64_t bytes = fg_cache_evict_workspace_bytes(&cache, t.width, u32(requests), budget);
+        const at::Tensor work = workspace(c, bytes);
+        at::Tensor left = c.empty({requests}, at::kInt), freed = c.empty({requests * t.width}, at::kInt), released = c.empty({1}, at::kInt);
+        check(fg_cache_evict(&cache, static_cast<float *>(weights.data_ptr()), t.at, t.row, t.width, lens, u32(requests), budget, window, sinks,
+                             static_cast<int32_t *>(left.data_ptr()), static_cast<int32_t *>(freed.data_ptr()), static_cast<int32_t *>(released.data_ptr()),
+                             start_of(work), static_cast<uint64_t>(bytes), c.stream));
+        written({&kc, &vc, &weights});
+        return pack({left, freed, released});
+    });
+}
+
+#define FG_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+PyMethodDef kMethods[] = {FG_METHOD(cache_plan), FG_METHOD(cache_append), FG_METHOD(attend), FG_METHOD(cache_bounds), FG_METHOD(select_blocks),
+                          FG_METHOD(attend_blocks), FG_METHOD(cache_weigh), FG_METHOD(cache_evict), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_attention", "The cache and attention entry points for torch tensors.", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -364,6 +364,94 @@ int fg_attend_retrieved(const fg_kv_cache *cache, const fg_attention *a, void *w
  * call would refuse. */
 int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
 
+/* Attention over selected pages, where no index is built over the keys: a bound of each
+ * page's keys (fg_cache_bounds) gives every page a score for a query, fg_select_blocks
+ * picks the pages that score highest, fg_attend_blocks attends to them.  A block is a
+ * page of the cache: block b of a request holds its tokens b * page_size and on.  In
+ * these calls fg_attention's sinks and window count blocks: the row at position p, whose
+ * block is c = p div page_size, sees of the tokens j <= p those of the first `sinks`
+ * blocks, of the last `window` ones (c - window + 1 .. c, window >= 1), and of the blocks
+ * on its list, which lie between: sinks <= b <= c - window. */
+
+/* For each of `tokens` slots that is the last of its page, 8-bit bounds of that page's keys
+ * (cache->v is not read): with M the largest |key| of a page and key/value head and 2^s the
+ * least power of two with M <= 127 * 2^s, not below 2^-126,
+ *   d_scales[page * heads_kv + head]                       2^s
+ *   d_bounds[((page * heads_kv + head) * 2 + 0) * dim + d] the largest key of channel d / 2^s, rounded up
+ *   d_bounds[((page * heads_kv + head) * 2 + 1) * dim + d] the smallest, rounded down
+ * so every key lies between its bounds times 2^s.  A page with an infinity or NaN among
+ * the head's keys gets scale +infinity and bounds 0.  The slots are fg_cache_append's, so a
+ * page's bounds are there once it is full; pages without them are not read by
+ * fg_select_blocks as long as window >= 1.  Keys that are moved or written again need
+ * their pages' last slots passed again.  d_bounds 16-byte aligned. */
+int fg_cache_bounds(const fg_kv_cache *cache, const int64_t *d_slots, uint32_t tokens, int8_t *d_bounds, float *d_scales,
+                    void *stream);
+
+/* The a->nids blocks that score highest for each row of q and each of a->lists lists, ids
+ * ascending, -1 behind them: d_ids[(token * lists + list) * nids + i].  lists is a multiple
+ * of heads_kv that divides heads, as for fg_attend_retrieved.  With q+ and q- the sums over a
+ * list's query heads, in order and in 32 bits, of max(q, 0) and min(q, 0), and c+ and c- those
+ * divided by the least power of two that leaves 127 at most (as for the bounds) and rounded
+ * to the nearest integer, ties to even:
+ *   score(b) = 2^s (c+ . upper bounds + c- . lower bounds)
+ * which is, rounding of c aside, the sum over the heads of the most that a key of block b can
+ * give q . k.  It is exact in 32 bits (an integer below 2^24 times a power of two; what is past
+ * the largest float is infinite), so the same blocks come out however the work is split;
+ * equal scores go to the lower block.  A block of scale +infinity scores +infinity; a row
+ * whose q+ or q- is not finite has c+ = c- = 0.  Only blocks between the first and the last
+ * ones whose table entry names a page are selected.  cache gives the shape and dtype (of
+ * q); its k and v are not read and may be NULL.  a: q, table, q_starts, kv_lens, sinks, window,
+ * lists, nids (1 or more, at most 4,096); out, lse, ids, scale and max_q are not used.  Rows outside every
+ * request are left alone.  tokens at most 4,194,304, tokens * lists * nids < 2^31. */
+int fg_select_blocks(const fg_kv_cache *cache, const fg_attention *a, const int8_t *d_bounds, const float *d_scales,
+                     int32_t *d_ids, void *workspace, uint64_t workspace_bytes, void *stream);
+int64_t fg_select_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
+
+/* Attention of chunks of new tokens (rows as for fg_attend) over the first and last blocks
+ * and those of lists: a->ids is (tokens, lists, nids) int32, a list for each row and `lists`,
+ * as fg_select_blocks writes them.  An id that is not above all before it in its list, or
+ * lies outside [sinks, c - window], adds nothing.  nids at most 4,096, 0 allowed; tokens
+ * at most 4,194,304. */
+int fg_attend_blocks(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes,
+                     void *stream);
+int64_t fg_attend_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
+
+/* Holding a cache to a budget: fg_cache_weigh sums the attention weight that each cached token
+ * draws, fg_cache_evict keeps the tokens that drew most.
+ *
+ * d_weights is float32 of shape (pages, heads_kv, page_size), contiguous: a weight for each
+ * slot and key/value head.  For token j of request r and its slot,
+ *   weight (+)= sum over the request's rows of q at positions p >= j and the query heads of
+ *               the key/value head of exp(scale q . k_j - lse)
+ * with q's rows placed as for fg_attend and a->lse, read here, what fg_attend gave for them.
+ * Tokens j >= d_known[r] have no weight yet: theirs is set, the others' is added to.  A row
+ * whose lse is -infinity adds nothing; a token without a page gets no weight.  Of rows that
+ * are not all given (the last ones of a prompt, say) the sum is over those.  Pages that
+ * several requests of a call share add up (in no fixed order).  a: q, lse, table, q_starts,
+ * kv_lens, scale; cache->v is not read. */
+int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_weights, const int32_t *d_known,
+                   void *stream);
+
+/* Each request of more than `budget` tokens back to budget: for each key/value head its first
+ * `sinks` tokens stay, its last `window` ones, and of those between the ones of largest
+ * weight (equal ones: the earlier; NaN counts as +infinity, a token without a page as less than any).
+ * With H = budget - window, kept tokens below place H stay where they are; those above move,
+ * in order, to the places below H whose tokens go, also in order; the last `window` tokens
+ * move to H .. budget - 1.  Keys, values and weights move together, head by head, so a slot's
+ * heads may hold different tokens; positions that were rotated into keys stay theirs.
+ * Attention (fg_attend without a window) sees the same whatever the order.  Outputs:
+ *   d_kv_lens  requests                min(length, budget); lengths past the table's room count as that
+ *   d_freed    requests * table_width  the table's entries past that, requests in order; -1 behind them
+ *   d_released 1                       how many those are
+ * The table itself stays: fg_cache_plan writes a new page over an entry when the request
+ * grows again.  No page may belong to two requests of the call.  Bounds of pages whose keys
+ * moved are void.  1 <= requests <= 4096, sinks + window <= budget, 1 <= budget. */
+int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_table, int64_t table_row, uint32_t table_width,
+                   const int32_t *d_kv_lens, uint32_t requests, uint32_t budget, uint32_t window, uint32_t sinks,
+                   int32_t *d_new_lens, int32_t *d_freed, int32_t *d_released, void *workspace, uint64_t workspace_bytes,
+                   void *stream);
+int64_t fg_cache_evict_workspace_bytes(const fg_kv_cache *cache, uint32_t table_width, uint32_t requests, uint32_t budget);
+
 const char *fg_last_error(void);
 const char *fg_version(void);
 
