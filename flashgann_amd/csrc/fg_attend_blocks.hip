@@ -440,7 +440,7 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     P.per = fast_div(per);
     P.head_parts = (P.group + kTileRows - 1) / kTileRows;
     P.tile = fast_div(tokens);
-    plan->tiles = a->tokens / tokens + a->requests;
+    plan->tiles = a->tokens / tokens + (tokens > 1 ? a->requests : 0);
     plan->lds = tokens * P.nids * 12;
     const uint64_t items = static_cast<uint64_t>(plan->tiles) * P.lists * P.head_parts;
     const uint64_t blocks = std::min<uint64_t>(a->table_width, static_cast<uint64_t>(P.first) + P.last + P.nids);

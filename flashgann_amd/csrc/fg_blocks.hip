@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kBoundsThreads) void fg_cache_bounds_kernel(BoundsP
 
 // ---------------------------------------------------------------- selection
 
-constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kSelectRows = 16;
+constexpr uint32_t kSelectThreads = 512, kSelectWaves = kSelectThreads / 64, kSelectRows = 16;
 constexpr uint32_t kSelectLds = 128 * 1024;  // bytes of keys that a workgroup holds
 
 struct SelectParams {
@@ -140,6 +140,7 @@ struct SelectParams {
     FastDiv rows;       // query rows of a tile
     uint32_t stride;    // keys of a row
     uint32_t parts;     // workgroups that share a tile's blocks
+    uint32_t tiles;
     FastDiv page_size;
 };
 
@@ -202,20 +203,15 @@ __device__ __forceinline__ void code_queries(const SelectParams &P, const Tile &
     }
 }
 
-// The P.count largest of n keys (0: none) by their places, ascending, -1 behind them.
-template <uint32_t WAVES, class Keys>
-__device__ __forceinline__ void pick(Keys keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, Picking<WAVES> &S) {
-    const uint32_t lane = threadIdx.x % 64, wave = WAVES > 1 ? uniform(threadIdx.x / 64) : 0;
-    const Border B = border_of<WAVES>(keys, n, count, S);
-    const Run run = run_of<WAVES>(n);
+// The `count` largest keys of a run by their places, ascending, -1 behind them.
+template <uint32_t WAVES, class Run>
+__device__ __forceinline__ void pick(const Run &run, uint32_t count, uint32_t first, int32_t *ids, Picking<WAVES> &S) {
+    const uint32_t lane = threadIdx.x % 64, wave = team_wave<WAVES>();
+    const Border B = border_of<WAVES>(run, count, S);
     uint32_t at = 0, equal = 0;  // ids written, and keys equal to the border, before this wave's run
     if constexpr (WAVES > 1) {
         uint32_t above = 0, same = 0;
-#pragma unroll 4
-        for (uint32_t i = run.begin + lane; i < run.end; i += 64) {
-            const uint32_t x = keys[i];
-            above += x > B.border, same += x == B.border;
-        }
+        run.each([&](uint32_t x, uint32_t) { above += x > B.border, same += x == B.border; });
         above = wave_sum(above), same = wave_sum(same);
         if (lane == 0) S.count[0][wave] = above, S.count[1][wave] = same;
         __syncthreads();
@@ -224,44 +220,59 @@ __device__ __forceinline__ void pick(Keys keys, uint32_t n, uint32_t count, uint
             equal += S.count[1][w];
         }
     }
-    for (uint32_t i0 = run.begin; B.valid && i0 < run.end; i0 += 64) {
-        const uint32_t i = i0 + lane, x = i < run.end ? static_cast<uint32_t>(keys[i]) : 0;
-        const bool take = taken(B, x, equal);
-        const uint64_t all = __ballot(take);
-        if (take) ids[at + __popcll(all & ((1ull << lane) - 1))] = static_cast<int32_t>(first + i);
-        at += __popcll(all);
-    }
+    if (B.valid)
+        run.each([&](uint32_t x, uint32_t i) {
+            const bool take = taken(B, x, equal);
+            const uint64_t all = __ballot(take);
+            if (take) ids[at + __popcll(all & ((1ull << lane) - 1))] = static_cast<int32_t>(first + i);
+            at += __popcll(all);
+        });
     for (uint32_t i = min(B.valid, count) + (WAVES > 1 ? threadIdx.x : lane); i < count; i += 64 * WAVES) ids[i] = -1;
+}
+
+// Keys in registers where they fit.
+template <uint32_t WAVES, class Keys>
+__device__ __forceinline__ void pick_from(Keys keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, Picking<WAVES> &S) {
+    if (run_size<WAVES>(n) <= 64 * 4) pick<WAVES>(held_run<WAVES, 4>(keys, n), count, first, ids, S);
+    else if (run_size<WAVES>(n) <= 64 * 16) pick<WAVES>(held_run<WAVES, 16>(keys, n), count, first, ids, S);
+    else pick<WAVES>(stored_run<WAVES>(keys, n), count, first, ids, S);
 }
 
 enum { kFused, kScratch, kScore, kPick };  // keys in LDS; in a scratch of the workgroup; made only; picked from only
 
-// A workgroup takes a tile of rows of one list: queries coded once, then each wave a group
-// of 16 blocks at a time through the matrix unit, rows against blocks.
+// A workgroup takes a tile of rows of one list: queries coded once, then each wave groups of
+// 16 blocks through the matrix unit, rows against blocks.  Workgroups of neighbouring numbers
+// take a tile's lists, so that an XCD, to which every eighth goes, sees few heads' bounds.
 template <class T, int D, int MODE, bool TEAM>
-__global__ __launch_bounds__(kSelectThreads) void fg_select_kernel(SelectParams P) {
-    constexpr int STEPS = 2 * D / 64;
+__global__ __launch_bounds__(kSelectThreads, 4) void fg_select_kernel(SelectParams P) {
+    constexpr int STEPS = 2 * D / 64, U = D <= 128 ? 2 : 1;  // groups of blocks under way at a time
     constexpr uint32_t QROW = 2 * D + 16;  // bytes of a row's codes in LDS
+    constexpr uint32_t WAVES = TEAM ? kSelectWaves : 1;
     extern __shared__ uint32_t held[];
     __shared__ __attribute__((aligned(16))) char codes[kSelectRows * QROW];
-    constexpr uint32_t WAVES = TEAM ? kSelectWaves : 1;
-    __shared__ Picking<WAVES> picking[TEAM ? 1 : kSelectRows];
+    __shared__ Picking<WAVES> picking[TEAM ? 1 : kSelectWaves];
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 16, quarter = lane / 16;
-    const uint32_t list = blockIdx.y, part = MODE == kScore ? blockIdx.z : 0;
-    const uint32_t tiles = P.rows.div(P.tokens) + P.requests;
-    const uint64_t scratch = MODE == kScratch ? static_cast<uint64_t>(blockIdx.y) * gridDim.x + blockIdx.x : 0;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const uint32_t part = MODE == kScore ? blockIdx.y : 0, items = P.tiles * P.lists;
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t tile = item / P.lists, list = item - tile * P.lists;
         const Tile t = tile_of(P.q_starts, P.kv_lens, P.requests, P.tokens, P.rows, tile);
         if (t.rows == 0) continue;
         const int32_t first = static_cast<int32_t>(min(P.first, P.table_width)), end = end_of(P, t.pos + t.rows - 1);
         const uint32_t n = static_cast<uint32_t>(max(end - first, 0));
-        uint32_t *const stored = MODE == kScratch ? P.keys + scratch * P.rows.d * P.stride
-                                                  : P.keys + (static_cast<uint64_t>(list) * tiles + tile) * P.rows.d * P.stride;
+        uint32_t *const stored = P.keys + static_cast<uint64_t>(MODE == kScratch ? blockIdx.x : item) * P.rows.d * P.stride;
         const auto put = [&](uint32_t row, uint32_t i, uint32_t key) {
             if constexpr (MODE == kFused) held[row * P.stride + i] = key;
             else stored[static_cast<uint64_t>(row) * P.stride + i] = key;
         };
         if constexpr (MODE != kPick) {
+            const uint32_t kv_head = list / P.list_heads;
+            const int32_t *row = P.table + t.request * P.table_row + first;
+            const uint32_t groups = (n + 15) / 16, step = kSelectWaves * (MODE == kScore ? P.parts : 1);
+            const auto page_of = [&](uint32_t g) { return g < groups && g * 16 + col < n ? row[g * 16 + col] : -1; };
+            const uint32_t g0 = wave + kSelectWaves * part;
+            int32_t page[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) page[u] = page_of(g0 + u * step);
             code_queries<T, D>(P, t, list, codes, QROW);
             __syncthreads();
             i32x4 qv[STEPS];
@@ -269,32 +280,36 @@ __global__ __launch_bounds__(kSelectThreads) void fg_select_kernel(SelectParams 
             for (int s = 0; s < STEPS; ++s) qv[s] = *reinterpret_cast<const i32x4 *>(codes + col * QROW + 64 * s + 16 * quarter);
             int32_t ends[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ends[i] = end_of(P, t.pos + static_cast<int32_t>(4 * quarter) + i);
-            const uint32_t kv_head = list / P.list_heads;
-            const int32_t *row = P.table + t.request * P.table_row;
-            const uint32_t groups = (n + 15) / 16, step = kSelectWaves * (MODE == kScore ? P.parts : 1);
-            uint32_t g = wave + kSelectWaves * part;
-            int32_t page = g < groups && g * 16 + col < n ? row[first + g * 16 + col] : -1;
-            for (; g < groups; g += step) {
-                const bool real = static_cast<uint32_t>(page) < P.pages;
-                const int64_t at = static_cast<int64_t>(real ? page : 0) * P.heads_kv + kv_head;
-                const int8_t *src = P.bounds + at * (2 * D) + 16 * quarter;
-                i32x4 b[STEPS];
+            for (int i = 0; i < 4; ++i) ends[i] = end_of(P, t.pos + static_cast<int32_t>(4 * quarter) + i) - first;
+            for (uint32_t g = g0; g < groups; g += U * step) {
+                i32x4 b[U][STEPS];
+                float scale[U];
+                bool real[U];
 #pragma unroll
-                for (int s = 0; s < STEPS; ++s) b[s] = *reinterpret_cast<const i32x4 *>(src + 64 * s);
-                const float scale = P.scales[at];
-                const uint32_t i16 = g * 16 + col, next = g + step;
-                page = next < groups && next * 16 + col < n ? row[first + next * 16 + col] : -1;
-                i32x4 s4 = {0, 0, 0, 0};
+                for (int u = 0; u < U; ++u) {
+                    real[u] = static_cast<uint32_t>(page[u]) < P.pages;
+                    const int64_t at = static_cast<int64_t>(real[u] ? page[u] : 0) * P.heads_kv + kv_head;
+                    const int8_t *src = P.bounds + at * (2 * D) + 16 * quarter;
 #pragma unroll
-                for (int s = 0; s < STEPS; ++s) s4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(qv[s], b[s], s4, 0, 0, 0);
-                if (i16 < n) {
+                    for (int s = 0; s < STEPS; ++s) b[u][s] = *reinterpret_cast<const i32x4 *>(src + 64 * s);
+                    scale[u] = P.scales[at];
+                }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t r = 4 * quarter + i;
-                        if (r < static_cast<uint32_t>(t.rows)) {
-                            const float score = scale == INFINITY ? INFINITY : static_cast<float>(s4[i]) * scale;
-                            put(r, i16, real && first + static_cast<int32_t>(i16) < ends[i] ? key_of(score) : 0u);
+                for (int u = 0; u < U; ++u) page[u] = page_of(g + (U + u) * step);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    i32x4 s4 = {0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s) s4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(qv[s], b[u][s], s4, 0, 0, 0);
+                    const uint32_t i16 = (g + u * step) * 16 + col;
+                    if (g + u * step < groups && i16 < n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t r = 4 * quarter + i;
+                            if (r < static_cast<uint32_t>(t.rows)) {
+                                const float score = scale[u] == INFINITY ? INFINITY : static_cast<float>(s4[i]) * scale[u];
+                                put(r, i16, real[u] && static_cast<int32_t>(i16) < ends[i] ? key_of(score) : 0u);
+                            }
                         }
                     }
                 }
@@ -304,8 +319,8 @@ __global__ __launch_bounds__(kSelectThreads) void fg_select_kernel(SelectParams 
         if constexpr (MODE != kScore) {
             for (uint32_t r = TEAM ? 0 : wave; r < static_cast<uint32_t>(t.rows); r += TEAM ? 1 : kSelectWaves) {
                 int32_t *out = P.ids + ((t.q0 + static_cast<uint64_t>(r)) * P.lists + list) * P.count;
-                if constexpr (MODE == kFused) pick<WAVES>(held + r * P.stride, n, P.count, first, out, picking[TEAM ? 0 : r]);
-                else pick<WAVES>(static_cast<const uint32_t *>(stored) + static_cast<uint64_t>(r) * P.stride, n, P.count, first, out, picking[TEAM ? 0 : r]);
+                if constexpr (MODE == kFused) pick_from<WAVES>(held + r * P.stride, n, P.count, first, out, picking[TEAM ? 0 : wave]);
+                else pick_from<WAVES>(static_cast<const uint32_t *>(stored) + static_cast<uint64_t>(r) * P.stride, n, P.count, first, out, picking[TEAM ? 0 : wave]);
             }
             __syncthreads();
         }
@@ -313,18 +328,18 @@ __global__ __launch_bounds__(kSelectThreads) void fg_select_kernel(SelectParams 
 }
 
 template <class T, int D>
-int launch_select(const SelectParams &P, int mode, dim3 grid, uint32_t lds, hipStream_t st) {
-    const auto go = [&](auto kernel, dim3 g, uint32_t bytes) -> int {
+int launch_select(const SelectParams &P, int mode, uint32_t grid, uint32_t lds, hipStream_t st) {
+    const auto go = [&](auto kernel, uint32_t parts, uint32_t bytes) -> int {
         if (bytes > 32 * 1024) FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kSelectLds), "selection LDS");
-        hipLaunchKernelGGL(kernel, g, dim3(kSelectThreads), bytes, st, P);
+        hipLaunchKernelGGL(kernel, dim3(grid, parts), dim3(kSelectThreads), bytes, st, P);
         return FG_OK;
     };
     int rc = FG_OK;
-    if (mode == kFused) rc = P.rows.d == 1 ? go(fg_select_kernel<T, D, kFused, true>, grid, lds) : go(fg_select_kernel<T, D, kFused, false>, grid, lds);
-    else if (mode == kScratch) rc = go(fg_select_kernel<T, D, kScratch, true>, grid, 0);
+    if (mode == kFused) rc = P.rows.d == 1 ? go(fg_select_kernel<T, D, kFused, true>, 1, lds) : go(fg_select_kernel<T, D, kFused, false>, 1, lds);
+    else if (mode == kScratch) rc = go(fg_select_kernel<T, D, kScratch, true>, 1, 0);
     else {
-        rc = go(fg_select_kernel<T, D, kScore, true>, dim3(grid.x, grid.y, P.parts), 0);
-        if (rc == FG_OK) rc = go(fg_select_kernel<T, D, kPick, true>, grid, 0);
+        rc = go(fg_select_kernel<T, D, kScore, true>, P.parts, 0);
+        if (rc == FG_OK) rc = go(fg_select_kernel<T, D, kPick, true>, 1, 0);
     }
     if (rc != FG_OK) return rc;
     FG_HIP(hipGetLastError(), "selection launch");
@@ -334,8 +349,7 @@ int launch_select(const SelectParams &P, int mode, dim3 grid, uint32_t lds, hipS
 // How a call is run.
 struct SelectPlan {
     int mode;
-    dim3 grid;
-    uint32_t lds;
+    uint32_t grid, lds;
     uint64_t workspace;
 };
 
@@ -381,21 +395,24 @@ int prepare_select(const fg_kv_cache *c, const fg_attention *a, SelectParams *ou
     uint32_t rows = kSelectRows;
     while (rows > 1 && (static_cast<uint64_t>(rows) * P.stride * 4 > kSelectLds || a->tokens <= 2 * static_cast<uint64_t>(a->requests))) rows /= 2;
     P.rows = fast_div(rows);
-    const uint64_t tiles = a->tokens / rows + static_cast<uint64_t>(a->requests), items = tiles * a->lists;
+    // (a row alone is a tile of its own number, and leaves none empty)
+    P.tiles = a->tokens / rows + (rows > 1 ? a->requests : 0);
+    const uint64_t items = static_cast<uint64_t>(P.tiles) * a->lists;
+    if (items > 0x7FFFFFFFull) return fail(FG_EINVAL, "tokens * lists must be below 2^31");
     P.parts = 1;
-    plan->grid = dim3(static_cast<uint32_t>(std::min<uint64_t>(tiles, 1u << 20)), a->lists);
+    plan->grid = static_cast<uint32_t>(std::min<uint64_t>(items, 1u << 20));
     plan->lds = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(rows) * P.stride * 4, 0xFFFFFFFFu));
     plan->workspace = 0;
     plan->mode = kFused;
     if (plan->lds > kSelectLds) {
         plan->mode = kScratch;
-        plan->grid.x = static_cast<uint32_t>(std::min<uint64_t>(tiles, std::max(1u, 512 / a->lists)));
-        plan->workspace = static_cast<uint64_t>(plan->grid.x) * a->lists * P.stride * 4;
+        plan->grid = static_cast<uint32_t>(std::min<uint64_t>(items, 512));
+        plan->workspace = static_cast<uint64_t>(plan->grid) * P.stride * 4;
     }
     // Few rows over many blocks: several workgroups make a row's keys, and one picks from them.
     if (rows == 1 && items < 128 && most >= 2048) {
         plan->mode = kScore;
-        plan->grid.x = static_cast<uint32_t>(tiles);
+        plan->grid = static_cast<uint32_t>(items);
         P.parts = std::min<uint32_t>((most + 16 * kSelectWaves - 1) / (16 * kSelectWaves), static_cast<uint32_t>(std::max<uint64_t>(1, 512 / items)));
         plan->workspace = items * P.stride * 4;
     }

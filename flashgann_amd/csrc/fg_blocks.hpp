@@ -10,7 +10,8 @@ constexpr uint32_t kMostBlocks = 4096;     // of a list: what attention over the
 constexpr uint32_t kMostTokens = 1u << 22; // of a call: its tiles are a grid's workgroups
 
 // Rows of q in tiles: those of request r are tiles q_starts[r] / rows + r and on, which leaves
-// room for the ragged last one of each, so a call has tokens / rows + requests at most.
+// room for the ragged last one of each, so a call has tokens / rows + requests at most.  A tile
+// of one row is that row.
 struct Tile {
     int32_t request, q0, rows, pos;  // first row of q; rows (0: no such tile); position of the first
 };
@@ -21,14 +22,14 @@ __device__ __forceinline__ Tile tile_of(const int32_t *q_starts, const int32_t *
     uint32_t lo = 0;  // the last request whose tiles begin at or before `tile`, by 64 guesses at a time
     for (uint32_t len = requests; len > 1;) {
         const uint32_t stride = (len + 63) / 64, guess = lane * stride;
-        const bool before = guess < len && rows.div(clampi(q_starts[lo + min(guess, len - 1)], 0, T)) + lo + guess <= tile;
+        const bool before = guess < len && rows.div(clampi(q_starts[lo + min(guess, len - 1)], 0, T)) + (rows.d > 1 ? lo + guess : 0) <= tile;
         const uint32_t n = max(static_cast<uint32_t>(__popcll(__ballot(before))), 1u) - 1;
         lo += n * stride;
         len = min(stride, len - n * stride);
     }
     lo = uniform(lo);
     const int32_t q0 = clampi(q_starts[lo], 0, T), n = clampi(q_starts[lo + 1], q0, T) - q0;
-    const int64_t row0 = (static_cast<int64_t>(tile) - static_cast<int64_t>(rows.div(q0) + lo)) * rows.d;
+    const int64_t row0 = (static_cast<int64_t>(tile) - static_cast<int64_t>(rows.div(q0) + (rows.d > 1 ? lo : 0))) * rows.d;
     Tile t{static_cast<int32_t>(lo), 0, 0, 0};
     if (row0 >= 0 && row0 < n) {
         t.q0 = q0 + static_cast<int32_t>(row0);

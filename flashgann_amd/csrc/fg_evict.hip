@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void fg_weigh_kernel(WeighParams P) {
 // ---------------------------------------------------------------- eviction
 
 constexpr uint32_t kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
-constexpr uint32_t kChooseKeys = 32768;     // weights that a workgroup holds in LDS
+constexpr uint32_t kFewKeys = 8 * kChooseThreads, kChooseKeys = 32 * kChooseThreads;  // weights that a workgroup holds in registers
 constexpr uint32_t kChooseWorkgroups = 512; // at most, where it does not
 constexpr uint32_t kEvictRequests = 4096;
 constexpr uint32_t kMoveThreads = 256, kMovePieces = 4;  // 16-byte pieces of a row that a workgroup moves
@@ -147,9 +147,9 @@ struct EvictParams {
     const int32_t *table, *kv_lens;
     int64_t table_row;
     int32_t *new_lens, *freed, *released;
-    int32_t *from, *to;  // slots, `most` for each request and head: places above H, and below
+    int32_t *from, *to;  // tokens, `most` for each request and head: places above H, and below
     uint32_t *counts;    // how many
-    uint32_t *keys;      // where LDS does not hold them: `room` for each workgroup
+    uint32_t *keys;      // where registers do not hold them: `room` for each workgroup
     uint32_t table_width, requests, heads_kv, budget, window, sinks;
     uint32_t room;       // tokens that the table names
     uint32_t most;       // min(budget, room)
@@ -212,76 +212,103 @@ __device__ __forceinline__ void list_freed(const EvictParams &P, uint32_t w, uin
     }
 }
 
+// The weights of tokens from + i on as keys, U at a time: their pages, then the weights.
+template <uint32_t U, class F>
+__device__ __forceinline__ void load_keys(const EvictParams &P, uint32_t r, uint32_t h, uint32_t from, uint32_t end, uint32_t step, F put) {
+    int32_t page[U];
+    float x[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t j = from + u * step;
+        page[u] = j < end ? P.table[r * P.table_row + P.cache.page_size.div(j)] : -1;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t j = from + u * step, at = j - P.cache.page_size.div(j) * P.cache.page_size.d;
+        const bool real = static_cast<uint32_t>(page[u]) < P.cache.pages;
+        x[u] = real ? P.weights[(static_cast<int64_t>(page[u]) * P.heads_kv + h) * P.cache.page_size.d + at] : 0.0f;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+        const bool real = static_cast<uint32_t>(page[u]) < P.cache.pages;
+        const uint32_t key = !real ? 1u : x[u] != x[u] ? key_of(INFINITY) : key_of(x[u] + 0.0f);  // (-0 as 0)
+        put(u, from + u * step < end ? key : 0u);
+    }
+}
+
 // A workgroup for a request and head: weights as ordered integers, the border of the heaviest,
-// then which slots move where.
-template <bool HELD>
-__global__ __launch_bounds__(kChooseThreads) void fg_evict_choose_kernel(EvictParams P) {
+// then which tokens move where.  K: a wave holds its run of up to 64 K weights in registers; 0: in
+// a scratch.
+template <uint32_t K>
+__global__ __launch_bounds__(kChooseThreads, K == 8 ? 8 : 4) void fg_evict_choose_kernel(EvictParams P) {
     extern __shared__ uint32_t dynamic[];
     __shared__ Picking<kChooseWaves> S;
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64);
     if (blockIdx.x >= P.choosers) {
-        list_freed(P, blockIdx.x - P.choosers, gridDim.x - P.choosers, dynamic, S.least);
+        list_freed(P, blockIdx.x - P.choosers, gridDim.x - P.choosers, dynamic, S.valid);
         return;
     }
-    uint32_t *const keys = HELD ? dynamic : P.keys + static_cast<uint64_t>(blockIdx.x) * P.room;
     for (uint32_t rh = blockIdx.x; rh < P.requests * P.heads_kv; rh += P.choosers) {
         const uint32_t r = rh / P.heads_kv, h = rh - r * P.heads_kv, n = length_of(P, r);
         if (n <= P.budget) {
             if (tid == 0) P.counts[rh] = 0;
             continue;
         }
-        // tokens sinks .. end - 1 are chosen from: `want` of them, so that `keep` stand before the last ones
-        const uint32_t end = n - P.window, keep = P.budget - P.window, want = keep - P.sinks, span = end - P.sinks;
-#pragma unroll 4
-        for (uint32_t i = tid; i < span; i += kChooseThreads) {
-            const int32_t slot = slot_of(P, r, P.sinks + i);
-            uint32_t key = 1;
-            if (slot >= 0) {
-                const float x = P.weights[weight_at(P, h, slot)];
-                key = x != x ? key_of(INFINITY) : key_of(x + 0.0f);  // (-0 as 0)
+        // tokens sinks .. end - 1 are chosen from: `low` of them, so that they end before place `keep`
+        const uint32_t end = n - P.window, keep = P.budget - P.window, low = keep - P.sinks, span = end - P.sinks;
+        const uint32_t per = run_size<kChooseWaves>(span), begin = min(wave * per, span), stop = min(begin + per, span);
+        const auto choose = [&](const auto &run) {
+            Border B{0xFFFFFFFFu, 0, 0};
+            if (low) B = border_of<kChooseWaves>(run, low, S);
+            // what each wave's run holds: keys above the border and equal to it, below place `keep` and from there on
+            uint32_t above[2] = {0, 0}, same[2] = {0, 0};
+            run.each([&](uint32_t x, uint32_t i) {
+                const uint32_t late = i >= low, a = x > B.border, s = x == B.border;
+                above[0] += a & ~late, above[1] += a & late, same[0] += s & ~late, same[1] += s & late;
+            });
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t a = wave_sum(above[c]), s = wave_sum(same[c]);
+                if (lane == 0) S.count[c][wave] = a, S.count[2 + c][wave] = s;
             }
-            keys[i] = key;
+            __syncthreads();
+            // a lane a wave: equal keys before it are the first to be taken
+            const uint32_t w = lane % kChooseWaves, s0 = S.count[2][w], s1 = S.count[3][w];
+            const uint32_t seen = sum_upto(s0 + s1) - (s0 + s1);  // (of the first lanes; the others' say nothing)
+            const uint32_t gone = min(w * per + per, low) - min(w * per, low) - S.count[0][w] - (min(seen + s0, B.ties) - min(seen, B.ties));
+            const uint32_t late = S.count[1][w] + min(seen + s0 + s1, B.ties) - min(seen + s0, B.ties);
+            const uint32_t gones = sum_upto(gone), lates = sum_upto(late);
+            const uint32_t holes = of_lane(static_cast<int32_t>(gones), kChooseWaves - 1);
+            uint32_t equal = of_lane(static_cast<int32_t>(seen), wave), at_hole = of_lane(static_cast<int32_t>(gones - gone), wave),
+                     at_late = of_lane(static_cast<int32_t>(lates - late), wave);
+            int32_t *const to = P.to + static_cast<uint64_t>(rh) * P.most, *const from = P.from + static_cast<uint64_t>(rh) * P.most;
+            run.each([&](uint32_t x, uint32_t i) {
+                const bool in = i < stop, take = taken(B, x, equal), hole = in && i < low && !take, rises = in && i >= low && take;
+                const uint64_t hs = __ballot(hole), rs = __ballot(rises), before = (1ull << lane) - 1;
+                if (hole) to[at_hole + __popcll(hs & before)] = static_cast<int32_t>(P.sinks + i);
+                if (rises) from[at_late + __popcll(rs & before)] = static_cast<int32_t>(P.sinks + i);
+                at_hole += __popcll(hs), at_late += __popcll(rs);
+            });
+            if (tid == 0) P.counts[rh] = holes;
+        };
+        if constexpr (K > 0) {
+            Held<K> run;
+            run.begin = begin, run.steps = (stop - begin + 63) / 64;
+            constexpr uint32_t U = K > 8 ? 8 : 4;
+#pragma unroll
+            for (uint32_t u0 = 0; u0 < K; u0 += U)
+                if (u0 < run.steps)
+                    load_keys<U>(P, r, h, P.sinks + begin + u0 * 64 + lane, P.sinks + stop, 64, [&](uint32_t u, uint32_t key) { run.key[u0 + u] = key; });
+            choose(run);
+        } else {
+            uint32_t *const keys = P.keys + static_cast<uint64_t>(blockIdx.x) * P.room;
+            for (uint32_t i0 = begin; i0 < stop; i0 += 8 * 64)
+                load_keys<8>(P, r, h, P.sinks + i0 + lane, P.sinks + stop, 64, [&](uint32_t u, uint32_t key) {
+                    if (i0 + u * 64 + lane < stop) keys[i0 + u * 64 + lane] = key;
+                });
+            // (a wave reads its own run alone: what it has written itself)
+            choose(Stored<const uint32_t *>{keys, begin, stop});
         }
-        __syncthreads();
-        Border B{0xFFFFFFFFu, 0, 0};
-        if (want) B = border_of<kChooseWaves>(static_cast<const uint32_t *>(keys), span, want, S);
-        const Run run = run_of<kChooseWaves>(span);
-        uint32_t same = 0;
-#pragma unroll 4
-        for (uint32_t i = run.begin + lane; i < run.end; i += 64) same += keys[i] == B.border;
-        same = wave_sum(same);
-        if (lane == 0) S.count[0][wave] = same;
-        __syncthreads();
-        uint32_t equal = 0;
-        for (uint32_t w = 0; w < wave; ++w) equal += S.count[0][w];
-        __syncthreads();
-        const uint32_t equal0 = equal, low = keep - P.sinks;  // places from `low` on are above
-        uint32_t holes = 0, late = 0;
-        for (uint32_t i0 = run.begin; i0 < run.end; i0 += 64) {
-            const uint32_t i = i0 + lane;
-            const bool in = i < run.end, take = taken(B, in ? keys[i] : 0u, equal) && want;
-            holes += __popcll(__ballot(in && i < low && !take));
-            late += __popcll(__ballot(in && i >= low && take));
-        }
-        if (lane == 0) S.count[0][wave] = holes, S.count[1][wave] = late;
-        __syncthreads();
-        uint32_t at_hole = 0, at_late = 0, moved = 0;
-        for (uint32_t w = 0; w < kChooseWaves; ++w) {
-            if (w < wave) at_hole += S.count[0][w], at_late += S.count[1][w];
-            moved += S.count[0][w];
-        }
-        int32_t *const to = P.to + static_cast<uint64_t>(rh) * P.most, *const from = P.from + static_cast<uint64_t>(rh) * P.most;
-        equal = equal0;
-        for (uint32_t i0 = run.begin; i0 < run.end; i0 += 64) {
-            const uint32_t i = i0 + lane;
-            const bool in = i < run.end, take = taken(B, in ? keys[i] : 0u, equal) && want;
-            const bool hole = in && i < low && !take, above = in && i >= low && take;
-            const uint64_t hs = __ballot(hole), as = __ballot(above), below = (1ull << lane) - 1;
-            if (hole) to[at_hole + __popcll(hs & below)] = slot_of(P, r, P.sinks + i);
-            if (above) from[at_late + __popcll(as & below)] = slot_of(P, r, P.sinks + i);
-            at_hole += __popcll(hs), at_late += __popcll(as);
-        }
-        if (tid == 0) P.counts[rh] = moved;
         __syncthreads();
     }
 }
@@ -333,7 +360,7 @@ __global__ __launch_bounds__(kMoveThreads) void fg_evict_move_kernel(EvictParams
         }
     };
     const int32_t *const from = P.from + static_cast<uint64_t>(rh) * P.most, *const to = P.to + static_cast<uint64_t>(rh) * P.most;
-    move(P.counts[rh], [&](uint32_t i) { return from[i]; }, [&](uint32_t i) { return to[i]; });
+    move(P.counts[rh], [&](uint32_t i) { return slot_of(P, r, from[i]); }, [&](uint32_t i) { return slot_of(P, r, to[i]); });
     __syncthreads();
     move(P.window, [&](uint32_t i) { return slot_of(P, r, n - P.window + i); }, [&](uint32_t i) { return slot_of(P, r, P.budget - P.window + i); });
 }
@@ -472,13 +499,8 @@ int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_
         hipStream_t st = reinterpret_cast<hipStream_t>(stream);
         const uint64_t entries = static_cast<uint64_t>(requests) * table_width;
         const uint32_t listers = static_cast<uint32_t>(std::min<uint64_t>(64, 1 + entries / (4 * kChooseThreads)));
-        const uint32_t lds = std::max<uint32_t>(plan.held ? P.room * 4 : 0, requests * 4);
-        if (plan.held) {
-            FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(fg_evict_choose_kernel<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kChooseKeys * 4), "eviction LDS");
-            hipLaunchKernelGGL(fg_evict_choose_kernel<true>, dim3(P.choosers + listers), dim3(kChooseThreads), lds, st, P);
-        } else {
-            hipLaunchKernelGGL(fg_evict_choose_kernel<false>, dim3(P.choosers + listers), dim3(kChooseThreads), lds, st, P);
-        }
+        const auto choose = P.room <= kFewKeys ? fg_evict_choose_kernel<8> : plan.held ? fg_evict_choose_kernel<32> : fg_evict_choose_kernel<0>;
+        hipLaunchKernelGGL(choose, dim3(P.choosers + listers), dim3(kChooseThreads), requests * 4, st, P);
         const uint32_t pieces = cache->dim / 8, slices = (2 * pieces + kMovePieces - 1) / kMovePieces;
         if (P.room > budget)
             hipLaunchKernelGGL(fg_evict_move_kernel, dim3(slices, cache->heads_kv, requests), dim3(kMoveThreads), 0, st, P, pieces);
