@@ -151,53 +151,54 @@ __device__ __forceinline__ int32_t end_of(const SelectParams &P, int32_t pos) {
     return static_cast<int32_t>(min(max(end, static_cast<int64_t>(0)), static_cast<int64_t>(P.table_width)));
 }
 
-// The codes of a tile's queries, 2 D bytes a row, into LDS; a wave a row.
+// The codes of a tile's queries, 2 D bytes a row, into LDS: a wave the rows wave, wave + 8.
 template <class T, int D>
 __device__ __forceinline__ void code_queries(const SelectParams &P, const Tile &t, uint32_t list, char *codes, uint32_t row_bytes) {
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    constexpr uint32_t PAIRS = D / 2, N = (PAIRS + 63) / 64;  // two channels a lane at a time
-    for (uint32_t row = wave; row < kSelectRows; row += kSelectWaves) {
-        float up[N][2] = {}, down[N][2] = {};
-        if (row < static_cast<uint32_t>(t.rows)) {
-            const char *src = P.q + (t.q0 + static_cast<int64_t>(row)) * P.q_token + static_cast<int64_t>(list) * P.group * P.q_head;
+    constexpr uint32_t PAIRS = D / 2, N = (PAIRS + 63) / 64, R = kSelectRows / kSelectWaves;  // two channels a lane at a time
+    float up[R][N][2] = {}, down[R][N][2] = {};
+    const char *src[R];  // (past the tile's rows the last one again: nobody asks for its scores)
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r)
+        src[r] = P.q + (t.q0 + static_cast<int64_t>(min(wave + r * kSelectWaves, static_cast<uint32_t>(t.rows) - 1))) * P.q_token +
+                 static_cast<int64_t>(list) * P.group * P.q_head;
 #pragma unroll 4
-            for (uint32_t h = 0; h < P.group; ++h) {
+    for (uint32_t h = 0; h < P.group; ++h) {
 #pragma unroll
-                for (uint32_t n = 0; n < N; ++n) {
-                    const uint32_t pair = n * 64 + lane;
-                    if (PAIRS % 64 == 0 || pair < PAIRS) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t *>(src + h * P.q_head + pair * 4);
+        for (uint32_t r = 0; r < R; ++r)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const float x = as_float<T>(c ? w >> 16 : w & 0xFFFF);
-                            // (not fmaxf: a NaN has to stay one)
-                            up[n][c] += x < 0.0f ? 0.0f : x;
-                            down[n][c] += x > 0.0f ? 0.0f : x;
-                        }
+            for (uint32_t n = 0; n < N; ++n) {
+                const uint32_t pair = n * 64 + lane;
+                if (PAIRS % 64 == 0 || pair < PAIRS) {
+                    const uint32_t w = *reinterpret_cast<const uint32_t *>(src[r] + h * P.q_head + pair * 4);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float x = as_float<T>(c ? w >> 16 : w & 0xFFFF);
+                        // (not fmaxf: a NaN has to stay one)
+                        up[r][n][c] += x < 0.0f ? 0.0f : x;
+                        down[r][n][c] += x > 0.0f ? 0.0f : x;
                     }
                 }
             }
-        }
-        float most = 0.0f;
-        bool special = false;
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+        char *const to = codes + (wave + r * kSelectWaves) * row_bytes;
+        uint32_t most = 0;  // magnitudes as integers: infinities and NaN past all others
 #pragma unroll
         for (uint32_t n = 0; n < N; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                special |= !(fabsf(up[n][c]) < INFINITY) | !(fabsf(down[n][c]) < INFINITY);
-                most = fmaxf(most, fmaxf(fabsf(up[n][c]), fabsf(down[n][c])));
-            }
-#pragma unroll
-        for (uint32_t d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-        const bool finite = !__any(special);
-        const float inv = finite ? inverse(scale_bits(most)) : 0.0f;
+            for (int c = 0; c < 2; ++c) most = max(most, max(__float_as_uint(up[r][n][c]) & 0x7FFFFFFFu, __float_as_uint(down[r][n][c]) & 0x7FFFFFFFu));
+        most = wave_max(most);
+        const bool finite = most < 0x7F800000u;
+        const float inv = finite ? inverse(scale_bits(__uint_as_float(most))) : 0.0f;
 #pragma unroll
         for (uint32_t n = 0; n < N; ++n) {
             const uint32_t pair = n * 64 + lane;
             if (PAIRS % 64 == 0 || pair < PAIRS) {
                 const auto code = [&](float x) { return finite ? static_cast<int>(rintf(x * inv)) & 0xFF : 0; };
-                *reinterpret_cast<uint16_t *>(codes + row * row_bytes + 2 * pair) = static_cast<uint16_t>(code(up[n][0]) | code(up[n][1]) << 8);
-                *reinterpret_cast<uint16_t *>(codes + row * row_bytes + D + 2 * pair) = static_cast<uint16_t>(code(down[n][0]) | code(down[n][1]) << 8);
+                *reinterpret_cast<uint16_t *>(to + 2 * pair) = static_cast<uint16_t>(code(up[r][n][0]) | code(up[r][n][1]) << 8);
+                *reinterpret_cast<uint16_t *>(to + D + 2 * pair) = static_cast<uint16_t>(code(down[r][n][0]) | code(down[r][n][1]) << 8);
             }
         }
     }
@@ -230,12 +231,71 @@ __device__ __forceinline__ void pick(const Run &run, uint32_t count, uint32_t fi
     for (uint32_t i = min(B.valid, count) + (WAVES > 1 ? threadIdx.x : lane); i < count; i += 64 * WAVES) ids[i] = -1;
 }
 
+// The lanes with the `count` largest of a wave's values, one each (0: none), bit by bit from
+// the highest in which they differ; among equal ones the lower lanes.  At least `count` lanes
+// have one, count >= 1.
+__device__ __forceinline__ uint64_t largest_lanes(uint32_t x, uint32_t count) {
+    uint64_t sure = 0, maybe = __ballot(x != 0);
+    if (static_cast<uint32_t>(__popcll(maybe)) == count) return maybe;
+    const uint32_t differ = wave_max(x) ^ wave_min(x ? x : 0xFFFFFFFFu);
+    for (uint32_t bit = differ ? 31 - __clz(differ) : 0u, mask = 1u << bit; mask; mask >>= 1) {
+        const uint64_t ones = __ballot((x & mask) != 0) & maybe;
+        const uint32_t n = __popcll(ones);
+        if (n >= count) {
+            maybe = ones;
+            if (n == count) return sure | maybe;
+        } else if (n) {
+            sure |= ones;
+            maybe &= ~ones;
+            count -= n;
+        }
+    }
+    while (static_cast<uint32_t>(__popcll(maybe)) > count) maybe &= ~(1ull << (63 - __clzll(maybe)));
+    return sure | maybe;
+}
+
+// pick() for few of 1 to 64 K keys, by a wave: the count-th largest of what each lane has at
+// most is a bound that at least `count` keys reach and few more, and those are sorted out one a
+// lane (16 of 1,000: 18 in the mean).  False, with nothing done, where that does not serve.
+template <uint32_t K>
+__device__ __forceinline__ bool pick_few(const uint32_t *keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, u32x2 *some) {
+    const uint32_t lane = threadIdx.x % 64;
+    const Held<K> run = held_run<1, K>(keys, n);
+    uint32_t most = 0;
+    run.each([&](uint32_t x, uint32_t) { most = max(most, x); });
+    if (static_cast<uint32_t>(__popcll(__ballot(most != 0))) < count) return false;
+    const uint64_t lanes = largest_lanes(most, count);
+    const uint32_t bound = wave_min(lanes >> lane & 1 ? most : 0xFFFFFFFFu);
+    uint32_t have = 0;
+    run.each([&](uint32_t x, uint32_t i) {
+        const uint64_t reach = __ballot(x >= bound);
+        const uint32_t at = have + __popcll(reach & ((1ull << lane) - 1));
+        if (x >= bound && at < 64) some[at] = u32x2{x, i};
+        have += __popcll(reach);
+    });
+    if (have > 64) return false;
+    team_sync<1>();
+    const u32x2 mine = some[lane];
+    const uint64_t chosen = largest_lanes(lane < have ? mine[0] : 0u, count);
+    if (chosen >> lane & 1) ids[__popcll(chosen & ((1ull << lane) - 1))] = static_cast<int32_t>(first + mine[1]);
+    team_sync<1>();
+    return true;
+}
+
 // Keys in registers where they fit.
-template <uint32_t WAVES, class Keys>
-__device__ __forceinline__ void pick_from(Keys keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, Picking<WAVES> &S) {
-    if (run_size<WAVES>(n) <= 64 * 4) pick<WAVES>(held_run<WAVES, 4>(keys, n), count, first, ids, S);
-    else if (run_size<WAVES>(n) <= 64 * 16) pick<WAVES>(held_run<WAVES, 16>(keys, n), count, first, ids, S);
-    else pick<WAVES>(stored_run<WAVES>(keys, n), count, first, ids, S);
+template <uint32_t WAVES>
+__device__ __forceinline__ void pick_from(const uint32_t *keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, Picking<WAVES> &S) {
+    if constexpr (WAVES == 1) {
+        u32x2 *const some = reinterpret_cast<u32x2 *>(S.bins[0]);
+        if (n && count <= 32 && n <= 64 * 16) {
+            if (n <= 64 * 8 ? pick_few<8>(keys, n, count, first, ids, some) : pick_few<16>(keys, n, count, first, ids, some)) return;
+        }
+    } else {
+        const uint32_t per = run_size<WAVES>(n);
+        if (n && per <= 64 * 2) return pick<WAVES>(held_run<WAVES, 2>(keys, n), count, first, ids, S);
+        if (n && per <= 64 * 16) return pick<WAVES>(held_run<WAVES, 16>(keys, n), count, first, ids, S);
+    }
+    pick<WAVES>(stored_run<WAVES>(keys, n), count, first, ids, S);
 }
 
 enum { kFused, kScratch, kScore, kPick };  // keys in LDS; in a scratch of the workgroup; made only; picked from only
@@ -260,19 +320,34 @@ __global__ __launch_bounds__(kSelectThreads, 4) void fg_select_kernel(SelectPara
         const int32_t first = static_cast<int32_t>(min(P.first, P.table_width)), end = end_of(P, t.pos + t.rows - 1);
         const uint32_t n = static_cast<uint32_t>(max(end - first, 0));
         uint32_t *const stored = P.keys + static_cast<uint64_t>(MODE == kScratch ? blockIdx.x : item) * P.rows.d * P.stride;
-        const auto put = [&](uint32_t row, uint32_t i, uint32_t key) {
-            if constexpr (MODE == kFused) held[row * P.stride + i] = key;
-            else stored[static_cast<uint64_t>(row) * P.stride + i] = key;
-        };
         if constexpr (MODE != kPick) {
             const uint32_t kv_head = list / P.list_heads;
             const int32_t *row = P.table + t.request * P.table_row + first;
             const uint32_t groups = (n + 15) / 16, step = kSelectWaves * (MODE == kScore ? P.parts : 1);
-            const auto page_of = [&](uint32_t g) { return g < groups && g * 16 + col < n ? row[g * 16 + col] : -1; };
-            const uint32_t g0 = wave + kSelectWaves * part;
+            const auto page_of = [&](uint32_t g) {  // (past the last block nothing is stored)
+                return n ? row[min(g * 16 + col, n - 1)] : 0;
+            };
+            i32x4 b[U][STEPS];
+            float scale[U];
+            const auto load = [&](const int32_t (&page)[U]) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool real = static_cast<uint32_t>(page[u]) < P.pages;
+                    const int64_t at = static_cast<int64_t>(real ? page[u] : 0) * P.heads_kv + kv_head;
+                    const int8_t *src = P.bounds + at * (2 * D) + 16 * quarter;
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s) b[u][s] = *reinterpret_cast<const i32x4 *>(src + 64 * s);
+                    const float of_page = P.scales[at];
+                    scale[u] = real ? of_page : NAN;
+                }
+            };
+            uint32_t g = wave + kSelectWaves * part;
             int32_t page[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) page[u] = page_of(g0 + u * step);
+            for (int u = 0; u < U; ++u) page[u] = page_of(g + u * step);
+            load(page);
+#pragma unroll
+            for (int u = 0; u < U; ++u) page[u] = page_of(g + (U + u) * step);
             code_queries<T, D>(P, t, list, codes, QROW);
             __syncthreads();
             i32x4 qv[STEPS];
@@ -281,36 +356,43 @@ __global__ __launch_bounds__(kSelectThreads, 4) void fg_select_kernel(SelectPara
             int32_t ends[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) ends[i] = end_of(P, t.pos + static_cast<int32_t>(4 * quarter) + i) - first;
-            for (uint32_t g = g0; g < groups; g += U * step) {
-                i32x4 b[U][STEPS];
-                float scale[U];
-                bool real[U];
+            const uint32_t rows = static_cast<uint32_t>(t.rows);
+            const int32_t all = end_of(P, t.pos) - first;  // blocks that every row selects from
+            uint32_t *const to = (MODE == kFused ? held : stored) + static_cast<uint64_t>(4 * quarter) * P.stride;
+            for (; g < groups; g += U * step) {
+                i32x4 s4[U];
+                float times[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    real[u] = static_cast<uint32_t>(page[u]) < P.pages;
-                    const int64_t at = static_cast<int64_t>(real[u] ? page[u] : 0) * P.heads_kv + kv_head;
-                    const int8_t *src = P.bounds + at * (2 * D) + 16 * quarter;
+                    s4[u] = i32x4{0, 0, 0, 0};
+                    times[u] = scale[u];
 #pragma unroll
-                    for (int s = 0; s < STEPS; ++s) b[u][s] = *reinterpret_cast<const i32x4 *>(src + 64 * s);
-                    scale[u] = P.scales[at];
+                    for (int s = 0; s < STEPS; ++s) s4[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(qv[s], b[u][s], s4[u], 0, 0, 0);
+                }
+                if (g + U * step < groups) {
+                    load(page);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) page[u] = page_of(g + (2 * U + u) * step);
                 }
 #pragma unroll
-                for (int u = 0; u < U; ++u) page[u] = page_of(g + (U + u) * step);
-#pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    i32x4 s4 = {0, 0, 0, 0};
-#pragma unroll
-                    for (int s = 0; s < STEPS; ++s) s4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(qv[s], b[u][s], s4, 0, 0, 0);
                     const uint32_t i16 = (g + u * step) * 16 + col;
-                    if (g + u * step < groups && i16 < n) {
+                    if (g + u * step >= groups) break;
+                    uint32_t key[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t r = 4 * quarter + i;
-                            if (r < static_cast<uint32_t>(t.rows)) {
-                                const float score = scale[u] == INFINITY ? INFINITY : static_cast<float>(s4[i]) * scale[u];
-                                put(r, i16, real[u] && static_cast<int32_t>(i16) < ends[i] ? key_of(score) : 0u);
-                            }
-                        }
+                    for (int i = 0; i < 4; ++i) key[i] = key_of(static_cast<float>(s4[u][i]) * times[u]);
+                    if (__any(!(times[u] < INFINITY))) {  // a page that is not finite, or none
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) key[i] = times[u] != times[u] ? 0u : times[u] == INFINITY ? key_of(INFINITY) : key[i];
+                    }
+                    if (static_cast<int32_t>((g + u * step) * 16 + 16) > all) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) key[i] = static_cast<int32_t>(i16) < ends[i] ? key[i] : 0u;
+                    }
+                    if (i16 < n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (4 * quarter + i < rows) to[i * P.stride + i16] = key[i];
                     }
                 }
             }
@@ -320,7 +402,7 @@ __global__ __launch_bounds__(kSelectThreads, 4) void fg_select_kernel(SelectPara
             for (uint32_t r = TEAM ? 0 : wave; r < static_cast<uint32_t>(t.rows); r += TEAM ? 1 : kSelectWaves) {
                 int32_t *out = P.ids + ((t.q0 + static_cast<uint64_t>(r)) * P.lists + list) * P.count;
                 if constexpr (MODE == kFused) pick_from<WAVES>(held + r * P.stride, n, P.count, first, out, picking[TEAM ? 0 : wave]);
-                else pick_from<WAVES>(static_cast<const uint32_t *>(stored) + static_cast<uint64_t>(r) * P.stride, n, P.count, first, out, picking[TEAM ? 0 : wave]);
+                else pick_from<WAVES>(stored + static_cast<uint64_t>(r) * P.stride, n, P.count, first, out, picking[TEAM ? 0 : wave]);
             }
             __syncthreads();
         }

@@ -212,27 +212,25 @@ __device__ __forceinline__ void list_freed(const EvictParams &P, uint32_t w, uin
     }
 }
 
-// The weights of tokens from + i on as keys, U at a time: their pages, then the weights.
+// The weights of U tokens j, j + step .. as keys, 0 from token `end` (1 or more) on: their pages
+// first, then the weights.
 template <uint32_t U, class F>
-__device__ __forceinline__ void load_keys(const EvictParams &P, uint32_t r, uint32_t h, uint32_t from, uint32_t end, uint32_t step, F put) {
+__device__ __forceinline__ void load_keys(const EvictParams &P, uint32_t r, uint32_t h, uint32_t j, uint32_t end, uint32_t step, F put) {
     int32_t page[U];
     float x[U];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t j = from + u * step;
-        page[u] = j < end ? P.table[r * P.table_row + P.cache.page_size.div(j)] : -1;
-    }
+    for (uint32_t u = 0; u < U; ++u) page[u] = P.table[r * P.table_row + P.cache.page_size.div(min(j + u * step, end - 1))];
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t j = from + u * step, at = j - P.cache.page_size.div(j) * P.cache.page_size.d;
-        const bool real = static_cast<uint32_t>(page[u]) < P.cache.pages;
-        x[u] = real ? P.weights[(static_cast<int64_t>(page[u]) * P.heads_kv + h) * P.cache.page_size.d + at] : 0.0f;
+        const uint32_t at = min(j + u * step, end - 1), off = at - P.cache.page_size.div(at) * P.cache.page_size.d;
+        const int64_t real = static_cast<uint32_t>(page[u]) < P.cache.pages ? page[u] : 0;
+        x[u] = P.weights[(real * P.heads_kv + h) * P.cache.page_size.d + off];
     }
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
         const bool real = static_cast<uint32_t>(page[u]) < P.cache.pages;
         const uint32_t key = !real ? 1u : x[u] != x[u] ? key_of(INFINITY) : key_of(x[u] + 0.0f);  // (-0 as 0)
-        put(u, from + u * step < end ? key : 0u);
+        put(u, j + u * step < end ? key : 0u);
     }
 }
 
@@ -293,12 +291,11 @@ __global__ __launch_bounds__(kChooseThreads, K == 8 ? 8 : 4) void fg_evict_choos
         };
         if constexpr (K > 0) {
             Held<K> run;
-            run.begin = begin, run.steps = (stop - begin + 63) / 64;
+            run.begin = begin, run.end = stop;
             constexpr uint32_t U = K > 8 ? 8 : 4;
 #pragma unroll
             for (uint32_t u0 = 0; u0 < K; u0 += U)
-                if (u0 < run.steps)
-                    load_keys<U>(P, r, h, P.sinks + begin + u0 * 64 + lane, P.sinks + stop, 64, [&](uint32_t u, uint32_t key) { run.key[u0 + u] = key; });
+                if (u0 == 0 || begin + u0 * 64 < stop) load_keys<U>(P, r, h, P.sinks + begin + u0 * 64 + lane, P.sinks + max(stop, 1u), 64, [&](uint32_t u, uint32_t key) { run.key[u0 + u] = key; });
             choose(run);
         } else {
             uint32_t *const keys = P.keys + static_cast<uint64_t>(blockIdx.x) * P.room;

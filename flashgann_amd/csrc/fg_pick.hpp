@@ -43,15 +43,18 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 template <uint32_t WAVES>
 __device__ __forceinline__ uint32_t run_size(uint32_t n) { return (n + 64 * WAVES - 1) / (64 * WAVES) * 64; }
 
-// A wave's run in registers, up to 64 * K keys; 0 past its end.
+// A wave's run in registers, up to 64 * K keys; 0 past its end.  Four are gone through at a time:
+// a branch around each costs more.
 template <uint32_t K>
 struct Held {
-    uint32_t key[K], begin, steps;
+    uint32_t key[K], begin, end;
     template <class F>
     __device__ __forceinline__ void each(F f) const {
 #pragma unroll
-        for (uint32_t u = 0; u < K; ++u)
-            if (u < steps) f(key[u], begin + u * 64 + threadIdx.x % 64);
+        for (uint32_t u = 0; u < K; ++u) {
+            if (u % 4 == 0 && u && begin + u * 64 >= end) break;
+            f(key[u], begin + u * 64 + threadIdx.x % 64);
+        }
     }
 };
 // In memory.
@@ -79,15 +82,14 @@ __device__ __forceinline__ Stored<Keys> stored_run(Keys keys, uint32_t n) {
     return {keys, begin, min(begin + per, n)};
 }
 template <uint32_t WAVES, uint32_t K, class Keys>
-__device__ __forceinline__ Held<K> held_run(Keys keys, uint32_t n) {  // run_size(n) <= 64 * K
+__device__ __forceinline__ Held<K> held_run(Keys keys, uint32_t n) {  // 1 <= n, run_size(n) <= 64 * K
     const uint32_t per = run_size<WAVES>(n), begin = min(team_wave<WAVES>() * per, n), end = min(begin + per, n);
     Held<K> h;
-    h.begin = begin, h.steps = (end - begin + 63) / 64;
+    h.begin = begin, h.end = end;
 #pragma unroll
-    for (uint32_t u = 0; u < K; ++u) {
-        const uint32_t i = begin + u * 64 + threadIdx.x % 64;
-        h.key[u] = u < h.steps && i < end ? static_cast<uint32_t>(keys[i]) : 0u;
-    }
+    for (uint32_t u = 0; u < K; ++u) h.key[u] = keys[min(begin + u * 64 + threadIdx.x % 64, n - 1)];
+#pragma unroll
+    for (uint32_t u = 0; u < K; ++u) h.key[u] = begin + u * 64 + threadIdx.x % 64 < end ? h.key[u] : 0u;
     return h;
 }
 
