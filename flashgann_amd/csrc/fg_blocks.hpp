@@ -7,7 +7,8 @@
 namespace fgk {
 
 constexpr uint32_t kMostBlocks = 4096;     // of a list: what attention over them holds in LDS
-constexpr uint32_t kMostTokens = 1u << 22; // of a call: its tiles are a grid's workgroups
+constexpr uint32_t kMostTokens = 1u << 22; // of a call
+constexpr uint32_t kMostItems = 1u << 23;  // tiles and lists of a call, a grid's workgroups
 
 // Rows of q in tiles: those of request r are tiles q_starts[r] / rows + r and on, which leaves
 // room for the ragged last one of each, so a call has tokens / rows + requests at most.  A tile

@@ -304,7 +304,15 @@ def test_attend_single_tokens(dtype, dim, heads, heads_kv, lists, page, layout):
 def test_attend_chunks(dtype, dim, heads, heads_kv, lists, page, first, last, k):
     """Rows of a tile with different lists; chunks and single tokens in one batch, a request with nothing new."""
     new, kv = [1, 0, 3, 21, 17, 1], [9, 77, 3, 90, 217, 260]
-    compare_attend(new, kv, heads, heads_kv, dim, page, dtype, lists, k, first, last, "hnd" if page == 24 else "nhd")
+    layout = "hnd" if page == 24 else "nhd"
+    compare_attend(new, kv, heads, heads_kv, dim, page, dtype, lists, k, first, last, layout)
+    compare_attend([70, 0, 1, 33], [75, 77, 3, 290], heads, heads_kv, dim, page, dtype, lists, k, first, last, layout, 1)
+
+
+@pytest.mark.parametrize("page,kv,k,first,last", ((1, 3000, 20, 3, 2), (1, 700, 300, 0, 600), (2, 4000, 5, 900, 1), (8, 9000, 3, 0, 1), (200, 5000, 2, 1, 1), (64, 3000, 4, 0, 2)))
+def test_attend_windows_of_blocks(page, kv, k, first, last):
+    """Chunks whose blocks are far apart, next to each other over many windows, larger than a tile."""
+    compare_attend([30, 9], [kv, kv // 2], 4, 1, 64, page, BF, 2, k, first, last, seed=page)
 
 
 def test_attend_lists_of_any_order():
