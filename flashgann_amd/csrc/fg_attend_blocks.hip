@@ -7,6 +7,7 @@
 // tokens see, each block with a mask of the tokens that see it: neighbours ask for much the
 // same, and where they do not, the rows that a block is not for cost matrix work only.
 #include "fg_blocks.hpp"
+#include "fg_pick.hpp"
 
 namespace fgk {
 namespace {
@@ -389,86 +390,95 @@ __global__ __launch_bounds__(256) void fg_blocks_join_kernel(BlocksParams P) {
 
 // ---------------------------------------------------------------- chunks
 //
-// Four waves of 16 rows each share tiles of 64 tokens in LDS: what the tokens of all four see
-// between them is read once, and a wave goes through the tiles that one of its own rows sees.  The
-// union of a chunk's lists is made a window of blocks at a time, a word of tokens for each block,
-// so its blocks come in order and none twice.
-constexpr uint32_t kWaves = 4, kShared = 64;  // waves of a workgroup; tokens of a tile
-constexpr uint32_t kWindow = 256;             // blocks whose tokens are known at a time
-
-// The barrier that publishes LDS and nothing else: loads in flight from global memory stay
-// in flight.
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
+// 32 rows a workgroup, so that what neighbours both select is read once for twice as many tokens,
+// on 32 x 32 matrix tiles; as above each of the four waves takes every fourth tile of 32 tokens and
+// nothing is waited for but its own loads.  A lane loads the keys of the token whose place it has
+// worked out.  The union of the lists is made a window of blocks at a time, a word of
+// tokens for each block, so its blocks come in order and none twice.
+constexpr uint32_t kChunkRows = 32;
+constexpr uint32_t kWindow = 1024;  // blocks whose tokens are known at a time
 
 // The tokens (a bit each, the first at position pos) at or after position j.
-__device__ __forceinline__ uint64_t tokens_from(int32_t pos, int64_t j) {
+__device__ __forceinline__ uint32_t tokens_from(int32_t pos, int64_t j) {
     const int64_t i = j - pos;
-    return i <= 0 ? ~0ull : i >= 64 ? 0ull : ~0ull << i;
+    return i <= 0 ? ~0u : i >= 32 ? 0u : ~0u << i;
+}
+
+// Whether an infinity or NaN is among N pieces of 16-bit values: their magnitudes' maximum, two
+// values an instruction.
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+template <class T, int N>
+__device__ __forceinline__ bool any_specials(const u32x4 (&w)[N]) {
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[k][i]) << static_cast<uint16_t>(1));
+    return max(most[0], most[1]) >= 2 * T::kExponent;
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_tiles_kernel(BlocksParams P) {
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_chunk_kernel(BlocksParams P) {
     using vec = typename T::vec;
-    constexpr int STEPS = D / 32, DB = D / 16, CHUNKS = D / 8, PER = kShared * CHUNKS / 256;
-    // LDS rows are longer than the data: 16 rows' 16-byte pieces of K, and of V 16 rows' 32-byte
-    // pieces, then meet every bank equally often
-    constexpr uint32_t KROW = 2 * D + 16, VROW = 2 * D + 32;
+    constexpr int STEPS = D / 16, DB = D / 32, CHUNKS = D / 8;
+    constexpr uint32_t VROW = 2 * D + (D == 96 ? 128 : 64);  // bytes of a row of V in LDS: eight rows' 64-byte pieces meet every bank equally often
+    constexpr uint32_t OROW = D + 4;                         // floats of a row of O in LDS
     constexpr float UP = T::kTopWeight, DOWN = 1.0f / (1 << T::kTopWeight);
-    __shared__ __attribute__((aligned(16))) char kbuf[2][kShared * KROW];
-    __shared__ __attribute__((aligned(16))) char vbuf[2][kShared * VROW];
-    __shared__ unsigned long long seen[kWindow];  // tokens that see a block of the window; then of an entry
-    __shared__ int32_t entry_page[kWindow], entry_block[kWindow];
-    __shared__ longlong2 place[2][kShared];       // of a tile's tokens: bytes from the head's first key and value
-    __shared__ uint64_t shown[4][kShared];        // the tokens that see each
-    __shared__ unsigned long long special[4];     // which of a tile's values hold an infinity or NaN
+    // values of a tile of each wave, the window's blocks and those of its entries; then the waves' outputs
+    struct Blocks {
+        uint32_t seen[kWindow];                   // the tokens that have a block on their list
+        int32_t entry_page[kWindow], entry_block[kWindow];
+        uint32_t entry_seen[kWindow];             // of the blocks that some token sees
+    };
+    constexpr uint32_t VBYTES = 4 * 32 * VROW, OBYTES = 4 * kChunkRows * OROW * 4;
+    __shared__ __attribute__((aligned(16))) char lds[VBYTES + sizeof(Blocks) > OBYTES ? VBYTES + sizeof(Blocks) : OBYTES];
+    __shared__ float wave_m[4][kChunkRows], wave_l[4][kChunkRows];
     __shared__ uint32_t found[4], next_block;
+    __shared__ int64_t value_at[4][2][32];  // where a wave's tile's values lie, from the head's first; of the next one
+    Blocks &B = *reinterpret_cast<Blocks *>(lds + VBYTES);
 
-    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 16, quarter = lane / 16;
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 32, half = lane / 32;
     const uint32_t tile = blockIdx.x / P.lanes, lane_of = blockIdx.x - tile * P.lanes;
-    const uint32_t list = lane_of / P.head_parts, head0 = (lane_of - list * P.head_parts) * kTileRows;
+    const uint32_t list = lane_of / P.head_parts, head0 = (lane_of - list * P.head_parts) * kChunkRows;
     const Tile t = tile_of(P.q_starts, P.kv_lens, P.requests, P.tokens, P.tile, tile);
     if (t.rows == 0) return;
-    const uint32_t tokens = t.rows, nids = P.nids, page_size = P.cache.page_size.d, wave_tokens = P.tile.d / kWaves;
+    const uint32_t tokens = t.rows, nids = P.nids, page_size = P.cache.page_size.d;
     const int32_t *const table = P.table + t.request * P.table_row;
     const auto block_of = [&](int32_t pos) { return pos < 0 ? -1 : static_cast<int32_t>(P.cache.page_size.div(pos)); };
     const uint32_t blocks = static_cast<uint32_t>(min(block_of(t.pos + t.rows - 1), static_cast<int32_t>(P.table_width) - 1) + 1);
     const uint32_t dense = static_cast<uint32_t>(min(max(static_cast<int64_t>(block_of(t.pos)) - P.last + 1, static_cast<int64_t>(0)), static_cast<int64_t>(blocks)));
-    const uint64_t everyone = tokens >= 64 ? ~0ull : (1ull << tokens) - 1;
+    const uint32_t everyone = tokens >= 32 ? ~0u : (1u << tokens) - 1;
 
-    // this lane's row, and its wave's tokens
-    const uint32_t token0 = wave * wave_tokens, mine = token0 < tokens ? min(tokens - token0, wave_tokens) : 0;
-    const uint32_t token = P.per.div(col), heads = min(P.group - head0, P.per.d);
-    const bool real = token < mine && col - token * P.per.d < heads;
-    const int64_t qrow = t.q0 + static_cast<int64_t>(token0 + token), head = static_cast<int64_t>(list) * P.group + head0 + (col - token * P.per.d);
+    // this lane's row
+    const uint32_t rows = tokens * P.per.d, token = P.per.div(col), heads = min(P.group - head0, P.per.d);
+    const bool real = col < rows && col - token * P.per.d < heads;
+    const int64_t head = static_cast<int64_t>(list) * P.group + head0 + (col - token * P.per.d);
     vec qv[STEPS];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         u32x4 v = {0, 0, 0, 0};
-        if (real) v = *reinterpret_cast<const u32x4 *>(P.q + qrow * P.q_token + head * P.q_head + quarter * 16 + 64 * s);
+        if (real) v = *reinterpret_cast<const u32x4 *>(P.q + (t.q0 + static_cast<int64_t>(token)) * P.q_token + head * P.q_head + half * 16 + 32 * s);
         qv[s] = __builtin_bit_cast(vec, v);
     }
     const uint32_t kv_head = list / P.list_heads;
-    const char *const kbase = P.cache.k + kv_head * P.cache.k_head, *const vbase = P.cache.v + kv_head * P.cache.v_head;
+    const char *const kbase = P.cache.k + kv_head * P.cache.k_head + half * 16, *const vbase = P.cache.v + kv_head * P.cache.v_head;
+    char *const vmine = lds + wave * 32 * VROW;
 
     float m = -INFINITY, l = 0.0f;
-    f32x4 o[DB];
+    f32x16 o[DB];
 #pragma unroll
-    for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < DB; ++i) o[i] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
     for (uint32_t w0 = 0; w0 < blocks;) {
         const uint32_t w1 = min(w0 + kWindow, blocks);
         __syncthreads();
-        seen[tid] = 0;
+        *reinterpret_cast<u32x4 *>(B.seen + 4 * tid) = u32x4{0, 0, 0, 0};
         if (tid == 0) next_block = blocks;
         __syncthreads();
         // the lists' blocks in the window, an id counting where the running maximum rises
-        for (uint32_t i = wave; i < tokens; i += kWaves) {
+        for (uint32_t i = wave; i < tokens; i += 4) {
             const int32_t *src = P.ids + ((t.q0 + static_cast<uint64_t>(i)) * P.lists + list) * nids;
-            const int32_t room = static_cast<int32_t>(max(min(static_cast<int64_t>(block_of(t.pos + static_cast<int32_t>(i))) - P.last, static_cast<int64_t>(blocks) - 1), static_cast<int64_t>(-1)));
+            const int64_t room = min(static_cast<int64_t>(block_of(t.pos + static_cast<int32_t>(i))) - P.last, static_cast<int64_t>(blocks) - 1);
             int32_t most = -1;
             for (uint32_t k0 = 0; k0 < nids; k0 += 64) {
                 const int32_t id = k0 + lane < nids ? src[k0 + lane] : -1;
@@ -481,127 +491,127 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_tiles_kernel(B
                 x = max(x, most);
                 const int32_t up = __shfl_up(x, 1), before = lane ? up : most;
                 most = of_lane(x, 63);
-                if (id > before && id <= room && id >= 0 && static_cast<uint32_t>(id) >= P.first) {
-                    if (static_cast<uint32_t>(id) >= w0 && static_cast<uint32_t>(id) < w1) atomicOr(&seen[id - w0], 1ull << i);
+                if (id > before && id <= room && static_cast<uint32_t>(id) >= P.first) {
+                    if (static_cast<uint32_t>(id) >= w0 && static_cast<uint32_t>(id) < w1) atomicOr(&B.seen[id - w0], 1u << i);
                     else if (static_cast<uint32_t>(id) >= w1) atomicMin(&next_block, static_cast<uint32_t>(id));
                 }
             }
         }
         __syncthreads();
-        // those that some token sees, in order
-        const uint32_t b = w0 + tid;
-        uint64_t mask = 0;
-        int32_t page = -1;
-        if (b < w1) {
-            mask = seen[tid];
-            if (b < P.first) mask = ~0ull;
-            // among the last blocks of the tokens before position (b + last) * page_size
-            mask |= ~tokens_from(t.pos, (static_cast<int64_t>(b) + P.last) * page_size);
-            mask &= tokens_from(t.pos, static_cast<int64_t>(b) * page_size) & everyone;
-            if (mask) page = table[b];
-            if (static_cast<uint32_t>(page) >= P.cache.pages) mask = 0;
-        }
-        const uint64_t which = __ballot(mask != 0);
-        if (lane == 0) found[wave] = __popcll(which);
-        __syncthreads();
-        uint32_t at = __popcll(which & ((1ull << lane) - 1)), entries = 0;
+        // those that some token sees, in order; four a thread
+        const u32x4 listed = *reinterpret_cast<const u32x4 *>(B.seen + 4 * tid);
+        uint32_t mask[4], count = 0;
+        int32_t page[4];
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) {
+        for (uint32_t u = 0; u < 4; ++u) {
+            const uint32_t b = w0 + 4 * tid + u;
+            mask[u] = listed[u];
+            if (b < P.first) mask[u] = ~0u;
+            // among the last blocks of the tokens before position (b + last) * page_size
+            mask[u] |= ~tokens_from(t.pos, (static_cast<int64_t>(b) + P.last) * page_size);
+            mask[u] &= tokens_from(t.pos, static_cast<int64_t>(b) * page_size) & everyone;
+            if (b >= w1) mask[u] = 0;
+            page[u] = mask[u] ? table[b] : -1;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            if (static_cast<uint32_t>(page[u]) >= P.cache.pages) mask[u] = 0;
+            count += mask[u] != 0;
+        }
+        const uint32_t upto = sum_upto(count);
+        if (lane == 63) found[wave] = upto;
+        __syncthreads();
+        uint32_t at = upto - count, entries = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) {
             if (w < wave) at += found[w];
             entries += found[w];
         }
-        if (mask) seen[at] = mask, entry_page[at] = page, entry_block[at] = static_cast<int32_t>(b);
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+            if (mask[u]) {
+                B.entry_page[at] = page[u], B.entry_block[at] = static_cast<int32_t>(w0 + 4 * tid + u), B.entry_seen[at] = mask[u];
+                ++at;
+            }
         entries = uniform(entries);
         // where the next window begins
-        uint32_t next = next_block;
+        uint32_t next = min(next_block, max(dense, w1));
         if (w1 < P.first) next = w1;
-        next = min(next, max(dense, w1));
         w0 = uniform(max(next, w1));
         __syncthreads();
 
-        const int32_t total = static_cast<int32_t>(entries * page_size), tiles = (total + static_cast<int32_t>(kShared) - 1) / static_cast<int32_t>(kShared);
-        if (tiles == 0) continue;
-        const auto note = [&](int32_t i) {  // by one wave
-            const int32_t n = i * static_cast<int32_t>(kShared) + static_cast<int32_t>(lane);
-            uint64_t sees = 0;
-            longlong2 where = {0, 0};
-            if (n < total) {
-                const uint32_t e = P.cache.page_size.div(n);
-                const int64_t off = n - static_cast<int32_t>(e * page_size), p = entry_page[e];
-                sees = seen[e] & tokens_from(t.pos, static_cast<int64_t>(entry_block[e]) * page_size + off);
-                where = longlong2{p * P.cache.k_page + off * P.cache.k_token, p * P.cache.v_page + off * P.cache.v_token};
-            }
-            place[i % 2][lane] = where;
-            shown[i % 4][lane] = sees;
-            if (lane == 0) special[i % 4] = 0;
+        const int32_t total = static_cast<int32_t>(entries * page_size);
+        u32x4 kr[STEPS], vr[STEPS];
+        uint32_t sees;  // the tokens that see this lane's token of the tile
+        // (a lane loads its token's keys, as the product wants them, and of the values 16 bytes
+        // beside its neighbours')
+        const char *ks;
+        const auto find = [&](int32_t i) {
+            const int32_t n = i * 32 + static_cast<int32_t>(col), in = min(n, total - 1);
+            const uint32_t e = P.cache.page_size.div(in);
+            const int64_t off = in - static_cast<int32_t>(e * page_size), p = B.entry_page[e];
+            sees = n < total ? B.entry_seen[e] & tokens_from(t.pos, static_cast<int64_t>(B.entry_block[e]) * page_size + off) : 0u;
+            ks = kbase + p * P.cache.k_page + off * P.cache.k_token;
+            if (half == 0) value_at[wave][i / 4 % 2][col] = p * P.cache.v_page + off * P.cache.v_token;
         };
-        u32x4 kr[PER], vr[PER];
-        const auto load = [&](int32_t i) {
+        const auto load_k = [&] {
 #pragma unroll
-            for (int c = 0; c < PER; ++c) {
-                const uint32_t at = tid + c * 256;
-                const longlong2 where = place[i % 2][at / CHUNKS];
-                kr[c] = *reinterpret_cast<const u32x4 *>(kbase + where.x + at % CHUNKS * 16);
-                vr[c] = *reinterpret_cast<const u32x4 *>(vbase + where.y + at % CHUNKS * 16);
+            for (int s = 0; s < STEPS; ++s) kr[s] = *reinterpret_cast<const u32x4 *>(ks + 32 * s);
+        };
+        const auto load_v = [&](int32_t i) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const uint32_t at = s * 64 + lane;
+                vr[s] = *reinterpret_cast<const u32x4 *>(vbase + value_at[wave][i / 4 % 2][at / CHUNKS] + at % CHUNKS * 16);
             }
         };
-        const auto store = [&](int32_t i) {
+        if (static_cast<int32_t>(wave) * 32 < total) {
+            find(static_cast<int32_t>(wave));
+            load_k();
+            load_v(static_cast<int32_t>(wave));
+        }
+        for (int32_t i = static_cast<int32_t>(wave); i * 32 < total; i += 4) {
+            const uint32_t sees_now = sees;
+            const bool more = (i + 4) * 32 < total;
+            if (more) find(i + 4);
+            // scores: register k is that of token 8 (k / 4) + 4 half + k % 4
+            f32x16 s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < PER; ++c) {
-                const uint32_t at = tid + c * 256, row = at / CHUNKS;
-                *reinterpret_cast<u32x4 *>(kbuf[i % 2] + row * KROW + at % CHUNKS * 16) = kr[c];
-                u32x4 v = vr[c];
-                if (any_special<T>(v)) {
-                    // 0 * inf is NaN: infinities and NaNs are taken out of the product and added to
-                    // the rows that see them
-                    v = finite_part<T>(v);
-                    atomicOr(&special[i % 4], 1ull << row);
+            for (int k = 0; k < STEPS; ++k) s = T::mfma32(__builtin_bit_cast(vec, kr[k]), qv[k], s);
+            if (more) load_k();
+            uint32_t odd = 0;  // tokens whose values are not all finite
+            if (__any(any_specials<T>(vr))) {
+                // 0 * inf is NaN: infinities and NaNs are taken out of the product and added to the
+                // rows that see them
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                    if (any_special<T>(vr[k])) odd |= 1u << (k * 64 + lane) / CHUNKS;
+                    vr[k] = finite_part<T>(vr[k]);
                 }
-                *reinterpret_cast<u32x4 *>(vbuf[i % 2] + row * VROW + at % CHUNKS * 16) = v;
+                odd = last_lane(wave_scan(odd, 0, [](uint32_t a, uint32_t b) { return a | b; }));
             }
-        };
-        if (wave < 2) note(wave);
-        __syncthreads();
-        load(0);
-        __syncthreads();
-        if (wave == 2) note(2);
-        store(0);
-        load(1);
-
-        for (int32_t i = 0; i < tiles; ++i) {
-            lds_barrier();
-            if (i + 1 < tiles) store(i + 1);
-            if (wave == (i + 3) % kWaves) note(i + 3);
-            if (i + 2 < tiles) load(i + 2);
-
-            // the tile's tokens that each of the wave's tokens sees
-            const uint64_t sees = shown[i % 4][lane] >> token0;
-            uint64_t row_sees = 0, some = 0, all = ~0ull;
-            for (uint32_t x = 0; x < mine; ++x) {
-                const uint64_t those = __ballot((sees >> x) & 1);
-                some |= those, all &= those;
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                const uint32_t at = k * 64 + lane;
+                *reinterpret_cast<u32x4 *>(vmine + at / CHUNKS * VROW + at % CHUNKS * 16) = vr[k];
+            }
+            if (more) load_v(i + 4);
+            // the tile's tokens that this lane's row sees
+            uint32_t row_sees = 0, all = ~0u;
+            for (uint32_t x = 0; x < tokens; ++x) {
+                const uint32_t those = static_cast<uint32_t>(__ballot((sees_now >> x) & 1u));
+                all &= those;
                 row_sees = token == x ? those : row_sees;
             }
-            if (!some) continue;
-            const char *const kt = kbuf[i % 2] + col * KROW + 16 * quarter;
-            f32x4 s[4];  // register i of s[b] is token 16 b + 4 quarter + i
+            if (all != ~0u) {
+                const uint32_t bits = row_sees >> (4 * half);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                s[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k)
-                    s[b] = T::mfma16(__builtin_bit_cast(vec, *reinterpret_cast<const u32x4 *>(kt + 16 * b * KROW + 64 * k)), qv[k], s[b]);
+                for (int k = 0; k < 16; ++k) s[k] = keep_if(bits, k / 4 * 8 + k % 4, s[k]);
             }
             float top = -INFINITY;
-            if (all != ~0ull) {
-                const uint64_t bits = row_sees >> (4 * quarter);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) s[k / 4][k % 4] = keep_if(static_cast<uint32_t>(bits >> (k / 8 * 32)), k / 4 % 2 * 16 + k % 4, s[k / 4][k % 4]);
-            }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k / 4][k % 4]);
-            top = max_other32(max_other16(top)) * P.scale2;
-            top = fmaxf(m, top);
+            for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k]);
+            top = fmaxf(m, max_other32(top) * P.scale2);
             const float base = top == -INFINITY ? 0.0f : top;
             if (__any(top > m)) {
                 const float shrink = __builtin_amdgcn_exp2f(m - base);
@@ -612,56 +622,81 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_tiles_kernel(B
             }
             const float zero = UP - base;
             float sum = 0.0f;
-            u32x4 pk[2];
+            u32x4 pk[2];  // the weights of 16 tokens each
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                float p[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) p[k] = __builtin_amdgcn_exp2f(fmaf(s[b][k], P.scale2, zero));
-                sum += (p[0] + p[1]) + (p[2] + p[3]);
-                pk[b / 2][b % 2 * 2] = T::pack(p[0], p[1]), pk[b / 2][b % 2 * 2 + 1] = T::pack(p[2], p[3]);
+            for (int k = 0; k < 16; k += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[k], P.scale2, zero)), p1 = __builtin_amdgcn_exp2f(fmaf(s[k + 1], P.scale2, zero));
+                sum += p0 + p1;
+                pk[k / 8][k % 8 / 2] = T::pack(p0, p1);
             }
             l += sum;
-            const char *const vt = vbuf[i % 2] + (4 * quarter + col / 4) * VROW + (col % 4) * 8;
+            const char *const vt = vmine + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int k = 0; k < DB; ++k) {
-                    const s16x4 a0 = read_transposed(vt + 32 * h * VROW + 32 * k), a1 = read_transposed(vt + (32 * h + 16) * VROW + 32 * k);
-                    const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[k] = T::mfma16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, pk[h]), o[k]);
-                }
-            for (uint64_t odd = uniform(static_cast<uint64_t>(special[i % 4])) & some; odd; odd &= odd - 1) {
-                const uint32_t at = __ffsll(static_cast<unsigned long long>(odd)) - 1;
-                const int32_t n = i * static_cast<int32_t>(kShared) + static_cast<int32_t>(at);
-                const uint32_t e = P.cache.page_size.div(n);
-                const char *src = vbase + entry_page[e] * P.cache.v_page + static_cast<int64_t>(n - static_cast<int32_t>(e * page_size)) * P.cache.v_token + quarter * 8;
+            for (int n = 0; n < 2 * DB; ++n) {
+                const char *at = vt + 16 * (n / DB) * VROW + 64 * (n % DB);
+                const s16x8 a = __builtin_shufflevector(read_transposed(at), read_transposed(at + 8 * VROW), 0, 1, 2, 3, 4, 5, 6, 7);
+                o[n % DB] = T::mfma32(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, pk[n / DB]), o[n % DB]);
+            }
+            for (; odd; odd &= odd - 1) {
+                const int at = __ffs(odd) - 1;
+                const char *src = vbase + value_at[wave][i / 4 % 2][at] + half * 8;
                 const bool visible = (row_sees >> at) & 1u;
 #pragma unroll
-                for (int k = 0; k < DB; ++k) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(src + 32 * k);
-                    o[k][0] += visible ? special_part<T>(v.x & 0xFFFF) : 0.0f;
-                    o[k][1] += visible ? special_part<T>(v.x >> 16) : 0.0f;
-                    o[k][2] += visible ? special_part<T>(v.y & 0xFFFF) : 0.0f;
-                    o[k][3] += visible ? special_part<T>(v.y >> 16) : 0.0f;
-                }
+                for (int k = 0; k < DB; ++k)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {  // dimensions 32 k + 8 g + 4 half and on
+                        const uint2 v = *reinterpret_cast<const uint2 *>(src + 64 * k + 16 * g);
+                        o[k][4 * g] += visible ? special_part<T>(v.x & 0xFFFF) : 0.0f;
+                        o[k][4 * g + 1] += visible ? special_part<T>(v.x >> 16) : 0.0f;
+                        o[k][4 * g + 2] += visible ? special_part<T>(v.y & 0xFFFF) : 0.0f;
+                        o[k][4 * g + 3] += visible ? special_part<T>(v.y >> 16) : 0.0f;
+                    }
             }
         }
     }
 
-    l = add_other32(add_other16(l)) * DOWN;
-    if (!real) return;
-    const float inv = l == 0.0f ? 0.0f : DOWN / l;
-    char *const dst = P.out + qrow * P.out_token + head * P.out_head + quarter * 8;
+    // the four waves' softmaxes into one
+    l = add_other32(l);
+    if (half == 0) wave_m[wave][col] = m;
+    __syncthreads();
+    float top = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < DB; ++k) *reinterpret_cast<uint2 *>(dst + 32 * k) = uint2{T::pack(o[k][0] * inv, o[k][1] * inv), T::pack(o[k][2] * inv, o[k][3] * inv)};
-    if (quarter == 0 && P.lse) P.lse[qrow * P.heads + head] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, wave_m[i][col]);
+    const float mine = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top)) * DOWN;
+    if (half == 0) wave_l[wave][col] = l * mine;
+    float *const all_o = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int k = 0; k < DB; ++k)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4 *>(all_o + (wave * kChunkRows + col) * OROW + 32 * k + 8 * g + 4 * half) =
+                f32x4{o[k][4 * g], o[k][4 * g + 1], o[k][4 * g + 2], o[k][4 * g + 3]} * mine;
+    __syncthreads();
+    if (wave == 0 && half == 0 && real && P.lse) {
+        const float sum = wave_l[0][col] + wave_l[1][col] + wave_l[2][col] + wave_l[3][col];
+        P.lse[(t.q0 + static_cast<int64_t>(token)) * P.heads + head] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < kChunkRows * D / 4; e += 256) {
+        const uint32_t at = e + tid, orow = at / (D / 4), quad = at % (D / 4);
+        const uint32_t otoken = P.per.div(orow), ohead = orow - otoken * P.per.d;
+        if (orow < rows && ohead < heads) {
+            f32x4 a = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a += *reinterpret_cast<const f32x4 *>(all_o + (i * kChunkRows + orow) * OROW + 4 * quad);
+            const float sum = wave_l[0][orow] + wave_l[1][orow] + wave_l[2][orow] + wave_l[3][orow];
+            a *= sum == 0.0f ? 0.0f : 1.0f / sum;
+            char *dst = P.out + (t.q0 + static_cast<int64_t>(otoken)) * P.out_token +
+                        (static_cast<int64_t>(list) * P.group + head0 + ohead) * P.out_head;
+            *reinterpret_cast<uint2 *>(dst + 8 * quad) = uint2{T::pack(a[0], a[1]), T::pack(a[2], a[3])};
+        }
+    }
 }
 
 // ---------------------------------------------------------------- host side
 
 struct BlocksPlan {
-    bool shared;  // chunks: four waves' rows over tiles in LDS
+    bool chunk;  // which kernel
     uint32_t tiles, lds;
     uint64_t ml, workspace;
 };
@@ -708,24 +743,23 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     P.group = a->heads / a->lists;
     P.scale2 = a->scale * 1.44269504088896341f;
 
-    // A tile: the rows of as many tokens as 16 hold, their lists in LDS
-    const uint32_t per = std::min(P.group, kTileRows);
-    uint32_t tokens = kTileRows / per;
-    plan->shared = a->tokens >= 8 * static_cast<uint64_t>(a->requests) && a->table_width <= 4096;
-    if (plan->shared) tokens *= kWaves;
-    else if (P.nids) tokens = std::min(tokens, std::max(1u, kMostBlocks / P.nids));
+    // A tile: the rows of as many tokens as 16 (32) hold; the former's lists in LDS
+    plan->chunk = a->tokens >= 8 * static_cast<uint64_t>(a->requests) && a->table_width <= 16 * kWindow;
+    const uint32_t most_rows = plan->chunk ? kChunkRows : kTileRows, per = std::min(P.group, most_rows);
+    uint32_t tokens = most_rows / per;
+    if (!plan->chunk && P.nids) tokens = std::min(tokens, std::max(1u, kMostBlocks / P.nids));
     P.per = fast_div(per);
-    P.head_parts = (P.group + kTileRows - 1) / kTileRows;
+    P.head_parts = (P.group + most_rows - 1) / most_rows;
     P.tile = fast_div(tokens);
     P.lanes = P.lists * P.head_parts;
     plan->tiles = a->tokens / tokens + (tokens > 1 ? a->requests : 0);
-    plan->lds = plan->shared ? 0 : tokens * P.nids * 12;
+    plan->lds = plan->chunk ? 0 : tokens * P.nids * 12;
     const uint64_t items = static_cast<uint64_t>(plan->tiles) * P.lanes;
     if (items > kMostItems) return fail(FG_EINVAL, "more than 2^23 tiles of rows: attend to fewer tokens a call");
     const uint64_t blocks = std::min<uint64_t>(a->table_width, static_cast<uint64_t>(P.first) + P.last + P.nids);
     const uint64_t most = blocks * c->page_size;
     P.parts = 1;
-    while (!plan->shared && P.parts < kMostParts && items * P.parts < 512 && most > 2 * P.parts * kSplitTokens) P.parts *= 2;
+    while (!plan->chunk && P.parts < kMostParts && items * P.parts < 512 && most > 2 * P.parts * kSplitTokens) P.parts *= 2;
     const uint64_t slots = items * P.parts * kTileRows;
     plan->ml = slots * c->dim * 4;
     plan->workspace = P.parts > 1 ? slots * (c->dim * 4 + 8) : 0;
@@ -734,8 +768,8 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
 
 template <class T, int D>
 int launch(const BlocksParams &P, const BlocksPlan &plan, hipStream_t st) {
-    if (plan.shared) {
-        hipLaunchKernelGGL((fg_blocks_tiles_kernel<T, D>), dim3(plan.tiles * P.lanes), dim3(256), 0, st, P);
+    if (plan.chunk) {
+        hipLaunchKernelGGL((fg_blocks_chunk_kernel<T, D>), dim3(plan.tiles * P.lanes), dim3(256), 0, st, P);
         FG_HIP(hipGetLastError(), "attention launch");
         return FG_OK;
     }
