@@ -418,7 +418,7 @@ __device__ __forceinline__ bool any_specials(const u32x4 (&w)[N]) {
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_chunk_kernel(BlocksParams P) {
+__global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P) {
     using vec = typename T::vec;
     constexpr int STEPS = D / 16, DB = D / 32, CHUNKS = D / 8;
     constexpr uint32_t VROW = 2 * D + (D == 96 ? 128 : 64);  // bytes of a row of V in LDS: eight rows' 64-byte pieces meet every bank equally often
@@ -744,7 +744,8 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     P.scale2 = a->scale * 1.44269504088896341f;
 
     // A tile: the rows of as many tokens as 16 (32) hold; the former's lists in LDS
-    plan->chunk = a->tokens >= 8 * static_cast<uint64_t>(a->requests) && a->table_width <= 16 * kWindow;
+    // (at dim 256 the chunk kernel's rows do not fit the registers)
+    plan->chunk = c->dim <= 128 && a->tokens >= 8 * static_cast<uint64_t>(a->requests) && a->table_width <= 16 * kWindow;
     const uint32_t most_rows = plan->chunk ? kChunkRows : kTileRows, per = std::min(P.group, most_rows);
     uint32_t tokens = most_rows / per;
     if (!plan->chunk && P.nids) tokens = std::min(tokens, std::max(1u, kMostBlocks / P.nids));
@@ -768,10 +769,12 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
 
 template <class T, int D>
 int launch(const BlocksParams &P, const BlocksPlan &plan, hipStream_t st) {
-    if (plan.chunk) {
-        hipLaunchKernelGGL((fg_blocks_chunk_kernel<T, D>), dim3(plan.tiles * P.lanes), dim3(256), 0, st, P);
-        FG_HIP(hipGetLastError(), "attention launch");
-        return FG_OK;
+    if constexpr (D <= 128) {
+        if (plan.chunk) {
+            hipLaunchKernelGGL((fg_blocks_chunk_kernel<T, D>), dim3(plan.tiles * P.lanes), dim3(256), 0, st, P);
+            FG_HIP(hipGetLastError(), "attention launch");
+            return FG_OK;
+        }
     }
     FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(fg_blocks_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, kMostBlocks * 12), "attention LDS");
     hipLaunchKernelGGL((fg_blocks_kernel<T, D>), dim3(plan.tiles * P.parts * P.lanes), dim3(256), plan.lds, st, P);
