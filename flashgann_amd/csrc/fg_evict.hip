@@ -32,14 +32,26 @@ struct WeighParams {
 // Each of the four waves holds the keys of 64 tokens in registers and goes through the rows,
 // which all share from LDS, 16 at a time on the matrix unit: a lane's column is a token, so
 // its sum stays in one register till the end.
+// The barrier that publishes LDS and nothing else: loads in flight from global memory stay
+// in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <class T, int D>
-__global__ __launch_bounds__(256) void fg_weigh_kernel(WeighParams P) {
+__global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void fg_weigh_kernel(WeighParams P) {
     using vec = typename T::vec;
     constexpr int STEPS = D / 32;
     constexpr uint32_t QROW = 2 * D + 16;  // bytes of a row in LDS
-    __shared__ __attribute__((aligned(16))) char rows_of[kWeighRows * QROW];
-    __shared__ __attribute__((aligned(16))) float lse2[kWeighRows];
-    __shared__ __attribute__((aligned(16))) int32_t row_pos[kWeighRows];  // INT_MIN: the row counts nowhere
+    constexpr int PER = kWeighRows * (D / 8) / 256;
+    // rows of two steps: those being weighed and the next ones
+    __shared__ __attribute__((aligned(16))) char rows_of[2][kWeighRows * QROW];
+    __shared__ __attribute__((aligned(16))) float lse2[2][kWeighRows];
+    __shared__ __attribute__((aligned(16))) int32_t row_pos[2][kWeighRows];  // INT_MIN: the row counts nowhere
+    __shared__ uint32_t all_count[2];                                        // whether all of a step's rows count
+    static_assert(kWeighRows == 64);
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64), col = lane % 16, quarter = lane / 16;
     const uint64_t items = static_cast<uint64_t>(P.requests) * P.heads_kv * P.spread;
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
@@ -70,41 +82,54 @@ __global__ __launch_bounds__(256) void fg_weigh_kernel(WeighParams P) {
             float sum[4] = {0, 0, 0, 0};
             // rows before position j0 see none of these tokens
             const int32_t begin = max(j0 - pos0, 0) < fresh ? max(j0 - pos0, 0) * static_cast<int32_t>(P.group.d) : nrows;
-            for (int32_t base = begin; base < nrows; base += kWeighRows) {
-                __syncthreads();
+            u32x4 q_next[PER];
+            float z_next = 0.0f;
+            const auto load = [&](int32_t base) {
 #pragma unroll
-                for (uint32_t e0 = 0; e0 < kWeighRows * (D / 8); e0 += 256) {
-                    const uint32_t e = e0 + tid, i = e / (D / 8), piece = e % (D / 8);
-                    const int32_t row = base + static_cast<int32_t>(i), token = P.group.div(min(row, nrows - 1));
-                    u32x4 v = {0, 0, 0, 0};
-                    if (row < nrows)
-                        v = *reinterpret_cast<const u32x4 *>(P.q + (q0 + static_cast<int64_t>(token)) * P.q_token +
-                                                             (static_cast<int64_t>(h) * P.group.d + (row - token * static_cast<int32_t>(P.group.d))) * P.q_head + piece * 16);
-                    *reinterpret_cast<u32x4 *>(rows_of + i * QROW + piece * 16) = v;
+                for (int c = 0; c < PER; ++c) {
+                    const uint32_t e = c * 256 + tid;
+                    const int32_t row = min(base + static_cast<int32_t>(e / (D / 8)), nrows - 1), token = P.group.div(row);
+                    q_next[c] = *reinterpret_cast<const u32x4 *>(P.q + (q0 + static_cast<int64_t>(token)) * P.q_token +
+                                                                 (static_cast<int64_t>(h) * P.group.d + (row - token * static_cast<int32_t>(P.group.d))) * P.q_head + e % (D / 8) * 16);
                 }
                 if (tid < kWeighRows) {
-                    const int32_t row = base + static_cast<int32_t>(tid), token = P.group.div(min(row, nrows - 1));
-                    float z = 0.0f;
-                    int32_t pos = INT32_MIN;
-                    if (row < nrows) {
-                        z = P.lse[(q0 + static_cast<int64_t>(token)) * P.heads + h * P.group.d + (row - token * static_cast<int32_t>(P.group.d))];
-                        if (z != -INFINITY) pos = pos0 + token;
-                        else z = 0.0f;
-                    }
-                    lse2[tid] = z * 1.44269504088896341f;
-                    row_pos[tid] = pos;
+                    const int32_t row = min(base + static_cast<int32_t>(tid), nrows - 1), token = P.group.div(row);
+                    z_next = P.lse[(q0 + static_cast<int64_t>(token)) * P.heads + h * P.group.d + (row - token * static_cast<int32_t>(P.group.d))];
                 }
-                __syncthreads();
-                const int32_t here = min(nrows - base, static_cast<int32_t>(kWeighRows));
-                for (int32_t i0 = 0; i0 < here; i0 += 16) {
-                    const int32_t tail = base + min(i0 + 15, here - 1);
-                    if (pos0 + static_cast<int32_t>(P.group.div(tail)) < jw) continue;
+            };
+            const auto store = [&](int32_t base, uint32_t buf) {  // (rows past the last are repeated and count nowhere)
+#pragma unroll
+                for (int c = 0; c < PER; ++c) {
+                    const uint32_t e = c * 256 + tid;
+                    *reinterpret_cast<u32x4 *>(rows_of[buf] + e / (D / 8) * QROW + e % (D / 8) * 16) = q_next[c];
+                }
+                if (tid < kWeighRows) {
+                    const int32_t row = base + static_cast<int32_t>(tid);
+                    const bool counts = row < nrows && z_next != -INFINITY;
+                    lse2[buf][tid] = counts ? z_next * 1.44269504088896341f : 0.0f;
+                    row_pos[buf][tid] = counts ? pos0 + static_cast<int32_t>(P.group.div(row)) : INT32_MIN;
+                    const bool all = __all(counts);
+                    if (tid == 0) all_count[buf] = all;
+                }
+            };
+            __syncthreads();
+            if (begin < nrows) {
+                load(begin);
+                store(begin, 0);
+            }
+            wait_loads();  // of the keys: not known to have landed, they would be waited for in the loop, the next rows with them
+            if (begin + static_cast<int32_t>(kWeighRows) < nrows) load(begin + kWeighRows);
+            uint32_t buf = 0;
+            for (int32_t base = begin; base < nrows; base += kWeighRows, buf ^= 1) {
+                lds_barrier();
+                if (base + static_cast<int32_t>(kWeighRows) < nrows) store(base + kWeighRows, buf ^ 1);
+                if (base + 2 * static_cast<int32_t>(kWeighRows) < nrows) load(base + 2 * kWeighRows);
+                const auto weigh = [&](int32_t i0, auto masked) {
                     vec qf[STEPS];
 #pragma unroll
-                    for (int s = 0; s < STEPS; ++s) qf[s] = *reinterpret_cast<const vec *>(rows_of + (i0 + col) * QROW + 64 * s + 16 * quarter);
-                    const f32x4 z = *reinterpret_cast<const f32x4 *>(lse2 + i0 + 4 * quarter);
-                    const s32x4 pos = *reinterpret_cast<const s32x4 *>(row_pos + i0 + 4 * quarter);
-                    const bool all = __all(min(min(pos[0], pos[1]), min(pos[2], pos[3])) >= jw + 63);
+                    for (int s = 0; s < STEPS; ++s) qf[s] = *reinterpret_cast<const vec *>(rows_of[buf] + (i0 + col) * QROW + 64 * s + 16 * quarter);
+                    const f32x4 z = *reinterpret_cast<const f32x4 *>(lse2[buf] + i0 + 4 * quarter);
+                    const s32x4 pos = masked ? *reinterpret_cast<const s32x4 *>(row_pos[buf] + i0 + 4 * quarter) : s32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         f32x4 s = {0, 0, 0, 0};
@@ -113,12 +138,21 @@ __global__ __launch_bounds__(256) void fg_weigh_kernel(WeighParams P) {
                         float p[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], P.scale2, -z[i]));
-                        if (!all) {
+                        if (masked) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) p[i] = pos[i] >= jw + 16 * c + static_cast<int32_t>(col) ? p[i] : 0.0f;
                         }
                         sum[c] += (p[0] + p[1]) + (p[2] + p[3]);
                     }
+                };
+                // (rows are in order of position)
+                if (uniform(all_count[buf]) && pos0 + static_cast<int32_t>(P.group.div(base)) >= jw + 63) {
+#pragma unroll
+                    for (int32_t i0 = 0; i0 < static_cast<int32_t>(kWeighRows); i0 += 16) weigh(i0, std::false_type{});
+                } else {
+                    const int32_t here = min(nrows - base, static_cast<int32_t>(kWeighRows));
+                    for (int32_t i0 = 0; i0 < here; i0 += 16)
+                        if (pos0 + static_cast<int32_t>(P.group.div(base + min(i0 + 15, here - 1))) >= jw) weigh(i0, std::true_type{});
                 }
             }
 #pragma unroll
