@@ -173,7 +173,9 @@ constexpr uint32_t kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
 constexpr uint32_t kFewKeys = 8 * kChooseThreads, kChooseKeys = 32 * kChooseThreads;  // weights that a workgroup holds in registers
 constexpr uint32_t kChooseWorkgroups = 512; // at most, where it does not
 constexpr uint32_t kEvictRequests = 4096;
-constexpr uint32_t kMoveThreads = 256, kMovePieces = 4;  // 16-byte pieces of a row that a workgroup moves
+constexpr uint32_t kMoveThreads = 256, kMoveRows = 64;  // rows of a workgroup that fills holes
+constexpr uint32_t kShiftPieces = 4;                    // 16-byte pieces of a row that a workgroup of the last tokens' move takes
+constexpr uint32_t kFewMoves = 512;                     // that the workgroup which chose them makes itself
 
 struct EvictParams {
     CacheView cache;
@@ -188,16 +190,14 @@ struct EvictParams {
     uint32_t room;       // tokens that the table names
     uint32_t most;       // min(budget, room)
     uint32_t choosers;   // workgroups that choose; the others list the pages that go
+    uint32_t pieces;     // 16-byte pieces of a row of keys
+    uint32_t at_once;    // whether those that choose move too
 };
 
 __device__ __forceinline__ int32_t slot_of(const EvictParams &P, uint32_t r, uint32_t j) {
     const uint32_t b = P.cache.page_size.div(j);
     const int32_t page = P.table[r * P.table_row + b];
     return static_cast<uint32_t>(page) < P.cache.pages ? static_cast<int32_t>(page * P.cache.page_size.d + (j - b * P.cache.page_size.d)) : -1;
-}
-__device__ __forceinline__ int64_t weight_at(const EvictParams &P, uint32_t h, int32_t slot) {
-    const uint32_t page = P.cache.page_size.div(slot);
-    return (static_cast<int64_t>(page) * P.heads_kv + h) * P.cache.page_size.d + (slot - page * P.cache.page_size.d);
 }
 __device__ __forceinline__ uint32_t length_of(const EvictParams &P, uint32_t r) { return min(static_cast<uint32_t>(max(P.kv_lens[r], 0)), P.room); }
 __device__ __forceinline__ uint32_t pages_of(const EvictParams &P, uint32_t n) {
@@ -246,6 +246,59 @@ __device__ __forceinline__ void list_freed(const EvictParams &P, uint32_t w, uin
     }
 }
 
+// One thread's part of moving rows of a request and head: 16 bytes of each, of the keys, then the
+// values, and with the first of them the weight.
+struct Mover {
+    char *base;
+    int64_t page_step, token_step;
+    float *weights;  // of the head, page 0; nullptr: another thread moves them
+    uint32_t weight_step;
+    FastDiv page_size;
+    __device__ __forceinline__ Mover(const EvictParams &P, uint32_t h, uint32_t piece) : page_size(P.cache.page_size) {
+        const bool value = piece >= P.pieces;
+        base = const_cast<char *>(value ? P.cache.v + h * P.cache.v_head : P.cache.k + h * P.cache.k_head) + (value ? piece - P.pieces : piece) * 16;
+        page_step = value ? P.cache.v_page : P.cache.k_page, token_step = value ? P.cache.v_token : P.cache.k_token;
+        weights = piece == 0 ? P.weights + static_cast<int64_t>(h) * page_size.d : nullptr;
+        weight_step = P.heads_kv * page_size.d;
+    }
+    // U rows, source(u) to target(u), slots below 0 skipped; between loads and stores `between`
+    template <uint32_t U, class S, class D, class B>
+    __device__ __forceinline__ void move(S source, D target, B between) const {
+        int32_t from[U], to[U];
+        u32x4 x[U];
+        float w[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) from[u] = source(u), to[u] = target(u);
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t slot = max(from[u], 0), page = page_size.div(slot), at = slot - page * page_size.d;
+            x[u] = *reinterpret_cast<const u32x4 *>(base + page * page_step + at * token_step);
+            w[u] = weights ? weights[static_cast<int64_t>(page) * weight_step + at] : 0.0f;
+        }
+        between();
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            if (from[u] < 0 || to[u] < 0) continue;
+            const uint32_t page = page_size.div(to[u]), at = to[u] - page * page_size.d;
+            *reinterpret_cast<u32x4 *>(base + page * page_step + at * token_step) = x[u];
+            if (weights) weights[static_cast<int64_t>(page) * weight_step + at] = w[u];
+        }
+    }
+    // The last `window` of n tokens to places before `budget`, in steps of U * rows of them, this
+    // thread's the row-th of each `rows`.  They may go to places that others of them leave, but never to
+    // one that a later step reads, so a step loads all of its rows before it writes any.
+    template <uint32_t U>
+    __device__ __forceinline__ void shift(const EvictParams &P, uint32_t r, uint32_t n, uint32_t row, uint32_t rows, bool works) const {
+        for (uint32_t i0 = 0; i0 < P.window; i0 += rows * U)
+            move<U>([&](uint32_t u) { const uint32_t i = i0 + u * rows + row; return works && i < P.window ? slot_of(P, r, n - P.window + i) : -1; },
+                    [&](uint32_t u) { const uint32_t i = i0 + u * rows + row; return works && i < P.window ? slot_of(P, r, P.budget - P.window + i) : -1; },
+                    [] {
+                        wait_loads();
+                        __syncthreads();
+                    });
+    }
+};
+
 // The weights of U tokens j, j + step .. as keys, 0 from token `end` (1 or more) on: their pages
 // first, then the weights.
 template <uint32_t U, class F>
@@ -275,6 +328,7 @@ template <uint32_t K>
 __global__ __launch_bounds__(kChooseThreads, K == 8 ? 8 : 4) void fg_evict_choose_kernel(EvictParams P) {
     extern __shared__ uint32_t dynamic[];
     __shared__ Picking<kChooseWaves> S;
+    __shared__ int32_t few_to[K == 8 ? kFewMoves : 1], few_from[K == 8 ? kFewMoves : 1];
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = uniform(tid / 64);
     if (blockIdx.x >= P.choosers) {
         list_freed(P, blockIdx.x - P.choosers, gridDim.x - P.choosers, dynamic, S.valid);
@@ -313,7 +367,8 @@ __global__ __launch_bounds__(kChooseThreads, K == 8 ? 8 : 4) void fg_evict_choos
             const uint32_t holes = of_lane(static_cast<int32_t>(gones), kChooseWaves - 1);
             uint32_t equal = of_lane(static_cast<int32_t>(seen), wave), at_hole = of_lane(static_cast<int32_t>(gones - gone), wave),
                      at_late = of_lane(static_cast<int32_t>(lates - late), wave);
-            int32_t *const to = P.to + static_cast<uint64_t>(rh) * P.most, *const from = P.from + static_cast<uint64_t>(rh) * P.most;
+            const bool here = K == 8 && P.at_once;
+            int32_t *const to = here ? few_to : P.to + static_cast<uint64_t>(rh) * P.most, *const from = here ? few_from : P.from + static_cast<uint64_t>(rh) * P.most;
             run.each([&](uint32_t x, uint32_t i) {
                 const bool in = i < stop, take = taken(B, x, equal), hole = in && i < low && !take, rises = in && i >= low && take;
                 const uint64_t hs = __ballot(hole), rs = __ballot(rises), before = (1ull << lane) - 1;
@@ -321,7 +376,18 @@ __global__ __launch_bounds__(kChooseThreads, K == 8 ? 8 : 4) void fg_evict_choos
                 if (rises) from[at_late + __popcll(rs & before)] = static_cast<int32_t>(P.sinks + i);
                 at_hole += __popcll(hs), at_late += __popcll(rs);
             });
-            if (tid == 0) P.counts[rh] = holes;
+            if (here) {
+                const uint32_t pieces = 2 * P.pieces, rows = kChooseThreads / pieces, row = tid / pieces;
+                const Mover mover(P, h, tid - row * pieces);
+                __syncthreads();
+                for (uint32_t i0 = 0; i0 < holes; i0 += rows)
+                    mover.move<1>([&](uint32_t u) { const uint32_t i = i0 + u * rows + row; return row < rows && i < holes ? slot_of(P, r, few_from[i]) : -1; },
+                                  [&](uint32_t u) { const uint32_t i = i0 + u * rows + row; return row < rows && i < holes ? slot_of(P, r, few_to[i]) : -1; }, [] {});
+                __syncthreads();
+                mover.shift<1>(P, r, n, row, rows, row < rows);
+            } else if (tid == 0) {
+                P.counts[rh] = holes;
+            }
         };
         if constexpr (K > 0) {
             Held<K> run;
@@ -344,56 +410,28 @@ __global__ __launch_bounds__(kChooseThreads, K == 8 ? 8 : 4) void fg_evict_choos
     }
 }
 
-// A workgroup moves 64 bytes of every row of a request and head: the chosen ones, from above
-// into the holes below, which no other move touches; then the last `window` in order.  Those may
-// go to places that others of them leave, but never to one that a later step reads, so a step
-// loads all of its rows before it writes any.
-__global__ __launch_bounds__(kMoveThreads) void fg_evict_move_kernel(EvictParams P, uint32_t pieces) {
-    constexpr uint32_t ROWS = kMoveThreads / kMovePieces, U = 4;
-    const uint32_t tid = threadIdx.x, slice = blockIdx.x, h = blockIdx.y, r = blockIdx.z, rh = r * P.heads_kv + h;
-    const uint32_t n = length_of(P, r);
-    if (n <= P.budget) return;
-    const uint32_t piece = slice * kMovePieces + tid % kMovePieces, row = tid / kMovePieces;  // pieces of keys, then of values
-    const bool value = piece >= pieces, works = piece < 2 * pieces, weighs = piece == 0;
-    char *const base = const_cast<char *>(value ? P.cache.v + h * P.cache.v_head : P.cache.k + h * P.cache.k_head) + (value ? piece - pieces : piece) * 16;
-    const int64_t page_step = value ? P.cache.v_page : P.cache.k_page, token_step = value ? P.cache.v_token : P.cache.k_token;
-    const auto place = [&](int32_t slot) {
-        const uint32_t page = P.cache.page_size.div(slot);
-        return base + page * page_step + (slot - page * P.cache.page_size.d) * token_step;
-    };
-    const auto move = [&](uint32_t count, auto source, auto target) {
-        for (uint32_t i0 = 0; i0 < count; i0 += ROWS * U) {
-            int32_t from[U], to[U];
-            u32x4 x[U];
-            float w[U];
-#pragma unroll
-            for (uint32_t u = 0; u < U; ++u) {
-                const uint32_t i = i0 + u * ROWS + row;
-                const bool in = works && i < count;
-                from[u] = in ? source(i) : -1;
-                to[u] = in ? target(i) : -1;
-                if (from[u] < 0) to[u] = -1;
-            }
-#pragma unroll
-            for (uint32_t u = 0; u < U; ++u) {
-                x[u] = u32x4{0, 0, 0, 0};
-                w[u] = 0.0f;
-                if (to[u] >= 0) x[u] = *reinterpret_cast<const u32x4 *>(place(from[u]));
-                if (to[u] >= 0 && weighs) w[u] = P.weights[weight_at(P, h, from[u])];
-            }
-            wait_loads();
-            __syncthreads();
-#pragma unroll
-            for (uint32_t u = 0; u < U; ++u) {
-                if (to[u] >= 0) *reinterpret_cast<u32x4 *>(place(to[u])) = x[u];
-                if (to[u] >= 0 && weighs) P.weights[weight_at(P, h, to[u])] = w[u];
-            }
-        }
-    };
+// The chosen tokens into the holes below; no other move touches a place of theirs, so any
+// workgroup takes any of them.
+__global__ __launch_bounds__(kMoveThreads) void fg_evict_fill_kernel(EvictParams P) {
+    const uint32_t h = blockIdx.y, r = blockIdx.z, rh = r * P.heads_kv + h, tid = threadIdx.x;
+    if (length_of(P, r) <= P.budget) return;
+    const uint32_t count = P.counts[rh], pieces = 2 * P.pieces, rows = kMoveThreads / pieces, row = tid / pieces;
+    const Mover mover(P, h, tid - row * pieces);
     const int32_t *const from = P.from + static_cast<uint64_t>(rh) * P.most, *const to = P.to + static_cast<uint64_t>(rh) * P.most;
-    move(P.counts[rh], [&](uint32_t i) { return slot_of(P, r, from[i]); }, [&](uint32_t i) { return slot_of(P, r, to[i]); });
-    __syncthreads();
-    move(P.window, [&](uint32_t i) { return slot_of(P, r, n - P.window + i); }, [&](uint32_t i) { return slot_of(P, r, P.budget - P.window + i); });
+    for (uint32_t i0 = blockIdx.x * kMoveRows; i0 < count; i0 += gridDim.x * kMoveRows) {
+        const uint32_t end = min(i0 + kMoveRows, count);
+        for (uint32_t i1 = i0; i1 < end; i1 += rows * 4)
+            mover.move<4>([&](uint32_t u) { const uint32_t i = i1 + u * rows + row; return row < rows && i < end ? slot_of(P, r, from[i]) : -1; },
+                          [&](uint32_t u) { const uint32_t i = i1 + u * rows + row; return row < rows && i < end ? slot_of(P, r, to[i]) : -1; }, [] {});
+    }
+}
+
+// The last tokens behind them, once all have left their places: a workgroup 64 bytes of every row.
+__global__ __launch_bounds__(kMoveThreads) void fg_evict_shift_kernel(EvictParams P) {
+    const uint32_t h = blockIdx.y, r = blockIdx.z, n = length_of(P, r), piece = blockIdx.x * kShiftPieces + threadIdx.x % kShiftPieces;
+    if (n <= P.budget) return;
+    const bool works = piece < 2 * P.pieces;
+    Mover(P, h, works ? piece : 0).shift<4>(P, r, n, threadIdx.x / kShiftPieces, kMoveThreads / kShiftPieces, works);
 }
 
 // ---------------------------------------------------------------- host side
@@ -530,11 +568,17 @@ int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_
         hipStream_t st = reinterpret_cast<hipStream_t>(stream);
         const uint64_t entries = static_cast<uint64_t>(requests) * table_width;
         const uint32_t listers = static_cast<uint32_t>(std::min<uint64_t>(64, 1 + entries / (4 * kChooseThreads)));
+        P.pieces = cache->dim / 8;
+        // Few can move: in the kernel that chooses.
+        P.at_once = P.room <= kFewKeys && P.room <= budget + kFewMoves && window <= kFewMoves;
         const auto choose = P.room <= kFewKeys ? fg_evict_choose_kernel<8> : plan.held ? fg_evict_choose_kernel<32> : fg_evict_choose_kernel<0>;
         hipLaunchKernelGGL(choose, dim3(P.choosers + listers), dim3(kChooseThreads), requests * 4, st, P);
-        const uint32_t pieces = cache->dim / 8, slices = (2 * pieces + kMovePieces - 1) / kMovePieces;
-        if (P.room > budget)
-            hipLaunchKernelGGL(fg_evict_move_kernel, dim3(slices, cache->heads_kv, requests), dim3(kMoveThreads), 0, st, P, pieces);
+        if (P.room > budget && !P.at_once) {
+            const uint32_t moves = std::min(budget - window, P.room - budget);
+            const uint32_t wide = std::max<uint32_t>(1, std::min<uint64_t>((moves + kMoveRows - 1) / kMoveRows, 8192 / (static_cast<uint64_t>(requests) * cache->heads_kv)));
+            if (moves) hipLaunchKernelGGL(fg_evict_fill_kernel, dim3(wide, cache->heads_kv, requests), dim3(kMoveThreads), 0, st, P);
+            if (window) hipLaunchKernelGGL(fg_evict_shift_kernel, dim3((2 * P.pieces + kShiftPieces - 1) / kShiftPieces, cache->heads_kv, requests), dim3(kMoveThreads), 0, st, P);
+        }
         FG_HIP(hipGetLastError(), "eviction launch");
         return FG_OK;
     });
