@@ -757,10 +757,11 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     plan->lds = plan->chunk ? 0 : tokens * P.nids * 12;
     const uint64_t items = static_cast<uint64_t>(plan->tiles) * P.lanes;
     if (items > kMostItems) return fail(FG_EINVAL, "more than 2^23 tiles of rows: attend to fewer tokens a call");
-    const uint64_t blocks = std::min<uint64_t>(a->table_width, static_cast<uint64_t>(P.first) + P.last + P.nids);
+    const uint64_t at_a_time = std::min<uint64_t>(tokens, (a->tokens + a->requests - 1) / std::max(1u, a->requests));  // of a tile, in the mean
+    const uint64_t blocks = std::min<uint64_t>(a->table_width, static_cast<uint64_t>(P.first) + P.last + at_a_time * P.nids);
     const uint64_t most = blocks * c->page_size;
     P.parts = 1;
-    while (!plan->chunk && P.parts < kMostParts && items * P.parts < 512 && most > 2 * P.parts * kSplitTokens) P.parts *= 2;
+    while (!plan->chunk && P.parts < kMostParts && items * P.parts < 256 && most > 2 * P.parts * kSplitTokens) P.parts *= 2;
     const uint64_t slots = items * P.parts * kTileRows;
     plan->ml = slots * c->dim * 4;
     plan->workspace = P.parts > 1 ? slots * (c->dim * 4 + 8) : 0;

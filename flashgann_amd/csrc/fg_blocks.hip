@@ -79,15 +79,20 @@ __global__ __launch_bounds__(kBoundsThreads) void fg_cache_bounds_kernel(BoundsP
         for (int c = 0; c < 8; ++c) hi[c] = -INFINITY, lo[c] = INFINITY;
         bool special = false;
         if (works) {
-#pragma unroll 4
-            for (uint32_t row = sub; row < P.page_size.d; row += ROWS) {
-                const u32x4 w = *reinterpret_cast<const u32x4 *>(src + row * P.k_token);
-                special |= any_special<T>(w);
+            // (a row past the last is the last once more)
+            for (uint32_t row0 = 0; row0 < P.page_size.d; row0 += 8 * ROWS) {
+                u32x4 w[8];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float a = as_float<T>(w[c] & 0xFFFF), b = as_float<T>(w[c] >> 16);
-                    hi[2 * c] = fmaxf(hi[2 * c], a), lo[2 * c] = fminf(lo[2 * c], a);
-                    hi[2 * c + 1] = fmaxf(hi[2 * c + 1], b), lo[2 * c + 1] = fminf(lo[2 * c + 1], b);
+                for (uint32_t u = 0; u < 8; ++u) w[u] = *reinterpret_cast<const u32x4 *>(src + min(row0 + u * ROWS + sub, P.page_size.d - 1) * P.k_token);
+#pragma unroll
+                for (uint32_t u = 0; u < 8; ++u) {
+                    special |= any_special<T>(w[u]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float a = as_float<T>(w[u][c] & 0xFFFF), b = as_float<T>(w[u][c] >> 16);
+                        hi[2 * c] = fmaxf(hi[2 * c], a), lo[2 * c] = fminf(lo[2 * c], a);
+                        hi[2 * c + 1] = fmaxf(hi[2 * c + 1], b), lo[2 * c + 1] = fminf(lo[2 * c + 1], b);
+                    }
                 }
             }
         }
@@ -304,8 +309,8 @@ enum { kFused, kScratch, kScore, kPick };  // keys in LDS; in a scratch of the w
 // 16 blocks through the matrix unit, rows against blocks.  Workgroups of neighbouring numbers
 // take a tile's lists, so that an XCD, to which every eighth goes, sees few heads' bounds.
 template <class T, int D, int MODE, bool TEAM>
-__global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_select_kernel(SelectParams P) {
-    constexpr int STEPS = 2 * D / 64, U = D <= 128 ? 2 : 1;  // groups of blocks under way at a time
+__global__ __launch_bounds__(kSelectThreads, D > 128 || TEAM ? 2 : 4) void fg_select_kernel(SelectParams P) {
+    constexpr int STEPS = 2 * D / 64, U = D > 128 ? (TEAM ? 2 : 1) : TEAM ? 4 : 2;  // groups of blocks under way at a time
     constexpr uint32_t QROW = 2 * D + 16;  // bytes of a row's codes in LDS
     constexpr uint32_t WAVES = TEAM ? kSelectWaves : 1;
     extern __shared__ uint32_t held[];
@@ -349,7 +354,7 @@ __global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_s
 #pragma unroll
             for (int u = 0; u < U; ++u) page[u] = page_of(g + (U + u) * step);
             code_queries<T, D>(P, t, list, codes, QROW);
-            __syncthreads();
+            lds_barrier();  // (the bounds stay on their way)
             i32x4 qv[STEPS];
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) qv[s] = *reinterpret_cast<const i32x4 *>(codes + col * QROW + 64 * s + 16 * quarter);

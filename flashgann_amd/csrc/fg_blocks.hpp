@@ -10,6 +10,14 @@ constexpr uint32_t kMostBlocks = 4096;     // of a list: what attention over the
 constexpr uint32_t kMostTokens = 1u << 22; // of a call
 constexpr uint32_t kMostItems = 1u << 23;  // tiles and lists of a call, a grid's workgroups
 
+// The barrier that publishes LDS and nothing else: loads in flight from global memory stay
+// in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // Rows of q in tiles: those of request r are tiles q_starts[r] / rows + r and on, which leaves
 // room for the ragged last one of each, so a call has tokens / rows + requests at most.  A tile
 // of one row is that row.

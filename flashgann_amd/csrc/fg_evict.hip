@@ -32,14 +32,6 @@ struct WeighParams {
 // Each of the four waves holds the keys of 64 tokens in registers and goes through the rows,
 // which all share from LDS, 16 at a time on the matrix unit: a lane's column is a token, so
 // its sum stays in one register till the end.
-// The barrier that publishes LDS and nothing else: loads in flight from global memory stay
-// in flight.
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 template <class T, int D>
 __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void fg_weigh_kernel(WeighParams P) {
     using vec = typename T::vec;
