@@ -309,8 +309,8 @@ enum { kFused, kScratch, kScore, kPick };  // keys in LDS; in a scratch of the w
 // 16 blocks through the matrix unit, rows against blocks.  Workgroups of neighbouring numbers
 // take a tile's lists, so that an XCD, to which every eighth goes, sees few heads' bounds.
 template <class T, int D, int MODE, bool TEAM>
-__global__ __launch_bounds__(kSelectThreads, D > 128 || TEAM ? 2 : 4) void fg_select_kernel(SelectParams P) {
-    constexpr int STEPS = 2 * D / 64, U = D > 128 ? (TEAM ? 2 : 1) : TEAM ? 4 : 2;  // groups of blocks under way at a time
+__global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_select_kernel(SelectParams P) {
+    constexpr int STEPS = 2 * D / 64, U = D <= 128 ? 2 : 1;  // groups of blocks under way at a time
     constexpr uint32_t QROW = 2 * D + 16;  // bytes of a row's codes in LDS
     constexpr uint32_t WAVES = TEAM ? kSelectWaves : 1;
     extern __shared__ uint32_t held[];
