@@ -743,11 +743,18 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     P.group = a->heads / a->lists;
     P.scale2 = a->scale * 1.44269504088896341f;
 
-    // A tile: the rows of as many tokens as 16 (32) hold; the former's lists in LDS
-    // (at dim 256 the chunk kernel's rows do not fit the registers)
-    plan->chunk = c->dim <= 128 && a->tokens >= 8 * static_cast<uint64_t>(a->requests) && a->table_width <= 16 * kWindow;
+    // Tiles of 32 rows once they fill half the device, whole; before that those of 16 are split among
+    // workgroups.  24 of 250 pages of 32 (32 heads over 8, dim 128): 8 requests of 8 new tokens 45.8 us
+    // against 42.2, of 16 46.3 against 62.7, of 64 67 against 123; 32 requests of 2 46.5 against 51.6; one
+    // of 64 40.8 against 28.  Over many blocks windows cost more than lists in order: 256 tokens, 64 of
+    // 500 blocks 30 against 43, of 2,000 41 against 49, of 7,500 80 against 53.  (At dim 256 the chunk
+    // kernel's rows do not fit the registers.)
+    const auto tile_tokens = [&](uint32_t rows) { return rows / std::min(P.group, rows); };
+    const uint64_t chunk_tiles = std::max<uint64_t>(a->tokens / tile_tokens(kChunkRows), a->requests) * P.lists * ((P.group + kChunkRows - 1) / kChunkRows);
+    plan->chunk = c->dim <= 128 && a->tokens >= 2 * static_cast<uint64_t>(a->requests) && chunk_tiles >= 128 && a->table_width <= 4 * kWindow;
+    // A tile: the rows of as many tokens as it holds; for the former kernel with their lists in LDS.
     const uint32_t most_rows = plan->chunk ? kChunkRows : kTileRows, per = std::min(P.group, most_rows);
-    uint32_t tokens = most_rows / per;
+    uint32_t tokens = tile_tokens(most_rows);
     if (!plan->chunk && P.nids) tokens = std::min(tokens, std::max(1u, kMostBlocks / P.nids));
     P.per = fast_div(per);
     P.head_parts = (P.group + most_rows - 1) / most_rows;
@@ -760,6 +767,8 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     const uint64_t at_a_time = std::min<uint64_t>(tokens, (a->tokens + a->requests - 1) / std::max(1u, a->requests));  // of a tile, in the mean
     const uint64_t blocks = std::min<uint64_t>(a->table_width, static_cast<uint64_t>(P.first) + P.last + at_a_time * P.nids);
     const uint64_t most = blocks * c->page_size;
+    // Parts of a tile until every CU has one: 48 single tokens over 51 pages of 32, 480 tiles, 72.8 us
+    // whole, 76.9 in two parts; 4 drafts of 1 to 5, 32 tiles, 14.8 us in eight.
     P.parts = 1;
     while (!plan->chunk && P.parts < kMostParts && items * P.parts < 256 && most > 2 * P.parts * kSplitTokens) P.parts *= 2;
     const uint64_t slots = items * P.parts * kTileRows;

@@ -476,11 +476,15 @@ int prepare_select(const fg_kv_cache *c, const fg_attention *a, SelectParams *ou
     P.last = static_cast<uint32_t>(a->window);
     P.page_size = fast_div(c->page_size);
 
-    // Keys of a tile's rows are held in LDS: 16 rows where they fit, fewer over longer tables.
+    // Keys of a tile's rows are held in LDS: 16 rows where they fit, fewer over longer tables.  Up to two
+    // rows a CU, or where most tiles would hold one or two, a workgroup takes a row: 4 requests of 8
+    // new tokens over 1,000 blocks (8 lists) 17.4 us against 22.5, 32 of 1 22.0 against 32.8, of 2 27.3
+    // against 33.1, of 3 37.9 against 33.0.
     const uint32_t most = std::max(1u, a->table_width - std::min(a->table_width, P.first));
     P.stride = most | 1;  // (odd: the rows of a tile lie in different banks)
+    const bool one = a->tokens <= 2 * static_cast<uint64_t>(a->requests) || static_cast<uint64_t>(a->tokens) * a->lists <= 512;
     uint32_t rows = kSelectRows;
-    while (rows > 1 && (static_cast<uint64_t>(rows) * P.stride * 4 > kSelectLds || a->tokens <= 2 * static_cast<uint64_t>(a->requests))) rows /= 2;
+    while (rows > 1 && (static_cast<uint64_t>(rows) * P.stride * 4 > kSelectLds || one)) rows /= 2;
     P.rows = fast_div(rows);
     // (a row alone is a tile of its own number, and leaves none empty)
     P.tiles = a->tokens / rows + (rows > 1 ? a->requests : 0);
@@ -496,8 +500,11 @@ int prepare_select(const fg_kv_cache *c, const fg_attention *a, SelectParams *ou
         plan->grid = static_cast<uint32_t>(std::min<uint64_t>(items, 512));
         plan->workspace = static_cast<uint64_t>(plan->grid) * P.stride * 4;
     }
-    // Few rows over many blocks: several workgroups make a row's keys, and one picks from them.
-    if (rows == 1 && items < 128 && most >= 2048) {
+    // Few rows over many blocks: several workgroups make a row's keys, and one picks from them (8 rows over
+    // 500 blocks 11.7 us against 12.2, over 1,500 12.5 against 21.9, over 8,125 17.6 against 81; 96 over
+    // 500 14.8 against 13.2, over 1,500 20.4 against 24.5; 128 over 3,750 38.5 against 51.7; 256 over 1,500
+    // 31.8 against 30.3).
+    if (rows == 1 && items <= 160 && most >= 1024) {
         plan->mode = kScore;
         plan->grid = static_cast<uint32_t>(items);
         P.parts = std::min<uint32_t>((most + 16 * kSelectWaves - 1) / (16 * kSelectWaves), static_cast<uint32_t>(std::max<uint64_t>(1, 512 / items)));

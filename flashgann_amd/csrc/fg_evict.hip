@@ -447,6 +447,7 @@ int weigh(const fg_kv_cache *c, const fg_attention *a, float *weights, const int
     if (static_cast<uint64_t>(a->tokens) * a->heads > 0x7FFFFFFFull) return fail(FG_EINVAL, "tokens * heads must be below 2^31");
     if (a->table_width > 0x7FFFFFFFu || a->table_row < 0) return fail(FG_EINVAL, "table_width or table_row out of range");
     if (static_cast<uint64_t>(a->table_width) * c->page_size > 0x3FFFFFFFull) return fail(FG_EINVAL, "table_width * page_size must be below 2^30");
+    if (a->tokens > kMostTokens) return fail(FG_EINVAL, "tokens must be at most 4,194,304");
     if (a->requests > 65536) return fail(FG_EINVAL, "requests must be at most 65,536");
     if (a->requests == 0) return FG_OK;
     if (!a->kv_lens || !a->q_starts || !known || !weights || (a->tokens && (!a->q || !a->lse)) || (a->table_width && !a->table))
@@ -501,7 +502,7 @@ int plan_evict(const fg_kv_cache *c, uint32_t table_width, uint32_t requests, ui
     P.most = std::min(budget, P.room);
     const uint64_t pairs = static_cast<uint64_t>(requests) * c->heads_kv, slots = pairs * P.most;
     plan->held = P.room <= kChooseKeys;
-    P.choosers = static_cast<uint32_t>(plan->held ? pairs : std::min<uint64_t>(pairs, kChooseWorkgroups));
+    P.choosers = static_cast<uint32_t>(std::min<uint64_t>(pairs, plan->held ? 65536 : kChooseWorkgroups));
     plan->from = slots * 4;
     plan->counts = slots * 8;
     plan->keys = plan->counts + (pairs * 4 + 15) / 16 * 16;
@@ -561,7 +562,8 @@ int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_
         const uint64_t entries = static_cast<uint64_t>(requests) * table_width;
         const uint32_t listers = static_cast<uint32_t>(std::min<uint64_t>(64, 1 + entries / (4 * kChooseThreads)));
         P.pieces = cache->dim / 8;
-        // Few can move: in the kernel that chooses.
+        // Few can move: in the kernel that chooses (48 requests of 8 heads back to 4,096 tokens, 1 over, a window of 16
+        // 21 us against 31; 500 over 65 against 80, with a window of 400 104 against 128).
         P.at_once = P.room <= kFewKeys && P.room <= budget + kFewMoves && window <= kFewMoves;
         const auto choose = P.room <= kFewKeys ? fg_evict_choose_kernel<8> : plan.held ? fg_evict_choose_kernel<32> : fg_evict_choose_kernel<0>;
         hipLaunchKernelGGL(choose, dim3(P.choosers + listers), dim3(kChooseThreads), requests * 4, st, P);

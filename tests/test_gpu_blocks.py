@@ -234,6 +234,38 @@ def test_select_long(new, kv, heads, heads_kv, lists, page, k):
     assert torch.equal(ids, want)
 
 
+@pytest.mark.parametrize("new,kv,page,k", ((300, 4000, 4, 16), (300, 4000, 4, 32), (300, 4000, 4, 33), (300, 12000, 4, 20), (300, 30000, 4, 20), (300, 60000, 4, 300),
+                                           (300, 70000, 2, 9)))
+def test_select_tiles_of_rows(new, kv, page, k):
+    """Many rows at once: 16 of a tile in LDS, 8, 4 and 2 over longer tables, and more blocks than it holds, where
+    a workgroup takes several rows one after another; few and many to pick."""
+    from flashgann_amd import attention
+    q, kc, _, table, starts = case(17, [new], [kv], 4, 2, 64, page, BF)
+    bounds, scales = torch.zeros((kc.shape[0], 2, 2, 64), dtype=torch.int8, device="cuda"), torch.zeros((kc.shape[0], 2), device="cuda")
+    attention.cache_bounds(kc.cuda(), torch.arange(kc.shape[0] * page, device="cuda"), bounds, scales)
+    ids = attention.select_blocks(q.cuda(), bounds, scales, table.cuda(), ints(starts), ints([kv]), page_size=page, k=k)
+    assert torch.equal(ids, plain_select(q, bounds, scales, table, starts, [kv], page, k, 2, 1, 1))
+
+
+def test_select_ties_in_tiles_of_rows():
+    """Equal scores go to the lower block however rows are picked from: all equal, a few values, infinite ones."""
+    def same(n):
+        def change(kc, table):
+            for p in range(kc.shape[0]):
+                kc[p] = kc[p % n]
+        return change
+    for n, k in ((1, 7), (3, 7), (3, 32), (40, 20), (3, 60)):
+        compare_select([300], [700], 4, 2, 64, 4, BF, k, 2, 1, 1, n, same(n))
+    compare_select([300], [700], 4, 2, 64, 4, BF, 9, 2, 1, 1, 8, None, None, lambda q: q.zero_())
+
+    def odd(kc, table):
+        table[0, 3], table[0, 9] = -1, kc.shape[0]
+        for b, x in ((4, NAN), (7, INF), (20, -INF), (33, NAN)):
+            kc[int(table[0, b]), 1, 0, 5] = x
+    for k in (2, 3, 4, 9):
+        compare_select([300], [700], 4, 2, 64, 4, FP, k, 2, 1, 1, 3, odd)
+
+
 def _shared(new, kv, heads, heads_kv, page):
     """Requests whose tables name the same pages in different orders."""
     rng = np.random.default_rng(8)
@@ -397,3 +429,58 @@ def test_attend_strides_out_and_rows_outside():
     O.attend(q, kc, vc, table, starts, [90, 60], ids, 64 ** -0.5, 1, 1).check(od, lse)
     for rows in (slice(0, 5), slice(33, 40)):
         assert torch.all(od[rows] == 3) and torch.all(lse[rows] == 3)
+
+
+# ---------------------------------------------------------------- attend, tiles of 32 rows
+
+MANY = [1, 0, 3, 21, 40, 1, 2, 5, 1, 1, 9, 0, 33, 1, 1, 4]
+KV = [9, 77, 3, 90, 217, 60, 2, 130, 1, 40, 9, 5, 70, 300, 17, 111]
+
+
+@pytest.mark.parametrize("dtype,dim,heads,heads_kv,lists,page", ((BF, 128, 16, 8, 8, 16), (FP, 96, 24, 8, 8, 24), (BF, 64, 16, 2, 16, 5), (FP, 128, 32, 8, 8, 4), (BF, 96, 8, 8, 8, 1)))
+@pytest.mark.parametrize("first,last,k", ((0, 1, 3), (1, 2, 5), (0, 1, 0), (3, 40, 2), (50, 1, 4), (2, 3, 60)))
+def test_attend_many_requests(dtype, dim, heads, heads_kv, lists, page, first, last, k):
+    """Chunks, drafts and single tokens of many requests in one batch."""
+    compare_attend(MANY, KV, heads, heads_kv, dim, page, dtype, lists, k, first, last, "hnd" if page == 24 else "nhd", page)
+
+
+def test_attend_many_heads_of_a_list():
+    """More query heads of a list than a tile has rows."""
+    compare_attend(MANY * 2, KV * 2, 80, 2, 64, 8, BF, 2, 4, 1, 2)
+
+
+@pytest.mark.parametrize("page,kv,k,first,last", ((1, 2500, 20, 3, 2), (1, 700, 300, 0, 600), (2, 4000, 5, 900, 1), (8, 9000, 3, 0, 1), (200, 5000, 2, 1, 1), (64, 3000, 4, 0, 2)))
+def test_attend_many_windows_of_blocks(page, kv, k, first, last):
+    """Blocks far apart, next to each other over several windows, larger than a tile."""
+    compare_attend([5] + [2] * 7 + [9], [kv - 11 * r for r in range(9)], 16, 16, 64, page, BF, 16, k, first, last, seed=page)
+
+
+@pytest.mark.parametrize("dtype", (BF, FP))
+def test_attend_many_odd_lists_and_values(dtype):
+    """Ids out of order, pages missing, infinities and NaN where only some rows see them."""
+    def mess(q, kc, vc, table, ids):
+        rng = np.random.default_rng(5)
+        ids.copy_(torch.from_numpy(rng.choice(np.array([-5, -1, 0, 1, 2, 3, 3, 5, 8, 9, 12, 30, 90, (1 << 31) - 1], np.int32), ids.shape)))
+        ids[3:30] = ids[3:30].sort(-1).values
+    compare_attend(MANY, KV, 16, 8, 64, 8, dtype, 8, 7, 1, 2, seed=1, change=mess)
+
+    def gone(q, kc, vc, table, ids):
+        table[0, 1], table[4, 5], table[3, :], table[12, 3] = -1, kc.shape[0], -7, 1 << 30
+    compare_attend(MANY, KV, 16, 8, 128, 8, dtype, 8, 8, 1, 2, change=gone, width=30)
+
+    for what in (NAN, INF, -INF):
+        def odd(q, kc, vc, table, ids):
+            used = set(table.flatten().tolist())
+            for p in range(kc.shape[0]):
+                if p not in used:
+                    kc[p], vc[p] = what, what
+            for r in (3, 4, 7, 12):
+                n = KV[r]
+                if n % 8:
+                    kc[int(table[r, n // 8]), n % 8:] = what
+                    vc[int(table[r, n // 8]), n % 8:] = what
+                vc[int(table[r, (n - 1) // 8]), (n - 1) % 8, 1, 7] = what
+                vc[int(table[r, 3]), 5, 0, 33], kc[int(table[r, 2]), 3, 1, 9] = what, what
+            ids[:, :, :] = -1
+            ids[0::3, :, 0], ids[1::3, :, 0] = 3, 2
+        compare_attend(MANY, KV, 16, 8, 64, 8, dtype, 8, 3, 1, 1, change=odd)

@@ -125,7 +125,7 @@ def calls(args, bounds, scales, page):
     return ids, out, lse, w, *e, kc, vc
 
 
-@pytest.mark.parametrize("new,kv", (([1, 1], [900, 400]), ([70, 50], [500, 400])))
+@pytest.mark.parametrize("new,kv", (([1, 1], [900, 400]), ([70, 50], [500, 400]), ([2] * 64, [100] * 64), ([400], [900])))
 def test_on_another_stream(new, kv):
     from flashgann_amd import attention
     q, kc, vc, table, starts = case(10, new, kv, 8, 2, 128, 16, BF)
@@ -146,7 +146,7 @@ def test_on_another_stream(new, kv):
         assert all(torch.equal(a, b) for a, b in zip(g, want))
 
 
-@pytest.mark.parametrize("new,kv,page", (([1, 1], [900, 400], 16), ([70, 50], [500, 400], 16), ([1], [9000], 4), ([1, 1], [20000, 300], 8)))
+@pytest.mark.parametrize("new,kv,page", (([1, 1], [900, 400], 16), ([70, 50], [500, 400], 16), ([1], [9000], 4), ([1, 1], [20000, 300], 8), ([2] * 64, [100] * 64, 16), ([400], [900], 8)))
 def test_graph_replays(new, kv, page):
     """Captured calls follow what is in device memory: replayed over other queries and lengths, with eager work and
     allocations between, against the same calls made eagerly; two graphs in turn."""
