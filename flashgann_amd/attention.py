@@ -165,7 +165,8 @@ def cache_weigh(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     lse: what `attend` returned for them, without a window.  weights: (pages, heads_kv,
     page_size) float32, contiguous, written in place.  known: (requests,) int32, the tokens
     that have a weight already (the length before this step, say): those from there on are
-    set instead of added to.  Pages shared by requests of the call add up."""
+    set instead of added to.  Tokens that requests of the call share get all their sums if
+    each knows them; one that has to be set may belong to one request only."""
     _attention.cache_weigh(q, k_cache, block_table, q_starts, kv_lens, lse, weights, known, scale)
 
 
@@ -188,5 +189,6 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     `attend` without a window from then on; keys hold their own positions.  Returns the
     new lengths, the pages that are free now (the first `released` entries of `freed`, -1
     behind them) and their number; block_table keeps its entries, which `cache_plan` writes
-    over as the request grows.  Pages may not be shared.  1 to 4,096 requests a call."""
+    over as the request grows.  Pages may not be shared, k_cache and v_cache not be the same
+    memory.  1 to 4,096 requests a call."""
     return CacheEviction(*_attention.cache_evict(k_cache, v_cache, weights, block_table, kv_lens, budget, window, sinks))

@@ -544,6 +544,9 @@ int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_
         if (!d_weights || !d_kv_lens || !d_new_lens || !d_released || (table_width && (!d_table || !d_freed))) return fail(FG_EINVAL, "NULL device buffer");
         if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < plan.workspace)
             return fail(FG_EINVAL, "workspace must be 16-byte aligned and hold " + std::to_string(plan.workspace) + " bytes");
+        // rows of one memory would be moved twice, and lengths written while others read them
+        if (cache->k == cache->v) return fail(FG_EINVAL, "k and v must not be the same memory");
+        if (d_new_lens < d_kv_lens + requests && d_kv_lens < d_new_lens + requests) return fail(FG_EINVAL, "new lengths must not overlap kv_lens");
         char *base = static_cast<char *>(workspace);
         P.weights = d_weights;
         P.table = d_table;

@@ -411,7 +411,8 @@ int64_t fg_select_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_atte
  * and those of lists: a->ids is (tokens, lists, nids) int32, a list for each row and `lists`,
  * as fg_select_blocks writes them.  An id that is not above all before it in its list, or
  * lies outside [sinks, c - window], adds nothing.  nids at most 4,096, 0 allowed; tokens
- * at most 4,194,304. */
+ * at most 4,194,304, and at most 2^23 tiles of rows: (tokens + requests) * lists *
+ * ceil(heads / lists / 16) up to that always serves. */
 int fg_attend_blocks(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes,
                      void *stream);
 int64_t fg_attend_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
@@ -426,9 +427,10 @@ int64_t fg_attend_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_atte
  * with q's rows placed as for fg_attend and a->lse, read here, what fg_attend gave for them.
  * Tokens j >= d_known[r] have no weight yet: theirs is set, the others' is added to.  A row
  * whose lse is -infinity adds nothing; a token without a page gets no weight.  Of rows that
- * are not all given (the last ones of a prompt, say) the sum is over those.  Pages that
- * several requests of a call share add up (in no fixed order).  a: q, lse, table, q_starts,
- * kv_lens, scale; cache->v is not read. */
+ * are not all given (the last ones of a prompt, say) the sum is over those.  A token below
+ * d_known of every request that shares its page gets all their sums (in no fixed order); one that
+ * has to be set may belong to one request only.  a: q, lse, table, q_starts, kv_lens, scale;
+ * cache->v is not read.  tokens at most 4,194,304. */
 int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_weights, const int32_t *d_known,
                    void *stream);
 
@@ -444,8 +446,8 @@ int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_wei
  *   d_freed    requests * table_width  the table's entries past that, requests in order; -1 behind them
  *   d_released 1                       how many those are
  * The table itself stays: fg_cache_plan writes a new page over an entry when the request
- * grows again.  No page may belong to two requests of the call.  Bounds of pages whose keys
- * moved are void.  1 <= requests <= 4096, sinks + window <= budget, 1 <= budget. */
+ * grows again.  No page may belong to two requests of the call, k and v not be the same memory,
+ * d_new_lens not overlap d_kv_lens.  Bounds of pages whose keys moved are void.  1 <= requests <= 4096, sinks + window <= budget, 1 <= budget. */
 int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_table, int64_t table_row, uint32_t table_width,
                    const int32_t *d_kv_lens, uint32_t requests, uint32_t budget, uint32_t window, uint32_t sinks,
                    int32_t *d_new_lens, int32_t *d_freed, int32_t *d_released, void *workspace, uint64_t workspace_bytes,

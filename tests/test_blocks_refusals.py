@@ -129,6 +129,15 @@ def test_evict():
         refused(evict(**bad), word)
     for i in range(3):
         refused(evict(outs=tuple(None if j == i else AT for j in range(3))), "NULL")
+    # keys and values in one memory, lengths written over those that are read
+    refused(evict(cache_bytes(k=AT, v=AT)), "same memory")
+    apart = cache_bytes(k=AT, v=AT + 64)
+    for lens in (AT, AT + 8, AT - 8):
+        refused(evict(apart, lens=lens), "overlap")
+
+
+def test_more_tiles_of_rows_than_a_grid_holds():
+    refused(attend(cache_bytes(), blocks_bytes(tokens=1 << 22, heads=256, lists=256)), "2^23 tiles")
 
 
 def test_tensors_of_the_host_are_refused():
