@@ -62,6 +62,9 @@ __device__ __forceinline__ bool on_list(const int32_t *list, uint32_t n, int32_t
     return lo < n && list[lo] == b;
 }
 
+// Bound by the bytes of the union: 48 single tokens over 48 selected pages of 32 and the first and last
+// (32 heads over 8, dim 128) 66 us, 4.9 TB/s; of few tokens by latency, lists, union, table and keys one
+// after another: 5 requests of 1 to 5 tokens 11.4 us, and 4 to join their parts.
 template <class T, int D>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_kernel(BlocksParams P) {
     using vec = typename T::vec;
@@ -395,6 +398,12 @@ __global__ __launch_bounds__(256) void fg_blocks_join_kernel(BlocksParams P) {
 // nothing is waited for but its own loads.  A lane loads the keys of the token whose place it has
 // worked out.  The union of the lists is made a window of blocks at a time, a word of
 // tokens for each block, so its blocks come in order and none twice.
+//
+// A chunk of 2,048 tokens after 62,000 (32 heads over 8, dim 128, 16 pages of 64 each) 354 us; its
+// tiles of eight tokens read 59 blocks each of the 160 listed, 4 GB in all, of which the L2 has 69%.
+// Waves wait for loads 48% of their time, vector issue is 38% of it, the matrix unit 15%.  In tiles
+// of 16 rows 720 us; rows of several waves over tiles shared in LDS 546 us (a barrier a tile, and
+// each wave masks what only the others asked for).
 constexpr uint32_t kChunkRows = 32;
 constexpr uint32_t kWindow = 1024;  // blocks whose tokens are known at a time
 

@@ -52,7 +52,9 @@ struct BoundsParams {
 };
 
 // A workgroup looks through 256 slots for those that end a page; each wave then takes a page
-// of its head at a time, D / 8 lanes a row.  Bound by the keys' bytes, or by a launch.
+// of its head at a time, D / 8 lanes a row.  Eight loads a lane are under way.  Bound by the keys'
+// bytes: 30,000 tokens (8 heads, dim 128, pages of 64) 15.8 us, 3.9 TB/s;
+// of 64 single tokens by the latency of slots, then keys, 4.6 us.
 template <class T, int D>
 __global__ __launch_bounds__(kBoundsThreads) void fg_cache_bounds_kernel(BoundsParams P) {
     constexpr uint32_t LANES = D <= 64 ? 8 : D <= 128 ? 16 : 32, ROWS = 64 / LANES;  // (dim 96: 12 of 16 lanes work)
@@ -308,6 +310,12 @@ enum { kFused, kScratch, kScore, kPick };  // keys in LDS; in a scratch of the w
 // A workgroup takes a tile of rows of one list: queries coded once, then each wave groups of
 // 16 blocks through the matrix unit, rows against blocks.  Workgroups of neighbouring numbers
 // take a tile's lists, so that an XCD, to which every eighth goes, sees few heads' bounds.
+//
+// Bound by the latency of a short workgroup.  32 single tokens over 4,000 to 24,000 (8 lists, dim 128,
+// pages of 16) 25 us: the longest has 1,500 blocks, 13.5 us in the loop after 6.5 us of queries and
+// first loads, 3.2 us to pick; their bounds at memory's rate would take 11 us.  A chunk of 4,096 tokens over
+// 64,097 (pages of 64) 105 us: a workgroup 22 us, two a CU, in four rounds, its waves waiting for
+// half of it.  Two groups of blocks under way a wave: four slow the split form by half.
 template <class T, int D, int MODE, bool TEAM>
 __global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_select_kernel(SelectParams P) {
     constexpr int STEPS = 2 * D / 64, U = D <= 128 ? 2 : 1;  // groups of blocks under way at a time
