@@ -238,41 +238,30 @@ __device__ __forceinline__ void pick(const Run &run, uint32_t count, uint32_t fi
     for (uint32_t i = min(B.valid, count) + (WAVES > 1 ? threadIdx.x : lane); i < count; i += 64 * WAVES) ids[i] = -1;
 }
 
-// The lanes with the `count` largest of a wave's values, one each (0: none), bit by bit from
-// the highest in which they differ; among equal ones the lower lanes.  At least `count` lanes
-// have one, count >= 1.
-__device__ __forceinline__ uint64_t largest_lanes(uint32_t x, uint32_t count) {
-    uint64_t sure = 0, maybe = __ballot(x != 0);
-    if (static_cast<uint32_t>(__popcll(maybe)) == count) return maybe;
-    const uint32_t differ = wave_max(x) ^ wave_min(x ? x : 0xFFFFFFFFu);
-    for (uint32_t bit = differ ? 31 - __clz(differ) : 0u, mask = 1u << bit; mask; mask >>= 1) {
-        const uint64_t ones = __ballot((x & mask) != 0) & maybe;
-        const uint32_t n = __popcll(ones);
-        if (n >= count) {
-            maybe = ones;
-            if (n == count) return sure | maybe;
-        } else if (n) {
-            sure |= ones;
-            maybe &= ~ones;
-            count -= n;
-        }
-    }
-    while (static_cast<uint32_t>(__popcll(maybe)) > count) maybe &= ~(1ull << (63 - __clzll(maybe)));
-    return sure | maybe;
-}
-
-// pick() for few of 1 to 64 K keys, by a wave: the count-th largest of what each lane has at
-// most is a bound that at least `count` keys reach and few more, and those are sorted out one a
-// lane (16 of 1,000: 18 in the mean).  False, with nothing done, where that does not serve.
+// pick() for few of 1 to 64 K keys, by a wave.  Bits of what each lane has at most give a bound that
+// `count` lanes reach and a quarter more at most (none more past 20), or one that cannot be raised; the
+// keys that reach it are few (16 of 1,000: 21 in the mean) and each is ranked, one a lane, by those
+// above it.  False, with nothing done, where that does not serve.
 template <uint32_t K>
 __device__ __forceinline__ bool pick_few(const uint32_t *keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, u32x2 *some) {
     const uint32_t lane = threadIdx.x % 64;
     const Held<K> run = held_run<1, K>(keys, n);
-    uint32_t most = 0;
-    run.each([&](uint32_t x, uint32_t) { most = max(most, x); });
-    if (static_cast<uint32_t>(__popcll(__ballot(most != 0))) < count) return false;
-    const uint64_t lanes = largest_lanes(most, count);
-    const uint32_t bound = wave_min(lanes >> lane & 1 ? most : 0xFFFFFFFFu);
+    uint32_t top = 0;
+    run.each([&](uint32_t x, uint32_t) { top = max(top, x); });
+    if (static_cast<uint32_t>(__popcll(__ballot(top != 0))) < count) return false;
+    const uint32_t most = wave_max(top), least = wave_min(top ? top : 0xFFFFFFFFu);
+    uint32_t bound = least;
+    if (most != least) {
+        uint32_t mask = 0x80000000u >> __clz(most ^ least);
+        bound = most & ~(2 * mask - 1);
+        for (; mask; mask >>= 1) {
+            const uint32_t reach = __popcll(__ballot(top >= (bound | mask)));
+            if (reach < count) continue;
+            bound |= mask;
+            if (reach <= max(count, min(count + count / 4, 20u))) break;
+        }
+        bound = max(bound, least);
+    }
     uint32_t have = 0;
     run.each([&](uint32_t x, uint32_t i) {
         const uint64_t reach = __ballot(x >= bound);
@@ -283,7 +272,21 @@ __device__ __forceinline__ bool pick_few(const uint32_t *keys, uint32_t n, uint3
     if (have > 64) return false;
     team_sync<1>();
     const u32x2 mine = some[lane];
-    const uint64_t chosen = largest_lanes(lane < have ? mine[0] : 0u, count);
+    const uint32_t x = lane < have ? mine[0] : 0u;
+    uint32_t above = 0;
+    for (uint32_t i0 = 0; i0 < have; i0 += 8) {
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u) above += static_cast<uint32_t>(of_lane(static_cast<int32_t>(x), i0 + u)) > x;
+    }
+    uint64_t chosen = __ballot(x != 0 && above < count);
+    if (static_cast<uint32_t>(__popcll(chosen)) > count) {  // equal keys at the border: the first ones
+        const uint32_t border = wave_min(chosen >> lane & 1 ? x : 0xFFFFFFFFu);
+        uint64_t equal = __ballot(x == border);
+        for (uint32_t more = __popcll(chosen) - count; more; --more) {
+            const uint64_t last = 1ull << (63 - __clzll(equal));
+            chosen &= ~last, equal &= ~last;
+        }
+    }
     if (chosen >> lane & 1) ids[__popcll(chosen & ((1ull << lane) - 1))] = static_cast<int32_t>(first + mine[1]);
     team_sync<1>();
     return true;
@@ -314,7 +317,7 @@ enum { kFused, kScratch, kScore, kPick };  // keys in LDS; in a scratch of the w
 // Bound by the latency of a short workgroup.  32 single tokens over 4,000 to 24,000 (8 lists, dim 128,
 // pages of 16) 25 us: the longest has 1,500 blocks, 13.5 us in the loop after 6.5 us of queries and
 // first loads, 3.2 us to pick; their bounds at memory's rate would take 11 us.  A chunk of 4,096 tokens over
-// 64,097 (pages of 64) 105 us: a workgroup 22 us, two a CU, in four rounds, its waves waiting for
+// 64,097 (pages of 64) 99 us: a workgroup 21 us, two a CU, in four rounds, its waves waiting for
 // half of it.  Two groups of blocks under way a wave: four slow the split form by half.
 template <class T, int D, int MODE, bool TEAM>
 __global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_select_kernel(SelectParams P) {
