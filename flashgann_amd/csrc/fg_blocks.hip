@@ -238,14 +238,13 @@ __device__ __forceinline__ void pick(const Run &run, uint32_t count, uint32_t fi
     for (uint32_t i = min(B.valid, count) + (WAVES > 1 ? threadIdx.x : lane); i < count; i += 64 * WAVES) ids[i] = -1;
 }
 
-// pick() for few of 1 to 64 K keys, by a wave.  Bits of what each lane has at most give a bound that
+// pick() for few, by a wave.  Bits of what each lane has at most give a bound that
 // `count` lanes reach and a quarter more at most (none more past 20), or one that cannot be raised; the
 // keys that reach it are few (16 of 1,000: 21 in the mean) and each is ranked, one a lane, by those
 // above it.  False, with nothing done, where that does not serve.
-template <uint32_t K>
-__device__ __forceinline__ bool pick_few(const uint32_t *keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, u32x2 *some) {
+template <class Run>
+__device__ __forceinline__ bool pick_few(const Run &run, uint32_t count, uint32_t first, int32_t *ids, u32x2 *some) {
     const uint32_t lane = threadIdx.x % 64;
-    const Held<K> run = held_run<1, K>(keys, n);
     uint32_t top = 0;
     run.each([&](uint32_t x, uint32_t) { top = max(top, x); });
     if (static_cast<uint32_t>(__popcll(__ballot(top != 0))) < count) return false;
@@ -297,8 +296,11 @@ template <uint32_t WAVES>
 __device__ __forceinline__ void pick_from(const uint32_t *keys, uint32_t n, uint32_t count, uint32_t first, int32_t *ids, Picking<WAVES> &S) {
     if constexpr (WAVES == 1) {
         u32x2 *const some = reinterpret_cast<u32x2 *>(S.bins[0]);
-        if (n && count <= 32 && n <= 64 * 16) {
-            if (n <= 64 * 8 ? pick_few<8>(keys, n, count, first, ids, some) : pick_few<16>(keys, n, count, first, ids, some)) return;
+        if (n && count <= 32) {
+            if (n <= 64 * 8 ? pick_few(held_run<1, 8>(keys, n), count, first, ids, some)
+                            : n <= 64 * 16 ? pick_few(held_run<1, 16>(keys, n), count, first, ids, some)
+                                           : pick_few(stored_run<1>(keys, n), count, first, ids, some))
+                return;
         }
     } else {
         const uint32_t per = run_size<WAVES>(n);

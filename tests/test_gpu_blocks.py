@@ -266,6 +266,16 @@ def test_select_ties_in_tiles_of_rows():
         compare_select([300], [700], 4, 2, 64, 4, FP, k, 2, 1, 1, 3, odd)
 
 
+@pytest.mark.parametrize("n,k", ((1, 7), (3, 32), (40, 20), (70, 20), (0, 5)))
+def test_select_ties_in_long_tiles_of_rows(n, k):
+    """As above over 2,000 blocks, 8 rows a tile, and 9,000, two: n different pages in turn; 0: queries of zeros."""
+    def same(kc, table):
+        for p in range(kc.shape[0]):
+            kc[p] = kc[p % n]
+    compare_select([300], [8000], 4, 2, 64, 4, BF, k, 2, 1, 1, 11, same if n else None, None, None if n else (lambda q: q.zero_()))
+    compare_select([260], [18000], 4, 2, 64, 2, FP, k, 2, 1, 1, 12, same if n else None, None, None if n else (lambda q: q.zero_()))
+
+
 def _shared(new, kv, heads, heads_kv, page):
     """Requests whose tables name the same pages in different orders."""
     rng = np.random.default_rng(8)
