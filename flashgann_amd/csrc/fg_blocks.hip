@@ -337,7 +337,8 @@ __global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_s
         if (t.rows == 0) continue;
         const int32_t first = static_cast<int32_t>(min(P.first, P.table_width)), end = end_of(P, t.pos + t.rows - 1);
         const uint32_t n = static_cast<uint32_t>(max(end - first, 0));
-        uint32_t *const stored = P.keys + static_cast<uint64_t>(MODE == kScratch ? blockIdx.x : item) * P.rows.d * P.stride;
+        uint32_t *const stored = P.keys + (MODE == kScratch ? blockIdx.x : static_cast<uint64_t>(t.q0) * P.lists + list) * static_cast<uint64_t>(P.stride);
+        const uint32_t row_step = MODE == kScore ? P.lists * P.stride : P.stride;  // (of keys in memory: few enough where a tile has more than one row)
         if constexpr (MODE != kPick) {
             const uint32_t kv_head = list / P.list_heads;
             const int32_t *row = P.table + t.request * P.table_row + first;
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_s
             for (int i = 0; i < 4; ++i) ends[i] = end_of(P, t.pos + static_cast<int32_t>(4 * quarter) + i) - first;
             const uint32_t rows = static_cast<uint32_t>(t.rows);
             const int32_t all = end_of(P, t.pos) - first;  // blocks that every row selects from
-            uint32_t *const to = (MODE == kFused ? held : stored) + static_cast<uint64_t>(4 * quarter) * P.stride;
+            uint32_t *const to = (MODE == kFused ? held : stored) + 4 * quarter * row_step;
             for (; g < groups; g += U * step) {
                 i32x4 s4[U];
                 float times[U];
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_s
                     if (i16 < n) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (4 * quarter + i < rows) to[i * P.stride + i16] = key[i];
+                            if (4 * quarter + i < rows) to[i * row_step + i16] = key[i];
                     }
                 }
             }
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_s
             for (uint32_t r = TEAM ? 0 : wave; r < static_cast<uint32_t>(t.rows); r += TEAM ? 1 : kSelectWaves) {
                 int32_t *out = P.ids + ((t.q0 + static_cast<uint64_t>(r)) * P.lists + list) * P.count;
                 if constexpr (MODE == kFused) pick_from<WAVES>(held + r * P.stride, n, P.count, first, out, picking[TEAM ? 0 : wave]);
-                else pick_from<WAVES>(stored + static_cast<uint64_t>(r) * P.stride, n, P.count, first, out, picking[TEAM ? 0 : wave]);
+                else pick_from<WAVES>(stored, n, P.count, first, out, picking[0]);
             }
             __syncthreads();
         }
@@ -429,17 +430,20 @@ __global__ __launch_bounds__(kSelectThreads, D > 128 && !TEAM ? 2 : 4) void fg_s
 
 template <class T, int D>
 int launch_select(const SelectParams &P, int mode, uint32_t grid, uint32_t lds, hipStream_t st) {
-    const auto go = [&](auto kernel, uint32_t parts, uint32_t bytes) -> int {
+    const auto go = [&](auto kernel, const SelectParams &P, uint32_t grid, uint32_t parts, uint32_t bytes) -> int {
         if (bytes > 32 * 1024) FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kSelectLds), "selection LDS");
         hipLaunchKernelGGL(kernel, dim3(grid, parts), dim3(kSelectThreads), bytes, st, P);
         return FG_OK;
     };
     int rc = FG_OK;
-    if (mode == kFused) rc = P.rows.d == 1 ? go(fg_select_kernel<T, D, kFused, true>, 1, lds) : go(fg_select_kernel<T, D, kFused, false>, 1, lds);
-    else if (mode == kScratch) rc = go(fg_select_kernel<T, D, kScratch, true>, 1, 0);
+    if (mode == kFused) rc = P.rows.d == 1 ? go(fg_select_kernel<T, D, kFused, true>, P, grid, 1, lds) : go(fg_select_kernel<T, D, kFused, false>, P, grid, 1, lds);
+    else if (mode == kScratch) rc = go(fg_select_kernel<T, D, kScratch, true>, P, grid, 1, 0);
     else {
-        rc = go(fg_select_kernel<T, D, kScore, true>, P.parts, 0);
-        if (rc == FG_OK) rc = go(fg_select_kernel<T, D, kPick, true>, 1, 0);
+        rc = go(fg_select_kernel<T, D, kScore, true>, P, grid, P.parts, 0);
+        SelectParams each = P;  // rows are picked from one by one
+        each.rows = fast_div(1);
+        each.tiles = P.tokens;
+        if (rc == FG_OK) rc = go(fg_select_kernel<T, D, kPick, true>, each, static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(P.tokens) * P.lists, 1u << 20)), 1, 0);
     }
     if (rc != FG_OK) return rc;
     FG_HIP(hipGetLastError(), "selection launch");
@@ -513,15 +517,26 @@ int prepare_select(const fg_kv_cache *c, const fg_attention *a, SelectParams *ou
         plan->grid = static_cast<uint32_t>(std::min<uint64_t>(items, 512));
         plan->workspace = static_cast<uint64_t>(plan->grid) * P.stride * 4;
     }
-    // Few rows over many blocks: several workgroups make a row's keys, and one picks from them (8 rows over
-    // 500 blocks 11.7 us against 12.2, over 1,500 12.5 against 21.9, over 8,125 17.6 against 81; 96 over
-    // 500 14.8 against 13.2, over 1,500 20.4 against 24.5; 128 over 3,750 38.5 against 51.7; 256 over 1,500
-    // 31.8 against 30.3).
-    if (rows == 1 && items <= 160 && most >= 1024) {
+    // Rows by themselves that are few, over many blocks: several workgroups make a row's keys, and one picks
+    // from them (8 rows over 500 blocks 11.7 us against 12.2, over 1,500 12.5 against 21.9, over 8,125 17.6
+    // against 81; 96 over 500 14.8 against 13.2, over 1,500 20.4 against 24.5; 128 over 3,750 38.5 against
+    // 51.7; 256 over 1,500 31.8 against 30.3).  So with tiles, of 16 rows then, that are few (56 over 500 blocks
+    // 16.9 us against 14.1, over 1,000 19.0 against 19.0, over 2,000 26.6 against 36.7; 208 over 2,000 57.6 against
+    // 37.5), and over more blocks than LDS holds 8 rows of twice, while the keys take 1 GB at most (800 over 2,100
+    // 191 us against 142 with 8 rows, over 3,100 239 against 278, over 4,100 278 against 455; 200 over 3,000 72 against
+    // 79, over 8,000 130 against 356).
+    const uint64_t keys = static_cast<uint64_t>(a->tokens) * a->lists * P.stride * 4;
+    const uint64_t whole = one ? items : (static_cast<uint64_t>(a->tokens) / kSelectRows + a->requests) * a->lists;
+    const bool few = most >= 1024 && whole <= (one ? 160 : 64);
+    if (keys <= (1ull << 30) && (few || (!one && P.stride > 2304))) {
         plan->mode = kScore;
-        plan->grid = static_cast<uint32_t>(items);
-        P.parts = std::min<uint32_t>((most + 16 * kSelectWaves - 1) / (16 * kSelectWaves), static_cast<uint32_t>(std::max<uint64_t>(1, 512 / items)));
-        plan->workspace = items * P.stride * 4;
+        if (!one) {
+            P.rows = fast_div(kSelectRows);
+            P.tiles = a->tokens / kSelectRows + a->requests;
+        }
+        plan->grid = static_cast<uint32_t>(std::min<uint64_t>(whole, 1u << 20));
+        P.parts = std::min<uint32_t>((most + 16 * kSelectWaves - 1) / (16 * kSelectWaves), static_cast<uint32_t>(std::max<uint64_t>(1, (one ? 512 : 1024) / std::max<uint64_t>(1, whole))));
+        plan->workspace = keys;
     }
     return FG_OK;
 }

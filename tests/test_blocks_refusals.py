@@ -92,6 +92,17 @@ def test_lists_and_ranges():
         refused(attend(cache_bytes(), blocks_bytes(**bad)), word)
 
 
+def test_nothing_new_over_a_wide_table():
+    """No tokens or no requests: nothing to do, however wide the table."""
+    L = _lib.lib()
+    for width in (500, 5000, 500000):
+        for none in (dict(tokens=0), dict(requests=0), dict(requests=0, tokens=15, heads=256, lists=256), dict(requests=0, tokens=0)):
+            a = blocks_bytes(**{**none, "table_width": width})
+            assert L.fg_select_blocks_workspace_bytes(cache_bytes(), a) == 0
+            assert L.fg_attend_blocks_workspace_bytes(cache_bytes(), a) == 0
+            assert select(cache_bytes(), a) == _lib.FG_OK and attend(cache_bytes(), a) == _lib.FG_OK
+
+
 def test_workspaces():
     """What a call needs at most, from its sizes; a smaller, absent or odd one is refused."""
     L = _lib.lib()

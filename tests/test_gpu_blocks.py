@@ -237,8 +237,7 @@ def test_select_long(new, kv, heads, heads_kv, lists, page, k):
 @pytest.mark.parametrize("new,kv,page,k", ((300, 4000, 4, 16), (300, 4000, 4, 32), (300, 4000, 4, 33), (300, 12000, 4, 20), (300, 30000, 4, 20), (300, 60000, 4, 300),
                                            (300, 70000, 2, 9)))
 def test_select_tiles_of_rows(new, kv, page, k):
-    """Many rows at once: 16 of a tile in LDS, 8, 4 and 2 over longer tables, and more blocks than it holds, where
-    a workgroup takes several rows one after another; few and many to pick."""
+    """Many rows at once: 16 of a tile in LDS, and over longer tables with their keys in memory; few and many to pick."""
     from flashgann_amd import attention
     q, kc, _, table, starts = case(17, [new], [kv], 4, 2, 64, page, BF)
     bounds, scales = torch.zeros((kc.shape[0], 2, 2, 64), dtype=torch.int8, device="cuda"), torch.zeros((kc.shape[0], 2), device="cuda")
@@ -266,14 +265,36 @@ def test_select_ties_in_tiles_of_rows():
         compare_select([300], [700], 4, 2, 64, 4, FP, k, 2, 1, 1, 3, odd)
 
 
-@pytest.mark.parametrize("n,k", ((1, 7), (3, 32), (40, 20), (70, 20), (0, 5)))
+@pytest.mark.parametrize("new,kv,page,k", ((8400, 17000, 8, 16), (3400, 20000, 4, 33), (1700, 20000, 2, 20), (850, 20000, 1, 7), (490, 35000, 1, 9)))
+def test_select_more_keys_than_are_kept(new, kv, page, k):
+    """More than 1 GB of keys: tiles of 8, 4, 2 rows and one in LDS, and more blocks than it holds, where a workgroup
+    takes several rows one after another."""
+    from flashgann_amd import attention
+    q, kc, _, table, starts = case(18, [new], [kv], 16, 2, 64, page, BF)
+    bounds, scales = torch.zeros((kc.shape[0], 2, 2, 64), dtype=torch.int8, device="cuda"), torch.zeros((kc.shape[0], 2), device="cuda")
+    attention.cache_bounds(kc.cuda(), torch.arange(kc.shape[0] * page, device="cuda"), bounds, scales)
+    ids = attention.select_blocks(q.cuda(), bounds, scales, table.cuda(), ints(starts), ints([kv]), page_size=page, k=k, lists=16)
+    for i in range(0, new, 500):  # the rows some at a time, each part as the last of its request
+        n = min(500, new - i)
+        want = plain_select(q[i:i + n], bounds, scales, table, [0, n], [kv - new + i + n], page, k, 16, 1, 1)
+        assert torch.equal(ids[i:i + n], want), i
+
+
+@pytest.mark.parametrize("new,blocks", ((100, 1000), (100, 1030), (100, 2100), (33, 4000)))
+@pytest.mark.parametrize("lists,k", ((2, 16), (8, 64)))
+def test_select_few_tiles(new, blocks, lists, k):
+    """Few tiles of rows over many blocks, of two requests of different lengths and one without new tokens."""
+    compare_select([new, 0, 17], [4 * blocks, 50, 1500], 8, 2, 64, 4, BF, k, lists, 1, 1, 13)
+
+
+@pytest.mark.parametrize("n,k", ((1, 7), (3, 32), (40, 20), (0, 5)))
 def test_select_ties_in_long_tiles_of_rows(n, k):
-    """As above over 2,000 blocks, 8 rows a tile, and 9,000, two: n different pages in turn; 0: queries of zeros."""
+    """As above over 2,200 and 2,600 blocks: n different pages in turn; 0: queries of zeros."""
     def same(kc, table):
         for p in range(kc.shape[0]):
             kc[p] = kc[p % n]
-    compare_select([300], [8000], 4, 2, 64, 4, BF, k, 2, 1, 1, 11, same if n else None, None, None if n else (lambda q: q.zero_()))
-    compare_select([260], [18000], 4, 2, 64, 2, FP, k, 2, 1, 1, 12, same if n else None, None, None if n else (lambda q: q.zero_()))
+    compare_select([140], [8800], 8, 2, 64, 4, BF, k, 4, 1, 1, 11, same if n else None, None, None if n else (lambda q: q.zero_()))
+    compare_select([130], [5200], 8, 2, 64, 2, FP, k, 4, 1, 1, 12, same if n else None, None, None if n else (lambda q: q.zero_()))
 
 
 def _shared(new, kv, heads, heads_kv, page):
