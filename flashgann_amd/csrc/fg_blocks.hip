@@ -574,7 +574,7 @@ int fg_cache_bounds(const fg_kv_cache *cache, const int64_t *d_slots, uint32_t t
                     void *stream) {
     return guarded<int>([&]() -> int {
         CacheView view;
-        if (int rc = check_cache(cache, &view)) return rc;
+        if (int rc = check_cache(cache, &view, false)) return rc;
         if (tokens > 0x7FFFFFFFu) return fail(FG_EINVAL, "tokens must be below 2^31");
         if (tokens == 0) return FG_OK;
         if (!d_slots || !d_bounds || !d_scales) return fail(FG_EINVAL, "NULL device buffer");

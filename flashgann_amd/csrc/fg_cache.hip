@@ -173,9 +173,9 @@ int check_cache_shape(const fg_kv_cache *c) {
     return FG_OK;
 }
 
-int check_cache(const fg_kv_cache *c, CacheView *view) {
+int check_cache(const fg_kv_cache *c, CacheView *view, bool values) {
     if (int rc = check_cache_shape(c)) return rc;
-    if (!c->k || !c->v) return fail(FG_EINVAL, "NULL cache buffer");
+    if (!c->k || (values && !c->v)) return fail(FG_EINVAL, "NULL cache buffer");
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16)
         return fail(FG_EINVAL, "cache buffers must be 16-byte aligned");
     if ((c->k_page | c->k_token | c->k_head | c->v_page | c->v_token | c->v_head) % 8)

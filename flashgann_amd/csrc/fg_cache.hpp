@@ -32,8 +32,9 @@ struct CacheView {
 // Checks a cache's sizes and type, its pointers and strides aside; FG_OK or a reported failure.
 int check_cache_shape(const fg_kv_cache *c);
 
-// Checks the cache and fills its view; FG_OK or a reported failure.
-int check_cache(const fg_kv_cache *c, CacheView *view);
+// Checks the cache and fills its view; FG_OK or a reported failure.  Without `values`, for a
+// call that reads keys alone, v may be NULL.
+int check_cache(const fg_kv_cache *c, CacheView *view, bool values = true);
 
 }  // namespace fgk
 

@@ -447,7 +447,7 @@ void launch_weigh(const WeighParams &P, uint32_t dim, uint32_t grid, hipStream_t
 
 int weigh(const fg_kv_cache *c, const fg_attention *a, float *weights, const int32_t *known, void *stream) {
     WeighParams P{};
-    if (int rc = check_cache(c, &P.cache)) return rc;
+    if (int rc = check_cache(c, &P.cache, false)) return rc;
     if (!a) return fail(FG_EINVAL, "attention arguments are NULL");
     if (a->heads < 1 || a->heads > 1024 || a->heads % c->heads_kv) return fail(FG_EINVAL, "heads must be a multiple of heads_kv, at most 1024");
     if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return fail(FG_EINVAL, "scale must be positive and finite");

@@ -374,7 +374,7 @@ int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *
  * on its list, which lie between: sinks <= b <= c - window. */
 
 /* For each of `tokens` slots that is the last of its page, 8-bit bounds of that page's keys
- * (cache->v is not read): with M the largest |key| of a page and key/value head and 2^s the
+ * (cache->v is not read and may be NULL): with M the largest |key| of a page and key/value head and 2^s the
  * least power of two with M <= 127 * 2^s, not below 2^-126,
  *   d_scales[page * heads_kv + head]                       2^s
  *   d_bounds[((page * heads_kv + head) * 2 + 0) * dim + d] the largest key of channel d / 2^s, rounded up
@@ -430,7 +430,7 @@ int64_t fg_attend_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_atte
  * are not all given (the last ones of a prompt, say) the sum is over those.  A token below
  * d_known of every request that shares its page gets all their sums (in no fixed order); one that
  * has to be set may belong to one request only.  a: q, lse, table, q_starts, kv_lens, scale;
- * cache->v is not read.  tokens at most 4,194,304. */
+ * cache->v is not read and may be NULL.  tokens at most 4,194,304. */
 int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_weights, const int32_t *d_known,
                    void *stream);
 
