@@ -189,6 +189,6 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     `attend` without a window from then on; keys hold their own positions.  Returns the
     new lengths, the pages that are free now (the first `released` entries of `freed`, -1
     behind them) and their number; block_table keeps its entries, which `cache_plan` writes
-    over as the request grows.  Pages may not be shared, k_cache and v_cache not be the same
-    memory.  1 to 4,096 requests a call."""
+    over as the request grows.  No page may be named twice, and k_cache and v_cache may share
+    no memory, with each other or between their own places.  1 to 4,096 requests a call."""
     return CacheEviction(*_attention.cache_evict(k_cache, v_cache, weights, block_table, kv_lens, budget, window, sinks))

@@ -546,6 +546,10 @@ int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_
         EvictPlan plan;
         if (int rc = plan_evict(cache, table_width, requests, budget, &P, &plan)) return rc;
         if (int rc = check_cache(cache, &P.cache)) return rc;
+        // places that share memory (a head repeated by a stride of 0, say) would be moved by several workgroups
+        const bool shared = (cache->pages > 1 && (!cache->k_page || !cache->v_page)) || (cache->page_size > 1 && (!cache->k_token || !cache->v_token)) ||
+                            (cache->heads_kv > 1 && (!cache->k_head || !cache->v_head));
+        if (shared) return fail(FG_EINVAL, "a cache whose places share memory (a stride of 0) cannot be evicted from");
         if (static_cast<uint64_t>(window) + sinks > budget) return fail(FG_EINVAL, "window + sinks must be at most budget");
         if (table_row < 0) return fail(FG_EINVAL, "table_row out of range");
         if (!d_weights || !d_kv_lens || !d_new_lens || !d_released || (table_width && (!d_table || !d_freed))) return fail(FG_EINVAL, "NULL device buffer");

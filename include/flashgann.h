@@ -446,8 +446,8 @@ int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_wei
  *   d_freed    requests * table_width  the table's entries past that, requests in order; -1 behind them
  *   d_released 1                       how many those are
  * The table itself stays: fg_cache_plan writes a new page over an entry when the request
- * grows again.  No page may belong to two requests of the call, k and v not be the same memory,
- * d_new_lens not overlap d_kv_lens.  Bounds of pages whose keys moved are void.  1 <= requests <= 4096, sinks + window <= budget, 1 <= budget. */
+ * grows again.  No page may be named twice by the entries in use, no two places of the cache share
+ * memory, nor k and v (a stride of 0 and k == v are refused), d_new_lens not overlap d_kv_lens.  Bounds of pages whose keys moved are void.  1 <= requests <= 4096, sinks + window <= budget, 1 <= budget. */
 int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_table, int64_t table_row, uint32_t table_width,
                    const int32_t *d_kv_lens, uint32_t requests, uint32_t budget, uint32_t window, uint32_t sinks,
                    int32_t *d_new_lens, int32_t *d_freed, int32_t *d_released, void *workspace, uint64_t workspace_bytes,
