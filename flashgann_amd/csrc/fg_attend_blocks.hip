@@ -295,6 +295,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_kernel(BlocksP
             l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
             u32x4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
             const vec pv = __builtin_bit_cast(vec, pk);
+            team_sync<1>();  // (the values that other lanes have written)
             const char *vt = vmine + (4 * quarter + col / 4) * VROW + (col % 4) * 8;
 #pragma unroll
             for (int i = 0; i < DB; ++i) {
@@ -562,6 +563,7 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
             sees = n < total ? B.entry_seen[e] & tokens_from(t.pos, static_cast<int64_t>(B.entry_block[e]) * page_size + off) : 0u;
             ks = kbase + p * P.cache.k_page + off * P.cache.k_token;
             if (half == 0) value_at[wave][i / 4 % 2][col] = p * P.cache.v_page + off * P.cache.v_token;
+            team_sync<1>();  // (other lanes read it)
         };
         const auto load_k = [&] {
 #pragma unroll
@@ -639,6 +641,7 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
                 pk[k / 8][k % 8 / 2] = T::pack(p0, p1);
             }
             l += sum;
+            team_sync<1>();  // (the values that other lanes have written)
             const char *const vt = vmine + (4 * half + lane % 16 / 4) * VROW + (lane / 16 % 2) * 32 + (lane % 4) * 8;
 #pragma unroll
             for (int n = 0; n < 2 * DB; ++n) {
