@@ -119,10 +119,10 @@ __global__ __launch_bounds__(kBoundsThreads) void fg_cache_bounds_kernel(BoundsP
             int c[2][4];
 #pragma unroll
             for (int i8 = 0; i8 < 8; ++i8) {
-                // at least one code away from 0 where the key is not 0: the product with one that
-                // lies 2^149 times below the scale is 0 before it is rounded
-                const float x = sub ? fminf(floorf(lo[i8] * inv), lo[i8] < 0.0f ? -1.0f : 127.0f) : fmaxf(ceilf(hi[i8] * inv), hi[i8] > 0.0f ? 1.0f : -127.0f);
-                c[i8 / 4][i8 % 4] = finite ? static_cast<int>(x) : 0;
+                // (floor(x) is -ceil(-x)) at least one code away from 0 where the key is not 0: the
+                // product with one that lies 2^149 times below the scale is 0 before it is rounded
+                const float out = sub ? -lo[i8] : hi[i8], x = fmaxf(ceilf(out * inv), out > 0.0f ? 1.0f : -127.0f);
+                c[i8 / 4][i8 % 4] = finite ? static_cast<int>(sub ? -x : x) : 0;
             }
             *reinterpret_cast<uint2 *>(P.bounds + (at * 2 + sub) * D + piece * 8) = uint2{pack4(c[0]), pack4(c[1])};
         }
