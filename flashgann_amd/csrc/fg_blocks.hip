@@ -524,13 +524,17 @@ int prepare_select(const fg_kv_cache *c, const fg_attention *a, SelectParams *ou
     // against 81; 96 over 500 14.8 against 13.2, over 1,500 20.4 against 24.5; 128 over 3,750 38.5 against
     // 51.7; 256 over 1,500 31.8 against 30.3).  So with tiles, of 16 rows then, that are few (56 over 500 blocks
     // 16.9 us against 14.1, over 1,000 19.0 against 19.0, over 2,000 26.6 against 36.7; 208 over 2,000 57.6 against
-    // 37.5), and over more blocks than LDS holds 8 rows of twice, while the keys take 1 GB at most (800 over 2,100
-    // 191 us against 142 with 8 rows, over 3,100 239 against 278, over 4,100 278 against 455; 200 over 3,000 72 against
-    // 79, over 8,000 130 against 356).
+    // 37.5), and over long tables, while the keys take 1 GiB at most.  In LDS a tile has 8 rows then (4 past 4,096
+    // blocks): bounds are read twice as often, and past 2,160 blocks at dim 128, 2,030 at 256, two workgroups no
+    // longer fit a CU; smaller bounds are still read faster than keys.  Keys in memory against LDS, us, 8 lists: 1,600
+    // rows dim 64 3,199 blocks 198, 194, 3,699 210, 217; dim 96 2,699 209, 209, 3,199 224, 238; dim 128 2,149 201, 144,
+    // 2,199 204, 211; dim 256 1,999 227, 189, 2,049 230, 288.  400 rows dim 64 3,624 66, 63, 4,224 74, 98; dim 96 2,624
+    // 65, 59, 3,624 72, 77; dim 128 2,124 63, 48, 2,224 64, 62, 2,624 68, 70; dim 256 1,974 69, 49, 2,074 73, 86.
     const uint64_t keys = static_cast<uint64_t>(a->tokens) * a->lists * P.stride * 4;
     const uint64_t whole = one ? items : (static_cast<uint64_t>(a->tokens) / kSelectRows + a->requests) * a->lists;
     const bool few = most >= 1024 && whole <= (one ? 160 : 64);
-    if (keys <= (1ull << 30) && (few || (!one && P.stride > 2304))) {
+    const uint32_t held_well = c->dim <= 64 ? 3400 : c->dim <= 96 ? 2800 : c->dim <= 128 ? 2160 : 2030;  // blocks
+    if (keys <= (1ull << 30) && (few || (!one && P.stride > held_well))) {
         plan->mode = kScore;
         if (!one) {
             P.rows = fast_div(kSelectRows);

@@ -48,7 +48,8 @@ def select_into(ids, q, bounds, scales, table, starts, kv, page, k, lists):
     (700, 37, 641, 6000, 4, False),  # of 16 rows, more blocks
     (60, 5, 50, 12000, 4, True),     # few tiles over many blocks
     (3, 1, 1, 20000, 4, True),       # a row over many blocks
-    (700, 31, 640, 12000, 4, True),  # keys in memory
+    (700, 31, 640, 12000, 4, False), # of 8 rows
+    (700, 31, 640, 16000, 4, True),  # keys in memory
 ))
 @pytest.mark.parametrize("k", (7, 40))
 def test_select_leaves_rows_outside(rows, begin, new, kv, page, memory, k):
