@@ -162,7 +162,9 @@ def cache_weigh(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tenso
     rows that see it and the query heads of its key/value head of exp(scale q . k - lse).
 
     q, q_starts, kv_lens: as for `attend` (all new tokens, or a request's last ones only);
-    lse: what `attend` returned for them, without a window.  weights: (pages, heads_kv,
+    lse: what `attend` returned for them, without a window, so that a row's weights sum to 1
+    (with `attend_blocks`' they are shares of the selected pages, and a token outside those may
+    count for more than 1).  weights: (pages, heads_kv,
     page_size) float32, contiguous, written in place.  known: (requests,) int32, the tokens
     that have a weight already (the length before this step, say): those from there on are
     set instead of added to.  Tokens that requests of the call share get all their sums if

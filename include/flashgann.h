@@ -424,7 +424,9 @@ int64_t fg_attend_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_atte
  * slot and key/value head.  For token j of request r and its slot,
  *   weight (+)= sum over the request's rows of q at positions p >= j and the query heads of
  *               the key/value head of exp(scale q . k_j - lse)
- * with q's rows placed as for fg_attend and a->lse, read here, what fg_attend gave for them.
+ * with q's rows placed as for fg_attend and a->lse, read here, what fg_attend gave for them: each row's
+ * weights sum to 1.  (Any lse is taken as it is: with fg_attend_blocks' they are shares of the selected
+ * pages, and a token outside those may count for more than 1.)
  * Tokens j >= d_known[r] have no weight yet: theirs is set, the others' is added to.  A row
  * whose lse is -infinity adds nothing; a token without a page gets no weight.  Of rows that
  * are not all given (the last ones of a prompt, say) the sum is over those.  A token below
