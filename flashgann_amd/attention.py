@@ -191,6 +191,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     `attend` without a window from then on; keys hold their own positions.  Returns the
     new lengths, the pages that are free now (the first `released` entries of `freed`, -1
     behind them) and their number; block_table keeps its entries, which `cache_plan` writes
-    over as the request grows.  No page may be named twice, and k_cache and v_cache may share
+    over as the request grows.  A token whose place, or new place, has no page (cache_plan ran out
+    of them: used > the free pages) is lost, and entries without one are among `freed` as they
+    are: leave them out of the free pages.  No page may be named twice, and k_cache and v_cache may share
     no memory, with each other or between their own places.  1 to 4,096 requests a call."""
     return CacheEviction(*_attention.cache_evict(k_cache, v_cache, weights, block_table, kv_lens, budget, window, sinks))

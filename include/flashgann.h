@@ -441,11 +441,14 @@ int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_wei
  * weight (equal ones: the earlier; NaN counts as +infinity, a token without a page as less than any).
  * With H = budget - window, kept tokens below place H stay where they are; those above move,
  * in order, to the places below H whose tokens go, also in order; the last `window` tokens
- * move to H .. budget - 1.  Keys, values and weights move together, head by head, so a slot's
+ * move to H .. budget - 1.  A place without a page holds nothing: it may be one of those below H, and
+ * what would move to it, the heaviest and the last tokens too, is lost, as cache_append does not write
+ * it either.  Keys, values and weights move together, head by head, so a slot's
  * heads may hold different tokens; positions that were rotated into keys stay theirs.
  * Attention (fg_attend without a window) sees the same whatever the order.  Outputs:
  *   d_kv_lens  requests                min(length, budget); lengths past the table's room count as that
- *   d_freed    requests * table_width  the table's entries past that, requests in order; -1 behind them
+ *   d_freed    requests * table_width  the table's entries past that, requests in order and as they are
+ *                                      (one that names no page too); -1 behind them
  *   d_released 1                       how many those are
  * The table itself stays: fg_cache_plan writes a new page over an entry when the request
  * grows again.  No page may be named twice by the entries in use, no two places of the cache share
