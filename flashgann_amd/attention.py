@@ -139,7 +139,12 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, scales: torch.Tensor, b
     read anyway.  lists: a multiple of heads_kv that divides heads, heads_kv unless given; the
     query heads of a list select together, by the sum over them of the most that the bounds
     leave for q . key, with the summed queries in 8 bits too.  Scores are exact, and equal
-    ones go to the lower block.  1 to 4,096 pages a list; up to 4,194,304 rows a call."""
+    ones go to the lower block.  Rows outside every request are left uninitialised.  1 to 4,096
+    pages a list; up to 4,194,304 rows a call.
+
+    Pass the columns in use, block_table[:, :n]: the call is run, and takes up to 1 GiB of
+    workspace, by what the table has room for (4,096 rows over 1,000 pages 99 us, in a table of
+    8,192 columns 297 us and 1 GiB)."""
     return _attention.select_blocks(q, bounds, scales, block_table, q_starts, kv_lens, page_size, k, lists, first_blocks, last_blocks)
 
 
@@ -152,7 +157,8 @@ def attend_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 
     ids: (tokens, lists, k) int32 as `select_blocks` returns them, a list for each row; an
     id that is not above all before it in its list, or names one of the first or last blocks
-    or one after them, adds nothing.  Everything else, and (out, lse), as for `attend`."""
+    or one after them, adds nothing.  Everything else, and (out, lse), as for `attend`.  A
+    block_table of more than 4,096 columns makes chunks take twice as long: pass those in use."""
     return _attention.attend_blocks(q, k_cache, v_cache, block_table, q_starts, kv_lens, ids, first_blocks, last_blocks, scale, out, lse)
 
 
@@ -194,5 +200,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     over as the request grows.  A token whose place, or new place, has no page (cache_plan ran out
     of them: used > the free pages) is lost, and entries without one are among `freed` as they
     are: leave them out of the free pages.  No page may be named twice, and k_cache and v_cache may share
-    no memory, with each other or between their own places.  1 to 4,096 requests a call."""
+    no memory, with each other or between their own places.  1 to 4,096 requests a call.
+
+    Kernels and workspace (8 bytes a request, head and token of the budget at least) follow what the
+    table has room for: pass the columns in use, block_table[:, :n]."""
     return CacheEviction(*_attention.cache_evict(k_cache, v_cache, weights, block_table, kv_lens, budget, window, sinks))

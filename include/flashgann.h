@@ -371,7 +371,12 @@ int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *
  * these calls fg_attention's sinks and window count blocks: the row at position p, whose
  * block is c = p div page_size, sees of the tokens j <= p those of the first `sinks`
  * blocks, of the last `window` ones (c - window + 1 .. c, window >= 1), and of the blocks
- * on its list, which lie between: sinks <= b <= c - window. */
+ * on its list, which lie between: sinks <= b <= c - window.
+ *
+ * The host does not know the lengths, so kernels and workspaces of these calls and of eviction
+ * follow the table's room: let table_width be the columns in use, not those allocated.  One MI355X: a chunk
+ * of 4,096 tokens selecting from 1,000 pages 99 us, in a table of 8,192 columns 297 and of 32,768 1,930;
+ * attention of 2,048 over what they selected 341 us, past 4,096 columns 711. */
 
 /* For each of `tokens` slots that is the last of its page, 8-bit bounds of that page's keys
  * (cache->v is not read and may be NULL): with M the largest |key| of a page and key/value head and 2^s the
@@ -405,6 +410,9 @@ int fg_cache_bounds(const fg_kv_cache *cache, const int64_t *d_slots, uint32_t t
  * request are left alone.  tokens at most 4,194,304, tokens * lists * nids < 2^31. */
 int fg_select_blocks(const fg_kv_cache *cache, const fg_attention *a, const int8_t *d_bounds, const float *d_scales,
                      int32_t *d_ids, void *workspace, uint64_t workspace_bytes, void *stream);
+/* 0 where LDS holds the keys of the table's blocks for enough rows; else 4 bytes a row, list and column past
+ * the first blocks, up to 1 GiB, or, past that, up to 2,048 a column.  Used until the call's work on `stream`
+ * ends, as all workspaces here. */
 int64_t fg_select_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
 
 /* Attention of chunks of new tokens (rows as for fg_attend) over the first and last blocks
@@ -452,7 +460,13 @@ int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_wei
  *   d_released 1                       how many those are
  * The table itself stays: fg_cache_plan writes a new page over an entry when the request
  * grows again.  No page may be named twice by the entries in use, no two places of the cache share
- * memory, nor k and v (a stride of 0 and k == v are refused), d_new_lens not overlap d_kv_lens.  Bounds of pages whose keys moved are void.  1 <= requests <= 4096, sinks + window <= budget, 1 <= budget. */
+ * memory, nor k and v (a stride of 0 and k == v are refused), d_new_lens not overlap d_kv_lens.  Bounds of
+ * pages whose keys moved are void.  1 <= requests <= 4096, sinks + window <= budget, 1 <= budget.
+ *
+ * Workspace: 8 bytes a request, head and token of min(budget, table_width * page_size), and over tables that
+ * name more than 32,768 tokens 4 for each of those and up to 512 requests and heads.  A table that names at most
+ * 512 tokens past the budget, 8,192 in all, serves in one launch (48 requests a few over 4,096 tokens 26 us; in
+ * a table of 8,192 pages of 16 43 us and 215 MB instead of 13). */
 int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_table, int64_t table_row, uint32_t table_width,
                    const int32_t *d_kv_lens, uint32_t requests, uint32_t budget, uint32_t window, uint32_t sinks,
                    int32_t *d_new_lens, int32_t *d_freed, int32_t *d_released, void *workspace, uint64_t workspace_bytes,
