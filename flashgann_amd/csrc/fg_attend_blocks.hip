@@ -734,6 +734,7 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
         (a->q_token | a->q_head | a->out_token | a->out_head) % 8)
         return fail(FG_EINVAL, "q and out must be 16-byte aligned, strides multiples of 8 elements");
+    if ((a->tokens > 1 && !a->out_token) || (a->heads > 1 && !a->out_head)) return fail(FG_EINVAL, "rows of out share memory (a stride of 0)");
     P.q = static_cast<const char *>(a->q);
     P.out = static_cast<char *>(a->out);
     P.lse = a->lse;

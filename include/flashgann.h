@@ -420,7 +420,8 @@ int64_t fg_select_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_atte
  * as fg_select_blocks writes them.  An id that is not above all before it in its list, or
  * lies outside [sinks, c - window], adds nothing.  nids at most 4,096, 0 allowed; tokens
  * at most 4,194,304, and at most 2^23 tiles of rows: (tokens + requests) * lists *
- * ceil(heads / lists / 16) up to that always serves. */
+ * ceil(heads / lists / 16) up to that always serves.  No two rows of out may share memory (a stride
+ * of 0 is refused); out may be q itself. */
 int fg_attend_blocks(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes,
                      void *stream);
 int64_t fg_attend_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
