@@ -423,7 +423,10 @@ __device__ __forceinline__ bool any_specials(const u32x4 (&w)[N]) {
 #pragma unroll
     for (int k = 0; k < N; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[k][i]) << static_cast<uint16_t>(1));
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = w[k][i];  // (a bit cast of the vector's element itself takes the first one)
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x) << static_cast<uint16_t>(1));
+        }
     return max(most[0], most[1]) >= 2 * T::kExponent;
 }
 
