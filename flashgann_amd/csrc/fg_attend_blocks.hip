@@ -1,7 +1,7 @@
 // fg_attend_blocks.hip -- attention over selected pages of a paged cache.
 //
 // Softmax and products are those of fg_attend.hip's few-rows kernel: S' = K Q', then
-// O' = V' P', a running maximum and sum, weights rounded to the values' type.  What differs is
+// O' = V' P', a running maximum and sum.  What differs is
 // which tokens a row sees: the first blocks, the last ones and those of its list.  Rows of
 // neighbouring tokens share a tile of 16 rows, and the tile reads the union of what its
 // tokens see, each block with a mask of the tokens that see it: neighbours ask for much the
@@ -16,6 +16,32 @@ constexpr uint32_t kTileRows = 16;
 constexpr uint32_t kTokenPlaces = 1024;  // token places resolved at a time
 constexpr uint32_t kSplitTokens = 128;   // a part's tokens are a multiple: a tile of each wave
 constexpr uint32_t kMostParts = 64;
+
+// What rounding two weights to the values' type left of them, in that type too.  The matrix unit takes
+// 16 bits, and outputs are to be off by their own rounding alone: a weight goes in as the sum of two
+// such numbers (16 bits of it in bfloat16, 22 in float16), against the same values read once.  A chunk's
+// attention takes 6% longer for it (381 us against 359), single tokens and drafts do not; the error is
+// that of 32-bit weights (0.0017 relative in bfloat16, the output's rounding, against 0.0021 with one part).
+template <class T>
+__device__ __forceinline__ uint32_t rest_of(float a, float b, uint32_t rounded) {
+    return T::pack(a - as_float<T>(rounded & 0xFFFF), b - as_float<T>(rounded >> 16));
+}
+
+// Whether an infinity or NaN is among N pieces of 16-bit values: their magnitudes' maximum, two
+// values an instruction.
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+template <class T, int N>
+__device__ __forceinline__ bool any_specials(const u32x4 (&w)[N]) {
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = w[k][i];  // (a bit cast of the vector's element itself takes the first one)
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x) << static_cast<uint16_t>(1));
+        }
+    return max(most[0], most[1]) >= 2 * T::kExponent;
+}
 
 struct BlocksParams {
     CacheView cache;
@@ -160,7 +186,6 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_kernel(BlocksP
     const uint32_t rows = tokens * P.per.d, heads = min(P.group - head0, P.per.d);
     const uint32_t token = P.per.div(col), bit = min(token, 15u);
     const bool real = col < rows && col - token * P.per.d < heads;
-    const bool ragged = tokens > 1;
     const int64_t head = static_cast<int64_t>(list) * P.group + head0 + (col - token * P.per.d);
     vec qv[STEPS];
     {
@@ -248,24 +273,20 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_kernel(BlocksP
             uint32_t odd = 0;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                bool special = false;
+                u32x4 v[STEPS];  // (of a token that no row sees: zeros, whatever was read instead)
 #pragma unroll
-                for (int k = 0; k < STEPS; ++k) {
-                    // (a token that no row sees: whatever was read instead)
-                    u32x4 v = held[b] ? vr[b][k] : u32x4{0, 0, 0, 0};
-                    if (ragged && any_special<T>(v)) {
-                        // 0 * inf is NaN: where not every row sees a token, infinities and NaNs
-                        // are taken out of the product and added to the rows that see them
-                        special = true;
-                        v = finite_part<T>(v);
-                    }
-                    *reinterpret_cast<u32x4 *>(vmine + (16 * b + col) * VROW + 64 * k + 16 * quarter) = v;
-                }
-                if (ragged) {
-                    uint64_t any = __ballot(special);
-                    any |= any >> 32;
+                for (int k = 0; k < STEPS; ++k) v[k] = held[b] ? vr[b][k] : u32x4{0, 0, 0, 0};
+                // 0 * inf is NaN: infinities and NaNs are taken out of the product, whose weights, or
+                // parts of them, may be 0 or negative, and added to the rows that see them
+                const uint64_t special = __ballot(any_specials<T>(v));
+                if (special) {
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) v[k] = finite_part<T>(v[k]);
+                    const uint64_t any = special | special >> 32;
                     odd |= static_cast<uint32_t>((any | any >> 16) & 0xFFFF) << (16 * b);
                 }
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) *reinterpret_cast<u32x4 *>(vmine + (16 * b + col) * VROW + 64 * k + 16 * quarter) = v[k];
             }
             if ((at32 + 4) * 32 < n) load(at32 + 4);
 
@@ -294,7 +315,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_kernel(BlocksP
             for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(p[i] - zero);
             l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
             u32x4 pk = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
-            const vec pv = __builtin_bit_cast(vec, pk);
+            u32x4 pr;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pr[i] = rest_of<T>(p[2 * i], p[2 * i + 1], pk[i]);
+            const vec pv = __builtin_bit_cast(vec, pk), rv = __builtin_bit_cast(vec, pr);
             team_sync<1>();  // (the values that other lanes have written)
             const char *vt = vmine + (4 * quarter + col / 4) * VROW + (col % 4) * 8;
 #pragma unroll
@@ -302,6 +326,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_kernel(BlocksP
                 const s16x4 a0 = read_transposed(vt + 32 * i), a1 = read_transposed(vt + 16 * VROW + 32 * i);
                 const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
                 o[i] = T::mfma16(__builtin_bit_cast(vec, a), pv, o[i]);
+                o[i] = T::mfma16(__builtin_bit_cast(vec, a), rv, o[i]);
             }
             for (; odd; odd &= odd - 1) {
                 const int32_t at = at32 * 32 + __ffs(odd) - 1;
@@ -412,22 +437,6 @@ constexpr uint32_t kWindow = 1024;  // blocks whose tokens are known at a time
 __device__ __forceinline__ uint32_t tokens_from(int32_t pos, int64_t j) {
     const int64_t i = j - pos;
     return i <= 0 ? ~0u : i >= 32 ? 0u : ~0u << i;
-}
-
-// Whether an infinity or NaN is among N pieces of 16-bit values: their magnitudes' maximum, two
-// values an instruction.
-typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
-template <class T, int N>
-__device__ __forceinline__ bool any_specials(const u32x4 (&w)[N]) {
-    u16x2 most = {0, 0};
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t x = w[k][i];  // (a bit cast of the vector's element itself takes the first one)
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x) << static_cast<uint16_t>(1));
-        }
-    return max(most[0], most[1]) >= 2 * T::kExponent;
 }
 
 template <class T, int D>
@@ -595,8 +604,8 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
             if (more) load_k();
             uint32_t odd = 0;  // tokens whose values are not all finite
             if (__any(any_specials<T>(vr))) {
-                // 0 * inf is NaN: infinities and NaNs are taken out of the product and added to the
-                // rows that see them
+                // (as in the few-rows kernel) infinities and NaNs are taken out of the product and added to
+                // the rows that see them
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
                     if (any_special<T>(vr[k])) odd |= 1u << (k * 64 + lane) / CHUNKS;
@@ -636,12 +645,13 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
             }
             const float zero = UP - base;
             float sum = 0.0f;
-            u32x4 pk[2];  // the weights of 16 tokens each
+            u32x4 pk[2], pr[2];  // the weights of 16 tokens each, in two parts
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(s[k], P.scale2, zero)), p1 = __builtin_amdgcn_exp2f(fmaf(s[k + 1], P.scale2, zero));
                 sum += p0 + p1;
                 pk[k / 8][k % 8 / 2] = T::pack(p0, p1);
+                pr[k / 8][k % 8 / 2] = rest_of<T>(p0, p1, pk[k / 8][k % 8 / 2]);
             }
             l += sum;
             team_sync<1>();  // (the values that other lanes have written)
@@ -651,6 +661,7 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
                 const char *at = vt + 16 * (n / DB) * VROW + 64 * (n % DB);
                 const s16x8 a = __builtin_shufflevector(read_transposed(at), read_transposed(at + 8 * VROW), 0, 1, 2, 3, 4, 5, 6, 7);
                 o[n % DB] = T::mfma32(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, pk[n / DB]), o[n % DB]);
+                o[n % DB] = T::mfma32(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, pr[n / DB]), o[n % DB]);
             }
             for (; odd; odd &= odd - 1) {
                 const int at = __ffs(odd) - 1;

@@ -28,15 +28,6 @@ __device__ __forceinline__ uint32_t pack4(const int (&c)[4]) {
     return (c[0] & 0xFF) | (c[1] & 0xFF) << 8 | (c[2] & 0xFF) << 16 | static_cast<uint32_t>(c[3]) << 24;
 }
 
-template <class T>
-__device__ __forceinline__ float as_float(uint32_t bits16);
-template <>
-__device__ __forceinline__ float as_float<BF16>(uint32_t x) { return __uint_as_float(x << 16); }
-template <>
-__device__ __forceinline__ float as_float<F16>(uint32_t x) {
-    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x)));
-}
-
 // ---------------------------------------------------------------- bounds
 
 constexpr uint32_t kBoundsThreads = 256, kBoundsTokens = 256;

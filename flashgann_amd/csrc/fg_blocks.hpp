@@ -10,6 +10,16 @@ constexpr uint32_t kMostBlocks = 4096;     // of a list: what attention over the
 constexpr uint32_t kMostTokens = 1u << 22; // of a call
 constexpr uint32_t kMostItems = 1u << 23;  // tiles and lists of a call, a grid's workgroups
 
+// A value's 16 bits as a float.
+template <class T>
+__device__ __forceinline__ float as_float(uint32_t bits16);
+template <>
+__device__ __forceinline__ float as_float<BF16>(uint32_t x) { return __uint_as_float(x << 16); }
+template <>
+__device__ __forceinline__ float as_float<F16>(uint32_t x) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x)));
+}
+
 // The barrier that publishes LDS and nothing else: loads in flight from global memory stay
 // in flight.
 __device__ __forceinline__ void lds_barrier() {

@@ -421,7 +421,9 @@ int64_t fg_select_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_atte
  * lies outside [sinks, c - window], adds nothing.  nids at most 4,096, 0 allowed; tokens
  * at most 4,194,304, and at most 2^23 tiles of rows: (tokens + requests) * lists *
  * ceil(heads / lists / 16) up to that always serves.  No two rows of out may share memory (a stride
- * of 0 is refused); out may be q itself. */
+ * of 0 is refused); out may be q itself.  Weights go into the product with the values in two parts of
+ * the cache's type, so an output is off by its own rounding and that of 32-bit sums; an infinite value
+ * makes its channel infinite, or NaN, for the rows that see it and for no other. */
 int fg_attend_blocks(const fg_kv_cache *cache, const fg_attention *a, void *workspace, uint64_t workspace_bytes,
                      void *stream);
 int64_t fg_attend_blocks_workspace_bytes(const fg_kv_cache *cache, const fg_attention *a);
