@@ -20,15 +20,15 @@ constexpr uint32_t kMostParts = 64;
 // What rounding two weights to the values' type left of them, in that type too.  The matrix unit takes
 // 16 bits, and outputs are to be off by their own rounding alone: a weight goes in as the sum of two
 // such numbers (16 bits of it in bfloat16, 22 in float16), against the same values read once.  A chunk's
-// attention takes 6% longer for it (381 us against 359), single tokens and drafts do not; the error is
-// that of 32-bit weights (0.0017 relative in bfloat16, the output's rounding, against 0.0021 with one part).
+// attention takes 6% longer for it, single tokens and drafts do not; the error is that of 32-bit
+// weights (0.0017 relative in bfloat16, the output's rounding, against 0.0021 with one part).
 template <class T>
 __device__ __forceinline__ uint32_t rest_of(float a, float b, uint32_t rounded) {
     return T::pack(a - as_float<T>(rounded & 0xFFFF), b - as_float<T>(rounded >> 16));
 }
 
 // Whether an infinity or NaN is among N pieces of 16-bit values: 0 times any other is 0, two values
-// an instruction (their magnitudes' maximum takes two: 381 us of a chunk's attention against 377).
+// an instruction.
 __device__ __forceinline__ float plus_zero_times(BF16, uint32_t w, float sum) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{0.0f, 0.0f}, sum, false);
 }
@@ -473,6 +473,7 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
     const uint32_t blocks = static_cast<uint32_t>(min(block_of(t.pos + t.rows - 1), static_cast<int32_t>(P.table_width) - 1) + 1);
     const uint32_t dense = static_cast<uint32_t>(min(max(static_cast<int64_t>(block_of(t.pos)) - P.last + 1, static_cast<int64_t>(0)), static_cast<int64_t>(blocks)));
     const uint32_t everyone = tokens >= 32 ? ~0u : (1u << tokens) - 1;
+    const bool by_block = page_size * tokens > 32;  // fewer blocks in a tile of 32 places than tokens
 
     // this lane's row
     const uint32_t rows = tokens * P.per.d, token = P.per.div(col), heads = min(P.group - head0, P.per.d);
@@ -489,8 +490,11 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
     const char *const kbase = P.cache.k + kv_head * P.cache.k_head + half * 16, *const vbase = P.cache.v + kv_head * P.cache.v_head;
     char *const vmine = lds + wave * 32 * VROW;
 
-    float m = -INFINITY, l = 0.0f;
+    float m, l;
     f32x16 o[DB];
+    bool careful = false;  // whether infinities and NaN are taken out of the products
+again:
+    m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
@@ -574,8 +578,10 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
         const auto find = [&](int32_t i) {
             const int32_t n = i * 32 + static_cast<int32_t>(col), in = min(n, total - 1);
             const uint32_t e = P.cache.page_size.div(in);
-            const int64_t off = in - static_cast<int32_t>(e * page_size), p = B.entry_page[e];
+            int64_t off = in - static_cast<int32_t>(e * page_size);
+            const int64_t p = B.entry_page[e];
             sees = n < total ? B.entry_seen[e] & tokens_from(t.pos, static_cast<int64_t>(B.entry_block[e]) * page_size + off) : 0u;
+            off = sees ? off : 0;  // (whatever lies where no row sees it stays unread: the block's first token is seen)
             ks = kbase + p * P.cache.k_page + off * P.cache.k_token;
             if (half == 0) value_at[wave][i / 4 % 2][col] = p * P.cache.v_page + off * P.cache.v_token;
             team_sync<1>();  // (other lanes read it)
@@ -606,9 +612,7 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
             for (int k = 0; k < STEPS; ++k) s = T::mfma32(__builtin_bit_cast(vec, kr[k]), qv[k], s);
             if (more) load_k();
             uint32_t odd = 0;  // tokens whose values are not all finite
-            if (__any(any_specials<T>(vr))) {
-                // (as in the few-rows kernel) infinities and NaNs are taken out of the product and added to
-                // the rows that see them
+            if (careful) {
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
                     if (any_special<T>(vr[k])) odd |= 1u << (k * 64 + lane) / CHUNKS;
@@ -622,12 +626,24 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
                 *reinterpret_cast<u32x4 *>(vmine + at / CHUNKS * VROW + at % CHUNKS * 16) = vr[k];
             }
             if (more) load_v(i + 4);
-            // the tile's tokens that this lane's row sees
+            // the tile's tokens that this lane's row sees: those that the same tokens see, a block's as a rule,
+            // together (32 tokens a tile, pages of 64, 111 us of a chunk against 186 token by token; 8 and 16 144,
+            // 146), or token by token where a tile has no more of them than blocks
             uint32_t row_sees = 0, all = ~0u;
-            for (uint32_t x = 0; x < tokens; ++x) {
-                const uint32_t those = static_cast<uint32_t>(__ballot((sees_now >> x) & 1u));
-                all &= those;
-                row_sees = token == x ? those : row_sees;
+            if (by_block) {
+                for (uint32_t left = ~0u; left;) {
+                    const uint32_t seen_by = static_cast<uint32_t>(of_lane(static_cast<int32_t>(sees_now), __ffs(left) - 1));
+                    const uint32_t those = static_cast<uint32_t>(__ballot(sees_now == seen_by));
+                    left &= ~those;
+                    if (seen_by != everyone) all = 0;
+                    row_sees |= those & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int32_t>(seen_by), token, 1));
+                }
+            } else {
+                for (uint32_t x = 0; x < tokens; ++x) {
+                    const uint32_t those = static_cast<uint32_t>(__ballot((sees_now >> x) & 1u));
+                    all &= those;
+                    row_sees = token == x ? those : row_sees;
+                }
             }
             if (all != ~0u) {
                 const uint32_t bits = row_sees >> (4 * half);
@@ -681,6 +697,24 @@ __global__ __launch_bounds__(256, 2) void fg_blocks_chunk_kernel(BlocksParams P)
                         o[k][4 * g + 3] += visible ? special_part<T>(v.y >> 16) : 0.0f;
                     }
             }
+        }
+    }
+
+    if (!careful) {
+        // 0 * inf is NaN: a value that is not finite leaves no output of its channel finite, of rows that see
+        // it or not.  Then all again with such values taken out of the products and added to the rows that see them
+        float zero = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DB; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) zero = fmaf(o[k][i], 0.0f, zero);
+        const bool odd = __any(zero != zero);
+        __syncthreads();
+        if (lane == 0) found[wave] = odd;
+        __syncthreads();
+        if (uniform(found[0] | found[1] | found[2] | found[3])) {
+            careful = true;
+            goto again;
         }
     }
 
