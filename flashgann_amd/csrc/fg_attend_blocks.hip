@@ -93,7 +93,7 @@ __device__ __forceinline__ bool on_list(const int32_t *list, uint32_t n, int32_t
 
 // Bound by the bytes of the union: 48 single tokens over 48 selected pages of 32 and the first and last
 // (32 heads over 8, dim 128) 66 us, 4.9 TB/s; of few tokens by latency, lists, union, table and keys one
-// after another: 5 requests of 1 to 5 tokens 11.4 us, and 4 to join their parts.
+// after another: 5 requests of 1 to 5 tokens 11.0 us, and 4 to join their parts.
 template <class T, int D>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void fg_blocks_kernel(BlocksParams P) {
     using vec = typename T::vec;
@@ -428,11 +428,11 @@ __global__ __launch_bounds__(256) void fg_blocks_join_kernel(BlocksParams P) {
 // worked out.  The union of the lists is made a window of blocks at a time, a word of
 // tokens for each block, so its blocks come in order and none twice.
 //
-// A chunk of 2,048 tokens after 62,000 (32 heads over 8, dim 128, 16 pages of 64 each) 354 us; its
-// tiles of eight tokens read 59 blocks each of the 160 listed, 4 GB in all, of which the L2 has 69%.
-// Waves wait for loads 48% of their time, vector issue is 38% of it, the matrix unit 15%.  In tiles
-// of 16 rows 720 us; rows of several waves over tiles shared in LDS 546 us (a barrier a tile, and
-// each wave masks what only the others asked for).
+// A chunk of 2,048 tokens after 62,000 (32 heads over 8, dim 128, 16 pages of 64 each) 353 us; its
+// tiles of eight tokens read 59 blocks each of the 160 listed, 4 GB in all, of which the L2 has 67%.
+// Waves wait for loads 41% of their time, vector issue is 42% of it, the matrix unit 23%.  In tiles
+// of 16 rows 689 us; rows of several waves over tiles shared in LDS took 546 us against 354 (a barrier a
+// tile, and each wave masks what only the others asked for).
 constexpr uint32_t kChunkRows = 32;
 constexpr uint32_t kWindow = 1024;  // blocks whose tokens are known at a time
 
@@ -627,8 +627,8 @@ again:
             }
             if (more) load_v(i + 4);
             // the tile's tokens that this lane's row sees: those that the same tokens see, a block's as a rule,
-            // together (32 tokens a tile, pages of 64, 111 us of a chunk against 186 token by token; 8 and 16 144,
-            // 146), or token by token where a tile has no more of them than blocks
+            // together, or token by token where a tile has no more of those than blocks (1,024 tokens over 16
+            // pages of 64, dim 128: 32 tokens a tile 111 us against 186 token by token, 8 148 against 148)
             uint32_t row_sees = 0, all = ~0u;
             if (by_block) {
                 for (uint32_t left = ~0u; left;) {
@@ -808,10 +808,10 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     P.scale2 = a->scale * 1.44269504088896341f;
 
     // Tiles of 32 rows once they fill half the device, whole; before that those of 16 are split among
-    // workgroups.  24 of 250 pages of 32 (32 heads over 8, dim 128): 8 requests of 8 new tokens 45.8 us
-    // against 42.2, of 16 46.3 against 62.7, of 64 67 against 123; 32 requests of 2 46.5 against 51.6; one
-    // of 64 40.8 against 28.  Over many blocks windows cost more than lists in order: 256 tokens, 64 of
-    // 500 blocks 30 against 43, of 2,000 41 against 49, of 7,500 80 against 53.  (At dim 256 the chunk
+    // workgroups.  24 of 250 pages of 32 (32 heads over 8, dim 128): 8 requests of 8 new tokens 42.5 us
+    // against 41.1, of 16 43.2 against 59.9, of 64 67 against 117; 32 requests of 2 46.6 against 51.1; one
+    // of 64 37.9 against 26.6.  Over many blocks windows cost more than lists in order: 256 tokens, 64 of
+    // 500 blocks 30 against 42, of 2,000 41 against 48, of 7,500 81 against 52.  (At dim 256 the chunk
     // kernel's rows do not fit the registers.)
     const auto tile_tokens = [&](uint32_t rows) { return rows / std::min(P.group, rows); };
     const uint64_t chunk_tiles = std::max<uint64_t>(a->tokens / tile_tokens(kChunkRows), a->requests) * P.lists * ((P.group + kChunkRows - 1) / kChunkRows);
@@ -832,7 +832,7 @@ int prepare(const fg_kv_cache *c, const fg_attention *a, BlocksParams *out, Bloc
     const uint64_t blocks = std::min<uint64_t>(a->table_width, static_cast<uint64_t>(P.first) + P.last + at_a_time * P.nids);
     const uint64_t most = blocks * c->page_size;
     // Parts of a tile until every CU has one: 48 single tokens over 51 pages of 32, 480 tiles, 72.8 us
-    // whole, 76.9 in two parts; 4 drafts of 1 to 5, 32 tiles, 14.8 us in eight.
+    // whole, 76.9 in two parts; 4 drafts of 1 to 5, 32 tiles, 14.2 us in eight.
     P.parts = 1;
     while (!plan->chunk && P.parts < kMostParts && items * P.parts < 256 && most > 2 * P.parts * kSplitTokens) P.parts *= 2;
     const uint64_t slots = items * P.parts * kTileRows;

@@ -376,7 +376,7 @@ int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *
  * The host does not know the lengths, so kernels and workspaces of these calls and of eviction
  * follow the table's room: let table_width be the columns in use, not those allocated.  One MI355X: a chunk
  * of 4,096 tokens selecting from 1,000 pages 99 us, in a table of 8,192 columns 297 and of 32,768 1,930;
- * attention of 2,048 over what they selected 341 us, past 4,096 columns 711. */
+ * attention of 2,048 over what they selected 353 us, past 4,096 columns 689. */
 
 /* For each of `tokens` slots that is the last of its page, 8-bit bounds of that page's keys
  * (cache->v is not read and may be NULL): with M the largest |key| of a page and key/value head and 2^s the
