@@ -202,6 +202,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     are: leave them out of the free pages.  No page may be named twice, and k_cache and v_cache may share
     no memory, with each other or between their own places.  1 to 4,096 requests a call.
 
-    Kernels and workspace (8 bytes a request, head and token of the budget at least) follow what the
-    table has room for: pass the columns in use, block_table[:, :n]."""
+    Kernels and workspace (8 bytes a request, head and token that the table names past the budget, or
+    of the budget if that is less) follow what the table has room for: pass the columns in use,
+    block_table[:, :n]."""
     return CacheEviction(*_attention.cache_evict(k_cache, v_cache, weights, block_table, kv_lens, budget, window, sinks))

@@ -185,7 +185,7 @@ struct EvictParams {
     uint32_t *keys;      // where registers do not hold them: `room` for each workgroup
     uint32_t table_width, requests, heads_kv, budget, window, sinks;
     uint32_t room;       // tokens that the table names
-    uint32_t most;       // min(budget, room)
+    uint32_t most;       // tokens that may move into holes: min(budget, room - budget)
     uint32_t choosers;   // workgroups that choose; the others list the pages that go
     uint32_t pieces;     // 16-byte pieces of a row of keys
     uint32_t at_once;    // whether those that choose move too
@@ -506,7 +506,7 @@ int plan_evict(const fg_kv_cache *c, uint32_t table_width, uint32_t requests, ui
     P.heads_kv = c->heads_kv;
     P.budget = budget;
     P.room = table_width * c->page_size;
-    P.most = std::min(budget, P.room);
+    P.most = std::min(budget, P.room - std::min(P.room, budget));
     const uint64_t pairs = static_cast<uint64_t>(requests) * c->heads_kv, slots = pairs * P.most;
     plan->held = P.room <= kChooseKeys;
     P.choosers = static_cast<uint32_t>(std::min<uint64_t>(pairs, plan->held ? 65536 : kChooseWorkgroups));
