@@ -379,8 +379,8 @@ int64_t fg_attend_workspace_bytes(const fg_kv_cache *cache, const fg_attention *
  * attention of 2,048 over what they selected 353 us, past 4,096 columns 689. */
 
 /* For each of `tokens` slots that is the last of its page, 8-bit bounds of that page's keys
- * (cache->v is not read and may be NULL): with M the largest |key| of a page and key/value head and 2^s the
- * least power of two with M <= 127 * 2^s, not below 2^-126,
+ * (cache->v is not read and may be NULL): with M the largest |key| of a page and key/value head and
+ * 2^s the least power of two with M <= 127 * 2^s, not below 2^-126,
  *   d_scales[page * heads_kv + head]                       2^s
  *   d_bounds[((page * heads_kv + head) * 2 + 0) * dim + d] the largest key of channel d / 2^s, rounded up
  *   d_bounds[((page * heads_kv + head) * 2 + 1) * dim + d] the smallest, rounded down
@@ -466,10 +466,11 @@ int fg_cache_weigh(const fg_kv_cache *cache, const fg_attention *a, float *d_wei
  * memory, nor k and v (a stride of 0 and k == v are refused), d_new_lens not overlap d_kv_lens.  Bounds of
  * pages whose keys moved are void.  1 <= requests <= 4096, sinks + window <= budget, 1 <= budget.
  *
- * Workspace: 8 bytes a request, head and token that may move, min(budget, table_width * page_size - budget), and
- * over tables that name more than 32,768 tokens 4 for each of those and up to 512 requests and heads.  A table that names at most
- * 512 tokens past the budget, 8,192 in all, serves in one launch (48 requests a few over 4,096 tokens 26 us; in
- * a table of 8,192 pages of 16 43 us and 215 MB instead of 0.2). */
+ * Workspace: 8 bytes a request, head and token that may move, min(budget, table_width * page_size -
+ * budget), and over tables that name more than 32,768 tokens 4 for each of those and up to 512 requests
+ * and heads.  A table that names at most 512 tokens past the budget, 8,192 in all, serves in one launch if
+ * window is at most 512 (48 requests a few over 4,096 tokens 26 us; in a table of 8,192 pages of 16 43 us
+ * and 215 MB instead of 0.2). */
 int fg_cache_evict(const fg_kv_cache *cache, float *d_weights, const int32_t *d_table, int64_t table_row, uint32_t table_width,
                    const int32_t *d_kv_lens, uint32_t requests, uint32_t budget, uint32_t window, uint32_t sinks,
                    int32_t *d_new_lens, int32_t *d_freed, int32_t *d_released, void *workspace, uint64_t workspace_bytes,
